@@ -352,6 +352,54 @@ int mx_token_logprob_bwd_any(const void* logits, int64_t rows, int64_t vocab, in
                              const int64_t* target, const float* lse, const float* grad_logprob,
                              void* dlogits, int64_t ldd, void* stream);
 
+/* Token embedding (the first layer of torchtitan/models/common/decoder.py:59-155):
+ * out[t, :] = scale * weight[ids[t] - first, :], a row of zeros where ids[t] - first is not in [0, rows) (the
+ * table of a vocabulary shard).  ids int64 or, with ids_i64 = 0, int32 [n]; weight [rows, cols] (row stride ldw),
+ * out [n, cols] dense, each bf16 or float32; the product is formed in float32 and rounded once.
+ * mx_embedding_grad: grad[v, :] = scale * (sum of dout[t, :] over the t with ids[t] - first = v and ids[t] !=
+ * padding; an id outside the table: no padding), every row written, zeros where there is no such t; dout [n, cols]
+ * (row stride ldd), grad [rows, cols] dense.  Sums are float32, in the order of t within parts that depend on the ids
+ * alone: the same bits on every run.  workspace: mx_embedding_grad_workspace bytes, 16-byte aligned.
+ * Element-aligned tensors; any cols; n and rows below 2^31 - 1, else MX_ERR_UNSUPPORTED. */
+int mx_embedding(const void* ids, int ids_i64, int64_t n, const void* weight, int weight_f32, int64_t rows, int64_t cols,
+                 int64_t ldw, int64_t first, float scale, void* out, int out_f32, void* stream);
+int64_t mx_embedding_grad_workspace(int64_t n, int64_t rows, int64_t cols);
+int mx_embedding_grad(const void* ids, int ids_i64, int64_t n, const void* dout, int dout_f32, int64_t ldd, int64_t rows,
+                      int64_t cols, int64_t first, int64_t padding, float scale, void* grad, int grad_f32, void* workspace,
+                      void* stream);
+
+/* The residual sum behind a block with the norms on both its sides (torchtitan/models/common/rmsnorm.py:14-50 and the
+ * residual additions of a transformer block), in float32 for every row of h and r [rows, cols]:
+ *     n = post ? rms_norm(h) * post : h;   t = scale * r + (gate ? gate * n : n)
+ *     stream_out = t;   normed = rms_norm(t) * pre   (before t is rounded; pre NULL: not formed)
+ * rms_norm(x) = x / sqrt(mean x^2 + eps).  h and normed are bf16 or float32 (h_f32), r and stream_out are r_f32 (r float32
+ * where h is); row strides ldh and ldr, outputs dense.  post, pre [cols], gate [gate_rows, cols], gate_rows dividing rows: row i uses
+ * gate row i / (rows / gate_rows); each is float32 where its bit of weights_f32 is set (1 post, 2 gate, 4 pre), else
+ * bf16.  rstd (float32 [2, rows], may be NULL): both 1 / sqrt(...), which the backward needs.
+ * mx_residual_norm_bwd: from the gradients of stream_out and normed (dense; NULL: zero) those of h, r, post, gate and pre
+ * (NULL: not wanted), each in its operand's type; sums over rows in float32, in an order that depends on the sizes alone.
+ * workspace: mx_residual_norm_workspace bytes, 16-byte aligned.  Element-aligned tensors; any cols. */
+int mx_residual_norm(const void* h, int h_f32, const void* r, int r_f32, int64_t rows, int64_t cols, int64_t ldh, int64_t ldr,
+                     const void* post, const void* gate, const void* pre, int weights_f32, int64_t gate_rows, float scale,
+                     float eps, void* stream_out, void* normed, float* rstd, void* stream);
+int64_t mx_residual_norm_workspace(int64_t rows, int64_t cols, int64_t gate_rows);
+int mx_residual_norm_bwd(const void* h, int h_f32, const void* r, int r_f32, int64_t rows, int64_t cols, int64_t ldh,
+                         int64_t ldr, const void* post, const void* gate, const void* pre, int weights_f32, int64_t gate_rows,
+                         float scale, const float* rstd, const void* dstream, const void* dnormed, void* dh, void* dr,
+                         void* dpost, void* dgate, void* dpre, void* workspace, void* stream);
+
+/* The norm of n tensors (host arrays; bf16, or float32 where is_f32[i]; elems[i] values in one run of memory) taken as one
+ * vector, and their scaling (the clipping of gradients, torchtitan/distributed/utils.py:466-472 and around).  kind 0: sqrt(sum
+ * x^2), 1: sum |x|, 2: max |x|; sums in float64, norm: one float32 on the device.  workspace: mx_grad_norm_workspace(n)
+ * bytes, 8-byte aligned.
+ * mx_grad_scale: every value times min(1, limit / (*norm + 1e-6)), in float32, rounded to its type, in place; nothing
+ * is touched where that is exactly 1.  Tensors that share memory are scaled one after the other. */
+int64_t mx_grad_norm_workspace(int64_t n);
+int mx_grad_norm(int64_t n, void* const* grads, const int64_t* elems, const int32_t* is_f32, int kind, float* norm,
+                 void* workspace, void* stream);
+int mx_grad_scale(int64_t n, void* const* grads, const int64_t* elems, const int32_t* is_f32, const float* norm, float limit,
+                  void* stream);
+
 /* Re-order a row-major [rows, nblk] scale matrix into MX_SCALES_MFMA order
  * (the "blocked layout" step the reference leaves to torch._scaled_mm, docs/mxfp8.md:36). */
 int mx_scale_layout(const uint8_t* scales, int64_t rows, int64_t nblk, uint8_t* out, void* stream);

@@ -66,6 +66,17 @@ SIGNATURES = {
     "mx_swiglu_bwd_cast_dim0_dim1_ld": (c_int, [_P, _P, _P, _I, _I, _I, _I, _I, _P, _I, _P, _P, _I, _P, _P, c_int, c_int, _P]),
     "mx_swiglu_cast_dim0_dim1": (c_int, [_P, _P, _I, _I, _I, _I, _P, _P, _P, _P, _P, c_int, c_int, _P]),
     "mx_swiglu_bwd_cast_dim0_dim1": (c_int, [_P, _P, _P, _I, _I, _I, _I, _I, _P, _P, _P, _P, _P, c_int, c_int, _P]),
+    "mx_embedding": (c_int, [_P, c_int, _I, _P, c_int, _I, _I, _I, _I, ctypes.c_float, _P, c_int, _P]),
+    "mx_embedding_grad_workspace": (_I, [_I, _I, _I]),
+    "mx_embedding_grad": (c_int, [_P, c_int, _I, _P, c_int, _I, _I, _I, _I, _I, ctypes.c_float, _P, c_int, _P, _P]),
+    "mx_residual_norm": (c_int, [_P, c_int, _P, c_int, _I, _I, _I, _I, _P, _P, _P, c_int, _I, ctypes.c_float,
+                                 ctypes.c_float, _P, _P, _P, _P]),
+    "mx_residual_norm_workspace": (_I, [_I, _I, _I]),
+    "mx_residual_norm_bwd": (c_int, [_P, c_int, _P, c_int, _I, _I, _I, _I, _P, _P, _P, c_int, _I, ctypes.c_float,
+                                     _P, _P, _P, _P, _P, _P, _P, _P, _P, _P]),
+    "mx_grad_norm_workspace": (_I, [_I]),
+    "mx_grad_norm": (c_int, [_I, _P, _P, _P, c_int, _P, _P, _P]),
+    "mx_grad_scale": (c_int, [_I, _P, _P, _P, _P, ctypes.c_float, _P]),
     "mx_scale_layout": (c_int, [_P, _I, _I, _P, _P]),
     "mx_scale_unlayout": (c_int, [_P, _I, _I, _P, _P]),
     "mx_gemm_nt": (c_int, [_P, _P, _P, _P, _P, _I, _I, _I, _I, _P]),

@@ -971,6 +971,191 @@ def swiglu_bwd_to_mx_dim0_dim1(dg: torch.Tensor, a: torch.Tensor, b: torch.Tenso
     return half(0), half(1), dab
 
 
+# --------------------------------------------------------------------------- around the linears
+ROW_TYPES = (torch.bfloat16, torch.float32)  # of the embedding, the norms around a block and the gradients
+
+
+def plain_rows(*operands) -> bool:
+    """The kernels below take these tensors (None among them: no operand): plain ones on the GPU, bf16 or float32,
+    outside function transforms."""
+    return not _transformed() and all(
+        t is None or (type(t) in (torch.Tensor, torch.nn.Parameter) and t.is_cuda and t.dtype in ROW_TYPES) for t in operands)
+
+
+def _rows_as_they_lie(t: torch.Tensor) -> torch.Tensor:
+    """[rows, cols] with unit inner stride and rows that do not overlap (a copy where they do)."""
+    if (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+        return t.contiguous()
+    return t
+
+
+def _row_type(t: torch.Tensor, what: str) -> int:
+    if not t.is_cuda:
+        raise _lib.MXLibraryError(f"{what}: the kernels run on the GPU only; got a CPU tensor")
+    if t.dtype not in ROW_TYPES:
+        raise TypeError(f"{what} must be bfloat16 or float32, got {t.dtype}")
+    return int(t.dtype == torch.float32)
+
+
+def _check_ids(ids: torch.Tensor, like: torch.Tensor) -> torch.Tensor:
+    if ids.dtype not in (torch.int64, torch.int32):
+        raise TypeError(f"ids must be int64 or int32, got {ids.dtype}")
+    if ids.device != like.device:
+        raise ValueError(f"ids on {ids.device}, the rows on {like.device}")
+    return ids.contiguous()
+
+
+def embedding_fwd(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, first_row: int = 0,
+                  dtype: torch.dtype | None = None) -> torch.Tensor:
+    """`dtype` [*ids.shape, cols]: scale * weight[ids - first_row] (float32, rounded once), zeros for an id outside
+    the table's rows.  weight: bf16 or float32 [rows, cols]."""
+    w_f32, ids = _row_type(weight, "weight"), _check_ids(ids, weight)
+    weight = _rows_as_they_lie(weight)
+    (rows, cols), n = weight.shape, ids.numel()
+    out = torch.empty((*ids.shape, cols), dtype=dtype or weight.dtype, device=weight.device)
+    _call("mx_embedding", "embedding", weight.device, _ptr(ids), int(ids.dtype == torch.int64), n, _ptr(weight), w_f32, rows,
+          cols, weight.stride(0), first_row, scale, _ptr(out), _row_type(out, "dtype"), _stream(weight))
+    return out
+
+
+def embedding_bwd(ids: torch.Tensor, dout: torch.Tensor, rows: int, scale: float = 1.0, first_row: int = 0,
+                  padding_idx: int | None = None, dtype: torch.dtype | None = None) -> torch.Tensor:
+    """`dtype` [rows, cols], the gradient of `embedding_fwd`'s weight from dout [*ids.shape, cols]: equal ids summed in
+    float32 in an order that depends on the ids alone, rounded once; ids equal to `padding_idx` count for nothing."""
+    d_f32, ids = _row_type(dout, "dout"), _check_ids(ids, dout)
+    if dout.shape[:-1] != ids.shape:
+        raise ValueError(f"dout must be [*{tuple(ids.shape)}, cols], got {tuple(dout.shape)}")
+    cols, n = dout.shape[-1], ids.numel()
+    dout = _rows_as_they_lie(dout.reshape(n, cols))
+    grad = torch.empty((rows, cols), dtype=dtype or dout.dtype, device=dout.device)
+    work = torch.empty(_lib.load().mx_embedding_grad_workspace(n, rows, cols), dtype=torch.uint8, device=dout.device)
+    _call("mx_embedding_grad", "embedding_grad", dout.device, _ptr(ids), int(ids.dtype == torch.int64), n, _ptr(dout), d_f32,
+          dout.stride(0), rows, cols, first_row, first_row - 1 if padding_idx is None else padding_idx, scale, _ptr(grad),
+          _row_type(grad, "dtype"), _ptr(work), _stream(dout))
+    return grad
+
+
+def _norm_operands(h, residual, post, gate, pre):
+    """The matrices and vectors as the kernels read them, the types' flags and the number of gate rows."""
+    h_f32, r_f32 = _row_type(h, "h"), _row_type(residual, "residual")
+    if h_f32 and not r_f32:
+        raise TypeError("a float32 block output needs a float32 residual")
+    if h.dim() != 2 or residual.shape != h.shape:
+        raise ValueError(f"h and residual must be matrices of one shape, got {tuple(h.shape)} and {tuple(residual.shape)}")
+    rows, cols = h.shape
+    flags, weights = 0, []
+    for bit, (name, w) in enumerate((("post_weight", post), ("gate", gate), ("pre_weight", pre))):
+        if w is not None:
+            flags |= _row_type(w, name) << bit
+            if w.device != h.device:
+                raise ValueError(f"{name} on {w.device}, h on {h.device}")
+            if name == "gate":
+                if w.dim() != 2 or w.shape[1] != cols or not w.shape[0] or rows % w.shape[0]:
+                    raise ValueError(f"gate must be [n, {cols}] with n dividing {rows}, got {tuple(w.shape)}")
+            elif w.shape != (cols,):
+                raise ValueError(f"{name} must be [{cols}], got {tuple(w.shape)}")
+            w = w.contiguous()
+        weights.append(w)
+    if residual.device != h.device:
+        raise ValueError(f"residual on {residual.device}, h on {h.device}")
+    groups = 1 if gate is None else gate.shape[0]
+    return _rows_as_they_lie(h), h_f32, _rows_as_they_lie(residual), r_f32, weights, flags, groups
+
+
+def _optional_ptr(t: torch.Tensor | None):
+    return None if t is None else t.data_ptr()
+
+
+def residual_norm(h: torch.Tensor, residual: torch.Tensor, post: torch.Tensor | None, gate: torch.Tensor | None,
+                  pre: torch.Tensor | None, scale: float, eps: float, want_rstd: bool = False):
+    """(stream, normed or None, rstd or None) of `mx_residual_norm`: the residual sum scale * residual + gate *
+    (rms_norm(h) * post) in residual's type and its rms_norm * pre in h's, for matrices [rows, cols] and a gate
+    [n, cols], n dividing the rows; each of post, gate and pre may be None."""
+    h, h_f32, r, r_f32, weights, flags, groups = _norm_operands(h, residual, post, gate, pre)
+    (rows, cols), dev = h.shape, h.device
+    stream = torch.empty((rows, cols), dtype=r.dtype, device=dev)
+    normed = None if pre is None else torch.empty((rows, cols), dtype=h.dtype, device=dev)
+    rstd = torch.empty((2, rows), dtype=torch.float32, device=dev) if want_rstd else None
+    _call("mx_residual_norm", "residual_norm", dev, _ptr(h), h_f32, _ptr(r), r_f32, rows, cols, h.stride(0), r.stride(0),
+          *(_optional_ptr(w) for w in weights), flags, groups, scale, eps, _ptr(stream), _optional_ptr(normed),
+          _optional_ptr(rstd), _stream(h))
+    return stream, normed, rstd
+
+
+def residual_norm_bwd(h: torch.Tensor, residual: torch.Tensor, post: torch.Tensor | None, gate: torch.Tensor | None,
+                      pre: torch.Tensor | None, scale: float, rstd: torch.Tensor, dstream: torch.Tensor | None,
+                      dnormed: torch.Tensor | None, needs=(True, True, True, True, True)):
+    """Gradients of h, residual, post, gate and pre (None where `needs` says so or the operand is None) from those of
+    `residual_norm`'s outputs (None: zero) and its rstd."""
+    h, h_f32, r, r_f32, weights, flags, groups = _norm_operands(h, residual, post, gate, pre)
+    (rows, cols), dev = h.shape, h.device
+    if rstd.shape != (2, rows) or rstd.dtype != torch.float32 or rstd.device != dev:
+        raise TypeError(f"rstd must be float32 [2, {rows}] on h's device")
+    for d, like in ((dstream, r), (dnormed, h)):
+        if d is not None and (d.shape != like.shape or d.dtype != like.dtype or d.device != dev):
+            raise TypeError("gradients must have their outputs' shape, type and device")
+    dstream, dnormed = (None if d is None else d.contiguous() for d in (dstream, dnormed))
+    rstd = rstd.contiguous()
+    grads = [torch.empty(t.shape, dtype=t.dtype, device=dev) if need and t is not None else None
+             for need, t in zip(needs, (h, r, *weights))]
+    if rows == 0:  # sums over no row
+        return tuple(None if g is None else g.zero_() for g in grads)
+    work = torch.empty(_lib.load().mx_residual_norm_workspace(rows, cols, groups), dtype=torch.uint8, device=dev)
+    _call("mx_residual_norm_bwd", "residual_norm_bwd", dev, _ptr(h), h_f32, _ptr(r), r_f32, rows, cols, h.stride(0),
+          r.stride(0), *(_optional_ptr(w) for w in weights), flags, groups, scale, _ptr(rstd), _optional_ptr(dstream),
+          _optional_ptr(dnormed), *(_optional_ptr(g) for g in grads), _ptr(work), _stream(h))
+    return tuple(grads)
+
+
+GRAD_NORMS = {2.0: 0, 1.0: 1, float("inf"): 2}
+
+
+def _grad_lists(grads):
+    dev = grads[0].device
+    for t in grads:
+        _row_type(t, "gradients")
+        if t.device != dev:
+            raise ValueError(f"gradients on {dev} and {t.device}: one device a call")
+        if not is_dense(t):
+            raise ValueError(f"a gradient of shape {tuple(t.shape)} with strides {t.stride()} is not one run of memory")
+    return (len(grads), _host_table([_ptr(t) for t in grads], c_int64), _host_table([t.numel() for t in grads], c_int64),
+            _host_table([int(t.dtype == torch.float32) for t in grads], c_int32))
+
+
+def is_dense(t: torch.Tensor) -> bool:
+    """The tensor's elements are one run of memory, each once, in whatever order."""
+    if t.is_contiguous() or t.numel() == 0:
+        return True
+    need = 1
+    for stride, size in sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz > 1):
+        if stride != need:
+            return False
+        need *= size
+    return True
+
+
+def grad_norm(grads, norm_type: float = 2.0) -> torch.Tensor:
+    """float32 scalar: the 2-, 1- or infinity-norm of all tensors of the list (bf16 or float32, one GPU, dense) taken as
+    one vector, summed in float64."""
+    grads = list(grads)
+    lists = _grad_lists(grads)
+    dev = grads[0].device
+    norm = torch.empty((), dtype=torch.float32, device=dev)
+    work = torch.empty(_lib.load().mx_grad_norm_workspace(len(grads)), dtype=torch.uint8, device=dev)
+    _call("mx_grad_norm", "grad_norm", dev, *lists, GRAD_NORMS[float(norm_type)], _ptr(norm), _ptr(work), _stream(norm))
+    return norm
+
+
+def grad_scale_(grads, norm: torch.Tensor, limit: float) -> None:
+    """Every tensor of the list times min(1, limit / (norm + 1e-6)), in place; norm: a float32 scalar on their GPU."""
+    grads = list(grads)
+    lists = _grad_lists(grads)
+    if norm.dtype != torch.float32 or norm.numel() != 1 or norm.device != grads[0].device:
+        raise TypeError("the norm must be one float32 on the gradients' device")
+    torch.autograd.graph.increment_version(grads)
+    _call("mx_grad_scale", "grad_scale", grads[0].device, *lists, _ptr(norm), limit, _stream(norm))
+
+
 def scale_layout(scales: torch.Tensor) -> torch.Tensor:
     """Row-major [rows, nblk] scales -> flat buffer in MFMA order."""
     rows, nblk = scales.shape
