@@ -63,6 +63,134 @@ __device__ __forceinline__ T norm_rounded(float f) {
   else return (uint16_t)(__builtin_bit_cast(uint32_t, __builtin_convertvector(v2f_t{f, f}, v2bf_t)));
 }
 
+// ---- rows that fit the registers of their lanes: kV-element pieces, piece k of lane l at column (k LANES + l) kV.
+// Where the width is no multiple of kV the last piece lies kV in front of the row's end and covers columns of the one
+// before again: both lanes form and write the same values there, and the row's sums leave the second out.
+constexpr int kV = 8;
+
+template <int LANES, int N>
+struct NormShape {
+  static constexpr int kLanes = LANES, kPieces = N;              // of one row
+  static constexpr int kThreads = LANES > 64 ? LANES : 256;      // of a workgroup
+  static constexpr int kRows = kThreads / LANES;                 // that a workgroup works on at a time
+  static constexpr int kCols = LANES * N * kV;                   // a row's columns at most
+};
+
+// Where a lane's piece lies: from column `at` on, its first `skip` elements another lane's; none if not `in`.
+struct NormPlace {
+  int at, skip;
+  bool in;
+};
+template <class S>
+__device__ __forceinline__ NormPlace norm_place(int k, int lane, int cols) {
+  const int c = (k * S::kLanes + lane) * kV;
+  const int at = c < cols - kV ? c : cols - kV;
+  return {at, c - at, c < cols};
+}
+template <bool NT, class T>
+__device__ __forceinline__ void load_at(const T* row, const NormPlace& p, Piece<T, kV>& q) {
+  q = Piece<T, kV>{};
+  if (p.in) load_words<NT>(row + p.at, q);
+}
+template <class T>
+__device__ __forceinline__ void store_at(T* row, const NormPlace& p, const float (&f)[kV]) {
+  if (p.in) store_words<false>(row + p.at, from_floats<T>(f));
+}
+__device__ __forceinline__ void weight_at(const NormWeight& w, int64_t row, const NormPlace& p, float (&f)[kV]) {
+  if (!w.p) {
+#pragma unroll
+    for (int e = 0; e < kV; ++e) f[e] = 1.f;
+  } else if (w.f32) {
+    Piece<float, kV> q;
+    load_at<false>((const float*)w.p + row, p, q);
+    to_floats(q, f);
+  } else {
+    Piece<uint16_t, kV> q;
+    load_at<false>((const uint16_t*)w.p + row, p, q);
+    to_floats(q, f);
+  }
+}
+
+// Sum over the lanes of a row, in each of them.  Rows of more than a wave: `part` holds a float a wave, and a second
+// one has to be used in between before it is used again (one barrier a sum).
+template <int LANES>
+__device__ __forceinline__ float lanes_sum(float v, float* part) {
+#pragma unroll
+  for (int off = (LANES < 64 ? LANES : 64) / 2; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
+  if constexpr (LANES > 64) {
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = 0.f;
+#pragma unroll
+    for (int w = 0; w < LANES / 64; ++w) v += part[w];
+  }
+  return v;
+}
+
+template <class S, class H, class R>
+__global__ __launch_bounds__(S::kThreads) void residual_norm_kernel(NormArgs a, R* __restrict__ stream, H* __restrict__ normed,
+                                                                    float* __restrict__ rstd) {
+  constexpr int N = S::kPieces;
+  __shared__ float part[2][S::kLanes / 64 + 1];
+  const int lane = threadIdx.x % S::kLanes;
+  const int64_t row = (int64_t)blockIdx.x * S::kRows + threadIdx.x / S::kLanes;
+  if (row >= a.rows) return;  // (whole workgroups where rows share barriers)
+  const H* hp = (const H*)a.h + row * a.ldh;
+  const R* rp = (const R*)a.r + row * a.ldr;
+  const int64_t g0 = a.gate.p ? row / a.gate_each * a.cols : 0;
+  NormPlace at[N];
+  Piece<H, kV> h[N];
+  Piece<R, kV> r[N];
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    at[k] = norm_place<S>(k, lane, (int)a.cols);
+    load_at<true>(hp, at[k], h[k]);
+    load_at<true>(rp, at[k], r[k]);
+  }
+  float s1 = 1.f, s2 = 1.f;
+  if (a.post.p) {
+    float sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      float x[kV];
+      to_floats(h[k], x);
+#pragma unroll
+      for (int e = 0; e < kV; ++e) sum = __builtin_fmaf(x[e], e >= at[k].skip ? x[e] : 0.f, sum);
+    }
+    s1 = 1.f / sqrtf(lanes_sum<S::kLanes>(sum, part[0]) / (float)a.cols + a.eps);
+  }
+  float t[N][kV], sum = 0.f;
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    float x[kV], y[kV], p[kV], g[kV];
+    to_floats(h[k], x);
+    to_floats(r[k], y);
+    weight_at(a.post, 0, at[k], p);
+    weight_at(a.gate, g0, at[k], g);
+#pragma unroll
+    for (int e = 0; e < kV; ++e) {
+      t[k][e] = __builtin_fmaf(a.scale, y[e], g[e] * (x[e] * s1 * p[e]));
+      sum = __builtin_fmaf(t[k][e], e >= at[k].skip ? t[k][e] : 0.f, sum);
+    }
+    store_at(stream + row * a.cols, at[k], t[k]);
+  }
+  if (a.pre.p) {
+    s2 = 1.f / sqrtf(lanes_sum<S::kLanes>(sum, part[1]) / (float)a.cols + a.eps);
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      float w[kV];
+      weight_at(a.pre, 0, at[k], w);
+#pragma unroll
+      for (int e = 0; e < kV; ++e) w[e] *= t[k][e] * s2;
+      store_at(normed + row * a.cols, at[k], w);
+    }
+  }
+  if (rstd && lane == 0) {
+    rstd[row] = s1;
+    rstd[a.rows + row] = s2;
+  }
+}
+
 // Rows of any width, one workgroup a row, element by element; what a later step needs of an earlier one is formed again.
 template <class H, class R>
 __global__ __launch_bounds__(kNormThreads) void residual_norm_any_kernel(NormArgs a, R* __restrict__ stream,
@@ -177,16 +305,209 @@ __global__ __launch_bounds__(kNormThreads) void residual_norm_bwd_any_kernel(Nor
   }
 }
 
-// out[g, c] = sum over the parts p of group g, in order, of part[(g parts + p) stride + c].
-__global__ __launch_bounds__(kNormThreads) void residual_norm_join_kernel(const float* __restrict__ part, int64_t parts,
-                                                                          int64_t stride, int64_t cols, void* __restrict__ out,
-                                                                          int f32) {
-  const int64_t c = (int64_t)blockIdx.x * kNormThreads + threadIdx.x, g = blockIdx.y;
-  if (c >= cols) return;
-  float s = 0.f;
-  for (int64_t p = 0; p < parts; ++p) s += part[(g * parts + p) * stride + c];
-  if (f32) ((float*)out)[g * cols + c] = s;
-  else ((uint16_t*)out)[g * cols + c] = norm_rounded<uint16_t>(s);
+// A lane's sums of all rows of its workgroup: the rows' lanes add theirs to `lds` in turn.
+template <class S>
+__device__ __forceinline__ void rows_joined(float (&acc)[S::kPieces][kV], float* lds) {
+  if constexpr (S::kRows > 1) {
+    const int lane = threadIdx.x % S::kLanes, sub = threadIdx.x / S::kLanes;
+    for (int s = 0; s < S::kRows; ++s) {
+      if (sub == s) {
+#pragma unroll
+        for (int k = 0; k < S::kPieces; ++k)
+#pragma unroll
+          for (int e = 0; e < kV; ++e) {
+            float* at = lds + (k * kV + e) * S::kLanes + lane;  // (lanes side by side: no bank conflicts)
+            if (s > 0) acc[k][e] += *at;
+            *at = acc[k][e];
+          }
+      }
+      __syncthreads();
+    }
+#pragma unroll
+    for (int k = 0; k < S::kPieces; ++k)
+#pragma unroll
+      for (int e = 0; e < kV; ++e) acc[k][e] = lds[(k * kV + e) * S::kLanes + lane];
+    __syncthreads();
+  }
+}
+
+// SIDE: the block's side of the sum (norm behind it, gate) as well; else h has the gradient e.
+template <class S, bool SIDE, class H, class R>
+__global__ __launch_bounds__(S::kThreads) void residual_norm_bwd_kernel(NormArgs a, NormStrips strips,
+                                                                        const float* __restrict__ rstd, NormGrads o) {
+  constexpr int N = S::kPieces;
+  constexpr bool kHeld = N == 1;  // weights stay in registers; with two pieces a lane they are read again for every row
+  __shared__ float part[2][S::kLanes / 64 + 1];
+  __shared__ float lds[S::kRows > 1 ? S::kCols : 1];
+  const int lane = threadIdx.x % S::kLanes, sub = threadIdx.x / S::kLanes;
+  const float per = 1.f / (float)a.cols;
+  float dpre[N][kV] = {}, dpost[N][kV] = {};
+  NormPlace at[N];
+#pragma unroll
+  for (int k = 0; k < N; ++k) at[k] = norm_place<S>(k, lane, (int)a.cols);
+  float pre1[kV], post1[kV], gate1[kV];
+  if constexpr (kHeld) {
+    weight_at(a.pre, 0, at[0], pre1);
+    weight_at(a.post, 0, at[0], post1);
+  }
+  for (int64_t strip = blockIdx.x; strip < strips.total; strip += gridDim.x) {
+    const int64_t group = strip / strips.strips, part0 = (strip - group * strips.strips) * strips.each;
+    const int64_t first = group * a.gate_each + part0;
+    const int64_t end = first + (part0 + strips.each < a.gate_each ? strips.each : a.gate_each - part0);
+    const int64_t g0 = group * a.cols;
+    float dgate[N][kV] = {};
+    if constexpr (kHeld && SIDE) weight_at(a.gate, g0, at[0], gate1);
+    for (int64_t row = first + sub; row < end; row += S::kRows) {
+      Piece<H, kV> h[N], dy[N];
+      Piece<R, kV> r[N], ds[N];
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        load_at<true>((const H*)a.h + row * a.ldh, at[k], h[k]);
+        load_at<true>((const R*)a.r + row * a.ldr, at[k], r[k]);
+        dy[k] = Piece<H, kV>{};
+        ds[k] = Piece<R, kV>{};
+        if (o.dnormed) load_at<true>((const H*)o.dnormed + row * a.cols, at[k], dy[k]);
+        if (o.dstream) load_at<true>((const R*)o.dstream + row * a.cols, at[k], ds[k]);
+      }
+      const float s1 = rstd[row], s2 = rstd[a.rows + row];
+      float hat[N][kV], sum = 0.f;
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        float x[kV], y[kV], d[kV], w[kV];
+        to_floats(h[k], x);
+        to_floats(r[k], y);
+        to_floats(dy[k], d);
+        if constexpr (SIDE) {
+          float p[kV], g[kV];
+          if constexpr (!kHeld) {
+            weight_at(a.post, 0, at[k], p);
+            weight_at(a.gate, g0, at[k], g);
+          }
+#pragma unroll
+          for (int e = 0; e < kV; ++e) x[e] = (kHeld ? gate1[e] : g[e]) * (x[e] * s1 * (kHeld ? post1[e] : p[e]));
+        }
+        if constexpr (!kHeld) weight_at(a.pre, 0, at[k], w);
+#pragma unroll
+        for (int e = 0; e < kV; ++e) {
+          hat[k][e] = __builtin_fmaf(a.scale, y[e], x[e]) * s2;
+          dpre[k][e] = __builtin_fmaf(d[e], hat[k][e], dpre[k][e]);
+          sum = __builtin_fmaf(d[e] * (kHeld ? pre1[e] : w[e]), e >= at[k].skip ? hat[k][e] : 0.f, sum);
+        }
+      }
+      const float mean = lanes_sum<S::kLanes>(sum, part[0]) * per;
+      sum = 0.f;
+      float (&q)[N][kV] = hat;  // (in place: what h's gradient is formed from)
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        float d[kV], w[kV], e1[kV], dr[kV];
+        to_floats(dy[k], d);
+        to_floats(ds[k], e1);
+        if constexpr (!kHeld) weight_at(a.pre, 0, at[k], w);
+#pragma unroll
+        for (int e = 0; e < kV; ++e) {
+          e1[e] = __builtin_fmaf(s2, __builtin_fmaf(-hat[k][e], mean, d[e] * (kHeld ? pre1[e] : w[e])), e1[e]);
+          dr[e] = a.scale * e1[e];
+        }
+        if (o.dr) store_at((R*)o.dr + row * a.cols, at[k], dr);
+        if constexpr (SIDE) {
+          float x[kV], p[kV], g[kV];
+          to_floats(h[k], x);
+          if constexpr (!kHeld) {
+            weight_at(a.post, 0, at[k], p);
+            weight_at(a.gate, g0, at[k], g);
+          }
+#pragma unroll
+          for (int e = 0; e < kV; ++e) {
+            const float hs = x[e] * s1, qe = e1[e] * (kHeld ? gate1[e] : g[e]), pe = kHeld ? post1[e] : p[e];
+            dgate[k][e] = __builtin_fmaf(e1[e], hs * pe, dgate[k][e]);
+            dpost[k][e] = __builtin_fmaf(qe, hs, dpost[k][e]);
+            q[k][e] = qe * pe;
+            sum = __builtin_fmaf(q[k][e], e >= at[k].skip ? hs : 0.f, sum);
+          }
+        } else {
+          if (o.dh) store_at((H*)o.dh + row * a.cols, at[k], e1);
+        }
+      }
+      if constexpr (SIDE) {
+        const float all = lanes_sum<S::kLanes>(sum, part[1]) * per, mean1 = a.post.p ? all : 0.f;
+        if (o.dh) {
+#pragma unroll
+          for (int k = 0; k < N; ++k) {
+            float x[kV];
+            to_floats(h[k], x);
+#pragma unroll
+            for (int e = 0; e < kV; ++e) x[e] = s1 * __builtin_fmaf(-x[e] * s1, mean1, q[k][e]);
+            store_at((H*)o.dh + row * a.cols, at[k], x);
+          }
+        }
+      } else if constexpr (S::kLanes > 64) {
+        __syncthreads();  // (part[0] again)
+      }
+    }
+    if (SIDE && o.dgate) {
+      rows_joined<S>(dgate, lds);
+      if (sub == 0) {
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+          if (strips.strips > 1) store_at(o.gate_part + strip * a.cols, at[k], dgate[k]);
+          else if (o.dgate_f32) store_at((float*)o.dgate + g0, at[k], dgate[k]);
+          else store_at((uint16_t*)o.dgate + g0, at[k], dgate[k]);
+        }
+      }
+    }
+  }
+  float* out = o.rows_part + (int64_t)blockIdx.x * 3 * a.cols;
+  rows_joined<S>(dpre, lds);
+  if constexpr (SIDE) rows_joined<S>(dpost, lds);
+  if (sub == 0) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      store_at(out + a.cols, at[k], dpre[k]);
+      if constexpr (SIDE) store_at(out, at[k], dpost[k]);
+    }
+  }
+}
+
+// Sums of the workgroups' parts: blockIdx.y 0 post, 1 pre, from 2 on the rows of the gate, those without a place left
+// out.  A workgroup takes 64 columns; 16 lanes of four columns each, 16 such groups that take every 16th part, in order.
+struct NormJoin {
+  const float* rows_part;
+  const float* gate_part;
+  int64_t groups, strips;
+  void* out[3];
+  int f32[3];
+};
+__global__ __launch_bounds__(kNormThreads) void residual_norm_join_kernel(NormJoin j, int64_t cols) {
+  constexpr int kEach = 16;
+  __shared__ float sums[kEach][64];
+  const int which = blockIdx.y < 2 ? (int)blockIdx.y : 2;
+  if (!j.out[which]) return;
+  const int64_t g = which == 2 ? (int64_t)blockIdx.y - 2 : 0;
+  const int lane = threadIdx.x & 15, slice = threadIdx.x >> 4;
+  const int64_t c = (int64_t)blockIdx.x * 64 + lane * 4, left = cols - c;
+  const float* part = which == 2 ? j.gate_part + g * j.strips * cols : j.rows_part + which * cols;
+  const int64_t parts = which == 2 ? j.strips : j.groups, stride = which == 2 ? cols : 3 * cols;
+  float acc[4] = {};
+#pragma unroll 8
+  for (int64_t p = slice; p < parts; p += kEach) {
+    Piece<float, 4> q;
+    load_piece<false>(part + p * stride + c, left, q);
+    float f[4];
+    to_floats(q, f);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[e] += f[e];
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) sums[slice][lane * 4 + e] = acc[e];
+  __syncthreads();
+  const int64_t col = (int64_t)blockIdx.x * 64 + threadIdx.x;
+  if (threadIdx.x < 64 && col < cols) {
+    float s = 0.f;
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) s += sums[k][threadIdx.x];
+    if (j.f32[which]) ((float*)j.out[which])[g * cols + col] = s;
+    else ((uint16_t*)j.out[which])[g * cols + col] = norm_rounded<uint16_t>(s);
+  }
 }
 
 // Workgroups of the backward pass, and their strips.
@@ -199,6 +520,21 @@ static NormStrips norm_strips(int64_t rows, int64_t gate_rows) {
   const int64_t each = (n + strips - 1) / strips;
   strips = (n + each - 1) / each;
   return {each, strips, strips * gate_rows};
+}
+
+// Calls f(shape) with the smallest shape that holds a row, or f(0) for rows that none does.
+template <class F>
+static void norm_shape(int64_t cols, F&& f) {
+  if (cols < kV) f(0);
+  else if (cols <= NormShape<16, 1>::kCols) f(NormShape<16, 1>());
+  else if (cols <= NormShape<32, 1>::kCols) f(NormShape<32, 1>());
+  else if (cols <= NormShape<64, 1>::kCols) f(NormShape<64, 1>());
+  else if (cols <= NormShape<128, 1>::kCols) f(NormShape<128, 1>());
+  else if (cols <= NormShape<256, 1>::kCols) f(NormShape<256, 1>());
+  else if (cols <= NormShape<512, 1>::kCols) f(NormShape<512, 1>());
+  else if (cols <= NormShape<1024, 1>::kCols) f(NormShape<1024, 1>());
+  else if (cols <= NormShape<1024, 2>::kCols) f(NormShape<1024, 2>());
+  else f(0);
 }
 
 template <class F>
@@ -239,8 +575,15 @@ extern "C" int mx_residual_norm(const void* h, int h_f32, const void* r, int r_f
   norm_types(h_f32, r_f32, [&](auto ht, auto rt) {
     using H = decltype(ht);
     using R = decltype(rt);
-    hipLaunchKernelGGL((residual_norm_any_kernel<H, R>), dim3((unsigned)rows), dim3(kNormThreads), 0, (hipStream_t)stream, a,
-                       (R*)stream_out, (H*)normed, rstd);
+    norm_shape(cols, [&](auto shape) {
+      using S = decltype(shape);
+      if constexpr (std::is_same_v<S, int>)
+        hipLaunchKernelGGL((residual_norm_any_kernel<H, R>), dim3((unsigned)rows), dim3(kNormThreads), 0, (hipStream_t)stream,
+                           a, (R*)stream_out, (H*)normed, rstd);
+      else
+        hipLaunchKernelGGL((residual_norm_kernel<S, H, R>), dim3((unsigned)((rows + S::kRows - 1) / S::kRows)),
+                           dim3(S::kThreads), 0, (hipStream_t)stream, a, (R*)stream_out, (H*)normed, rstd);
+    });
   });
   return hipGetLastError() == hipSuccess ? MX_OK : MX_ERR_LAUNCH;
 }
@@ -275,20 +618,25 @@ extern "C" int mx_residual_norm_bwd(const void* h, int h_f32, const void* r, int
   const NormGrads o{dstream, dnormed, dh, dr, rows_part, gate_part, dgate, weights_f32 & 2};
   hipStream_t st = (hipStream_t)stream;
   norm_types(h_f32, r_f32, [&](auto ht, auto rt) {
-    hipLaunchKernelGGL((residual_norm_bwd_any_kernel<decltype(ht), decltype(rt)>), dim3((unsigned)groups), dim3(kNormThreads),
-                       0, st, a, s, rstd, o);
+    using H = decltype(ht);
+    using R = decltype(rt);
+    norm_shape(cols, [&](auto shape) {
+      using S = decltype(shape);
+      if constexpr (std::is_same_v<S, int>)
+        hipLaunchKernelGGL((residual_norm_bwd_any_kernel<H, R>), dim3((unsigned)groups), dim3(kNormThreads), 0, st, a, s, rstd, o);
+      else if (post || gate)
+        hipLaunchKernelGGL((residual_norm_bwd_kernel<S, true, H, R>), dim3((unsigned)groups), dim3(S::kThreads), 0, st, a, s,
+                           rstd, o);
+      else
+        hipLaunchKernelGGL((residual_norm_bwd_kernel<S, false, H, R>), dim3((unsigned)groups), dim3(S::kThreads), 0, st, a, s,
+                           rstd, o);
+    });
   });
-  const unsigned blocks = (unsigned)((cols + kNormThreads - 1) / kNormThreads);
-  auto join = [&](void* out, const float* part, int64_t parts, int64_t stride, int64_t many, int f32) {
-    for (int64_t g = 0; out && g < many; g += 65535) {  // (a grid has at most as many rows)
-      const int64_t now = many - g < 65535 ? many - g : 65535;
-      hipLaunchKernelGGL(residual_norm_join_kernel, dim3(blocks, (unsigned)now), dim3(kNormThreads), 0, st,
-                         part + g * parts * stride, parts, stride, cols,
-                         f32 ? (void*)((float*)out + g * cols) : (void*)((uint16_t*)out + g * cols), f32);
-    }
-  };
-  join(dpost, rows_part, groups, 3 * cols, 1, weights_f32 & 1);
-  join(dpre, rows_part + cols, groups, 3 * cols, 1, weights_f32 & 4);
-  if (s.strips > 1) join(dgate, gate_part, s.strips, cols, gate_rows, weights_f32 & 2);
+  const int64_t gates = dgate && s.strips > 1 ? gate_rows : 0;  // (fewer than kNormGroups of them)
+  if (dpost || dpre || gates) {
+    const NormJoin j{rows_part, gate_part, groups, s.strips, {dpost, dpre, dgate}, {weights_f32 & 1, weights_f32 & 4, weights_f32 & 2}};
+    hipLaunchKernelGGL(residual_norm_join_kernel, dim3((unsigned)((cols + 63) / 64), (unsigned)(2 + gates)), dim3(kNormThreads),
+                       0, st, j, cols);
+  }
   return hipGetLastError() == hipSuccess ? MX_OK : MX_ERR_LAUNCH;
 }
