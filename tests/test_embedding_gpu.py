@@ -209,3 +209,30 @@ def test_refusals(device):
     (grad,) = torch.autograd.grad(out.sum(), weight, create_graph=True)
     with pytest.raises(RuntimeError):
         grad.sum().backward()
+
+
+@pytest.mark.parametrize("tokens", [100, 8191, 8200, 33000, 90000])
+@pytest.mark.parametrize("cols", [5, 136, 2056])
+def test_runs_of_every_length(device, tokens, cols):
+    """Ids repeated 1 to 700 times, in any order: runs that begin and end anywhere in the pieces that are summed by one
+    workgroup, several long ones next to each other."""
+    if tokens * cols > 2 ** 26:
+        tokens = 2 ** 26 // cols
+    g = torch.Generator(device=device).manual_seed(tokens)
+    lengths = torch.randint(1, 20, (tokens,), generator=g, device=device)
+    lengths[::7] = 64
+    lengths[1::29] = torch.randint(100, 700, lengths[1::29].shape, generator=g, device=device)
+    ids = torch.arange(tokens, device=device).repeat_interleave(lengths)[:tokens] * 3
+    rows = int(ids.max()) + 5
+    ids = ids[torch.randperm(tokens, generator=g, device=device)]
+    weight = torch.randn((rows, cols), generator=g, device=device)
+    dout = torch.randn((tokens, cols), generator=g, device=device).to(torch.bfloat16)
+    check(ids, weight, 1.0, None, 0, torch.bfloat16, dout)
+    check(ids, weight[: rows // 2], 1.0, int(ids[0]), 0, torch.bfloat16, dout)  # half of the tokens have no row
+
+
+@pytest.mark.parametrize("rows", [511, 512, 300000, 2 ** 18 - 1, 2 ** 18])
+def test_tables_around_a_digit_of_the_sort(device, rows):
+    ids, weight, dout = make(device, 10007, rows, 8, torch.bfloat16, torch.bfloat16, rows)
+    ids[:3] = torch.tensor([0, rows - 1, rows], device=device)
+    check(ids, weight, 1.0, None, 0, torch.bfloat16, dout)

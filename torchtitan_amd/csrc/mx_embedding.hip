@@ -32,7 +32,7 @@ struct EmbIds {
 // One wave a token: the row's pieces are asked for four at a time.
 template <class W, class O>
 __global__ __launch_bounds__(kEmbThreads) void embedding_kernel(EmbIds ids, int64_t n, const W* __restrict__ weight,
-                                                                int64_t cols, int64_t ldw, float scale,
+                                                                int64_t cols, int64_t ldw, float scale, bool past,
                                                                 O* __restrict__ out) {
   constexpr int V = 8, U = 4;
   const int64_t t = (int64_t)blockIdx.x * kEmbWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -57,78 +57,418 @@ __global__ __launch_bounds__(kEmbThreads) void embedding_kernel(EmbIds ids, int6
 #pragma unroll
         for (int e = 0; e < V; ++e) f[e] *= scale;
       }
-      store_piece<false>(dst + c, cols - c, from_floats<O>(f));
+      const Piece<O, V> q = from_floats<O>(f);
+      if (past) store_piece<true>(dst + c, cols - c, q);
+      else store_piece<false>(dst + c, cols - c, q);
     }
   }
 }
 
-// Stable order of the tokens by their rows: a token's place is the number of tokens with a smaller row, or with its
-// row and in front of it.  A workgroup places 64 tokens; every wave counts over a sixteenth of the tokens.
-constexpr int kRankThreads = 1024, kRankTile = 8192;
+// ---- the order of the tokens by their rows, stable: up to kRankMost tokens in one launch, more by radix passes
 
-__global__ __launch_bounds__(kRankThreads) void embedding_rank_kernel(EmbIds ids, int64_t n, uint32_t* __restrict__ keys,
-                                                                      uint32_t* __restrict__ places) {
-  __shared__ uint32_t tile[kRankTile];
-  __shared__ uint32_t counts[kRankThreads / 64][64];
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int64_t t = (int64_t)blockIdx.x * 64 + lane;
-  const uint32_t mine = t < n ? ids.key(t) : 0xFFFFFFFFu;
+// A token's place is the number of tokens with a smaller row, or with its row and in front of it.  A workgroup places 64
+// tokens, one a lane; every wave counts over a sixteenth of all tokens, whose rows it reads from LDS four at a time.
+// Two instructions a pair: 2003 tokens XX us, 8192 XX us, where the radix passes take XX and XX.
+constexpr int kRankThreads = 1024, kRankMost = 8192;
+
+__global__ __launch_bounds__(kRankThreads) void embedding_rank_kernel(EmbIds ids, int n, uint32_t* __restrict__ keys,
+                                                                      uint32_t* __restrict__ places,
+                                                                      uint32_t* __restrict__ chains) {
+  constexpr int kWaves = kRankThreads / 64;
+  __shared__ alignas(16) uint32_t tile[kRankMost];
+  __shared__ uint32_t counts[kWaves][64];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int t0 = (int)blockIdx.x * 64, t = t0 + lane;
+  if (blockIdx.x == 0 && threadIdx.x == 0) *chains = 0;
+  const int padded = (n + 4 * kWaves - 1) / (4 * kWaves) * (4 * kWaves);  // (at most kRankMost)
+  for (int i = threadIdx.x; i < padded; i += kRankThreads) tile[i] = i < n ? ids.key(i) : 0xFFFFFFFFu;  // in front of nobody
+  __syncthreads();
+  const uint32_t mine = t < n ? tile[t] : 0u;
+  const int each = padded / kWaves, lo = wave * each, hi = lo + each;
   uint32_t before = 0;
-  for (int64_t base = 0; base < n; base += kRankTile) {
-    const int m = (int)(n - base < kRankTile ? n - base : kRankTile);
-    __syncthreads();
-    for (int i = threadIdx.x; i < m; i += kRankThreads) tile[i] = ids.key(base + i);
-    __syncthreads();
-    const int each = (m + 15) / 16, lo = wave * each, hi = lo + each < m ? lo + each : m;
-    for (int i = lo; i < hi; ++i) {
-      const uint32_t k = tile[i];
-      before += k < mine || (k == mine && base + i < t);
+  auto count = [&](int from, int to, auto&& limit) {
+    for (int i = from; i < to; i += 4) {
+      const u32x4 k = *reinterpret_cast<const u32x4*>(tile + i);
+      before += k.x < limit(i);
+      before += k.y < limit(i + 1);
+      before += k.z < limit(i + 2);
+      before += k.w < limit(i + 3);
     }
-  }
+  };
+  // (a row equal to mine counts where its token is in front: known for all of a wave's tokens but its own 64)
+  if (hi <= t0) count(lo, hi, [&](int) { return mine + 1; });
+  else if (lo >= t0 + 64) count(lo, hi, [&](int) { return mine; });
+  else count(lo, hi, [&](int i) { return mine + (i < t ? 1u : 0u); });
   counts[wave][lane] = before;
   __syncthreads();
   if (wave == 0 && t < n) {
     uint32_t at = 0;
-    for (int w = 0; w < kRankThreads / 64; ++w) at += counts[w][lane];
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) at += counts[w][lane];
     keys[at] = mine;
     places[at] = (uint32_t)t;
   }
 }
 
-__device__ __forceinline__ int64_t emb_lower_bound(const uint32_t* __restrict__ keys, int64_t n, uint32_t key) {
-  int64_t lo = 0, hi = n;
-  while (lo < hi) {
-    const int64_t mid = (lo + hi) >> 1;
-    if (keys[mid] < key) lo = mid + 1; else hi = mid;
+// A radix pass over digits of at most kDigitBits bits in three launches: every tile's counts of digits; for every digit
+// their sums over the tiles in front; every tile's tokens to their places.  No atomics beyond a workgroup's counts, so
+// the order is the same on every run.
+constexpr int kSortThreads = 256, kSortEach = 4, kSortTile = kSortThreads * kSortEach;
+constexpr int kDigitBits = 9, kDigits = 1 << kDigitBits;
+constexpr int kSortWaves = kSortThreads / 64;
+
+// Where a pass reads its rows and tokens: from the ids, or from what the pass before wrote.
+struct EmbSource {
+  EmbIds ids;
+  const uint32_t* keys;
+  const uint32_t* places;
+  __device__ __forceinline__ uint32_t key(int64_t i) const { return keys ? keys[i] : ids.key(i); }
+  __device__ __forceinline__ uint32_t place(int64_t i) const { return keys ? places[i] : (uint32_t)i; }
+};
+
+__global__ __launch_bounds__(kSortThreads) void embedding_count_kernel(EmbSource from, int64_t n, int shift, uint32_t* __restrict__ counts,
+                                                                       uint32_t* __restrict__ chains) {
+  __shared__ uint32_t digits[kDigits];
+  if (blockIdx.x == 0 && threadIdx.x == 0) *chains = 0;
+  for (int d = threadIdx.x; d < kDigits; d += kSortThreads) digits[d] = 0;
+  __syncthreads();
+  const int64_t base = (int64_t)blockIdx.x * kSortTile;
+#pragma unroll
+  for (int k = 0; k < kSortEach; ++k) {
+    const int64_t i = base + k * kSortThreads + threadIdx.x;
+    if (i < n) atomicAdd(&digits[from.key(i) >> shift & (kDigits - 1)], 1u);
+  }
+  __syncthreads();
+  for (int d = threadIdx.x; d < kDigits; d += kSortThreads) counts[(int64_t)d * gridDim.x + blockIdx.x] = digits[d];
+}
+
+__device__ __forceinline__ uint32_t wave_running_sum(uint32_t v) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const uint32_t u = __shfl_up(v, off, 64);
+    if (lane >= off) v += u;
+  }
+  return v;
+}
+
+// One wave a digit.
+__global__ __launch_bounds__(64) void embedding_offsets_kernel(uint32_t* __restrict__ counts, int64_t tiles,
+                                                               uint32_t* __restrict__ totals) {
+  uint32_t* mine = counts + (int64_t)blockIdx.x * tiles;
+  uint32_t sum = 0;
+  for (int64_t base = 0; base < tiles; base += 64) {
+    const int64_t i = base + threadIdx.x;
+    const uint32_t v = i < tiles ? mine[i] : 0u, upto = wave_running_sum(v);
+    if (i < tiles) mine[i] = sum + upto - v;
+    sum += __shfl(upto, 63, 64);
+  }
+  if (threadIdx.x == 0) totals[blockIdx.x] = sum;
+}
+
+__global__ __launch_bounds__(kSortThreads) void embedding_scatter_kernel(EmbSource from, int64_t n, int shift,
+                                                                         const uint32_t* __restrict__ offsets,
+                                                                         const uint32_t* __restrict__ totals,
+                                                                         uint32_t* __restrict__ keys,
+                                                                         uint32_t* __restrict__ places) {
+  __shared__ uint32_t counts[kSortWaves][kDigits];  // of a digit in a wave's tokens so far; then where the wave's begin
+  __shared__ uint32_t sums[kSortWaves];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  for (int d = threadIdx.x; d < kSortWaves * kDigits; d += kSortThreads) (&counts[0][0])[d] = 0;
+  __syncthreads();
+  uint32_t key[kSortEach], place[kSortEach], rank[kSortEach];
+  const int64_t base = (int64_t)blockIdx.x * kSortTile + wave * 64 * kSortEach;  // (a wave's tokens lie side by side)
+#pragma unroll
+  for (int k = 0; k < kSortEach; ++k) {
+    const int64_t i = base + k * 64 + lane;
+    const bool in = i < n;
+    key[k] = in ? from.key(i) : 0u;
+    place[k] = in ? from.place(i) : 0u;
+  }
+#pragma unroll
+  for (int k = 0; k < kSortEach; ++k) {
+    const bool in = base + k * 64 + lane < n;
+    const uint32_t d = key[k] >> shift & (kDigits - 1);
+    uint64_t same = __ballot(in);  // the wave's lanes with this lane's digit
+#pragma unroll
+    for (int b = 0; b < kDigitBits; ++b) {
+      const uint64_t ones = __ballot(d >> b & 1);
+      same &= d >> b & 1 ? ones : ~ones;
+    }
+    const uint64_t front = same & ((1ull << lane) - 1);
+    rank[k] = counts[wave][d] + (uint32_t)__popcll(front);
+    __syncthreads();
+    if (in && front == 0) counts[wave][d] += (uint32_t)__popcll(same);
+    __syncthreads();
+  }
+  // where every digit's tokens of this tile begin: behind all smaller digits, and this digit's of the tiles in front
+  constexpr int kEach = kDigits / kSortThreads;
+  uint32_t total[kEach], sum = 0;
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    total[e] = totals[threadIdx.x * kEach + e];
+    sum += total[e];
+  }
+  const uint32_t upto = wave_running_sum(sum);
+  if (lane == 63) sums[wave] = upto;
+  __syncthreads();
+  uint32_t at = upto - sum;
+  for (int w = 0; w < wave; ++w) at += sums[w];
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    const int d = threadIdx.x * kEach + e;
+    uint32_t here = at + offsets[(int64_t)d * gridDim.x + blockIdx.x];
+#pragma unroll
+    for (int w = 0; w < kSortWaves; ++w) {
+      const uint32_t c = counts[w][d];
+      counts[w][d] = here;
+      here += c;
+    }
+    at += total[e];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < kSortEach; ++k) {
+    if (base + k * 64 + lane >= n) break;
+    const uint32_t to = counts[wave][key[k] >> shift & (kDigits - 1)] + rank[k];
+    keys[to] = key[k];
+    places[to] = place[k];
+  }
+}
+
+// ---- sums of equal rows.  A run of equal rows in the sorted tokens is cut into pieces of `chunk` tokens from its first
+// token on, so that a row's sum depends on its own tokens alone, wherever its run lies.  A run of one piece is summed in
+// order; the others are chains: their pieces but the first leave float32 sums in `parts`, and another launch joins them.
+// The sorted tokens are cut into chunks of as many tokens; a workgroup sums the pieces that begin in its chunk (one at
+// most of a run that began before, whose slot of `parts` is the chunk's).
+struct EmbSums {
+  const uint32_t* keys;
+  const uint32_t* places;
+  int64_t n, rows, cols, ldd;
+  int chunk;        // tokens
+  float scale;
+  bool past;        // the gradient does not stay in the last cache: stored past it
+  float* parts;     // [chunks][cols]
+  uint32_t* chains; // how many; then the places that they begin at
+};
+
+constexpr int kChunkMost = 64;
+constexpr int kZeroRows = 64;  // rows of the table whose zeros one workgroup writes
+
+// First place whose row is not below `key` (between lo and hi), by the whole wave: 64 probes a step.
+__device__ __forceinline__ int64_t wave_lower_bound(const uint32_t* __restrict__ keys, int64_t lo, int64_t hi, uint32_t key) {
+  const int lane = threadIdx.x & 63;
+  while (lo < hi) {  // the answer is in [lo, hi]
+    const int64_t step = (hi - lo + 63) / 64, at = lo + lane * step;
+    const uint64_t below = __ballot(at < hi && keys[at < hi ? at : lo] < key);  // a prefix of the lanes
+    const int many = __popcll(below);
+    if (many == 0) return lo;
+    const int64_t last = lo + (many - 1) * step;  // below the key
+    hi = last + step < hi ? last + step : hi;
+    lo = last + 1;
   }
   return lo;
 }
 
-// One wave a row of the table: its tokens' gradients, found by a search in the sorted rows, summed in order.
+template <class G>
+__device__ __forceinline__ void store_row(G* to, int64_t left, const float* acc, float scale, bool past) {
+  float f[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) f[e] = acc[e] * scale;
+  const Piece<G, 8> q = from_floats<G>(f);
+  if (past) store_piece<true>(to, left, q);
+  else store_piece<false>(to, left, q);
+}
+
+// Workgroups [0, chunks): sums; behind them: zeros of the rows that no token has.  A lane holds 8 columns, blockIdx.y
+// says which of several slabs of blockDim.x * 8 columns; 8 tokens' pieces are asked for before the first is added.
 template <class D, class G>
-__global__ __launch_bounds__(kEmbThreads) void embedding_grad_kernel(const D* __restrict__ dout, int64_t n, int64_t ldd,
-                                                                     const uint32_t* __restrict__ keys,
-                                                                     const uint32_t* __restrict__ places, int64_t rows,
-                                                                     int64_t cols, float scale, G* __restrict__ grad) {
-  constexpr int V = 8;
-  const int64_t v = (int64_t)blockIdx.x * kEmbWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (v >= rows) return;
-  const int64_t lo = emb_lower_bound(keys, n, (uint32_t)v), hi = emb_lower_bound(keys, n, (uint32_t)v + 1);
-  for (int64_t c = (int64_t)(threadIdx.x & 63) * V; c < cols; c += 64 * V) {
+__global__ __launch_bounds__(256) void embedding_sums_kernel(EmbSums a, const D* __restrict__ dout, G* __restrict__ grad,
+                                                             int64_t chunks) {
+  constexpr int V = 8, U = 8;
+  __shared__ uint32_t keys[3 * kChunkMost + 2], places[2 * kChunkMost];
+  const int64_t c = ((int64_t)blockIdx.y * blockDim.x + threadIdx.x) * V, left = a.cols - c;
+  if (blockIdx.x >= chunks) {
+    const int64_t first = (int64_t)(blockIdx.x - chunks) * kZeroRows;
+    const int rows = (int)(a.rows - first < kZeroRows ? a.rows - first : kZeroRows), lane = threadIdx.x & 63;
+    // (every wave for itself: the first of its tokens, and for every row whether it has one)
+    const int64_t lo = wave_lower_bound(a.keys, 0, a.n, (uint32_t)first);
+    const int64_t hi = wave_lower_bound(a.keys, lo, a.n, (uint32_t)(first + rows));
+    int64_t from = lo, to = hi;
+    while (from < to) {
+      const int64_t mid = (from + to) >> 1;
+      if (a.keys[mid] < (uint32_t)(first + lane)) from = mid + 1; else to = mid;
+    }
+    const bool used = from < hi && a.keys[from] == (uint32_t)(first + lane);
+    uint64_t unused = ~__ballot(used);
+    if (rows < 64) unused &= (1ull << rows) - 1;
+    const float zeros[V] = {};
+    while (unused) {
+      const int r = __builtin_ctzll(unused);
+      unused &= unused - 1;
+      store_row(grad + (first + r) * a.cols + c, left, zeros, 0.f, a.past);
+    }
+    return;
+  }
+  // The rows of the chunk's tokens, of `chunk` and one tokens in front of them and of `chunk` behind.
+  const int C = a.chunk, lane = threadIdx.x & 63;
+  const int64_t c0 = (int64_t)blockIdx.x * C;
+  const int own = (int)(a.n - c0 < C ? a.n - c0 : C);
+  const uint32_t none = (uint32_t)a.rows;  // tokens without a row lie behind all others
+  for (int i = threadIdx.x; i < 3 * C + 2; i += blockDim.x) {
+    const int64_t at = c0 - C - 1 + i;
+    keys[i] = at >= 0 && at < a.n ? a.keys[at] : 0xFFFFFFFFu;
+    if (i > C && i <= 3 * C) places[i - C - 1] = at < a.n ? a.places[at] : 0u;
+  }
+  __syncthreads();
+  auto key = [&](int i) { return keys[i + C + 1]; };  // -C - 1 <= i <= 2 C
+  // Every wave for itself, a lane a token: the first tokens of runs, and the first place of the piece [lead, ...) of
+  // the run that began in front of the chunk, if one begins here.
+  const uint64_t starts = __ballot(lane < own && key(lane < C ? lane : 0) != key(lane < C ? lane - 1 : 0));
+  const uint32_t k0 = key(0);
+  int lead = -1;
+  if (!(starts & 1)) {
+    if (k0 == none) return;
+    int at;
+    if (key(-C) != k0) {  // it began less than a piece ago
+      at = C - __builtin_ctzll(~__ballot(lane < C && key(lane < C ? -1 - lane : 0) == k0));
+    } else {
+      const int64_t begin = wave_lower_bound(a.keys, 0, c0 - C, k0);
+      at = (int)((C - (c0 - begin) % C) % C);
+    }
+    if (at < own && key(at) == k0) lead = at;
+  }
+  if (lead < 0 && !starts) return;
+  const int lo = lead >= 0 ? lead : __builtin_ctzll(starts);
+  // the last piece that begins here, and its end
+  const int tail = starts ? 63 - __builtin_clzll(starts) : lead;
+  const uint32_t kt = key(tail);
+  const bool whole = key(tail + C) == kt;  // and the run goes on
+  int hi = tail;
+  if (starts && kt != none && whole) {
+    if (threadIdx.x == 0 && blockIdx.y == 0) a.chains[1 + atomicAdd(a.chains, 1u)] = (uint32_t)(c0 + tail);
+  } else if (kt != none) {
+    hi = whole ? tail + C : tail + 1 + __builtin_ctzll(__ballot(lane < C && key(tail + 1 + (lane < C ? lane : 0)) != kt));
+  }
+  float acc[V] = {};
+  for (int i0 = lo; i0 < hi; i0 += U) {
+    Piece<D, V> p[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u < hi ? i0 + u : hi - 1;
+      load_piece<true>(dout + (int64_t)places[i] * a.ldd + c, left, p[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u;
+      if (i >= hi) break;
+      const uint32_t k = key(i);
+      float f[V];
+      to_floats(p[u], f);
+#pragma unroll
+      for (int e = 0; e < V; ++e) acc[e] += f[e];
+      if (i + 1 == hi || key(i + 1) != k) {
+        if (lead >= 0 && k == k0) store_row(a.parts + (int64_t)blockIdx.x * a.cols + c, left, acc, 1.f, false);
+        else store_row(grad + (int64_t)k * a.cols + c, left, acc, a.scale, a.past);
+#pragma unroll
+        for (int e = 0; e < V; ++e) acc[e] = 0.f;
+      }
+    }
+  }
+}
+
+// The chains: the tokens of their first piece and the sums of the others, dealt out in turn to 16 groups of 16 lanes of
+// 8 columns each, whose sums are added in order.
+template <class D, class G>
+__global__ __launch_bounds__(256) void embedding_chains_kernel(EmbSums a, const D* __restrict__ dout, G* __restrict__ grad) {
+  constexpr int V = 8, kGroups = 16, kCols = 16 * V;
+  __shared__ float sums[kGroups][kCols];
+  const int64_t slabs = (a.cols + kCols - 1) / kCols, items = (int64_t)a.chains[0] * slabs;
+  const int group = threadIdx.x >> 4, lane = threadIdx.x & 15;
+  for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+    const int64_t begin = a.chains[1 + item / slabs], slab = item % slabs;
+    const uint32_t k = a.keys[begin];
+    const int64_t end = wave_lower_bound(a.keys, begin + a.chunk, a.n, k + 1);
+    const int64_t all = a.chunk + (end - begin - 1) / a.chunk;  // tokens of the first piece, then pieces
+    const int64_t c = slab * kCols + lane * V, left = a.cols - c;
+    const float* parts = a.parts + (begin / a.chunk + 1) * a.cols + c;
     float acc[V] = {};
-    for (int64_t i = lo; i < hi; ++i) {
+    for (int64_t i = group; i < a.chunk; i += kGroups) {
       Piece<D, V> p;
-      load_piece<false>(dout + (int64_t)places[i] * ldd + c, cols - c, p);
+      load_piece<false>(dout + (int64_t)a.places[begin + i] * a.ldd + c, left, p);
+      float f[V];
+      to_floats(p, f);
+#pragma unroll
+      for (int e = 0; e < V; ++e) acc[e] += f[e];
+    }
+#pragma unroll 4
+    for (int64_t i = group; i < all - a.chunk; i += kGroups) {
+      Piece<float, V> p;
+      load_piece<false>(parts + i * a.cols, left, p);
       float f[V];
       to_floats(p, f);
 #pragma unroll
       for (int e = 0; e < V; ++e) acc[e] += f[e];
     }
 #pragma unroll
-    for (int e = 0; e < V; ++e) acc[e] *= scale;
-    store_piece<false>(grad + v * cols + c, cols - c, from_floats<G>(acc));
+    for (int e = 0; e < V; ++e) sums[group][lane * V + e] = acc[e];
+    __syncthreads();
+    if (group == 0) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        acc[e] = 0.f;
+        for (int g = 0; g < kGroups; ++g) acc[e] += sums[g][lane * V + e];
+      }
+      store_row(grad + (int64_t)k * a.cols + c, left, acc, a.scale, false);
+    }
+    __syncthreads();
   }
 }
+
+// Tokens of a chunk: 64, fewer where there would not be a thousand chunks.
+static int emb_chunk(int64_t n) {
+  int c = 16;
+  while (c < kChunkMost && c * 1024 < n) c *= 2;
+  return c;
+}
+
+// The workspace, in 256-byte pieces.
+struct EmbPlan {
+  int64_t tiles, chunks, parts;
+  int passes, chunk;
+  int64_t keys[2], places[2], counts, totals, chains, sums, bytes;
+};
+static EmbPlan emb_plan(int64_t n, int64_t rows, int64_t cols) {
+  EmbPlan p{};
+  if (n <= 0 || rows <= 0 || cols <= 0) return p;
+  p.chunk = emb_chunk(n);
+  p.chunks = (n + p.chunk - 1) / p.chunk;
+  if (n > kRankMost) {
+    int bits = 1;
+    while (rows >> bits) ++bits;
+    p.passes = (bits + kDigitBits - 1) / kDigitBits;
+    p.tiles = (n + kSortTile - 1) / kSortTile;
+  }
+  auto take = [&](int64_t bytes) {
+    const int64_t at = p.bytes;
+    p.bytes += (bytes + 255) & ~int64_t{255};
+    return at;
+  };
+  for (int k = 0; k < (p.passes > 1 ? 2 : 1); ++k) {
+    p.keys[k] = take(4 * n);
+    p.places[k] = take(4 * n);
+  }
+  if (p.passes) {
+    p.counts = take(4 * kDigits * p.tiles);
+    p.totals = take(4 * kDigits);
+  }
+  p.chains = take(4 * (1 + p.chunks));
+  p.sums = take(4 * p.chunks * cols);
+  return p;
+}
+
+// Results that do not stay in the last cache (256 MB) until someone reads them are stored past it.
+static bool emb_past(int64_t bytes) { return bytes > (int64_t{384} << 20); }
 
 // Calls f(T()) with T the element type that the flag names.
 template <class F>
@@ -153,15 +493,15 @@ extern "C" int mx_embedding(const void* ids, int ids_i64, int64_t n, const void*
   of_type(weight_f32, [&](auto w) {
     of_type(out_f32, [&](auto o) {
       hipLaunchKernelGGL((embedding_kernel<decltype(w), decltype(o)>), dim3((unsigned)groups), dim3(kEmbThreads), 0,
-                         (hipStream_t)stream, e, n, (const decltype(w)*)weight, cols, ldw, scale, (decltype(o)*)out);
+                         (hipStream_t)stream, e, n, (const decltype(w)*)weight, cols, ldw, scale,
+                         emb_past(n * cols * (out_f32 ? 4 : 2)), (decltype(o)*)out);
     });
   });
   return hipGetLastError() == hipSuccess ? MX_OK : MX_ERR_LAUNCH;
 }
 
 extern "C" int64_t mx_embedding_grad_workspace(int64_t n, int64_t rows, int64_t cols) {
-  if (n <= 0 || rows <= 0 || cols <= 0) return 0;
-  return 8 * n;
+  return emb_plan(n, rows, cols).bytes;
 }
 
 extern "C" int mx_embedding_grad(const void* ids, int ids_i64, int64_t n, const void* dout, int dout_f32, int64_t ldd,
@@ -175,17 +515,45 @@ extern "C" int mx_embedding_grad(const void* ids, int ids_i64, int64_t n, const 
       ((uintptr_t)workspace & 15))
     return MX_ERR_ALIGNMENT;
   if (rows >= 0x7FFFFFFF || n >= 0x7FFFFFFF) return MX_ERR_UNSUPPORTED;
+  const EmbPlan p = emb_plan(n, rows, cols);
+  const int threads = cols > 1024 ? 256 : cols > 512 ? 128 : 64;
+  const int64_t slabs = (cols + threads * 8 - 1) / (threads * 8), groups = p.chunks + (rows + kZeroRows - 1) / kZeroRows;
+  if (slabs > 65535 || groups > 0x7FFFFFFF) return MX_ERR_UNSUPPORTED;
   hipStream_t st = (hipStream_t)stream;
-  uint32_t* keys = (uint32_t*)workspace;
-  uint32_t* places = keys + n;
+  uint8_t* ws = (uint8_t*)workspace;
+  auto words = [&](int64_t at) { return (uint32_t*)(ws + at); };
+  uint32_t* chains = words(p.chains);
   const EmbIds e{ids, ids_i64 != 0, first, rows, padding};
-  if (n > 0)
-    hipLaunchKernelGGL(embedding_rank_kernel, dim3((unsigned)((n + 63) / 64)), dim3(kRankThreads), 0, st, e, n, keys, places);
-  of_type(dout_f32, [&](auto d) {
-    of_type(grad_f32, [&](auto g) {
-      hipLaunchKernelGGL((embedding_grad_kernel<decltype(d), decltype(g)>), dim3((unsigned)((rows + kEmbWaves - 1) / kEmbWaves)),
-                         dim3(kEmbThreads), 0, st, (const decltype(d)*)dout, n, ldd, keys, places, rows, cols, scale,
-                         (decltype(g)*)grad);
+  int last = 0;  // which of the two lists holds the order
+  if (n > 0 && p.passes == 0) {
+    hipLaunchKernelGGL(embedding_rank_kernel, dim3((unsigned)((n + 63) / 64)), dim3(kRankThreads), 0, st, e, (int)n,
+                       words(p.keys[0]), words(p.places[0]), chains);
+  }
+  for (int pass = 0; pass < p.passes; ++pass) {
+    EmbSource from{e, nullptr, nullptr};
+    if (pass > 0) {
+      from.keys = words(p.keys[last]);
+      from.places = words(p.places[last]);
+      last ^= 1;
+    }
+    const int shift = pass * kDigitBits;
+    hipLaunchKernelGGL(embedding_count_kernel, dim3((unsigned)p.tiles), dim3(kSortThreads), 0, st, from, n, shift,
+                       words(p.counts), chains);
+    hipLaunchKernelGGL(embedding_offsets_kernel, dim3(kDigits), dim3(64), 0, st, words(p.counts), p.tiles, words(p.totals));
+    hipLaunchKernelGGL(embedding_scatter_kernel, dim3((unsigned)p.tiles), dim3(kSortThreads), 0, st, from, n, shift,
+                       words(p.counts), words(p.totals), words(p.keys[last]), words(p.places[last]));
+  }
+  const EmbSums a{words(p.keys[last]), words(p.places[last]), n, rows, cols, ldd, p.chunk, scale,
+                  emb_past(rows * cols * (grad_f32 ? 4 : 2)),
+                  (float*)(ws + p.sums), chains};
+  of_type(dout_f32, [&](auto dt) {
+    of_type(grad_f32, [&](auto gt) {
+      using D = decltype(dt);
+      using G = decltype(gt);
+      hipLaunchKernelGGL((embedding_sums_kernel<D, G>), dim3((unsigned)groups, (unsigned)slabs), dim3(threads), 0, st, a,
+                         (const D*)dout, (G*)grad, p.chunks);
+      if (n > p.chunk)  // (a chain is more than one piece)
+        hipLaunchKernelGGL((embedding_chains_kernel<D, G>), dim3(512), dim3(256), 0, st, a, (const D*)dout, (G*)grad);
     });
   });
   return hipGetLastError() == hipSuccess ? MX_OK : MX_ERR_LAUNCH;

@@ -13,6 +13,8 @@
 //
 // Sums over rows are float32 parts of one workgroup's rows each, joined in order by a second launch: the same result
 // on every run.  Row r of T uses row r / (T / G) of a gate of G rows.
+#include <algorithm>
+
 #include "mx_rows.h"
 
 namespace mx {
@@ -50,6 +52,7 @@ struct NormArgs {
   NormWeight post, gate, pre;
   int64_t gate_each;  // rows that share a row of the gate
   float scale, eps;
+  bool past;          // the matrices written are stored past the caches (see norm_past)
 };
 
 template <class T>
@@ -93,8 +96,11 @@ __device__ __forceinline__ void load_at(const T* row, const NormPlace& p, Piece<
   if (p.in) load_words<NT>(row + p.at, q);
 }
 template <class T>
-__device__ __forceinline__ void store_at(T* row, const NormPlace& p, const float (&f)[kV]) {
-  if (p.in) store_words<false>(row + p.at, from_floats<T>(f));
+__device__ __forceinline__ void store_at(T* row, const NormPlace& p, const float (&f)[kV], bool past = false) {
+  if (!p.in) return;
+  const Piece<T, kV> q = from_floats<T>(f);
+  if (past) store_words<true>(row + p.at, q);
+  else store_words<false>(row + p.at, q);
 }
 __device__ __forceinline__ void weight_at(const NormWeight& w, int64_t row, const NormPlace& p, float (&f)[kV]) {
   if (!w.p) {
@@ -111,12 +117,28 @@ __device__ __forceinline__ void weight_at(const NormWeight& w, int64_t row, cons
   }
 }
 
-// Sum over the lanes of a row, in each of them.  Rows of more than a wave: `part` holds a float a wave, and a second
-// one has to be used in between before it is used again (one barrier a sum).
+// gate * post: what a row's normalised block output is multiplied with.
+__device__ __forceinline__ void side_at(const NormArgs& a, int64_t g0, const NormPlace& p, float (&f)[kV]) {
+  float q[kV];
+  weight_at(a.post, 0, p, q);
+  weight_at(a.gate, g0, p, f);
+#pragma unroll
+  for (int e = 0; e < kV; ++e) f[e] *= q[e];
+}
+
+// Sum over the lanes of a row, in each of them.  Rows of more than a wave go through `part`, a float a wave, with one
+// barrier: whoever comes by here again before another barrier brings another `part`.
 template <int LANES>
 __device__ __forceinline__ float lanes_sum(float v, float* part) {
-#pragma unroll
-  for (int off = (LANES < 64 ? LANES : 64) / 2; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
+  v += __uint_as_float(dpp<kQuadXor1>(__float_as_uint(v)));
+  v += __uint_as_float(dpp<kQuadXor2>(__float_as_uint(v)));
+  v += __uint_as_float(dpp<kRowHalfMirror>(__float_as_uint(v)));
+  v += __uint_as_float(dpp<kRowMirror>(__float_as_uint(v)));  // (16 lanes)
+  if constexpr (LANES == 32) v += __shfl_xor(v, 16, 64);
+  if constexpr (LANES >= 64) {
+    auto of = [&](int lane) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), lane)); };
+    v = (of(0) + of(16)) + (of(32) + of(48));
+  }
   if constexpr (LANES > 64) {
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
     __syncthreads();
@@ -127,67 +149,104 @@ __device__ __forceinline__ float lanes_sum(float v, float* part) {
   return v;
 }
 
+// 1 / sqrt(x), x >= 0, within a few units in the last place: the hardware's, which takes no denormals.
+__device__ __forceinline__ float norm_rsqrt(float x) {
+  const bool tiny = x < 0x1p-100f;
+  const float s = __builtin_amdgcn_rsqf(tiny ? x * 0x1p100f : x);
+  return tiny ? s * 0x1p50f : s;
+}
+
+// Sum of a * b over a lane's pieces of a row; `ragged`: the width is no multiple of kV, and elements may be another
+// lane's.
+template <int N>
+__device__ __forceinline__ float own_products(const float (&a)[N][kV], const float (&b)[N][kV], const NormPlace (&at)[N],
+                                              bool ragged) {
+  float sum = 0.f;
+  if (ragged) {
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+#pragma unroll
+      for (int e = 0; e < kV; ++e) sum = __builtin_fmaf(a[k][e], e >= at[k].skip ? b[k][e] : 0.f, sum);
+  } else {
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+#pragma unroll
+      for (int e = 0; e < kV; ++e) sum = __builtin_fmaf(a[k][e], b[k][e], sum);
+  }
+  return sum;
+}
+
+// A workgroup takes every gridDim.x-th row (or kRows of them); the next row is on its way while one is worked on, and
+// the weights stay in registers (with two pieces a lane they are read for every row).
 template <class S, class H, class R>
 __global__ __launch_bounds__(S::kThreads) void residual_norm_kernel(NormArgs a, R* __restrict__ stream, H* __restrict__ normed,
                                                                     float* __restrict__ rstd) {
   constexpr int N = S::kPieces;
-  __shared__ float part[2][S::kLanes / 64 + 1];
+  constexpr bool kHeld = N == 1;
+  __shared__ float part[2][2][S::kLanes / 64 + 1];  // (two rows' worth: see lanes_sum)
   const int lane = threadIdx.x % S::kLanes;
-  const int64_t row = (int64_t)blockIdx.x * S::kRows + threadIdx.x / S::kLanes;
+  const int64_t step = (int64_t)gridDim.x * S::kRows;
+  int64_t row = (int64_t)blockIdx.x * S::kRows + threadIdx.x / S::kLanes;
   if (row >= a.rows) return;  // (whole workgroups where rows share barriers)
-  const H* hp = (const H*)a.h + row * a.ldh;
-  const R* rp = (const R*)a.r + row * a.ldr;
-  const int64_t g0 = a.gate.p ? row / a.gate_each * a.cols : 0;
+  struct Row {
+    Piece<H, kV> h[N];
+    Piece<R, kV> r[N];
+  };
   NormPlace at[N];
-  Piece<H, kV> h[N];
-  Piece<R, kV> r[N];
 #pragma unroll
-  for (int k = 0; k < N; ++k) {
-    at[k] = norm_place<S>(k, lane, (int)a.cols);
-    load_at<true>(hp, at[k], h[k]);
-    load_at<true>(rp, at[k], r[k]);
-  }
-  float s1 = 1.f, s2 = 1.f;
-  if (a.post.p) {
-    float sum = 0.f;
+  for (int k = 0; k < N; ++k) at[k] = norm_place<S>(k, lane, (int)a.cols);
+  auto fetch = [&](Row& q, int64_t i) {
 #pragma unroll
     for (int k = 0; k < N; ++k) {
-      float x[kV];
-      to_floats(h[k], x);
-#pragma unroll
-      for (int e = 0; e < kV; ++e) sum = __builtin_fmaf(x[e], e >= at[k].skip ? x[e] : 0.f, sum);
+      load_at<true>((const H*)a.h + i * a.ldh, at[k], q.h[k]);
+      load_at<true>((const R*)a.r + i * a.ldr, at[k], q.r[k]);
     }
-    s1 = 1.f / sqrtf(lanes_sum<S::kLanes>(sum, part[0]) / (float)a.cols + a.eps);
-  }
-  float t[N][kV], sum = 0.f;
+  };
+  Row now, next;
+  fetch(now, row);
+  // pre, and gate * post, of piece k
+  const bool ragged = a.cols % kV != 0;
+  const float per = 1.f / (float)a.cols;
+  float side1[kV], pre1[kV];
+  int64_t group = -1;
+  if constexpr (kHeld) weight_at(a.pre, 0, at[0], pre1);
+  for (int turn = 0;; turn ^= 1) {
+    const int64_t coming = row + step;
+    if (coming < a.rows) fetch(next, coming);
+    const int64_t g = a.gate.p ? row / a.gate_each : 0;
+    if (kHeld && g != group) side_at(a, g * a.cols, at[0], side1);
+    group = g;
+    float x[N][kV], s1 = 1.f, s2 = 1.f;
 #pragma unroll
-  for (int k = 0; k < N; ++k) {
-    float x[kV], y[kV], p[kV], g[kV];
-    to_floats(h[k], x);
-    to_floats(r[k], y);
-    weight_at(a.post, 0, at[k], p);
-    weight_at(a.gate, g0, at[k], g);
-#pragma unroll
-    for (int e = 0; e < kV; ++e) {
-      t[k][e] = __builtin_fmaf(a.scale, y[e], g[e] * (x[e] * s1 * p[e]));
-      sum = __builtin_fmaf(t[k][e], e >= at[k].skip ? t[k][e] : 0.f, sum);
-    }
-    store_at(stream + row * a.cols, at[k], t[k]);
-  }
-  if (a.pre.p) {
-    s2 = 1.f / sqrtf(lanes_sum<S::kLanes>(sum, part[1]) / (float)a.cols + a.eps);
+    for (int k = 0; k < N; ++k) to_floats(now.h[k], x[k]);
+    if (a.post.p) s1 = norm_rsqrt(__builtin_fmaf(lanes_sum<S::kLanes>(own_products(x, x, at, ragged), part[turn][0]), per, a.eps));
 #pragma unroll
     for (int k = 0; k < N; ++k) {
-      float w[kV];
-      weight_at(a.pre, 0, at[k], w);
+      float y[kV], w[kV];
+      to_floats(now.r[k], y);
+      if constexpr (!kHeld) side_at(a, g * a.cols, at[k], w);
 #pragma unroll
-      for (int e = 0; e < kV; ++e) w[e] *= t[k][e] * s2;
-      store_at(normed + row * a.cols, at[k], w);
+      for (int e = 0; e < kV; ++e) x[k][e] = __builtin_fmaf(a.scale, y[e], x[k][e] * s1 * (kHeld ? side1[e] : w[e]));
+      store_at(stream + row * a.cols, at[k], x[k], a.past);
     }
-  }
-  if (rstd && lane == 0) {
-    rstd[row] = s1;
-    rstd[a.rows + row] = s2;
+    if (a.pre.p) {
+      s2 = norm_rsqrt(__builtin_fmaf(lanes_sum<S::kLanes>(own_products(x, x, at, ragged), part[turn][1]), per, a.eps));
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        float w[kV];
+        if constexpr (!kHeld) weight_at(a.pre, 0, at[k], w);
+#pragma unroll
+        for (int e = 0; e < kV; ++e) x[k][e] = x[k][e] * s2 * (kHeld ? pre1[e] : w[e]);
+        store_at(normed + row * a.cols, at[k], x[k], a.past);
+      }
+    }
+    if (rstd && lane == 0) {
+      rstd[row] = s1;
+      rstd[a.rows + row] = s2;
+    }
+    if (coming >= a.rows) break;
+    row = coming;
+    now = next;
   }
 }
 
@@ -331,127 +390,140 @@ __device__ __forceinline__ void rows_joined(float (&acc)[S::kPieces][kV], float*
   }
 }
 
-// SIDE: the block's side of the sum (norm behind it, gate) as well; else h has the gradient e.
+// SIDE: the block's side of the sum (norm behind it, gate) as well; else h has the gradient e.  Over the rows of a strip,
+// which share a row of the gate, both weights of that side need the same sum of e h s1: times post it is the gate's
+// gradient, times the gate post's.
 template <class S, bool SIDE, class H, class R>
 __global__ __launch_bounds__(S::kThreads) void residual_norm_bwd_kernel(NormArgs a, NormStrips strips,
                                                                         const float* __restrict__ rstd, NormGrads o) {
   constexpr int N = S::kPieces;
-  constexpr bool kHeld = N == 1;  // weights stay in registers; with two pieces a lane they are read again for every row
-  __shared__ float part[2][S::kLanes / 64 + 1];
+  constexpr bool kHeld = N == 1;  // (as above)
+  __shared__ float part[2][2][S::kLanes / 64 + 1];
   __shared__ float lds[S::kRows > 1 ? S::kCols : 1];
   const int lane = threadIdx.x % S::kLanes, sub = threadIdx.x / S::kLanes;
   const float per = 1.f / (float)a.cols;
-  float dpre[N][kV] = {}, dpost[N][kV] = {};
+  struct Row {
+    Piece<H, kV> h[N], dy[N];
+    Piece<R, kV> r[N], ds[N];
+    float s1, s2;
+  };
   NormPlace at[N];
 #pragma unroll
   for (int k = 0; k < N; ++k) at[k] = norm_place<S>(k, lane, (int)a.cols);
-  float pre1[kV], post1[kV], gate1[kV];
-  if constexpr (kHeld) {
-    weight_at(a.pre, 0, at[0], pre1);
-    weight_at(a.post, 0, at[0], post1);
-  }
+  auto fetch = [&](Row& q, int64_t i) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      load_at<true>((const H*)a.h + i * a.ldh, at[k], q.h[k]);
+      load_at<true>((const R*)a.r + i * a.ldr, at[k], q.r[k]);
+      q.dy[k] = Piece<H, kV>{};
+      q.ds[k] = Piece<R, kV>{};
+      if (o.dnormed) load_at<true>((const H*)o.dnormed + i * a.cols, at[k], q.dy[k]);
+      if (o.dstream) load_at<true>((const R*)o.dstream + i * a.cols, at[k], q.ds[k]);
+    }
+    q.s1 = rstd[i];
+    q.s2 = rstd[a.rows + i];
+  };
+  // pre, and gate * post of the strip, of piece k
+  float pre1[kV], side1[kV];
+  auto pre_at = [&](int k, float (&f)[kV]) { weight_at(a.pre, 0, at[k], f); };
+  const bool ragged = a.cols % kV != 0;
+  if constexpr (kHeld) pre_at(0, pre1);
+  float dpre[N][kV] = {}, dpost[N][kV] = {};
+  int turn = 0;
   for (int64_t strip = blockIdx.x; strip < strips.total; strip += gridDim.x) {
     const int64_t group = strip / strips.strips, part0 = (strip - group * strips.strips) * strips.each;
     const int64_t first = group * a.gate_each + part0;
     const int64_t end = first + (part0 + strips.each < a.gate_each ? strips.each : a.gate_each - part0);
     const int64_t g0 = group * a.cols;
-    float dgate[N][kV] = {};
-    if constexpr (kHeld && SIDE) weight_at(a.gate, g0, at[0], gate1);
-    for (int64_t row = first + sub; row < end; row += S::kRows) {
-      Piece<H, kV> h[N], dy[N];
-      Piece<R, kV> r[N], ds[N];
-#pragma unroll
-      for (int k = 0; k < N; ++k) {
-        load_at<true>((const H*)a.h + row * a.ldh, at[k], h[k]);
-        load_at<true>((const R*)a.r + row * a.ldr, at[k], r[k]);
-        dy[k] = Piece<H, kV>{};
-        ds[k] = Piece<R, kV>{};
-        if (o.dnormed) load_at<true>((const H*)o.dnormed + row * a.cols, at[k], dy[k]);
-        if (o.dstream) load_at<true>((const R*)o.dstream + row * a.cols, at[k], ds[k]);
-      }
-      const float s1 = rstd[row], s2 = rstd[a.rows + row];
-      float hat[N][kV], sum = 0.f;
+    float both[N][kV] = {};
+    Row now, next;
+    int64_t row = first + sub;
+    if (kHeld && row < end) fetch(now, row);
+    if constexpr (kHeld && SIDE) side_at(a, g0, at[0], side1);
+    for (; row < end; row += S::kRows, turn ^= 1) {
+      if constexpr (!kHeld) fetch(now, row);
+      if (kHeld && row + S::kRows < end) fetch(next, row + S::kRows);
+      const float s1 = now.s1, s2 = now.s2;
+      float hat[N][kV], u[N][kV];
 #pragma unroll
       for (int k = 0; k < N; ++k) {
         float x[kV], y[kV], d[kV], w[kV];
-        to_floats(h[k], x);
-        to_floats(r[k], y);
-        to_floats(dy[k], d);
+        to_floats(now.h[k], x);
+        to_floats(now.r[k], y);
+        to_floats(now.dy[k], d);
         if constexpr (SIDE) {
-          float p[kV], g[kV];
-          if constexpr (!kHeld) {
-            weight_at(a.post, 0, at[k], p);
-            weight_at(a.gate, g0, at[k], g);
-          }
+          if constexpr (!kHeld) side_at(a, g0, at[k], w);
 #pragma unroll
-          for (int e = 0; e < kV; ++e) x[e] = (kHeld ? gate1[e] : g[e]) * (x[e] * s1 * (kHeld ? post1[e] : p[e]));
+          for (int e = 0; e < kV; ++e) x[e] = x[e] * s1 * (kHeld ? side1[e] : w[e]);
         }
-        if constexpr (!kHeld) weight_at(a.pre, 0, at[k], w);
+        if constexpr (!kHeld) pre_at(k, w);
 #pragma unroll
         for (int e = 0; e < kV; ++e) {
           hat[k][e] = __builtin_fmaf(a.scale, y[e], x[e]) * s2;
           dpre[k][e] = __builtin_fmaf(d[e], hat[k][e], dpre[k][e]);
-          sum = __builtin_fmaf(d[e] * (kHeld ? pre1[e] : w[e]), e >= at[k].skip ? hat[k][e] : 0.f, sum);
+          u[k][e] = d[e] * (kHeld ? pre1[e] : w[e]);
         }
       }
-      const float mean = lanes_sum<S::kLanes>(sum, part[0]) * per;
-      sum = 0.f;
-      float (&q)[N][kV] = hat;  // (in place: what h's gradient is formed from)
+      const float mean = lanes_sum<S::kLanes>(own_products(u, hat, at, ragged), part[turn][0]) * per;
+      float (&q)[N][kV] = u;  // (in place: what h's gradient is formed from)
 #pragma unroll
       for (int k = 0; k < N; ++k) {
-        float d[kV], w[kV], e1[kV], dr[kV];
-        to_floats(dy[k], d);
-        to_floats(ds[k], e1);
-        if constexpr (!kHeld) weight_at(a.pre, 0, at[k], w);
+        float w[kV], e1[kV], dr[kV];
+        to_floats(now.ds[k], e1);
 #pragma unroll
         for (int e = 0; e < kV; ++e) {
-          e1[e] = __builtin_fmaf(s2, __builtin_fmaf(-hat[k][e], mean, d[e] * (kHeld ? pre1[e] : w[e])), e1[e]);
+          e1[e] = __builtin_fmaf(s2, __builtin_fmaf(-hat[k][e], mean, u[k][e]), e1[e]);
           dr[e] = a.scale * e1[e];
         }
-        if (o.dr) store_at((R*)o.dr + row * a.cols, at[k], dr);
+        if (o.dr) store_at((R*)o.dr + row * a.cols, at[k], dr, a.past);
         if constexpr (SIDE) {
-          float x[kV], p[kV], g[kV];
-          to_floats(h[k], x);
-          if constexpr (!kHeld) {
-            weight_at(a.post, 0, at[k], p);
-            weight_at(a.gate, g0, at[k], g);
-          }
+          float x[kV];
+          to_floats(now.h[k], x);
+          if constexpr (!kHeld) side_at(a, g0, at[k], w);
 #pragma unroll
           for (int e = 0; e < kV; ++e) {
-            const float hs = x[e] * s1, qe = e1[e] * (kHeld ? gate1[e] : g[e]), pe = kHeld ? post1[e] : p[e];
-            dgate[k][e] = __builtin_fmaf(e1[e], hs * pe, dgate[k][e]);
-            dpost[k][e] = __builtin_fmaf(qe, hs, dpost[k][e]);
-            q[k][e] = qe * pe;
-            sum = __builtin_fmaf(q[k][e], e >= at[k].skip ? hs : 0.f, sum);
+            hat[k][e] = x[e] * s1;  // (h's share from here on)
+            both[k][e] = __builtin_fmaf(e1[e], hat[k][e], both[k][e]);
+            q[k][e] = e1[e] * (kHeld ? side1[e] : w[e]);
           }
         } else {
-          if (o.dh) store_at((H*)o.dh + row * a.cols, at[k], e1);
+          if (o.dh) store_at((H*)o.dh + row * a.cols, at[k], e1, a.past);
         }
       }
       if constexpr (SIDE) {
-        const float all = lanes_sum<S::kLanes>(sum, part[1]) * per, mean1 = a.post.p ? all : 0.f;
+        const float mean1 = a.post.p ? lanes_sum<S::kLanes>(own_products(q, hat, at, ragged), part[turn][1]) * per : 0.f;
         if (o.dh) {
 #pragma unroll
           for (int k = 0; k < N; ++k) {
-            float x[kV];
-            to_floats(h[k], x);
 #pragma unroll
-            for (int e = 0; e < kV; ++e) x[e] = s1 * __builtin_fmaf(-x[e] * s1, mean1, q[k][e]);
-            store_at((H*)o.dh + row * a.cols, at[k], x);
+            for (int e = 0; e < kV; ++e) q[k][e] = s1 * __builtin_fmaf(-hat[k][e], mean1, q[k][e]);
+            store_at((H*)o.dh + row * a.cols, at[k], q[k], a.past);
           }
         }
-      } else if constexpr (S::kLanes > 64) {
-        __syncthreads();  // (part[0] again)
       }
+      if constexpr (kHeld) now = next;
     }
-    if (SIDE && o.dgate) {
-      rows_joined<S>(dgate, lds);
-      if (sub == 0) {
+    if constexpr (SIDE) {
 #pragma unroll
-        for (int k = 0; k < N; ++k) {
-          if (strips.strips > 1) store_at(o.gate_part + strip * a.cols, at[k], dgate[k]);
-          else if (o.dgate_f32) store_at((float*)o.dgate + g0, at[k], dgate[k]);
-          else store_at((uint16_t*)o.dgate + g0, at[k], dgate[k]);
+      for (int k = 0; k < N; ++k) {
+        float g[kV];
+        weight_at(a.gate, g0, at[k], g);
+#pragma unroll
+        for (int e = 0; e < kV; ++e) dpost[k][e] = __builtin_fmaf(g[e], both[k][e], dpost[k][e]);
+      }
+      if (o.dgate) {
+        rows_joined<S>(both, lds);
+        if (sub == 0) {
+#pragma unroll
+          for (int k = 0; k < N; ++k) {
+            float p[kV];
+            weight_at(a.post, 0, at[k], p);
+#pragma unroll
+            for (int e = 0; e < kV; ++e) p[e] *= both[k][e];
+            if (strips.strips > 1) store_at(o.gate_part + strip * a.cols, at[k], p);
+            else if (o.dgate_f32) store_at((float*)o.dgate + g0, at[k], p);
+            else store_at((uint16_t*)o.dgate + g0, at[k], p);
+          }
         }
       }
     }
@@ -510,12 +582,21 @@ __global__ __launch_bounds__(kNormThreads) void residual_norm_join_kernel(NormJo
   }
 }
 
-// Workgroups of the backward pass, and their strips.
-constexpr int kNormGroups = 512;
+// Stores go past the caches where two matrices of this size do not stay in the last one (256 MB) until the next operator
+// reads them.  us forward and backward, past / through: 16384 x 4096 (2 x 134 MB) 89 + 162 / 85 + 144; x 8192 196 + 323 /
+// 212 + 339; 147456 x 2048 424 + 663 / 445 + 704.
+static bool norm_past(int64_t elements, int h_f32, int r_f32) { return elements * (2 * (2 + !!h_f32 + !!r_f32)) > (384 << 20); }
 
-static NormStrips norm_strips(int64_t rows, int64_t gate_rows) {
+// Workgroups: `waves` in all.
+static int64_t norm_groups(int64_t cols, int64_t waves) {
+  return waves * 64 / (cols <= 512 ? 256 : cols <= 1024 ? 128 : cols <= 2048 ? 256 : cols <= 4096 ? 512 : 1024);
+}
+// The backward pass has as many waves as its registers let a CU hold (two a SIMD with the block's side, four without).
+static int64_t norm_bwd_groups(int64_t cols, bool side) { return norm_groups(cols, side ? 2048 : 4096); }
+
+static NormStrips norm_strips(int64_t rows, int64_t gate_rows, int64_t groups) {
   const int64_t n = rows / gate_rows;
-  int64_t strips = kNormGroups / gate_rows;
+  int64_t strips = groups / gate_rows;
   strips = strips < 1 ? 1 : strips > n ? n : strips;
   const int64_t each = (n + strips - 1) / strips;
   strips = (n + each - 1) / each;
@@ -571,7 +652,7 @@ extern "C" int mx_residual_norm(const void* h, int h_f32, const void* r, int r_f
   if (((uintptr_t)stream_out & (r_f32 ? 3 : 1)) || ((uintptr_t)normed & (h_f32 ? 3 : 1)) || ((uintptr_t)rstd & 3))
     return MX_ERR_ALIGNMENT;
   const NormArgs a{h, r, rows, cols, ldh, ldr, {post, weights_f32 & 1}, {gate, weights_f32 & 2}, {pre, weights_f32 & 4},
-                   rows / gate_rows, scale, eps};
+                   rows / gate_rows, scale, eps, norm_past(rows * cols, h_f32, r_f32)};
   norm_types(h_f32, r_f32, [&](auto ht, auto rt) {
     using H = decltype(ht);
     using R = decltype(rt);
@@ -581,7 +662,7 @@ extern "C" int mx_residual_norm(const void* h, int h_f32, const void* r, int r_f
         hipLaunchKernelGGL((residual_norm_any_kernel<H, R>), dim3((unsigned)rows), dim3(kNormThreads), 0, (hipStream_t)stream,
                            a, (R*)stream_out, (H*)normed, rstd);
       else
-        hipLaunchKernelGGL((residual_norm_kernel<S, H, R>), dim3((unsigned)((rows + S::kRows - 1) / S::kRows)),
+        hipLaunchKernelGGL((residual_norm_kernel<S, H, R>), dim3((unsigned)std::min<int64_t>((rows + S::kRows - 1) / S::kRows, norm_groups(cols, 4096))),
                            dim3(S::kThreads), 0, (hipStream_t)stream, a, (R*)stream_out, (H*)normed, rstd);
     });
   });
@@ -590,9 +671,12 @@ extern "C" int mx_residual_norm(const void* h, int h_f32, const void* r, int r_f
 
 extern "C" int64_t mx_residual_norm_workspace(int64_t rows, int64_t cols, int64_t gate_rows) {
   if (rows <= 0 || cols <= 0 || gate_rows < 1 || rows % gate_rows) return 0;
-  const NormStrips s = norm_strips(rows, gate_rows);
-  const int64_t groups = s.total < kNormGroups ? s.total : kNormGroups;
-  return 4 * cols * (3 * groups + (s.strips > 1 ? s.total : 0));
+  int64_t most = 0;
+  for (bool side : {false, true}) {
+    const NormStrips s = norm_strips(rows, gate_rows, norm_bwd_groups(cols, side));
+    most = std::max(most, 3 * std::min(s.total, norm_bwd_groups(cols, side)) + (s.strips > 1 ? s.total : 0));
+  }
+  return 4 * cols * most;
 }
 
 extern "C" int mx_residual_norm_bwd(const void* h, int h_f32, const void* r, int r_f32, int64_t rows, int64_t cols,
@@ -610,9 +694,9 @@ extern "C" int mx_residual_norm_bwd(const void* h, int h_f32, const void* r, int
       odd(dgate, weights_f32 & 2) || odd(dpre, weights_f32 & 4) || odd(rstd, 1) || ((uintptr_t)workspace & 15))
     return MX_ERR_ALIGNMENT;
   const NormArgs a{h, r, rows, cols, ldh, ldr, {post, weights_f32 & 1}, {gate, weights_f32 & 2}, {pre, weights_f32 & 4},
-                   rows / gate_rows, scale, 0.f};
-  const NormStrips s = norm_strips(rows, gate_rows);
-  const int64_t groups = s.total < kNormGroups ? s.total : kNormGroups;
+                   rows / gate_rows, scale, 0.f, norm_past(rows * cols, h_f32, r_f32)};
+  const NormStrips s = norm_strips(rows, gate_rows, norm_bwd_groups(cols, post || gate));
+  const int64_t groups = std::min(s.total, norm_bwd_groups(cols, post || gate));
   float* rows_part = (float*)workspace;
   float* gate_part = rows_part + 3 * groups * cols;
   const NormGrads o{dstream, dnormed, dh, dr, rows_part, gate_part, dgate, weights_f32 & 2};
@@ -632,7 +716,7 @@ extern "C" int mx_residual_norm_bwd(const void* h, int h_f32, const void* r, int
                            rstd, o);
     });
   });
-  const int64_t gates = dgate && s.strips > 1 ? gate_rows : 0;  // (fewer than kNormGroups of them)
+  const int64_t gates = dgate && s.strips > 1 ? gate_rows : 0;  // (fewer than workgroups)
   if (dpost || dpre || gates) {
     const NormJoin j{rows_part, gate_part, groups, s.strips, {dpost, dpre, dgate}, {weights_f32 & 1, weights_f32 & 4, weights_f32 & 2}};
     hipLaunchKernelGGL(residual_norm_join_kernel, dim3((unsigned)((cols + 63) / 64), (unsigned)(2 + gates)), dim3(kNormThreads),

@@ -106,6 +106,9 @@ __device__ __forceinline__ Piece<T, V> from_floats(const float (&f)[V]) {
   return q;
 }
 
+// Lane exchange inside 16 lanes (see dpp): lane i from lane 15 - i; of 8, from lane 7 - i.
+constexpr int kRowMirror = 0x140, kRowHalfMirror = 0x141;
+
 __device__ __forceinline__ float wave_sum(float v) {
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
