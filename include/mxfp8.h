@@ -392,11 +392,13 @@ int mx_residual_norm_bwd(const void* h, int h_f32, const void* r, int r_f32, int
  * vector, and their scaling (the clipping of gradients, torchtitan/distributed/utils.py:466-472 and around).  kind 0: sqrt(sum
  * x^2), 1: sum |x|, 2: max |x|; sums in float64, norm: one float32 on the device.  workspace: mx_grad_norm_workspace(n)
  * bytes, 8-byte aligned.
- * mx_grad_scale: every value times min(1, limit / (*norm + 1e-6)), in float32, rounded to its type, in place; nothing
+ * mx_grad_scale (mx_grad_clip: the norm and then this): every value times min(1, limit / (*norm + 1e-6)), in float32, rounded to its type, in place; nothing
  * is touched where that is exactly 1.  Tensors that share memory are scaled one after the other. */
 int64_t mx_grad_norm_workspace(int64_t n);
 int mx_grad_norm(int64_t n, void* const* grads, const int64_t* elems, const int32_t* is_f32, int kind, float* norm,
                  void* workspace, void* stream);
+int mx_grad_clip(int64_t n, void* const* grads, const int64_t* elems, const int32_t* is_f32, int kind, float* norm,
+                 float limit, void* workspace, void* stream);
 int mx_grad_scale(int64_t n, void* const* grads, const int64_t* elems, const int32_t* is_f32, const float* norm, float limit,
                   void* stream);
 

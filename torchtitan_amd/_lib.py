@@ -76,6 +76,7 @@ SIGNATURES = {
                                      _P, _P, _P, _P, _P, _P, _P, _P, _P, _P]),
     "mx_grad_norm_workspace": (_I, [_I]),
     "mx_grad_norm": (c_int, [_I, _P, _P, _P, c_int, _P, _P, _P]),
+    "mx_grad_clip": (c_int, [_I, _P, _P, _P, c_int, _P, ctypes.c_float, _P, _P]),
     "mx_grad_scale": (c_int, [_I, _P, _P, _P, _P, ctypes.c_float, _P]),
     "mx_scale_layout": (c_int, [_P, _I, _I, _P, _P]),
     "mx_scale_unlayout": (c_int, [_P, _I, _I, _P, _P]),

@@ -1,5 +1,7 @@
 // The launches of a converted linear, of the SwiGLU block and of the routed experts, forward and backward, from one
 // native call each; and the single launches around them (gate, routing, log-probabilities, lists of casts), likewise.
+// The embedding and the norms around a block come with their autograd nodes: their launches take 5 us at small sizes, an
+// autograd function in Python around them 60 forward and backward.
 //
 // On inputs of up to a few thousand tokens these blocks wait for their host side: between two launches
 // (3.3 us each) Python made operands, asked tensors for their pointers and strides and passed them on, 4 to 8 us
@@ -9,6 +11,8 @@
 // case -- bf16 or float32 matrices on the current GPU whose rows the casts read as they lie -- and returns None
 // otherwise: the caller then takes the general path.
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
 #include <array>
@@ -57,6 +61,14 @@ struct Library {
   decltype(&mx_token_logprob_bwd_any) logprob_bwd = nullptr;
   decltype(&mx_cast_rows_many) rows_many = nullptr;
   decltype(&mx_dequant_many) dequant_many = nullptr;
+  decltype(&mx_embedding) embedding = nullptr;
+  decltype(&mx_embedding_grad_workspace) embedding_grad_workspace = nullptr;
+  decltype(&mx_embedding_grad) embedding_grad = nullptr;
+  decltype(&mx_residual_norm) residual_norm = nullptr;
+  decltype(&mx_residual_norm_workspace) residual_norm_workspace = nullptr;
+  decltype(&mx_residual_norm_bwd) residual_norm_bwd = nullptr;
+  decltype(&mx_grad_norm_workspace) grad_norm_workspace = nullptr;
+  decltype(&mx_grad_clip) grad_clip = nullptr;
 } lib;
 PyObject* check_status = nullptr;  // _lib.check, never released
 
@@ -98,6 +110,14 @@ void bind(const py::dict& addresses, const py::object& check) {
   set("mx_token_logprob_bwd_any", lib.logprob_bwd);
   set("mx_cast_rows_many", lib.rows_many);
   set("mx_dequant_many", lib.dequant_many);
+  set("mx_embedding", lib.embedding);
+  set("mx_embedding_grad_workspace", lib.embedding_grad_workspace);
+  set("mx_embedding_grad", lib.embedding_grad);
+  set("mx_residual_norm", lib.residual_norm);
+  set("mx_residual_norm_workspace", lib.residual_norm_workspace);
+  set("mx_residual_norm_bwd", lib.residual_norm_bwd);
+  set("mx_grad_norm_workspace", lib.grad_norm_workspace);
+  set("mx_grad_clip", lib.grad_clip);
   check_status = check.ptr();
   Py_INCREF(check_status);
 }
@@ -774,6 +794,244 @@ std::optional<std::vector<Tensor>> dequant_many(const std::vector<Tensor>& codes
   return out;
 }
 
+// ---- around the linears: embedding, norms with the residual sum, clipping (modules/embedding.py, modules/norm.py and
+// gradients.py have their meaning and their general path)
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+// bf16 or float32 on the GPU, no subclass that sees its operations
+bool row_tensor(const Tensor& t) {
+  return t.is_cuda() && t.layout() == at::kStrided && (t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kFloat) &&
+         !t.unsafeGetTensorImpl()->is_python_dispatch();
+}
+int is_f32(const Tensor& t) { return t.scalar_type() == at::kFloat; }
+// Elements between the rows of [..., cols], 0 where they do not lie one after the other at one distance
+int64_t row_pitch(const Tensor& t, int64_t cols) {
+  if (t.is_contiguous()) return cols;
+  return t.dim() == 2 && t.stride(1) == 1 && t.stride(0) >= cols ? t.stride(0) : 0;
+}
+void* pointer(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+Tensor or_none(const std::optional<Tensor>& t) { return t ? *t : Tensor(); }
+
+// A saved tensor as the kernels read it: hooks may have replaced it by another with the same values.
+Tensor saved_rows(const Tensor& t, const Tensor& like, at::IntArrayRef sizes) {
+  if (!t.defined()) return t;
+  TORCH_CHECK(t.device() == like.device() && t.sizes() == sizes, "a saved tensor came back as ", t.sizes(), " on ", t.device(),
+              "; expected ", sizes, " on ", like.device());
+  return row_pitch(t, sizes.back()) ? t : t.contiguous();
+}
+
+// Gradients that cannot be differentiated again: asking for it is an error.
+variable_list once(const variable_list& from, variable_list grads) {
+  bool again = false;
+  for (const Tensor& t : from) again |= t.defined() && t.requires_grad();
+  if (!again || !at::GradMode::is_enabled()) return grads;
+  for (Tensor& t : grads)
+    if (t.defined()) t = t.detach().set_requires_grad(true);
+  std::shared_ptr<torch::autograd::Node> error(
+      new torch::autograd::DelayedError("this operator's gradients cannot be differentiated again", static_cast<int64_t>(grads.size())),
+      torch::autograd::deleteNode);
+  return (*error)(std::move(grads));
+}
+
+Tensor embedding_launch(const Tensor& ids, const Tensor& weight, double scale, int64_t first, bool out_f32) {
+  std::vector<int64_t> sizes = ids.sizes().vec();
+  const int64_t cols = weight.size(1);
+  sizes.push_back(cols);
+  const Tensor out = at::empty(sizes, weight.options().dtype(out_f32 ? at::kFloat : at::kBFloat16));
+  checked(lib.embedding(ids.data_ptr(), ids.scalar_type() == at::kLong, ids.numel(), weight.data_ptr(), is_f32(weight),
+                        weight.size(0), cols, weight.stride(0), first, static_cast<float>(scale), out.data_ptr(), out_f32,
+                        stream_of(weight)),
+          "mx_embedding");
+  return out;
+}
+
+struct EmbeddingNode : torch::autograd::Function<EmbeddingNode> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& ids, const Tensor& weight, double scale, int64_t padding,
+                        int64_t first, bool out_f32) {
+    ctx->save_for_backward({ids});
+    for (auto& [name, value] : std::initializer_list<std::pair<const char*, c10::IValue>>{
+             {"scale", scale}, {"padding", padding}, {"first", first}, {"rows", weight.size(0)}, {"f32", is_f32(weight) != 0}})
+      ctx->saved_data[name] = value;
+    return embedding_launch(ids, weight, scale, first, out_f32);
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    Tensor ids = ctx->get_saved_variables()[0].contiguous(), dout = grads[0];
+    TORCH_CHECK(ids.device() == dout.device() && (ids.scalar_type() == at::kLong || ids.scalar_type() == at::kInt),
+                "the saved ids came back as ", ids.scalar_type(), " on ", ids.device());
+    const c10::DeviceGuard guard(dout.device());
+    const int64_t n = ids.numel(), cols = dout.size(-1), rows = ctx->saved_data["rows"].toInt();
+    TORCH_CHECK(dout.numel() == n * cols, "the saved ids came back as ", ids.sizes(), " for a gradient of ", dout.sizes());
+    const bool f32 = ctx->saved_data["f32"].toBool();
+    if (!row_pitch(dout, cols)) dout = dout.contiguous();
+    const Tensor grad = at::empty({rows, cols}, dout.options().dtype(f32 ? at::kFloat : at::kBFloat16));
+    const Tensor work = at::empty({lib.embedding_grad_workspace(n, rows, cols)}, dout.options().dtype(at::kByte));
+    checked(lib.embedding_grad(ids.data_ptr(), ids.scalar_type() == at::kLong, n, dout.data_ptr(), is_f32(dout),
+                               row_pitch(dout, cols), rows, cols, ctx->saved_data["first"].toInt(),
+                               ctx->saved_data["padding"].toInt(), static_cast<float>(ctx->saved_data["scale"].toDouble()),
+                               grad.data_ptr(), f32, work.data_ptr(), stream_of(dout)),
+            "mx_embedding_grad");
+    return once(grads, {Tensor(), grad, Tensor(), Tensor(), Tensor(), Tensor()});
+  }
+};
+
+std::optional<Tensor> scaled_embedding(const Tensor& ids, const Tensor& weight, double scale, std::optional<int64_t> padding,
+                                       int64_t first, bool out_f32) {
+  if (!row_tensor(weight) || weight.dim() != 2 || !on_current_device(weight) || ids.device() != weight.device() ||
+      (ids.scalar_type() != at::kLong && ids.scalar_type() != at::kInt) || !ids.is_contiguous() || weight.numel() == 0 ||
+      ids.unsafeGetTensorImpl()->is_python_dispatch() || !row_pitch(weight, weight.size(1)))
+    return std::nullopt;
+  Unlocked unlocked(std::in_place);
+  if (at::GradMode::is_enabled() && weight.requires_grad())
+    return EmbeddingNode::apply(ids, weight, scale, padding.value_or(first - 1), first, out_f32);
+  return embedding_launch(ids, weight, scale, first, out_f32);
+}
+
+// The kernels' view of the norm's operands: rows of h and residual, the weights and their types
+struct NormOperands {
+  int64_t rows, cols, groups;
+  int flags;
+};
+NormOperands norm_operands(const Tensor& h, const Tensor& post, const Tensor& gate, const Tensor& pre) {
+  const int64_t cols = h.size(-1);
+  auto flag = [](const Tensor& t, int bit) { return t.defined() && is_f32(t) ? bit : 0; };
+  return {h.numel() / cols, cols, gate.defined() ? gate.numel() / cols : 1, flag(post, 1) | flag(gate, 2) | flag(pre, 4)};
+}
+
+// (stream, normed or nothing, rstd or nothing)
+std::array<Tensor, 3> norm_launch(const Tensor& h, const Tensor& r, const Tensor& post, const Tensor& gate, const Tensor& pre,
+                                  double scale, double eps, bool want_rstd) {
+  const auto [rows, cols, groups, flags] = norm_operands(h, post, gate, pre);
+  const Tensor stream = at::empty(h.sizes(), r.options()), normed = pre.defined() ? at::empty(h.sizes(), h.options()) : Tensor(),
+               rstd = want_rstd ? at::empty({2, rows}, h.options().dtype(at::kFloat)) : Tensor();
+  checked(lib.residual_norm(h.data_ptr(), is_f32(h), r.data_ptr(), is_f32(r), rows, cols, row_pitch(h, cols), row_pitch(r, cols),
+                            pointer(post), pointer(gate), pointer(pre), flags, groups, static_cast<float>(scale),
+                            static_cast<float>(eps), stream.data_ptr(), pointer(normed), static_cast<float*>(pointer(rstd)),
+                            stream_of(h)),
+          "mx_residual_norm");
+  return {stream, normed, rstd};
+}
+
+struct ResidualNormNode : torch::autograd::Function<ResidualNormNode> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& h, const Tensor& r, const std::optional<Tensor>& post_weight,
+                               const std::optional<Tensor>& gate_rows, const std::optional<Tensor>& pre_weight, double scale,
+                               double eps) {
+    const Tensor post = or_none(post_weight), gate = or_none(gate_rows), pre = or_none(pre_weight);
+    const auto [stream, normed, rstd] = norm_launch(h, r, post, gate, pre, scale, eps, true);
+    int64_t wanted = 0, bit = 1;
+    for (const Tensor& t : {h, r, post, gate, pre}) {
+      if (t.defined() && t.requires_grad()) wanted |= bit;
+      bit *= 2;
+    }
+    ctx->saved_data["wanted"] = wanted;
+    ctx->save_for_backward({h, r, post, gate, pre, rstd});
+    ctx->saved_data["scale"] = scale;
+    ctx->set_materialize_grads(false);
+    return normed.defined() ? variable_list{stream, normed} : variable_list{stream};
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    variable_list out(7);
+    Tensor dstream = grads[0], dnormed = grads.size() > 1 ? grads[1] : Tensor();
+    if (!dstream.defined() && !dnormed.defined()) return out;
+    const variable_list saved = ctx->get_saved_variables();
+    const Tensor& like = dstream.defined() ? dstream : dnormed;
+    const c10::DeviceGuard guard(like.device());
+    const auto sizes = like.sizes();
+    const Tensor h = saved_rows(saved[0], like, sizes), r = saved_rows(saved[1], like, sizes);
+    const std::array<Tensor, 3> weights = {saved[2].defined() ? saved[2].contiguous() : Tensor(),
+                                           saved[3].defined() ? saved[3].contiguous() : Tensor(),
+                                           saved[4].defined() ? saved[4].contiguous() : Tensor()};
+    const auto& [post, gate, pre] = weights;
+    const Tensor rstd = saved[5].contiguous();
+    const auto [rows, cols, groups, flags] = norm_operands(h, post, gate, pre);
+    TORCH_CHECK(row_tensor(h) && row_tensor(r) && (!is_f32(h) || is_f32(r)) && rstd.scalar_type() == at::kFloat &&
+                    rstd.numel() == 2 * rows && rstd.device() == h.device(),
+                "a saved tensor came back with another type or size");
+    for (const Tensor& w : weights)
+      TORCH_CHECK(!w.defined() || (row_tensor(w) && w.device() == h.device() && w.size(-1) == cols),
+                  "a saved weight came back with another type or size");
+    if (dstream.defined()) dstream = dstream.contiguous();
+    if (dnormed.defined()) dnormed = dnormed.contiguous();
+    const int64_t wanted = ctx->saved_data["wanted"].toInt();
+    const std::array<const Tensor*, 5> of = {&h, &r, &post, &gate, &pre};
+    for (size_t i = 0; i < 5; ++i)
+      if (wanted >> i & 1) out[i] = at::empty(of[i]->sizes(), of[i]->options());
+    const Tensor work = at::empty({lib.residual_norm_workspace(rows, cols, groups)}, h.options().dtype(at::kByte));
+    checked(lib.residual_norm_bwd(h.data_ptr(), is_f32(h), r.data_ptr(), is_f32(r), rows, cols, row_pitch(h, cols),
+                                  row_pitch(r, cols), pointer(post), pointer(gate), pointer(pre), flags, groups,
+                                  static_cast<float>(ctx->saved_data["scale"].toDouble()), rstd.data_ptr<float>(),
+                                  pointer(dstream), pointer(dnormed), pointer(out[0]), pointer(out[1]), pointer(out[2]),
+                                  pointer(out[3]), pointer(out[4]), work.data_ptr(), stream_of(h)),
+            "mx_residual_norm_bwd");
+    return once(grads, std::move(out));
+  }
+};
+
+// (stream, normed or None)
+py::object residual_rms_norm(const Tensor& h, const Tensor& r, const std::optional<Tensor>& post_weight,
+                             const std::optional<Tensor>& gate_rows, const std::optional<Tensor>& pre_weight, double scale,
+                             double eps) {
+  const Tensor post = or_none(post_weight), gate = or_none(gate_rows), pre = or_none(pre_weight);
+  if (!row_tensor(h) || !row_tensor(r) || h.dim() == 0 || h.sizes() != r.sizes() || h.numel() == 0 || (is_f32(h) && !is_f32(r)) ||
+      r.device() != h.device() || !on_current_device(h))
+    return py::none();
+  const int64_t cols = h.size(-1);
+  if (!row_pitch(h, cols) || !row_pitch(r, cols)) return py::none();
+  auto weight = [&](const Tensor& w) { return row_tensor(w) && w.device() == h.device() && w.is_contiguous(); };
+  for (const Tensor& w : {post, pre})
+    if (w.defined() && (!weight(w) || w.dim() != 1 || w.size(0) != cols)) return py::none();
+  if (gate.defined()) {
+    if (!weight(gate) || gate.size(-1) != cols || (gate.dim() != 1 && gate.dim() != h.dim())) return py::none();
+    bool shared = false;  // h's leading dimensions up to one, ones behind it
+    for (int64_t i = 0; i + 1 < gate.dim(); ++i) {
+      if (gate.size(i) != h.size(i)) shared = true;
+      if (shared && gate.size(i) != 1) return py::none();
+    }
+  }
+  Unlocked unlocked(std::in_place);
+  bool grads = false;
+  for (const Tensor& t : {h, r, post, gate, pre}) grads |= t.defined() && t.requires_grad();
+  if (grads && at::GradMode::is_enabled()) {
+    const variable_list out = ResidualNormNode::apply(h, r, post_weight, gate_rows, pre_weight, scale, eps);
+    unlocked.reset();
+    return py::make_tuple(out[0], out.size() > 1 ? py::cast(out[1]) : py::none());
+  }
+  const auto [stream, normed, rstd] = norm_launch(h, r, post, gate, pre, scale, eps, false);
+  unlocked.reset();
+  return py::make_tuple(stream, normed.defined() ? py::cast(normed) : py::none());
+}
+
+// The norm of the parameters' gradients, which are scaled to `limit`
+std::optional<Tensor> clip_gradients(const std::vector<Tensor>& parameters, double limit, int kind) {
+  std::vector<Tensor> grads;
+  grads.reserve(parameters.size());
+  for (const Tensor& p : parameters) {
+    const Tensor& g = p.grad();
+    if (!g.defined()) continue;
+    if (!row_tensor(g) || !g.is_non_overlapping_and_dense() || g.device() != (grads.empty() ? g : grads[0]).device())
+      return std::nullopt;
+    grads.push_back(g);
+  }
+  if (grads.empty() || !on_current_device(grads[0])) return std::nullopt;
+  const size_t n = grads.size();
+  Unlocked unlocked(std::in_place);
+  std::vector<void*> data(n);
+  std::vector<int64_t> elems(n);
+  std::vector<int32_t> f32(n);
+  for (size_t i = 0; i < n; ++i) {
+    data[i] = grads[i].data_ptr();
+    elems[i] = grads[i].numel();
+    f32[i] = is_f32(grads[i]);
+    if (!grads[i].is_inference()) grads[i].unsafeGetTensorImpl()->bump_version();
+  }
+  const auto bytes = at::TensorOptions().device(grads[0].device()).dtype(at::kByte);
+  const Tensor norm = at::empty({}, bytes.dtype(at::kFloat)), work = at::empty({lib.grad_norm_workspace(n)}, bytes);
+  checked(lib.grad_clip(n, data.data(), elems.data(), f32.data(), kind, norm.data_ptr<float>(), static_cast<float>(limit),
+                        work.data_ptr(), stream_of(norm)),
+          "mx_grad_clip");
+  return norm;
+}
+
 // The capture that `stream` is part of, a number of its own for every capture (0: none).
 unsigned long long capture_id(uintptr_t stream) {
   hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
@@ -805,4 +1063,7 @@ PYBIND11_MODULE(_blocks, m) {
   m.def("token_logprob_bwd", torch::wrap_pybind_function(token_logprob_bwd));
   m.def("rows_many", torch::wrap_pybind_function(rows_many));
   m.def("dequant_many", torch::wrap_pybind_function(dequant_many));
+  m.def("scaled_embedding", torch::wrap_pybind_function(scaled_embedding));
+  m.def("residual_rms_norm", torch::wrap_pybind_function(residual_rms_norm));
+  m.def("clip_gradients", torch::wrap_pybind_function(clip_gradients));
 }

@@ -81,12 +81,23 @@ __global__ __launch_bounds__(kRankThreads) void embedding_rank_kernel(EmbIds ids
   const int t0 = (int)blockIdx.x * 64, t = t0 + lane;
   if (blockIdx.x == 0 && threadIdx.x == 0) *chains = 0;
   const int padded = (n + 4 * kWaves - 1) / (4 * kWaves) * (4 * kWaves);  // (at most kRankMost)
-  for (int i = threadIdx.x; i < padded; i += kRankThreads) tile[i] = i < n ? ids.key(i) : 0xFFFFFFFFu;  // in front of nobody
+  uint32_t own[kRankMost / kRankThreads];  // (all asked for before the first is written)
+#pragma unroll
+  for (int k = 0; k < kRankMost / kRankThreads; ++k) {
+    const int i = k * kRankThreads + threadIdx.x;
+    own[k] = i < n ? ids.key(i) : 0xFFFFFFFFu;  // (in front of nobody)
+  }
+#pragma unroll
+  for (int k = 0; k < kRankMost / kRankThreads; ++k) {
+    const int i = k * kRankThreads + threadIdx.x;
+    if (i < padded) tile[i] = own[k];
+  }
   __syncthreads();
   const uint32_t mine = t < n ? tile[t] : 0u;
   const int each = padded / kWaves, lo = wave * each, hi = lo + each;
   uint32_t before = 0;
   auto count = [&](int from, int to, auto&& limit) {
+#pragma unroll 4
     for (int i = from; i < to; i += 4) {
       const u32x4 k = *reinterpret_cast<const u32x4*>(tile + i);
       before += k.x < limit(i);
@@ -393,6 +404,7 @@ __global__ __launch_bounds__(256) void embedding_chains_kernel(EmbSums a, const 
     const int64_t c = slab * kCols + lane * V, left = a.cols - c;
     const float* parts = a.parts + (begin / a.chunk + 1) * a.cols + c;
     float acc[V] = {};
+#pragma unroll 4
     for (int64_t i = group; i < a.chunk; i += kGroups) {
       Piece<D, V> p;
       load_piece<false>(dout + (int64_t)a.places[begin + i] * a.ldd + c, left, p);
@@ -553,7 +565,7 @@ extern "C" int mx_embedding_grad(const void* ids, int ids_i64, int64_t n, const 
       hipLaunchKernelGGL((embedding_sums_kernel<D, G>), dim3((unsigned)groups, (unsigned)slabs), dim3(threads), 0, st, a,
                          (const D*)dout, (G*)grad, p.chunks);
       if (n > p.chunk)  // (a chain is more than one piece)
-        hipLaunchKernelGGL((embedding_chains_kernel<D, G>), dim3(512), dim3(256), 0, st, a, (const D*)dout, (G*)grad);
+        hipLaunchKernelGGL((embedding_chains_kernel<D, G>), dim3(1280), dim3(256), 0, st, a, (const D*)dout, (G*)grad);
     });
   });
   return hipGetLastError() == hipSuccess ? MX_OK : MX_ERR_LAUNCH;

@@ -18,6 +18,7 @@ constexpr int kGradPieces = 8;                                   // 16-byte piec
 constexpr int64_t kGradChunk = 16 * kGradThreads * kGradPieces;  // bytes
 constexpr int kGradTensors = 160;                                // of one launch
 constexpr int kGradGroups = 2048;                                // workgroups of one launch
+constexpr int64_t kGradPartsMost = 2 * kGradGroups;              // parts that every workgroup joins for itself
 
 struct GradEntry {
   void* p;
@@ -98,14 +99,21 @@ __global__ __launch_bounds__(kGradThreads) void grad_norm_kernel(GradTable table
   if (threadIdx.x == 0) parts[blockIdx.x] = acc;
 }
 
+// The norm from its parts, in every lane of the workgroup.
+template <int KIND>
+__device__ __forceinline__ float grad_joined(const double* __restrict__ parts, int64_t n, double* part) {
+  double acc = 0.0;
+#pragma unroll 8
+  for (int64_t i = threadIdx.x; i < n; i += kGradThreads) acc = grad_join<KIND>(acc, parts[i]);
+  acc = grad_group_join<KIND>(acc, part);
+  return (float)(KIND == kGradTwo ? __builtin_sqrt(acc) : acc);
+}
 template <int KIND>
 __global__ __launch_bounds__(kGradThreads) void grad_norm_join_kernel(const double* __restrict__ parts, int64_t n,
                                                                       float* __restrict__ norm) {
   __shared__ double part[kGradThreads / 64];
-  double acc = 0.0;
-  for (int64_t i = threadIdx.x; i < n; i += kGradThreads) acc = grad_join<KIND>(acc, parts[i]);
-  acc = grad_group_join<KIND>(acc, part);
-  if (threadIdx.x == 0) *norm = (float)(KIND == kGradTwo ? __builtin_sqrt(acc) : acc);
+  const float all = grad_joined<KIND>(parts, n, part);
+  if (threadIdx.x == 0) *norm = all;
 }
 
 template <class T>
@@ -128,12 +136,29 @@ __device__ __forceinline__ void grad_scale_chunk(T* p, int64_t left, float f) {
   }
 }
 
-// A factor of exactly 1 leaves every gradient as it is: nothing is read.
-__global__ __launch_bounds__(kGradThreads) void grad_scale_kernel(GradTable table, int n, uint32_t chunks,
-                                                                  const float* __restrict__ norm, float limit) {
-  const float f0 = limit / (*norm + 1e-6f), f = f0 > 1.f ? 1.f : f0;  // (NaN stays)
+// f from the norm, or (count > 0) from its parts, joined here by every workgroup: one launch less.  A factor of exactly 1
+// leaves every gradient as it is: nothing is read.  Chunks are taken from the last to the first: what the norm has read
+// last is still in the last cache.
+struct GradFactor {
+  const double* parts;
+  int64_t count;
+  float* norm;  // read, or (count > 0) written
+  float limit;
+};
+template <int KIND>
+__global__ __launch_bounds__(kGradThreads) void grad_scale_kernel(GradTable table, int n, uint32_t chunks, GradFactor by) {
+  __shared__ double part[kGradThreads / 64];
+  float norm;
+  if (by.count > 0) {
+    norm = grad_joined<KIND>(by.parts, by.count, part);
+    if (blockIdx.x == 0 && threadIdx.x == 0) *by.norm = norm;
+  } else {
+    norm = *by.norm;
+  }
+  const float f0 = by.limit / (norm + 1e-6f), f = f0 > 1.f ? 1.f : f0;  // (NaN stays)
   if (f == 1.f) return;
-  for (uint32_t chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
+  for (uint32_t i = blockIdx.x; i < chunks; i += gridDim.x) {
+    const uint32_t chunk = chunks - 1 - i;
     const GradEntry e = table.e[grad_find(table, n, chunk)];
     const int64_t at = (int64_t)(chunk - e.first) * (kGradChunk / (e.f32 ? 4 : 2));
     if (e.f32) grad_scale_chunk((float*)e.p + at, e.elems - at, f);
@@ -214,24 +239,49 @@ extern "C" int64_t mx_grad_norm_workspace(int64_t n) {
   return n <= 0 ? 0 : 8 * kGradGroups * ((n + kGradTensors - 1) / kGradTensors);
 }
 
-extern "C" int mx_grad_norm(int64_t n, void* const* grads, const int64_t* elems, const int32_t* is_f32, int kind, float* norm,
-                            void* workspace, void* stream) {
+// The parts of the norm in `parts`, how many in `count`.
+template <int KIND>
+static int grad_parts(int64_t n, void* const* grads, const int64_t* elems, const int32_t* is_f32, double* parts, int64_t& count,
+                      hipStream_t st) {
+  count = 0;
+  return grad_launches(n, grads, elems, is_f32, kGradTensors, [&](const GradTable& t, int m, uint32_t chunks) {
+    const unsigned groups = grad_groups(chunks);
+    hipLaunchKernelGGL(grad_norm_kernel<KIND>, dim3(groups), dim3(kGradThreads), 0, st, t, m, chunks, parts + count);
+    count += groups;
+  });
+}
+
+template <int KIND>
+static int grad_joined_launch(const double* parts, int64_t count, float* norm, hipStream_t st) {
+  hipLaunchKernelGGL(grad_norm_join_kernel<KIND>, dim3(1), dim3(kGradThreads), 0, st, parts, count, norm);
+  return hipGetLastError() == hipSuccess ? MX_OK : MX_ERR_LAUNCH;
+}
+
+template <int KIND>
+static int grad_scaled(int64_t n, void* const* grads, const int64_t* elems, const int32_t* is_f32, const GradFactor& by,
+                       hipStream_t st) {
+  // tensors that share memory are scaled one after the other, as a loop over them would
+  const int most = grad_overlap(n, grads, elems, is_f32) ? 1 : kGradTensors;
+  return grad_launches(n, grads, elems, is_f32, most, [&](const GradTable& t, int m, uint32_t chunks) {
+    hipLaunchKernelGGL(grad_scale_kernel<KIND>, dim3(grad_groups(chunks)), dim3(kGradThreads), 0, st, t, m, chunks, by);
+  });
+}
+
+static int grad_norm_check(int64_t n, void* const* grads, const int64_t* elems, const int32_t* is_f32, int kind,
+                           const float* norm, const void* workspace) {
   if (const int rc = grad_check(n, grads, elems, is_f32)) return rc;
   if (kind < kGradTwo || kind > kGradMax || !norm || (n > 0 && !workspace)) return MX_ERR_INVALID_ARG;
-  if (((uintptr_t)norm & 3) || ((uintptr_t)workspace & 7)) return MX_ERR_ALIGNMENT;
-  hipStream_t st = (hipStream_t)stream;
-  double* parts = (double*)workspace;
-  int64_t used = 0;
+  return ((uintptr_t)norm & 3) || ((uintptr_t)workspace & 7) ? MX_ERR_ALIGNMENT : MX_OK;
+}
+
+extern "C" int mx_grad_norm(int64_t n, void* const* grads, const int64_t* elems, const int32_t* is_f32, int kind, float* norm,
+                            void* workspace, void* stream) {
+  if (const int rc = grad_norm_check(n, grads, elems, is_f32, kind, norm, workspace)) return rc;
   return grad_kind(kind, [&](auto k) {
     constexpr int K = decltype(k)::value;
-    const int rc = grad_launches(n, grads, elems, is_f32, kGradTensors, [&](const GradTable& t, int m, uint32_t chunks) {
-      const unsigned groups = grad_groups(chunks);
-      hipLaunchKernelGGL(grad_norm_kernel<K>, dim3(groups), dim3(kGradThreads), 0, st, t, m, chunks, parts + used);
-      used += groups;
-    });
-    if (rc) return rc;
-    hipLaunchKernelGGL(grad_norm_join_kernel<K>, dim3(1), dim3(kGradThreads), 0, st, parts, used, norm);
-    return hipGetLastError() == hipSuccess ? (int)MX_OK : (int)MX_ERR_LAUNCH;
+    int64_t count;
+    if (const int rc = grad_parts<K>(n, grads, elems, is_f32, (double*)workspace, count, (hipStream_t)stream)) return rc;
+    return grad_joined_launch<K>((const double*)workspace, count, norm, (hipStream_t)stream);
   });
 }
 
@@ -240,10 +290,24 @@ extern "C" int mx_grad_scale(int64_t n, void* const* grads, const int64_t* elems
   if (const int rc = grad_check(n, grads, elems, is_f32)) return rc;
   if (!norm) return MX_ERR_INVALID_ARG;
   if ((uintptr_t)norm & 3) return MX_ERR_ALIGNMENT;
-  // tensors that share memory are scaled one after the other, as a loop over them would
-  const int most = grad_overlap(n, grads, elems, is_f32) ? 1 : kGradTensors;
-  return grad_launches(n, grads, elems, is_f32, most, [&](const GradTable& t, int m, uint32_t chunks) {
-    hipLaunchKernelGGL(grad_scale_kernel, dim3(grad_groups(chunks)), dim3(kGradThreads), 0, (hipStream_t)stream, t, m, chunks,
-                       norm, limit);
+  return grad_scaled<kGradTwo>(n, grads, elems, is_f32, {nullptr, 0, const_cast<float*>(norm), limit}, (hipStream_t)stream);
+}
+
+extern "C" int mx_grad_clip(int64_t n, void* const* grads, const int64_t* elems, const int32_t* is_f32, int kind, float* norm,
+                            float limit, void* workspace, void* stream) {
+  if (const int rc = grad_norm_check(n, grads, elems, is_f32, kind, norm, workspace)) return rc;
+  hipStream_t st = (hipStream_t)stream;
+  return grad_kind(kind, [&](auto k) {
+    constexpr int K = decltype(k)::value;
+    const double* parts = (const double*)workspace;
+    int64_t count;
+    if (const int rc = grad_parts<K>(n, grads, elems, is_f32, (double*)workspace, count, st)) return rc;
+    // more parts than a few launches' worth are joined once, not by every workgroup of every launch (and with none,
+    // where all tensors are empty, nobody else writes the norm)
+    if (count == 0 || count > kGradPartsMost) {
+      if (const int rc = grad_joined_launch<K>(parts, count, norm, st)) return rc;
+      count = 0;
+    }
+    return grad_scaled<K>(n, grads, elems, is_f32, {parts, count, norm, limit}, st);
   });
 }

@@ -8,7 +8,7 @@ from __future__ import annotations
 
 import torch
 
-from . import ops
+from . import _lib, ops
 
 
 def _ours(grads, norm_type: float) -> bool:
@@ -63,6 +63,10 @@ def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_i
     ``torch.nn.utils.clip_grad_norm_``.  A caller whose gradients are spread over ranks adds up the powers of
     ``get_total_norm`` and calls ``clip_grads_with_norm_`` with the result."""
     parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
+    if parameters and norm_type in ops.GRAD_NORMS and not error_if_nonfinite and ops.native_rows(parameters[0]):
+        norm = _lib.blocks().clip_gradients(parameters, max_norm, ops.GRAD_NORMS[norm_type])
+        if norm is not None:
+            return norm
     total_norm = get_total_norm(_grads(parameters), norm_type, error_if_nonfinite, foreach)
     clip_grads_with_norm_(parameters, max_norm, total_norm, foreach)
     return total_norm

@@ -13,7 +13,7 @@ import torch
 import torch.nn as nn
 from torch.autograd.function import once_differentiable
 
-from .. import ops
+from .. import _lib, ops
 from ..protocols import Module
 
 
@@ -52,6 +52,11 @@ def scaled_embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0
     zeros and no gradient: the rows of a vocabulary shard add up over the shards.  Tokens whose id is
     `padding_idx` have their row, but no gradient.  weight: [rows, dim].  The gradient is dense, sums of equal ids in
     float32 in an order that depends on the ids alone; it cannot be differentiated again."""
+    if (dtype is None or dtype in ops.ROW_TYPES) and ops.native_rows(weight):
+        out = _lib.blocks().scaled_embedding(ids, weight, scale, padding_idx, first_row,
+                                             (dtype or weight.dtype) == torch.float32)
+        if out is not None:
+            return out
     if ids.dtype not in (torch.int64, torch.int32):
         raise TypeError(f"ids must be int64 or int32, got {ids.dtype}")
     if weight.dim() != 2 or not weight.is_floating_point():

@@ -18,7 +18,7 @@ import torch
 import torch.nn as nn
 from torch.autograd.function import once_differentiable
 
-from .. import ops
+from .. import _lib, ops
 from ..protocols import Module
 
 
@@ -81,6 +81,10 @@ def residual_rms_norm(h: torch.Tensor, residual: torch.Tensor, *, post_weight: t
     h: output of a block, residual: the stream around it, both [..., dim]; h may be bf16 where the stream is float32.
     post_weight, pre_weight: [dim].  gate: [dim], or with h's dimensions: its leading ones up to some point, ones
     behind it, dim ([batch, 1, dim]: a row for every sequence).  The gradients cannot be differentiated again."""
+    if ops.native_rows(h):
+        out = _lib.blocks().residual_rms_norm(h, residual, post_weight, gate, pre_weight, residual_scale, eps)
+        if out is not None:
+            return out
     dim = h.shape[-1] if h.dim() else 0
     if h.dim() == 0 or residual.shape != h.shape:
         raise ValueError(f"h and residual must have one shape with a last dimension, got {tuple(h.shape)} and {tuple(residual.shape)}")

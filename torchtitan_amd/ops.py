@@ -975,6 +975,12 @@ def swiglu_bwd_to_mx_dim0_dim1(dg: torch.Tensor, a: torch.Tensor, b: torch.Tenso
 ROW_TYPES = (torch.bfloat16, torch.float32)  # of the embedding, the norms around a block and the gradients
 
 
+def native_rows(t: torch.Tensor) -> bool:
+    """One call of the native module may do an operator on t whole, with its autograd node; it returns None for what it
+    does not take."""
+    return _single(t) and not _transformed()
+
+
 def plain_rows(*operands) -> bool:
     """The kernels below take these tensors (None among them: no operand): plain ones on the GPU, bf16 or float32,
     outside function transforms."""
