@@ -66,21 +66,27 @@ __global__ __launch_bounds__(kEmbThreads) void embedding_kernel(EmbIds ids, int6
 
 // ---- the order of the tokens by their rows, stable: up to kRankMost tokens in one launch, more by radix passes
 
-// A token's place is the number of tokens with a smaller row, or with its row and in front of it.  A workgroup places 64
-// tokens, one a lane; every wave counts over a sixteenth of all tokens, whose rows it reads from LDS four at a time.
-// Two instructions a pair: 2003 tokens XX us, 8192 XX us, where the radix passes take XX and XX.
-constexpr int kRankThreads = 1024, kRankMost = 8192;
+// A token's place is the number of tokens with a smaller row, or with its row and in front of it.  A workgroup places
+// kRankThreads / parts tokens: every one is held by `parts` lanes, which count over a share of all tokens each, four rows
+// a read of LDS.  Two instructions a pair; parts so that there is a workgroup for every CU.
+constexpr int kRankThreads = 1024, kRankMost = 8192, kRankKeys = kRankMost + 4 * kRankThreads / 8;
 
-__global__ __launch_bounds__(kRankThreads) void embedding_rank_kernel(EmbIds ids, int n, uint32_t* __restrict__ keys,
+// Tokens of a workgroup, and how many rows a lane compares with: an odd number of fours, so that the shares of lanes
+// next to each other begin in different banks.
+static int rank_tokens(int64_t n) { return n > 4096 ? 32 : n > 2048 ? 16 : 8; }
+__host__ __device__ inline int rank_share(int n, int parts) {
+  const int fours = (n + 4 * parts - 1) / (4 * parts);
+  return 4 * (fours | 1);
+}
+
+__global__ __launch_bounds__(kRankThreads) void embedding_rank_kernel(EmbIds ids, int n, int tokens, uint32_t* __restrict__ keys,
                                                                       uint32_t* __restrict__ places,
                                                                       uint32_t* __restrict__ chains) {
-  constexpr int kWaves = kRankThreads / 64;
-  __shared__ alignas(16) uint32_t tile[kRankMost];
-  __shared__ uint32_t counts[kWaves][64];
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const int t0 = (int)blockIdx.x * 64, t = t0 + lane;
+  __shared__ alignas(16) uint32_t tile[kRankKeys];
+  __shared__ uint32_t counts[kRankThreads];
+  const int parts = kRankThreads / tokens, share = rank_share(n, parts);
+  const int part = threadIdx.x / tokens, at = threadIdx.x % tokens, t0 = (int)blockIdx.x * tokens, t = t0 + at;
   if (blockIdx.x == 0 && threadIdx.x == 0) *chains = 0;
-  const int padded = (n + 4 * kWaves - 1) / (4 * kWaves) * (4 * kWaves);  // (at most kRankMost)
   uint32_t own[kRankMost / kRankThreads];  // (all asked for before the first is written)
 #pragma unroll
   for (int k = 0; k < kRankMost / kRankThreads; ++k) {
@@ -88,17 +94,15 @@ __global__ __launch_bounds__(kRankThreads) void embedding_rank_kernel(EmbIds ids
     own[k] = i < n ? ids.key(i) : 0xFFFFFFFFu;  // (in front of nobody)
   }
 #pragma unroll
-  for (int k = 0; k < kRankMost / kRankThreads; ++k) {
-    const int i = k * kRankThreads + threadIdx.x;
-    if (i < padded) tile[i] = own[k];
-  }
+  for (int k = 0; k < kRankMost / kRankThreads; ++k) tile[k * kRankThreads + threadIdx.x] = own[k];
+  for (int i = kRankMost + threadIdx.x; i < kRankKeys; i += kRankThreads) tile[i] = 0xFFFFFFFFu;
   __syncthreads();
   const uint32_t mine = t < n ? tile[t] : 0u;
-  const int each = padded / kWaves, lo = wave * each, hi = lo + each;
+  const int lo = part * share, hi = lo + share;
   uint32_t before = 0;
-  auto count = [&](int from, int to, auto&& limit) {
+  auto count = [&](auto&& limit) {
 #pragma unroll 4
-    for (int i = from; i < to; i += 4) {
+    for (int i = lo; i < hi; i += 4) {
       const u32x4 k = *reinterpret_cast<const u32x4*>(tile + i);
       before += k.x < limit(i);
       before += k.y < limit(i + 1);
@@ -106,18 +110,17 @@ __global__ __launch_bounds__(kRankThreads) void embedding_rank_kernel(EmbIds ids
       before += k.w < limit(i + 3);
     }
   };
-  // (a row equal to mine counts where its token is in front: known for all of a wave's tokens but its own 64)
-  if (hi <= t0) count(lo, hi, [&](int) { return mine + 1; });
-  else if (lo >= t0 + 64) count(lo, hi, [&](int) { return mine; });
-  else count(lo, hi, [&](int i) { return mine + (i < t ? 1u : 0u); });
-  counts[wave][lane] = before;
+  // (a row equal to mine counts where its token is in front: the same answer for all of a share but those around t)
+  if (hi <= t0) count([&](int) { return mine + 1; });
+  else if (lo >= t0 + tokens) count([&](int) { return mine; });
+  else count([&](int i) { return mine + (i < t ? 1u : 0u); });
+  counts[threadIdx.x] = before;
   __syncthreads();
-  if (wave == 0 && t < n) {
-    uint32_t at = 0;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) at += counts[w][lane];
-    keys[at] = mine;
-    places[at] = (uint32_t)t;
+  if (part == 0 && t < n) {
+    uint32_t to = 0;
+    for (int p = 0; p < parts; ++p) to += counts[p * tokens + at];
+    keys[to] = mine;
+    places[to] = (uint32_t)t;
   }
 }
 
@@ -264,7 +267,7 @@ struct EmbSums {
 };
 
 constexpr int kChunkMost = 64;
-constexpr int kZeroRows = 64;  // rows of the table whose zeros one workgroup writes
+constexpr int kZeroRows = 64;  // of the table whose zeros one workgroup writes
 
 // First place whose row is not below `key` (between lo and hi), by the whole wave: 64 probes a step.
 __device__ __forceinline__ int64_t wave_lower_bound(const uint32_t* __restrict__ keys, int64_t lo, int64_t hi, uint32_t key) {
@@ -291,7 +294,30 @@ __device__ __forceinline__ void store_row(G* to, int64_t left, const float* acc,
   else store_piece<false>(to, left, q);
 }
 
-// Workgroups [0, chunks): sums; behind them: zeros of the rows that no token has.  A lane holds 8 columns, blockIdx.y
+// Zeros of those of the piece's kZeroRows rows that no token has, in columns [c0, c0 + width), by the whole workgroup.
+template <class G>
+__device__ __forceinline__ void zero_rows(const EmbSums& a, int64_t piece, int64_t c0, int64_t width, G* __restrict__ grad) {
+  const int64_t first = piece * kZeroRows;
+  const int rows = (int)(a.rows - first < kZeroRows ? a.rows - first : kZeroRows), lane = threadIdx.x & 63;
+  // (every wave for itself: the first of the rows' tokens, and for every row whether it has one)
+  const int64_t lo = wave_lower_bound(a.keys, 0, a.n, (uint32_t)first);
+  const int64_t hi = wave_lower_bound(a.keys, lo, a.n, (uint32_t)(first + rows));
+  int64_t from = lo, to = hi;
+  while (from < to) {
+    const int64_t mid = (from + to) >> 1;
+    if (a.keys[mid] < (uint32_t)(first + lane)) from = mid + 1; else to = mid;
+  }
+  const uint64_t used = __ballot(from < hi && a.keys[from] == (uint32_t)(first + lane));
+  if (width > a.cols - c0) width = a.cols - c0;
+  const int each = (int)((width + 7) / 8);  // lanes of a row
+  const float zeros[8] = {};
+  for (int i = threadIdx.x; i < rows * each; i += blockDim.x) {
+    const int r = i / each, c = (i - r * each) * 8;
+    if (!(used >> r & 1)) store_row(grad + (first + r) * a.cols + c0 + c, width - c, zeros, 0.f, a.past);
+  }
+}
+
+// Workgroups [0, chunks): sums; behind them: zeros of the rows without tokens.  A lane holds 8 columns, blockIdx.y
 // says which of several slabs of blockDim.x * 8 columns; 8 tokens' pieces are asked for before the first is added.
 template <class D, class G>
 __global__ __launch_bounds__(256) void embedding_sums_kernel(EmbSums a, const D* __restrict__ dout, G* __restrict__ grad,
@@ -300,25 +326,7 @@ __global__ __launch_bounds__(256) void embedding_sums_kernel(EmbSums a, const D*
   __shared__ uint32_t keys[3 * kChunkMost + 2], places[2 * kChunkMost];
   const int64_t c = ((int64_t)blockIdx.y * blockDim.x + threadIdx.x) * V, left = a.cols - c;
   if (blockIdx.x >= chunks) {
-    const int64_t first = (int64_t)(blockIdx.x - chunks) * kZeroRows;
-    const int rows = (int)(a.rows - first < kZeroRows ? a.rows - first : kZeroRows), lane = threadIdx.x & 63;
-    // (every wave for itself: the first of its tokens, and for every row whether it has one)
-    const int64_t lo = wave_lower_bound(a.keys, 0, a.n, (uint32_t)first);
-    const int64_t hi = wave_lower_bound(a.keys, lo, a.n, (uint32_t)(first + rows));
-    int64_t from = lo, to = hi;
-    while (from < to) {
-      const int64_t mid = (from + to) >> 1;
-      if (a.keys[mid] < (uint32_t)(first + lane)) from = mid + 1; else to = mid;
-    }
-    const bool used = from < hi && a.keys[from] == (uint32_t)(first + lane);
-    uint64_t unused = ~__ballot(used);
-    if (rows < 64) unused &= (1ull << rows) - 1;
-    const float zeros[V] = {};
-    while (unused) {
-      const int r = __builtin_ctzll(unused);
-      unused &= unused - 1;
-      store_row(grad + (first + r) * a.cols + c, left, zeros, 0.f, a.past);
-    }
+    zero_rows(a, blockIdx.x - chunks, (int64_t)blockIdx.y * blockDim.x * V, blockDim.x * V, grad);
     return;
   }
   // The rows of the chunk's tokens, of `chunk` and one tokens in front of them and of `chunk` behind.
@@ -388,21 +396,20 @@ __global__ __launch_bounds__(256) void embedding_sums_kernel(EmbSums a, const D*
   }
 }
 
-// The chains: the tokens of their first piece and the sums of the others, dealt out in turn to 16 groups of 16 lanes of
-// 8 columns each, whose sums are added in order.
+// The chains: the tokens of their first piece and the sums of the others, dealt out in turn to 8 groups of 32 lanes of 8
+// columns each, whose sums are added in order.
+constexpr int kChainGroups = 2048;
+
 template <class D, class G>
 __global__ __launch_bounds__(256) void embedding_chains_kernel(EmbSums a, const D* __restrict__ dout, G* __restrict__ grad) {
-  constexpr int V = 8, kGroups = 16, kCols = 16 * V;
+  constexpr int V = 8, kLanes = 32, kGroups = 256 / kLanes, kCols = kLanes * V;
   __shared__ float sums[kGroups][kCols];
   const int64_t slabs = (a.cols + kCols - 1) / kCols, items = (int64_t)a.chains[0] * slabs;
-  const int group = threadIdx.x >> 4, lane = threadIdx.x & 15;
+  const int group = threadIdx.x / kLanes, lane = threadIdx.x % kLanes;
   for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
     const int64_t begin = a.chains[1 + item / slabs], slab = item % slabs;
-    const uint32_t k = a.keys[begin];
-    const int64_t end = wave_lower_bound(a.keys, begin + a.chunk, a.n, k + 1);
-    const int64_t all = a.chunk + (end - begin - 1) / a.chunk;  // tokens of the first piece, then pieces
     const int64_t c = slab * kCols + lane * V, left = a.cols - c;
-    const float* parts = a.parts + (begin / a.chunk + 1) * a.cols + c;
+    const uint32_t k = a.keys[begin];
     float acc[V] = {};
 #pragma unroll 4
     for (int64_t i = group; i < a.chunk; i += kGroups) {
@@ -413,8 +420,11 @@ __global__ __launch_bounds__(256) void embedding_chains_kernel(EmbSums a, const 
 #pragma unroll
       for (int e = 0; e < V; ++e) acc[e] += f[e];
     }
+    const int64_t end = wave_lower_bound(a.keys, begin + a.chunk, a.n, k + 1);
+    const int64_t pieces = (end - begin - 1) / a.chunk;  // behind the first
+    const float* parts = a.parts + (begin / a.chunk + 1) * a.cols + c;
 #pragma unroll 4
-    for (int64_t i = group; i < all - a.chunk; i += kGroups) {
+    for (int64_t i = group; i < pieces; i += kGroups) {
       Piece<float, V> p;
       load_piece<false>(parts + i * a.cols, left, p);
       float f[V];
@@ -538,8 +548,9 @@ extern "C" int mx_embedding_grad(const void* ids, int ids_i64, int64_t n, const 
   const EmbIds e{ids, ids_i64 != 0, first, rows, padding};
   int last = 0;  // which of the two lists holds the order
   if (n > 0 && p.passes == 0) {
-    hipLaunchKernelGGL(embedding_rank_kernel, dim3((unsigned)((n + 63) / 64)), dim3(kRankThreads), 0, st, e, (int)n,
-                       words(p.keys[0]), words(p.places[0]), chains);
+    const int tokens = rank_tokens(n);
+    hipLaunchKernelGGL(embedding_rank_kernel, dim3((unsigned)((n + tokens - 1) / tokens)), dim3(kRankThreads), 0, st, e, (int)n,
+                       tokens, words(p.keys[0]), words(p.places[0]), chains);
   }
   for (int pass = 0; pass < p.passes; ++pass) {
     EmbSource from{e, nullptr, nullptr};
@@ -565,7 +576,7 @@ extern "C" int mx_embedding_grad(const void* ids, int ids_i64, int64_t n, const 
       hipLaunchKernelGGL((embedding_sums_kernel<D, G>), dim3((unsigned)groups, (unsigned)slabs), dim3(threads), 0, st, a,
                          (const D*)dout, (G*)grad, p.chunks);
       if (n > p.chunk)  // (a chain is more than one piece)
-        hipLaunchKernelGGL((embedding_chains_kernel<D, G>), dim3(1280), dim3(256), 0, st, a, (const D*)dout, (G*)grad);
+        hipLaunchKernelGGL((embedding_chains_kernel<D, G>), dim3(kChainGroups), dim3(256), 0, st, a, (const D*)dout, (G*)grad);
     });
   });
   return hipGetLastError() == hipSuccess ? MX_OK : MX_ERR_LAUNCH;
