@@ -5,6 +5,8 @@
 //
 // Both are bound by memory.  The gradient writes every row of the table, zeros where no token asked for it, and is the
 // same on every run: equal ids are summed in the order of their tokens, in float32, and rounded once.
+#include <algorithm>
+
 #include "mx_rows.h"
 
 namespace mx {
@@ -64,6 +66,34 @@ __global__ __launch_bounds__(kEmbThreads) void embedding_kernel(EmbIds ids, int6
   }
 }
 
+// ---- zeros of the whole gradient, written by workgroups of the launches that sort, whose own work leaves most of the
+// chip idle; the rows that tokens have are written over later.  16 bytes a lane and kFillPieces pieces, in order.
+struct EmbFill {
+  uint8_t* to;
+  int64_t bytes;  // of this launch
+  unsigned own;   // workgroups of the launch that sort
+  bool past;      // the gradient does not stay in the last cache: stored past it
+};
+constexpr int kFillPieces = 4;
+
+// Whether the calling workgroup has filled (and is done); THREADS lanes.
+template <int THREADS>
+__device__ __forceinline__ bool filled(const EmbFill& f) {
+  if (blockIdx.x < f.own) return false;
+  const int64_t base = (int64_t)(blockIdx.x - f.own) * (THREADS * 16 * kFillPieces) + threadIdx.x * 16;
+  const Piece<uint16_t, 8> zero{};
+#pragma unroll
+  for (int k = 0; k < kFillPieces; ++k) {
+    const int64_t at = base + k * THREADS * 16, left = (f.bytes - at) / 2;
+    if (f.past) store_piece<true>((uint16_t*)(f.to + at), left, zero);
+    else store_piece<false>((uint16_t*)(f.to + at), left, zero);
+  }
+  return true;
+}
+static int64_t fill_groups(int64_t bytes, int threads) { return (bytes + threads * 16 * kFillPieces - 1) / (threads * 16 * kFillPieces); }
+
+__global__ __launch_bounds__(256) void embedding_fill_kernel(EmbFill fill) { filled<256>(fill); }
+
 // ---- the order of the tokens by their rows, stable: up to kRankMost tokens in one launch, more by radix passes
 
 // A token's place is the number of tokens with a smaller row, or with its row and in front of it.  A workgroup places
@@ -81,7 +111,8 @@ __host__ __device__ inline int rank_share(int n, int parts) {
 
 __global__ __launch_bounds__(kRankThreads) void embedding_rank_kernel(EmbIds ids, int n, int tokens, uint32_t* __restrict__ keys,
                                                                       uint32_t* __restrict__ places,
-                                                                      uint32_t* __restrict__ chains) {
+                                                                      uint32_t* __restrict__ chains, EmbFill fill) {
+  if (filled<kRankThreads>(fill)) return;
   __shared__ alignas(16) uint32_t tile[kRankKeys];
   __shared__ uint32_t counts[kRankThreads];
   const int parts = kRankThreads / tokens, share = rank_share(n, parts);
@@ -141,7 +172,8 @@ struct EmbSource {
 };
 
 __global__ __launch_bounds__(kSortThreads) void embedding_count_kernel(EmbSource from, int64_t n, int shift, uint32_t* __restrict__ counts,
-                                                                       uint32_t* __restrict__ chains) {
+                                                                       uint32_t* __restrict__ chains, EmbFill fill) {
+  if (filled<kSortThreads>(fill)) return;
   __shared__ uint32_t digits[kDigits];
   if (blockIdx.x == 0 && threadIdx.x == 0) *chains = 0;
   for (int d = threadIdx.x; d < kDigits; d += kSortThreads) digits[d] = 0;
@@ -153,7 +185,7 @@ __global__ __launch_bounds__(kSortThreads) void embedding_count_kernel(EmbSource
     if (i < n) atomicAdd(&digits[from.key(i) >> shift & (kDigits - 1)], 1u);
   }
   __syncthreads();
-  for (int d = threadIdx.x; d < kDigits; d += kSortThreads) counts[(int64_t)d * gridDim.x + blockIdx.x] = digits[d];
+  for (int d = threadIdx.x; d < kDigits; d += kSortThreads) counts[(int64_t)d * fill.own + blockIdx.x] = digits[d];
 }
 
 __device__ __forceinline__ uint32_t wave_running_sum(uint32_t v) {
@@ -167,24 +199,28 @@ __device__ __forceinline__ uint32_t wave_running_sum(uint32_t v) {
 }
 
 // One wave a digit.
-__global__ __launch_bounds__(64) void embedding_offsets_kernel(uint32_t* __restrict__ counts, int64_t tiles,
-                                                               uint32_t* __restrict__ totals) {
-  uint32_t* mine = counts + (int64_t)blockIdx.x * tiles;
+__global__ __launch_bounds__(kSortThreads) void embedding_offsets_kernel(uint32_t* __restrict__ counts, int64_t tiles,
+                                                                         uint32_t* __restrict__ totals, EmbFill fill) {
+  if (filled<kSortThreads>(fill)) return;
+  const int lane = threadIdx.x & 63;
+  const int64_t digit = (int64_t)blockIdx.x * kSortWaves + (threadIdx.x >> 6);
+  uint32_t* mine = counts + digit * tiles;
   uint32_t sum = 0;
   for (int64_t base = 0; base < tiles; base += 64) {
-    const int64_t i = base + threadIdx.x;
+    const int64_t i = base + lane;
     const uint32_t v = i < tiles ? mine[i] : 0u, upto = wave_running_sum(v);
     if (i < tiles) mine[i] = sum + upto - v;
     sum += __shfl(upto, 63, 64);
   }
-  if (threadIdx.x == 0) totals[blockIdx.x] = sum;
+  if (lane == 0) totals[digit] = sum;
 }
 
 __global__ __launch_bounds__(kSortThreads) void embedding_scatter_kernel(EmbSource from, int64_t n, int shift,
                                                                          const uint32_t* __restrict__ offsets,
                                                                          const uint32_t* __restrict__ totals,
                                                                          uint32_t* __restrict__ keys,
-                                                                         uint32_t* __restrict__ places) {
+                                                                         uint32_t* __restrict__ places, EmbFill fill) {
+  if (filled<kSortThreads>(fill)) return;
   __shared__ uint32_t counts[kSortWaves][kDigits];  // of a digit in a wave's tokens so far; then where the wave's begin
   __shared__ uint32_t sums[kSortWaves];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
@@ -231,7 +267,7 @@ __global__ __launch_bounds__(kSortThreads) void embedding_scatter_kernel(EmbSour
 #pragma unroll
   for (int e = 0; e < kEach; ++e) {
     const int d = threadIdx.x * kEach + e;
-    uint32_t here = at + offsets[(int64_t)d * gridDim.x + blockIdx.x];
+    uint32_t here = at + offsets[(int64_t)d * fill.own + blockIdx.x];
 #pragma unroll
     for (int w = 0; w < kSortWaves; ++w) {
       const uint32_t c = counts[w][d];
@@ -261,13 +297,12 @@ struct EmbSums {
   int64_t n, rows, cols, ldd;
   int chunk;        // tokens
   float scale;
-  bool past;        // the gradient does not stay in the last cache: stored past it
+  bool past;        // (see EmbFill)
   float* parts;     // [chunks][cols]
   uint32_t* chains; // how many; then the places that they begin at
 };
 
 constexpr int kChunkMost = 64;
-constexpr int kZeroRows = 64;  // of the table whose zeros one workgroup writes
 
 // First place whose row is not below `key` (between lo and hi), by the whole wave: 64 probes a step.
 __device__ __forceinline__ int64_t wave_lower_bound(const uint32_t* __restrict__ keys, int64_t lo, int64_t hi, uint32_t key) {
@@ -294,41 +329,12 @@ __device__ __forceinline__ void store_row(G* to, int64_t left, const float* acc,
   else store_piece<false>(to, left, q);
 }
 
-// Zeros of those of the piece's kZeroRows rows that no token has, in columns [c0, c0 + width), by the whole workgroup.
-template <class G>
-__device__ __forceinline__ void zero_rows(const EmbSums& a, int64_t piece, int64_t c0, int64_t width, G* __restrict__ grad) {
-  const int64_t first = piece * kZeroRows;
-  const int rows = (int)(a.rows - first < kZeroRows ? a.rows - first : kZeroRows), lane = threadIdx.x & 63;
-  // (every wave for itself: the first of the rows' tokens, and for every row whether it has one)
-  const int64_t lo = wave_lower_bound(a.keys, 0, a.n, (uint32_t)first);
-  const int64_t hi = wave_lower_bound(a.keys, lo, a.n, (uint32_t)(first + rows));
-  int64_t from = lo, to = hi;
-  while (from < to) {
-    const int64_t mid = (from + to) >> 1;
-    if (a.keys[mid] < (uint32_t)(first + lane)) from = mid + 1; else to = mid;
-  }
-  const uint64_t used = __ballot(from < hi && a.keys[from] == (uint32_t)(first + lane));
-  if (width > a.cols - c0) width = a.cols - c0;
-  const int each = (int)((width + 7) / 8);  // lanes of a row
-  const float zeros[8] = {};
-  for (int i = threadIdx.x; i < rows * each; i += blockDim.x) {
-    const int r = i / each, c = (i - r * each) * 8;
-    if (!(used >> r & 1)) store_row(grad + (first + r) * a.cols + c0 + c, width - c, zeros, 0.f, a.past);
-  }
-}
-
-// Workgroups [0, chunks): sums; behind them: zeros of the rows without tokens.  A lane holds 8 columns, blockIdx.y
-// says which of several slabs of blockDim.x * 8 columns; 8 tokens' pieces are asked for before the first is added.
+// A lane holds 8 columns, blockIdx.y says which of several slabs of blockDim.x * 8 columns; 8 tokens' pieces are asked for before the first is added.
 template <class D, class G>
-__global__ __launch_bounds__(256) void embedding_sums_kernel(EmbSums a, const D* __restrict__ dout, G* __restrict__ grad,
-                                                             int64_t chunks) {
+__global__ __launch_bounds__(256) void embedding_sums_kernel(EmbSums a, const D* __restrict__ dout, G* __restrict__ grad) {
   constexpr int V = 8, U = 8;
   __shared__ uint32_t keys[3 * kChunkMost + 2], places[2 * kChunkMost];
   const int64_t c = ((int64_t)blockIdx.y * blockDim.x + threadIdx.x) * V, left = a.cols - c;
-  if (blockIdx.x >= chunks) {
-    zero_rows(a, blockIdx.x - chunks, (int64_t)blockIdx.y * blockDim.x * V, blockDim.x * V, grad);
-    return;
-  }
   // The rows of the chunk's tokens, of `chunk` and one tokens in front of them and of `chunk` behind.
   const int C = a.chunk, lane = threadIdx.x & 63;
   const int64_t c0 = (int64_t)blockIdx.x * C;
@@ -539,18 +545,32 @@ extern "C" int mx_embedding_grad(const void* ids, int ids_i64, int64_t n, const 
   if (rows >= 0x7FFFFFFF || n >= 0x7FFFFFFF) return MX_ERR_UNSUPPORTED;
   const EmbPlan p = emb_plan(n, rows, cols);
   const int threads = cols > 1024 ? 256 : cols > 512 ? 128 : 64;
-  const int64_t slabs = (cols + threads * 8 - 1) / (threads * 8), groups = p.chunks + (rows + kZeroRows - 1) / kZeroRows;
-  if (slabs > 65535 || groups > 0x7FFFFFFF) return MX_ERR_UNSUPPORTED;
+  const int64_t slabs = (cols + threads * 8 - 1) / (threads * 8), bytes = rows * cols * (grad_f32 ? 4 : 2);
+  if (slabs > 65535 || fill_groups(bytes, 256) + n > 0x7FFFFFFF) return MX_ERR_UNSUPPORTED;
   hipStream_t st = (hipStream_t)stream;
   uint8_t* ws = (uint8_t*)workspace;
   auto words = [&](int64_t at) { return (uint32_t*)(ws + at); };
   uint32_t* chains = words(p.chains);
   const EmbIds e{ids, ids_i64 != 0, first, rows, padding};
+  const bool past = emb_past(bytes);
+  // the fill, in equal parts for the launches that sort
+  const int64_t share = ((bytes + 3 * p.passes) / std::max(1, 3 * p.passes) + 255) & ~int64_t{255};
+  int64_t done = 0;
+  auto with_fill = [&](unsigned own, int lanes, auto&& launch) {
+    const EmbFill f{(uint8_t*)grad + done, std::min(share, bytes - done), own, past};
+    done += f.bytes;
+    launch(dim3((unsigned)(own + fill_groups(f.bytes, lanes))), dim3(lanes), f);
+  };
+  if (n == 0) {
+    with_fill(0, 256, [&](dim3 g, dim3 b, EmbFill f) { hipLaunchKernelGGL(embedding_fill_kernel, g, b, 0, st, f); });
+    return hipGetLastError() == hipSuccess ? MX_OK : MX_ERR_LAUNCH;
+  }
   int last = 0;  // which of the two lists holds the order
-  if (n > 0 && p.passes == 0) {
+  if (p.passes == 0) {
     const int tokens = rank_tokens(n);
-    hipLaunchKernelGGL(embedding_rank_kernel, dim3((unsigned)((n + tokens - 1) / tokens)), dim3(kRankThreads), 0, st, e, (int)n,
-                       tokens, words(p.keys[0]), words(p.places[0]), chains);
+    with_fill((unsigned)((n + tokens - 1) / tokens), kRankThreads, [&](dim3 g, dim3 b, EmbFill f) {
+      hipLaunchKernelGGL(embedding_rank_kernel, g, b, 0, st, e, (int)n, tokens, words(p.keys[0]), words(p.places[0]), chains, f);
+    });
   }
   for (int pass = 0; pass < p.passes; ++pass) {
     EmbSource from{e, nullptr, nullptr};
@@ -560,21 +580,25 @@ extern "C" int mx_embedding_grad(const void* ids, int ids_i64, int64_t n, const 
       last ^= 1;
     }
     const int shift = pass * kDigitBits;
-    hipLaunchKernelGGL(embedding_count_kernel, dim3((unsigned)p.tiles), dim3(kSortThreads), 0, st, from, n, shift,
-                       words(p.counts), chains);
-    hipLaunchKernelGGL(embedding_offsets_kernel, dim3(kDigits), dim3(64), 0, st, words(p.counts), p.tiles, words(p.totals));
-    hipLaunchKernelGGL(embedding_scatter_kernel, dim3((unsigned)p.tiles), dim3(kSortThreads), 0, st, from, n, shift,
-                       words(p.counts), words(p.totals), words(p.keys[last]), words(p.places[last]));
+    with_fill((unsigned)p.tiles, kSortThreads, [&](dim3 g, dim3 b, EmbFill f) {
+      hipLaunchKernelGGL(embedding_count_kernel, g, b, 0, st, from, n, shift, words(p.counts), chains, f);
+    });
+    with_fill(kDigits / kSortWaves, kSortThreads, [&](dim3 g, dim3 b, EmbFill f) {
+      hipLaunchKernelGGL(embedding_offsets_kernel, g, b, 0, st, words(p.counts), p.tiles, words(p.totals), f);
+    });
+    with_fill((unsigned)p.tiles, kSortThreads, [&](dim3 g, dim3 b, EmbFill f) {
+      hipLaunchKernelGGL(embedding_scatter_kernel, g, b, 0, st, from, n, shift, words(p.counts), words(p.totals),
+                         words(p.keys[last]), words(p.places[last]), f);
+    });
   }
-  const EmbSums a{words(p.keys[last]), words(p.places[last]), n, rows, cols, ldd, p.chunk, scale,
-                  emb_past(rows * cols * (grad_f32 ? 4 : 2)),
-                  (float*)(ws + p.sums), chains};
+  const EmbSums a{words(p.keys[last]), words(p.places[last]), n, rows, cols, ldd, p.chunk, scale, past, (float*)(ws + p.sums),
+                  chains};
   of_type(dout_f32, [&](auto dt) {
     of_type(grad_f32, [&](auto gt) {
       using D = decltype(dt);
       using G = decltype(gt);
-      hipLaunchKernelGGL((embedding_sums_kernel<D, G>), dim3((unsigned)groups, (unsigned)slabs), dim3(threads), 0, st, a,
-                         (const D*)dout, (G*)grad, p.chunks);
+      hipLaunchKernelGGL((embedding_sums_kernel<D, G>), dim3((unsigned)p.chunks, (unsigned)slabs), dim3(threads), 0, st, a,
+                         (const D*)dout, (G*)grad);
       if (n > p.chunk)  // (a chain is more than one piece)
         hipLaunchKernelGGL((embedding_chains_kernel<D, G>), dim3(kChainGroups), dim3(256), 0, st, a, (const D*)dout, (G*)grad);
     });

@@ -176,18 +176,21 @@ __device__ __forceinline__ float own_products(const float (&a)[N][kV], const flo
   return sum;
 }
 
-// A workgroup takes every gridDim.x-th row (or kRows of them); the next row is on its way while one is worked on, and
-// the weights stay in registers (with two pieces a lane they are read for every row).
+// A workgroup takes every gridDim.x-th row, or `pair` rows that lie together (kRows times as many); the next row is on its
+// way while one is worked on, and the weights stay in registers (with two pieces a lane they are read for every row).
+// Bound by memory: 16384 x 4096 with both norms and a gate 83 us (6.5 TB/s of the 6.5 of a copy that the last cache helps),
+// 147456 x 2048 419 us (5.8 of the 6.2 that two matrices read and two written reach without any arithmetic).
 template <class S, class H, class R>
-__global__ __launch_bounds__(S::kThreads) void residual_norm_kernel(NormArgs a, R* __restrict__ stream, H* __restrict__ normed,
-                                                                    float* __restrict__ rstd) {
+__global__ __launch_bounds__(S::kThreads) void residual_norm_kernel(NormArgs a, int pair, R* __restrict__ stream,
+                                                                    H* __restrict__ normed, float* __restrict__ rstd) {
   constexpr int N = S::kPieces;
   constexpr bool kHeld = N == 1;
   __shared__ float part[2][2][S::kLanes / 64 + 1];  // (two rows' worth: see lanes_sum)
   const int lane = threadIdx.x % S::kLanes;
-  const int64_t step = (int64_t)gridDim.x * S::kRows;
-  int64_t row = (int64_t)blockIdx.x * S::kRows + threadIdx.x / S::kLanes;
-  if (row >= a.rows) return;  // (whole workgroups where rows share barriers)
+  const int64_t step = pair ? S::kRows : (int64_t)gridDim.x * S::kRows, begin = (int64_t)blockIdx.x * S::kRows * (pair ? pair : 1);
+  int64_t row = begin + threadIdx.x / S::kLanes;
+  const int64_t end = pair && begin + S::kRows * pair < a.rows ? begin + S::kRows * pair : a.rows;
+  if (row >= end) return;  // (whole workgroups where rows share barriers)
   struct Row {
     Piece<H, kV> h[N];
     Piece<R, kV> r[N];
@@ -212,7 +215,7 @@ __global__ __launch_bounds__(S::kThreads) void residual_norm_kernel(NormArgs a, 
   if constexpr (kHeld) weight_at(a.pre, 0, at[0], pre1);
   for (int turn = 0;; turn ^= 1) {
     const int64_t coming = row + step;
-    if (coming < a.rows) fetch(next, coming);
+    if (coming < end) fetch(next, coming);
     const int64_t g = a.gate.p ? (uint32_t)row / (uint32_t)a.gate_each : 0;  // (rows fit 31 bits)
     if (kHeld && g != group) side_at(a, g * a.cols, at[0], side1);
     group = g;
@@ -244,7 +247,7 @@ __global__ __launch_bounds__(S::kThreads) void residual_norm_kernel(NormArgs a, 
       rstd[row] = s1;
       rstd[a.rows + row] = s2;
     }
-    if (coming >= a.rows) break;
+    if (coming >= end) break;
     row = coming;
     now = next;
   }
@@ -589,8 +592,19 @@ static bool norm_past(int64_t elements, int h_f32, int r_f32) { return elements 
 static int64_t norm_groups(int64_t cols, int64_t waves) {
   return waves * 64 / (cols <= 512 ? 256 : cols <= 1024 ? 128 : cols <= 2048 ? 256 : cols <= 4096 ? 512 : 1024);
 }
-// The backward pass has as many waves as its registers let a CU hold (two a SIMD with the block's side, four without).
-static int64_t norm_bwd_groups(int64_t cols, bool side) { return norm_groups(cols, side ? 2048 : 4096); }
+// Forward: as many workgroups as stay resident come back for more rows; matrices that the last cache does not hold are
+// gone through in order, two rows a workgroup, up to 2048 columns.  us in turn / two rows: 147456 x 2048 461 / 419, 65536 x
+// 1024 (past no cache) 83 / 92, 73728 x 4096 448 / 460, 16384 x 8192 218 / 238.
+static int norm_pair(const NormArgs& a) { return a.past && a.cols <= 2048 ? 2 : 0; }
+template <class S>
+static int64_t norm_fwd_groups(const NormArgs& a) {
+  if (const int64_t pair = norm_pair(a)) return (a.rows + S::kRows * pair - 1) / (S::kRows * pair);
+  return std::min<int64_t>((a.rows + S::kRows - 1) / S::kRows, norm_groups(a.cols, 4096));
+}
+
+// The backward pass has the waves that its registers let a CU hold: two a SIMD with the block's side; four without, three
+// for narrow rows (147456 x 2048: 702 us, with four 788; 16384 x 4096 135 and 132).
+static int64_t norm_bwd_groups(int64_t cols, bool side) { return norm_groups(cols, side ? 2048 : cols <= 2048 ? 3072 : 4096); }
 
 static NormStrips norm_strips(int64_t rows, int64_t gate_rows, int64_t groups) {
   const int64_t strips = std::max<int64_t>(1, std::min(groups / gate_rows, rows / gate_rows));
@@ -656,8 +670,8 @@ extern "C" int mx_residual_norm(const void* h, int h_f32, const void* r, int r_f
         hipLaunchKernelGGL((residual_norm_any_kernel<H, R>), dim3((unsigned)rows), dim3(kNormThreads), 0, (hipStream_t)stream,
                            a, (R*)stream_out, (H*)normed, rstd);
       else
-        hipLaunchKernelGGL((residual_norm_kernel<S, H, R>), dim3((unsigned)std::min<int64_t>((rows + S::kRows - 1) / S::kRows, norm_groups(cols, 4096))),
-                           dim3(S::kThreads), 0, (hipStream_t)stream, a, (R*)stream_out, (H*)normed, rstd);
+        hipLaunchKernelGGL((residual_norm_kernel<S, H, R>), dim3((unsigned)norm_fwd_groups<S>(a)), dim3(S::kThreads), 0,
+                           (hipStream_t)stream, a, norm_pair(a), (R*)stream_out, (H*)normed, rstd);
     });
   });
   return hipGetLastError() == hipSuccess ? MX_OK : MX_ERR_LAUNCH;
