@@ -209,6 +209,21 @@ def test_rows_of_zeros_and_what_is_not_finite(device):
     assert dh[[0, 1, 4, 5]].isfinite().all() and dr[[0, 1, 4, 5]].isfinite().all()
 
 
+@pytest.mark.parametrize("cols", [9, 20, 131, 250, 1030, 4099, 9001, 16390])
+@pytest.mark.parametrize("from_end", [0, 3, 7, 8])
+def test_an_infinity_leaves_the_rest_of_its_row_as_the_formula_does(device, cols, from_end):
+    """An infinite element makes its row's norm infinite: the others are 0 behind the norm, itself NaN."""
+    h, r, post, _, pre = make(device, 3, cols, (True, False, True))
+    at = cols - 1 - from_end
+    h[1, at] = float("inf")
+    stream, _ = residual_rms_norm(h, r, post_weight=post)
+    _, normed = residual_rms_norm(h, r, pre_weight=pre)
+    others = torch.arange(cols, device=device) != at
+    assert torch.equal(stream[1, others], r[1, others]) and stream[1, at].isnan()
+    assert not normed[1, others].any() and normed[1, at].isnan()
+    assert stream[[0, 2]].isfinite().all() and normed[[0, 2]].isfinite().all()
+
+
 def test_only_some_gradients_are_wanted(device):
     operands = make(device, 7, 768, (True, True, True))
     every = [t.clone().requires_grad_(True) for t in operands]

@@ -178,7 +178,8 @@ static int grad_check(int64_t n, void* const* p, const int64_t* elems, const int
   for (int64_t i = 0; i < n; ++i) {
     if (elems[i] < 0 || (elems[i] > 0 && !p[i])) return MX_ERR_INVALID_ARG;
     if ((uintptr_t)p[i] & (is_f32[i] ? 3 : 1)) return MX_ERR_ALIGNMENT;
-    if ((chunks += grad_chunks(elems[i], is_f32[i])) > 0x7FFFFFFF) return MX_ERR_UNSUPPORTED;
+    // (a workgroup each, and a launch has fewer than 2^32 lanes: 256 GB)
+    if ((chunks += grad_chunks(elems[i], is_f32[i])) > 0xFFFFFF) return MX_ERR_UNSUPPORTED;
   }
   return MX_OK;
 }

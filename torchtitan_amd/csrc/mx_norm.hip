@@ -166,7 +166,8 @@ __device__ __forceinline__ float own_products(const float (&a)[N][kV], const flo
 #pragma unroll
     for (int k = 0; k < N; ++k)
 #pragma unroll
-      for (int e = 0; e < kV; ++e) sum = __builtin_fmaf(a[k][e], e >= at[k].skip ? b[k][e] : 0.f, sum);
+      for (int e = 0; e < kV; ++e)  // (the product is left out, not made zero: infinity times 0 is no zero)
+        sum = e >= at[k].skip ? __builtin_fmaf(a[k][e], b[k][e], sum) : sum;
   } else {
 #pragma unroll
     for (int k = 0; k < N; ++k)
@@ -588,9 +589,9 @@ __global__ __launch_bounds__(kNormThreads) void residual_norm_join_kernel(NormJo
 // 212 + 339; 147456 x 2048 424 + 663 / 445 + 704.
 static bool norm_past(int64_t elements, int h_f32, int r_f32) { return elements * (2 * (2 + !!h_f32 + !!r_f32)) > (384 << 20); }
 
-// Workgroups: `waves` in all.
-static int64_t norm_groups(int64_t cols, int64_t waves) {
-  return waves * 64 / (cols <= 512 ? 256 : cols <= 1024 ? 128 : cols <= 2048 ? 256 : cols <= 4096 ? 512 : 1024);
+// Workgroups of `waves` waves for every CU.
+static int64_t norm_groups(int64_t cols, int waves) {
+  return 256 * 64 * waves / (cols <= 512 ? 256 : cols <= 1024 ? 128 : cols <= 2048 ? 256 : cols <= 4096 ? 512 : 1024);
 }
 // Forward: as many workgroups as stay resident come back for more rows; matrices that the last cache does not hold are
 // gone through in order, two rows a workgroup, up to 2048 columns.  us in turn / two rows: 147456 x 2048 461 / 419, 65536 x
@@ -599,12 +600,12 @@ static int norm_pair(const NormArgs& a) { return a.past && a.cols <= 2048 ? 2 : 
 template <class S>
 static int64_t norm_fwd_groups(const NormArgs& a) {
   if (const int64_t pair = norm_pair(a)) return (a.rows + S::kRows * pair - 1) / (S::kRows * pair);
-  return std::min<int64_t>((a.rows + S::kRows - 1) / S::kRows, norm_groups(a.cols, 4096));
+  return std::min<int64_t>((a.rows + S::kRows - 1) / S::kRows, norm_groups(a.cols, 16));
 }
 
 // The backward pass has the waves that its registers let a CU hold: two a SIMD with the block's side; four without, three
 // for narrow rows (147456 x 2048: 702 us, with four 788; 16384 x 4096 135 and 132).
-static int64_t norm_bwd_groups(int64_t cols, bool side) { return norm_groups(cols, side ? 2048 : cols <= 2048 ? 3072 : 4096); }
+static int64_t norm_bwd_groups(int64_t cols, bool side) { return norm_groups(cols, side ? 8 : cols <= 2048 ? 12 : 16); }
 
 static NormStrips norm_strips(int64_t rows, int64_t gate_rows, int64_t groups) {
   const int64_t strips = std::max<int64_t>(1, std::min(groups / gate_rows, rows / gate_rows));
@@ -642,7 +643,9 @@ static int norm_check(const void* h, int h_f32, const void* r, int r_f32, int64_
   auto odd = [](const void* p, int f32) { return ((uintptr_t)p & (f32 ? 3 : 1)) != 0; };
   if (odd(h, h_f32) || odd(r, r_f32) || odd(post, weights_f32 & 1) || odd(gate, weights_f32 & 2) || odd(pre, weights_f32 & 4))
     return MX_ERR_ALIGNMENT;
-  if (rows > 0x7FFFFFFF || cols > 0x7FFFFFFF) return MX_ERR_UNSUPPORTED;
+  // (a launch has fewer than 2^32 lanes: rows with a workgroup each)
+  const bool any = cols < kV || cols > NormShape<1024, 2>::kCols;
+  if (rows > (any ? 0xFFFFFF : 0x7FFFFFFF) || cols > 0x7FFFFFFF) return MX_ERR_UNSUPPORTED;
   return MX_OK;
 }
 
