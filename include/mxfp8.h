@@ -360,7 +360,8 @@ int mx_token_logprob_bwd_any(const void* logits, int64_t rows, int64_t vocab, in
  * padding; an id outside the table: no padding), every row written, zeros where there is no such t; dout [n, cols]
  * (row stride ldd), grad [rows, cols] dense.  Sums are float32, in the order of t within parts that depend on the ids
  * alone: the same bits on every run.  workspace: mx_embedding_grad_workspace bytes, 16-byte aligned.
- * Element-aligned tensors; any cols; n and rows below 2^31 - 1, else MX_ERR_UNSUPPORTED. */
+ * Element-aligned tensors; any cols; rows below 2^31 - 1, n up to 2^26 - 4 (forward) and 2^29 (gradient), and
+ * a gradient's rows of ceil(bytes / 16) pieces each fewer than 15 * 2^28 pieces in all, else MX_ERR_UNSUPPORTED. */
 int mx_embedding(const void* ids, int ids_i64, int64_t n, const void* weight, int weight_f32, int64_t rows, int64_t cols,
                  int64_t ldw, int64_t first, float scale, void* out, int out_f32, void* stream);
 int64_t mx_embedding_grad_workspace(int64_t n, int64_t rows, int64_t cols);

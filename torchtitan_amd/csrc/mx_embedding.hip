@@ -3,8 +3,10 @@
 //   out[t, :]  = scale * W[id(t) - first, :]                  (zeros where that row is not in the table)
 //   dW[v, :]   = scale * sum over t with id(t) - first = v, id(t) != padding, of dout[t, :]
 //
-// Both are bound by memory.  The gradient writes every row of the table, zeros where no token asked for it, and is the
-// same on every run: equal ids are summed in the order of their tokens, in float32, and rounded once.
+// Both are bound by memory.  The gradient writes every row of the table, zeros where no token asked for it: the tokens
+// are put in order by their rows, and every run of equal rows is summed in float32 and rounded once.  Which sums are
+// formed of a row depends on its own tokens and the number of all tokens alone, so the gradient is the same on every
+// run, and that of a part of the table the same as those rows of the whole's.
 #include <algorithm>
 
 #include "mx_rows.h"
@@ -13,6 +15,7 @@ namespace mx {
 
 constexpr int kEmbThreads = 256;
 constexpr int kEmbWaves = kEmbThreads / 64;
+constexpr int64_t kEmbGroups = 0xFFFFFF;  // workgroups of at most 256 lanes: a launch has fewer than 2^32 lanes
 
 struct EmbIds {
   const void* ids;
@@ -66,39 +69,60 @@ __global__ __launch_bounds__(kEmbThreads) void embedding_kernel(EmbIds ids, int6
   }
 }
 
-// ---- zeros of the whole gradient, written by workgroups of the launches that sort, whose own work leaves most of the
-// chip idle; the rows that tokens have are written over later.  16 bytes a lane and kFillPieces pieces, in order.
-struct EmbFill {
-  uint8_t* to;
-  int64_t bytes;  // of this launch
-  unsigned own;   // workgroups of the launch that sort
-  bool past;      // the gradient does not stay in the last cache: stored past it
+// ---- work that rides along in the launches that sort, whose own work leaves most of the chip idle: workgroups behind the
+// first `own` write zeros, 16 bytes a lane, in the order of memory (6.3 TB/s; workgroups that each go through a part of
+// their own reach 5.2).  Either all of a piece of memory (rows that tokens have are written over
+// later), or the rows of the gradient that no token has, by the flags that an earlier launch has set.
+enum { kRideFill = 0, kRideMark = 1, kRideUnused = 2 };
+struct EmbRide {
+  int mode;
+  unsigned own;    // workgroups of the launch's own work
+  uint8_t* to;     // memory to fill, the flags to set, or the gradient
+  int64_t count;   // bytes, tokens, or 16-byte pieces of rows from piece `from` on
+  bool past;       // the gradient does not stay in the last cache: stored past it
+  EmbIds ids;
+  const uint8_t* used;  // a flag a row
+  int64_t from, row_bytes;
 };
-constexpr int kFillPieces = 4;
 
-// Whether the calling workgroup has filled (and is done); THREADS lanes.
-template <int THREADS>
-__device__ __forceinline__ bool filled(const EmbFill& f) {
-  if (blockIdx.x < f.own) return false;
-  const int64_t base = (int64_t)(blockIdx.x - f.own) * (THREADS * 16 * kFillPieces) + threadIdx.x * 16;
+__device__ __forceinline__ void store_zeros(uint8_t* to, int64_t bytes, bool past) {
   const Piece<uint16_t, 8> zero{};
-#pragma unroll
-  for (int k = 0; k < kFillPieces; ++k) {
-    const int64_t at = base + k * THREADS * 16, left = (f.bytes - at) / 2;
-    if (f.past) store_piece<true>((uint16_t*)(f.to + at), left, zero);
-    else store_piece<false>((uint16_t*)(f.to + at), left, zero);
+  if (past) store_piece<true>((uint16_t*)to, bytes / 2, zero);
+  else store_piece<false>((uint16_t*)to, bytes / 2, zero);
+}
+
+// Whether the calling workgroup of THREADS lanes has ridden along (and is done).
+template <int THREADS>
+__device__ __forceinline__ bool rode(const EmbRide& q) {
+  if (blockIdx.x < q.own) return false;
+  const int64_t base = (int64_t)(blockIdx.x - q.own) * THREADS, i = base + threadIdx.x;
+  if (q.mode == kRideFill) {
+    store_zeros(q.to + i * 16, q.count - i * 16, q.past);
+  } else if (i < q.count) {
+    if (q.mode == kRideMark) {
+      const uint32_t r = q.ids.key(i);
+      if (r < (uint32_t)q.ids.rows) q.to[r] = 1;  // (whoever sets a flag sets it to 1)
+    } else {
+      // one division of long numbers a workgroup, a short one for its lanes
+      const uint32_t each = (uint32_t)((q.row_bytes + 15) / 16);
+      const int64_t row0 = (q.from + base) / each;
+      const uint32_t piece = (uint32_t)(q.from + base - row0 * each) + threadIdx.x, r = piece / each;
+      const int64_t c = (int64_t)(piece - r * each) * 16;
+      if (!q.used[row0 + r]) store_zeros(q.to + (row0 + r) * q.row_bytes + c, q.row_bytes - c, q.past);
+    }
   }
   return true;
 }
-static int64_t fill_groups(int64_t bytes, int threads) { return (bytes + threads * 16 * kFillPieces - 1) / (threads * 16 * kFillPieces); }
+static int64_t ride_groups(int64_t pieces, int threads) { return (pieces + threads - 1) / threads; }
 
-__global__ __launch_bounds__(256) void embedding_fill_kernel(EmbFill fill) { filled<256>(fill); }
+__global__ __launch_bounds__(256) void embedding_zeros_kernel(EmbRide ride) { rode<256>(ride); }
 
 // ---- the order of the tokens by their rows, stable: up to kRankMost tokens in one launch, more by radix passes
 
 // A token's place is the number of tokens with a smaller row, or with its row and in front of it.  A workgroup places
 // kRankThreads / parts tokens: every one is held by `parts` lanes, which count over a share of all tokens each, four rows
-// a read of LDS.  Two instructions a pair; parts so that there is a workgroup for every CU.
+// a read of LDS.  Two instructions a pair; parts so that there is a workgroup for every CU: 2003 tokens 5.9 us, 8192 16.6,
+// where two radix passes take 33.
 constexpr int kRankThreads = 1024, kRankMost = 8192, kRankKeys = kRankMost + 4 * kRankThreads / 8;
 
 // Tokens of a workgroup, and how many rows a lane compares with: an odd number of fours, so that the shares of lanes
@@ -111,8 +135,8 @@ __host__ __device__ inline int rank_share(int n, int parts) {
 
 __global__ __launch_bounds__(kRankThreads) void embedding_rank_kernel(EmbIds ids, int n, int tokens, uint32_t* __restrict__ keys,
                                                                       uint32_t* __restrict__ places,
-                                                                      uint32_t* __restrict__ chains, EmbFill fill) {
-  if (filled<kRankThreads>(fill)) return;
+                                                                      uint32_t* __restrict__ chains, EmbRide ride) {
+  if (rode<kRankThreads>(ride)) return;
   __shared__ alignas(16) uint32_t tile[kRankKeys];
   __shared__ uint32_t counts[kRankThreads];
   const int parts = kRankThreads / tokens, share = rank_share(n, parts);
@@ -172,8 +196,8 @@ struct EmbSource {
 };
 
 __global__ __launch_bounds__(kSortThreads) void embedding_count_kernel(EmbSource from, int64_t n, int shift, uint32_t* __restrict__ counts,
-                                                                       uint32_t* __restrict__ chains, EmbFill fill) {
-  if (filled<kSortThreads>(fill)) return;
+                                                                       uint32_t* __restrict__ chains, EmbRide ride) {
+  if (rode<kSortThreads>(ride)) return;
   __shared__ uint32_t digits[kDigits];
   if (blockIdx.x == 0 && threadIdx.x == 0) *chains = 0;
   for (int d = threadIdx.x; d < kDigits; d += kSortThreads) digits[d] = 0;
@@ -185,7 +209,7 @@ __global__ __launch_bounds__(kSortThreads) void embedding_count_kernel(EmbSource
     if (i < n) atomicAdd(&digits[from.key(i) >> shift & (kDigits - 1)], 1u);
   }
   __syncthreads();
-  for (int d = threadIdx.x; d < kDigits; d += kSortThreads) counts[(int64_t)d * fill.own + blockIdx.x] = digits[d];
+  for (int d = threadIdx.x; d < kDigits; d += kSortThreads) counts[(int64_t)d * ride.own + blockIdx.x] = digits[d];
 }
 
 __device__ __forceinline__ uint32_t wave_running_sum(uint32_t v) {
@@ -200,8 +224,8 @@ __device__ __forceinline__ uint32_t wave_running_sum(uint32_t v) {
 
 // One wave a digit.
 __global__ __launch_bounds__(kSortThreads) void embedding_offsets_kernel(uint32_t* __restrict__ counts, int64_t tiles,
-                                                                         uint32_t* __restrict__ totals, EmbFill fill) {
-  if (filled<kSortThreads>(fill)) return;
+                                                                         uint32_t* __restrict__ totals, EmbRide ride) {
+  if (rode<kSortThreads>(ride)) return;
   const int lane = threadIdx.x & 63;
   const int64_t digit = (int64_t)blockIdx.x * kSortWaves + (threadIdx.x >> 6);
   uint32_t* mine = counts + digit * tiles;
@@ -219,8 +243,8 @@ __global__ __launch_bounds__(kSortThreads) void embedding_scatter_kernel(EmbSour
                                                                          const uint32_t* __restrict__ offsets,
                                                                          const uint32_t* __restrict__ totals,
                                                                          uint32_t* __restrict__ keys,
-                                                                         uint32_t* __restrict__ places, EmbFill fill) {
-  if (filled<kSortThreads>(fill)) return;
+                                                                         uint32_t* __restrict__ places, EmbRide ride) {
+  if (rode<kSortThreads>(ride)) return;
   __shared__ uint32_t counts[kSortWaves][kDigits];  // of a digit in a wave's tokens so far; then where the wave's begin
   __shared__ uint32_t sums[kSortWaves];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
@@ -267,7 +291,7 @@ __global__ __launch_bounds__(kSortThreads) void embedding_scatter_kernel(EmbSour
 #pragma unroll
   for (int e = 0; e < kEach; ++e) {
     const int d = threadIdx.x * kEach + e;
-    uint32_t here = at + offsets[(int64_t)d * fill.own + blockIdx.x];
+    uint32_t here = at + offsets[(int64_t)d * ride.own + blockIdx.x];
 #pragma unroll
     for (int w = 0; w < kSortWaves; ++w) {
       const uint32_t c = counts[w][d];
@@ -297,7 +321,7 @@ struct EmbSums {
   int64_t n, rows, cols, ldd;
   int chunk;        // tokens
   float scale;
-  bool past;        // (see EmbFill)
+  bool past;        // (see EmbRide)
   float* parts;     // [chunks][cols]
   uint32_t* chains; // how many; then the places that they begin at
 };
@@ -464,7 +488,7 @@ static int emb_chunk(int64_t n) {
 struct EmbPlan {
   int64_t tiles, chunks, parts;
   int passes, chunk;
-  int64_t keys[2], places[2], counts, totals, chains, sums, bytes;
+  int64_t keys[2], places[2], counts, totals, used, chains, sums, bytes;
 };
 static EmbPlan emb_plan(int64_t n, int64_t rows, int64_t cols) {
   EmbPlan p{};
@@ -489,6 +513,7 @@ static EmbPlan emb_plan(int64_t n, int64_t rows, int64_t cols) {
   if (p.passes) {
     p.counts = take(4 * kDigits * p.tiles);
     p.totals = take(4 * kDigits);
+    p.used = take(rows);
   }
   p.chains = take(4 * (1 + p.chunks));
   p.sums = take(4 * p.chunks * cols);
@@ -516,7 +541,7 @@ extern "C" int mx_embedding(const void* ids, int ids_i64, int64_t n, const void*
   const uintptr_t w_odd = weight_f32 ? 3 : 1, o_odd = out_f32 ? 3 : 1;
   if (((uintptr_t)ids & (ids_i64 ? 7 : 3)) || ((uintptr_t)weight & w_odd) || ((uintptr_t)out & o_odd)) return MX_ERR_ALIGNMENT;
   const int64_t groups = (n + kEmbWaves - 1) / kEmbWaves;
-  if (rows >= 0x7FFFFFFF || groups > 0x7FFFFFFF) return MX_ERR_UNSUPPORTED;
+  if (rows >= 0x7FFFFFFF || groups > kEmbGroups) return MX_ERR_UNSUPPORTED;
   const EmbIds e{ids, ids_i64 != 0, first, rows, 0};
   of_type(weight_f32, [&](auto w) {
     of_type(out_f32, [&](auto o) {
@@ -546,32 +571,57 @@ extern "C" int mx_embedding_grad(const void* ids, int ids_i64, int64_t n, const 
   const EmbPlan p = emb_plan(n, rows, cols);
   const int threads = cols > 1024 ? 256 : cols > 512 ? 128 : 64;
   const int64_t slabs = (cols + threads * 8 - 1) / (threads * 8), bytes = rows * cols * (grad_f32 ? 4 : 2);
-  if (slabs > 65535 || fill_groups(bytes, 256) + n > 0x7FFFFFFF) return MX_ERR_UNSUPPORTED;
+  const int64_t row_bytes = cols * (grad_f32 ? 4 : 2), pieces = rows * ((row_bytes + 15) / 16);
+  if (slabs > 65535 || ride_groups(pieces, 256) + p.tiles + kDigits > kEmbGroups || p.chunks > kEmbGroups || row_bytes > 0x7FFFFFFF)
+    return MX_ERR_UNSUPPORTED;
   hipStream_t st = (hipStream_t)stream;
   uint8_t* ws = (uint8_t*)workspace;
   auto words = [&](int64_t at) { return (uint32_t*)(ws + at); };
   uint32_t* chains = words(p.chains);
   const EmbIds e{ids, ids_i64 != 0, first, rows, padding};
   const bool past = emb_past(bytes);
-  // the fill, in equal parts for the launches that sort
-  const int64_t share = ((bytes + 3 * p.passes) / std::max(1, 3 * p.passes) + 255) & ~int64_t{255};
-  int64_t done = 0;
-  auto with_fill = [&](unsigned own, int lanes, auto&& launch) {
-    const EmbFill f{(uint8_t*)grad + done, std::min(share, bytes - done), own, past};
-    done += f.bytes;
-    launch(dim3((unsigned)(own + fill_groups(f.bytes, lanes))), dim3(lanes), f);
+  uint8_t* out = (uint8_t*)grad;
+  auto nothing = [&](unsigned own) { return EmbRide{kRideFill, own, out, 0, past, e, nullptr, 0, 0}; };
+  auto fill = [&](unsigned own, uint8_t* to, int64_t from, int64_t many) {
+    return EmbRide{kRideFill, own, to + from, many, past, e, nullptr, 0, 0};
   };
+  auto launch = [&](const EmbRide& q, int lanes, auto&& f) {
+    const int64_t riding = q.mode == kRideFill ? (q.count + 15) / 16 : q.count;
+    f(dim3((unsigned)(q.own + ride_groups(riding, lanes))), dim3(lanes));
+  };
+  auto zeros = [&](int64_t from) {
+    const EmbRide q = fill(0, out, from, bytes - from);
+    if (q.count > 0)
+      launch(q, 256, [&](dim3 g, dim3 b) { hipLaunchKernelGGL(embedding_zeros_kernel, g, b, 0, st, q); });
+  };
+  int last = 0;  // which of the two lists holds the order
   if (n == 0) {
-    with_fill(0, 256, [&](dim3 g, dim3 b, EmbFill f) { hipLaunchKernelGGL(embedding_fill_kernel, g, b, 0, st, f); });
+    zeros(0);
     return hipGetLastError() == hipSuccess ? MX_OK : MX_ERR_LAUNCH;
   }
-  int last = 0;  // which of the two lists holds the order
   if (p.passes == 0) {
+    // Past the caches the launch's large workgroups fill at 5 TB/s: no more of the zeros there than the placing hides
+    // (2003 tokens, 622 MB: 116 us, with all of them 124; 8192 tokens, 311 MB through the caches: 105 and 100).
     const int tokens = rank_tokens(n);
-    with_fill((unsigned)((n + tokens - 1) / tokens), kRankThreads, [&](dim3 g, dim3 b, EmbFill f) {
-      hipLaunchKernelGGL(embedding_rank_kernel, g, b, 0, st, e, (int)n, tokens, words(p.keys[0]), words(p.places[0]), chains, f);
+    const int64_t here = past ? std::min<int64_t>(bytes, int64_t{48} << 20) : bytes;
+    const EmbRide q = fill((unsigned)((n + tokens - 1) / tokens), out, 0, here);
+    launch(q, kRankThreads, [&](dim3 g, dim3 b) {
+      hipLaunchKernelGGL(embedding_rank_kernel, g, b, 0, st, e, (int)n, tokens, words(p.keys[0]), words(p.places[0]), chains, q);
     });
+    zeros(here);
   }
+  // One pass: a small table, filled by the first launch.  More: the first launch clears the rows' flags, the second sets
+  // them, the others share the unused rows' zeros.
+  int launched = 0;
+  const int64_t parts = 3 * p.passes - 2, share = parts > 0 ? (pieces + parts - 1) / parts : 0;
+  auto ride = [&](unsigned own) {
+    const int k = launched++;
+    if (p.passes == 1) return k == 0 ? fill(own, out, 0, bytes) : nothing(own);
+    if (k == 0) return fill(own, ws + p.used, 0, (rows + 255) & ~int64_t{255});
+    if (k == 1) return EmbRide{kRideMark, own, ws + p.used, n, false, e, nullptr, 0, 0};
+    const int64_t from = std::min(pieces, share * (k - 2));
+    return EmbRide{kRideUnused, own, out, std::min(share, pieces - from), past, e, ws + p.used, from, row_bytes};
+  };
   for (int pass = 0; pass < p.passes; ++pass) {
     EmbSource from{e, nullptr, nullptr};
     if (pass > 0) {
@@ -580,15 +630,16 @@ extern "C" int mx_embedding_grad(const void* ids, int ids_i64, int64_t n, const 
       last ^= 1;
     }
     const int shift = pass * kDigitBits;
-    with_fill((unsigned)p.tiles, kSortThreads, [&](dim3 g, dim3 b, EmbFill f) {
-      hipLaunchKernelGGL(embedding_count_kernel, g, b, 0, st, from, n, shift, words(p.counts), chains, f);
+    const EmbRide q0 = ride((unsigned)p.tiles), q1 = ride(kDigits / kSortWaves), q2 = ride((unsigned)p.tiles);
+    launch(q0, kSortThreads, [&](dim3 g, dim3 b) {
+      hipLaunchKernelGGL(embedding_count_kernel, g, b, 0, st, from, n, shift, words(p.counts), chains, q0);
     });
-    with_fill(kDigits / kSortWaves, kSortThreads, [&](dim3 g, dim3 b, EmbFill f) {
-      hipLaunchKernelGGL(embedding_offsets_kernel, g, b, 0, st, words(p.counts), p.tiles, words(p.totals), f);
+    launch(q1, kSortThreads, [&](dim3 g, dim3 b) {
+      hipLaunchKernelGGL(embedding_offsets_kernel, g, b, 0, st, words(p.counts), p.tiles, words(p.totals), q1);
     });
-    with_fill((unsigned)p.tiles, kSortThreads, [&](dim3 g, dim3 b, EmbFill f) {
+    launch(q2, kSortThreads, [&](dim3 g, dim3 b) {
       hipLaunchKernelGGL(embedding_scatter_kernel, g, b, 0, st, from, n, shift, words(p.counts), words(p.totals),
-                         words(p.keys[last]), words(p.places[last]), f);
+                         words(p.keys[last]), words(p.places[last]), q2);
     });
   }
   const EmbSums a{words(p.keys[last]), words(p.places[last]), n, rows, cols, ldd, p.chunk, scale, past, (float*)(ws + p.sums),
