@@ -159,3 +159,36 @@ def test_entry_points_check_their_arguments_before_any_launch():
     sizes[0] = 1 << 60
     assert lib.mx_grad_scale(1, ptrs, sizes, kinds, a, 1.0, None) == 4
     assert lib.mx_grad_norm_workspace(0) == 0 and lib.mx_grad_norm_workspace(161) == 2 * lib.mx_grad_norm_workspace(160)
+
+
+def test_embedding_and_norms_trace_without_a_break():
+    """Off the GPU their formulas are traced, one graph; on it (fake tensors) one operator each."""
+    class Two(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.tokens = Embedding.Config(scale=2.0).build(num_embeddings=9, embedding_dim=32)
+            self.seam = ResidualRMSNorm.Config(post_norm=True, gate=True).build(dim=32)
+
+        def forward(self, ids):
+            x = self.tokens(ids)
+            return self.seam(x, x)
+
+    graphs = []
+    module, ids = Two(), torch.zeros((2, 3), dtype=torch.int64)
+    traced = torch.compile(module, backend=lambda graph, example: graphs.append(graph) or graph.forward, fullgraph=True)
+    assert all(torch.equal(a, b) for a, b in zip(traced(ids), module(ids))) and len(graphs) == 1
+    torch._dynamo.reset()
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    with FakeTensorMode():
+        w, ids = torch.empty((9, 32), dtype=torch.bfloat16, device="cuda"), torch.zeros((2, 3), dtype=torch.int64, device="cuda")
+        out = torch.ops.torchtitan_amd.embedding_fwd(ids, w, 2.0, None, 0, torch.float32)
+        assert out.shape == (2, 3, 32) and out.dtype == torch.float32
+        grad = torch.ops.torchtitan_amd.embedding_bwd(ids, out, 9, 2.0, 0, None, torch.bfloat16)
+        assert grad.shape == (9, 32) and grad.dtype == torch.bfloat16
+        h, r = torch.empty((6, 32), dtype=torch.bfloat16, device="cuda"), torch.empty((6, 32), device="cuda")
+        stream, normed, rstd = torch.ops.torchtitan_amd.residual_norm_fwd(h, r, w[0], None, w[1], 1.0, 1e-5)
+        assert stream.dtype == torch.float32 and normed.dtype == torch.bfloat16 and rstd.shape == (2, 6)
+        grads = torch.ops.torchtitan_amd.residual_norm_bwd(h, r, w[0], None, w[1], 1.0, rstd, stream, None,
+                                                           [True, False, True, True, True])
+        assert [tuple(g.shape) for g in grads] == [(6, 32), (0,), (32,), (0,), (32,)]

@@ -823,3 +823,98 @@ def mx_routed_experts_traced(x, top_scores, w1, w2, w3, tok_sorted, counts, scor
     return torch.ops.torchtitan_amd.mx_routed_experts_fwd(
         x, top_scores, w1, w2, w3, tok_sorted, counts, bool(score_before), ops.SCALE_MODES[cfg.scale_mode],
         cfg.cache_weight_casts, _wants_grad(x), _wants_grad(top_scores), _wants_grad(w1, w2, w3))[0]
+
+
+# ----------------------------------------------------------------------------- around the linears
+@torch.library.custom_op("torchtitan_amd::embedding_fwd", mutates_args=())
+def embedding_fwd(ids: torch.Tensor, weight: torch.Tensor, scale: float, padding_idx: int | None, first_row: int,
+                  dtype: torch.dtype) -> torch.Tensor:
+    """`ops.embedding_fwd` as a node of the graph (`padding_idx` is for its gradient)."""
+    return ops.embedding_fwd(ids, weight, scale, first_row, dtype)
+
+
+@embedding_fwd.register_fake
+def _(ids, weight, scale, padding_idx, first_row, dtype):
+    return weight.new_empty((*ids.shape, weight.shape[1]), dtype=dtype)
+
+
+@torch.library.custom_op("torchtitan_amd::embedding_bwd", mutates_args=())
+def embedding_bwd(ids: torch.Tensor, dout: torch.Tensor, rows: int, scale: float, first_row: int, padding_idx: int | None,
+                  dtype: torch.dtype) -> torch.Tensor:
+    return ops.embedding_bwd(ids, dout, rows, scale, first_row, padding_idx, dtype)
+
+
+@embedding_bwd.register_fake
+def _(ids, dout, rows, scale, first_row, padding_idx, dtype):
+    return dout.new_empty((rows, dout.shape[-1]), dtype=dtype)
+
+
+def _embedding_setup(ctx, inputs, output):
+    ids, weight, *ctx.call = inputs
+    ctx.save_for_backward(ids)
+    ctx.rows, ctx.w_dtype = weight.shape[0], weight.dtype
+
+
+def _embedding_backward(ctx, dout):
+    (ids,), (scale, padding_idx, first_row, _) = ctx.saved_tensors, ctx.call
+    grad = torch.ops.torchtitan_amd.embedding_bwd(ids, dout, ctx.rows, scale, first_row, padding_idx, ctx.w_dtype)
+    return None, grad, None, None, None, None
+
+
+embedding_fwd.register_autograd(_embedding_backward, setup_context=_embedding_setup)
+
+
+@torch.library.custom_op("torchtitan_amd::residual_norm_fwd", mutates_args=())
+def residual_norm_fwd(h: torch.Tensor, residual: torch.Tensor, post: torch.Tensor | None, gate: torch.Tensor | None,
+                      pre: torch.Tensor | None, scale: float,
+                      eps: float) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """`ops.residual_norm` on matrices as a node of the graph: (stream, normed -- empty without `pre` --, rstd)."""
+    stream, normed, rstd = ops.residual_norm(h, residual, post, gate, pre, scale, eps, want_rstd=True)
+    return stream, _empty(h.device) if normed is None else normed, rstd
+
+
+@residual_norm_fwd.register_fake
+def _(h, residual, post, gate, pre, scale, eps):
+    normed = _empty(h.device) if pre is None else h.new_empty(h.shape)
+    return residual.new_empty(h.shape), normed, h.new_empty((2, h.shape[0]), dtype=torch.float32)
+
+
+@torch.library.custom_op("torchtitan_amd::residual_norm_bwd", mutates_args=())
+def residual_norm_bwd(h: torch.Tensor, residual: torch.Tensor, post: torch.Tensor | None, gate: torch.Tensor | None,
+                      pre: torch.Tensor | None, scale: float, rstd: torch.Tensor, dstream: torch.Tensor | None,
+                      dnormed: torch.Tensor | None, needs: list[bool]) -> list[torch.Tensor]:
+    """Gradients of h, residual, post, gate and pre; empty where not asked for."""
+    grads = ops.residual_norm_bwd(h, residual, post, gate, pre, scale, rstd, dstream, dnormed, needs)
+    return [_empty(h.device) if g is None else g for g in grads]
+
+
+@residual_norm_bwd.register_fake
+def _(h, residual, post, gate, pre, scale, rstd, dstream, dnormed, needs):
+    return [t.new_empty(t.shape) if need and t is not None else _empty(h.device)
+            for need, t in zip(needs, (h, residual, post, gate, pre))]
+
+
+def _residual_norm_setup(ctx, inputs, output):
+    *operands, ctx.scale, _ = inputs
+    ctx.save_for_backward(*operands, output[2])
+    ctx.set_materialize_grads(False)
+
+
+def _residual_norm_backward(ctx, dstream, dnormed, drstd):
+    h, residual, post, gate, pre, rstd = ctx.saved_tensors
+    needs = [bool(n) for n in ctx.needs_input_grad[:5]]
+    if dstream is None and dnormed is None:
+        return None, None, None, None, None, None, None
+    grads = torch.ops.torchtitan_amd.residual_norm_bwd(h, residual, post, gate, pre, ctx.scale, rstd, dstream,
+                                                       None if pre is None else dnormed, needs)
+    wanted = [n and t is not None for n, t in zip(needs, (h, residual, post, gate, pre))]
+    return (*(g if w else None for g, w in zip(grads, wanted)), None, None)
+
+
+residual_norm_fwd.register_autograd(_residual_norm_backward, setup_context=_residual_norm_setup)
+
+
+def residual_norm_traced(h, residual, post, gate, pre, scale: float, eps: float):
+    """(stream, normed or None) of matrices while a graph is being traced."""
+    stream, normed, _ = torch.ops.torchtitan_amd.residual_norm_fwd(h, residual, post, gate, pre, scale, eps)
+    return stream, None if pre is None else normed

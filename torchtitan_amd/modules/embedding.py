@@ -52,7 +52,8 @@ def scaled_embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0
     zeros and no gradient: the rows of a vocabulary shard add up over the shards.  Tokens whose id is
     `padding_idx` have their row, but no gradient.  weight: [rows, dim].  The gradient is dense, sums of equal ids in
     float32 in an order that depends on the ids alone; it cannot be differentiated again."""
-    if (dtype is None or dtype in ops.ROW_TYPES) and ops.native_rows(weight):
+    tracing = torch.compiler.is_compiling()
+    if not tracing and (dtype is None or dtype in ops.ROW_TYPES) and ops.native_rows(weight):
         out = _lib.blocks().scaled_embedding(ids, weight, scale, padding_idx, first_row,
                                              (dtype or weight.dtype) == torch.float32)
         if out is not None:
@@ -64,7 +65,11 @@ def scaled_embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0
     if ids.device != weight.device:
         raise ValueError(f"ids on {ids.device}, weight on {weight.device}")
     dtype = dtype or weight.dtype
-    if not (ops.plain_rows(weight) and type(ids) is torch.Tensor and dtype in ops.ROW_TYPES):
+    if tracing and weight.is_cuda and weight.dtype in ops.ROW_TYPES and dtype in ops.ROW_TYPES:
+        from .. import compiled  # noqa: F401  (the same launches as nodes of the graph)
+
+        return torch.ops.torchtitan_amd.embedding_fwd(ids, weight, float(scale), padding_idx, first_row, dtype)
+    if tracing or not (ops.plain_rows(weight) and type(ids) is torch.Tensor and dtype in ops.ROW_TYPES):
         return _in_torch_ops(ids, weight, scale, padding_idx, first_row, dtype)
     if torch.is_grad_enabled() and weight.requires_grad:
         return _ScaledEmbedding.apply(ids, weight, scale, padding_idx, first_row, dtype)

@@ -81,7 +81,8 @@ def residual_rms_norm(h: torch.Tensor, residual: torch.Tensor, *, post_weight: t
     h: output of a block, residual: the stream around it, both [..., dim]; h may be bf16 where the stream is float32.
     post_weight, pre_weight: [dim].  gate: [dim], or with h's dimensions: its leading ones up to some point, ones
     behind it, dim ([batch, 1, dim]: a row for every sequence).  The gradients cannot be differentiated again."""
-    if ops.native_rows(h):
+    tracing = torch.compiler.is_compiling()
+    if not tracing and ops.native_rows(h):
         out = _lib.blocks().residual_rms_norm(h, residual, post_weight, gate, pre_weight, residual_scale, eps)
         if out is not None:
             return out
@@ -97,11 +98,16 @@ def residual_rms_norm(h: torch.Tensor, residual: torch.Tensor, *, post_weight: t
         if w is not None and w.shape != (dim,):
             raise ValueError(f"{name} must be [{dim}], got {tuple(w.shape)}")
     rows = None if gate is None else _gate_as_matrix(gate, h.shape)
-    if (h.numel() == 0 or not ops.plain_rows(*operands)
-            or (h.dtype == torch.float32 and residual.dtype == torch.bfloat16)):
+    ours = all(t.is_cuda and t.dtype in ops.ROW_TYPES for t in operands) and (
+        h.dtype == torch.bfloat16 or residual.dtype == torch.float32)
+    if not ours or h.numel() == 0 or not (tracing or ops.plain_rows(*operands)):
         return _in_torch_ops(h, residual, post_weight, gate, pre_weight, residual_scale, eps)
     h2, r2 = h.reshape(-1, dim), residual.reshape(-1, dim)
-    if torch.is_grad_enabled() and any(t.requires_grad for t in operands):
+    if tracing:
+        from ..compiled import residual_norm_traced  # the same launches as nodes of the graph
+
+        stream, normed = residual_norm_traced(h2, r2, post_weight, rows, pre_weight, float(residual_scale), float(eps))
+    elif torch.is_grad_enabled() and any(t.requires_grad for t in operands):
         stream, normed = _ResidualRMSNorm.apply(h2, r2, post_weight, rows, pre_weight, residual_scale, eps)
     else:
         stream, normed, _ = ops.residual_norm(h2, r2, post_weight, rows, pre_weight, residual_scale, eps)
