@@ -34,38 +34,40 @@ struct EmbIds {
   }
 };
 
-// One wave a token: the row's pieces are asked for four at a time.
+// One wave for 1024 columns of a token, all asked for before the first is stored: 147456 x 2048 151 us (604 MB written and
+// as many read, most of them from the caches; with 2048 columns a wave 156), 8192 x 4096 of a shard 18 (with a wave for the
+// whole row 24).
+constexpr int kEmbPieces = 2, kEmbSlab = 64 * 8 * kEmbPieces;
 template <class W, class O>
 __global__ __launch_bounds__(kEmbThreads) void embedding_kernel(EmbIds ids, int64_t n, const W* __restrict__ weight,
-                                                                int64_t cols, int64_t ldw, float scale, bool past,
+                                                                int64_t cols, int64_t ldw, float scale, bool past, uint32_t slabs,
                                                                 O* __restrict__ out) {
-  constexpr int V = 8, U = 4;
-  const int64_t t = (int64_t)blockIdx.x * kEmbWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  constexpr int V = 8, U = kEmbPieces;
+  const uint32_t item = blockIdx.x * (uint32_t)kEmbWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), t = item / slabs;
   if (t >= n) return;
   const uint32_t r = __builtin_amdgcn_readfirstlane(ids.row(t));
   const bool in = r < (uint32_t)ids.rows;
+  const int64_t c0 = (int64_t)(item - t * slabs) * kEmbSlab + (threadIdx.x & 63) * V;
   const W* src = weight + (in ? (int64_t)r * ldw : 0);
-  O* dst = out + t * cols;
-  for (int64_t c0 = (int64_t)(threadIdx.x & 63) * V; c0 < cols; c0 += 64 * V * U) {
-    Piece<W, V> p[U];
+  O* dst = out + (int64_t)t * cols;
+  Piece<W, V> p[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int64_t c = c0 + u * 64 * V;
-      if (in) load_piece<false>(src + c, cols - c, p[u]);
+  for (int u = 0; u < U; ++u) {
+    const int64_t c = c0 + u * 64 * V;
+    if (in) load_piece<false>(src + c, cols - c, p[u]);
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int64_t c = c0 + u * 64 * V;
+    float f[V] = {};
+    if (in) {
+      to_floats(p[u], f);
+#pragma unroll
+      for (int e = 0; e < V; ++e) f[e] *= scale;
     }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int64_t c = c0 + u * 64 * V;
-      float f[V] = {};
-      if (in) {
-        to_floats(p[u], f);
-#pragma unroll
-        for (int e = 0; e < V; ++e) f[e] *= scale;
-      }
-      const Piece<O, V> q = from_floats<O>(f);
-      if (past) store_piece<true>(dst + c, cols - c, q);
-      else store_piece<false>(dst + c, cols - c, q);
-    }
+    const Piece<O, V> q = from_floats<O>(f);
+    if (past) store_piece<true>(dst + c, cols - c, q);
+    else store_piece<false>(dst + c, cols - c, q);
   }
 }
 
@@ -326,7 +328,7 @@ struct EmbSums {
   uint32_t* chains; // how many; then the places that they begin at
 };
 
-constexpr int kChunkMost = 64;
+constexpr int kChunkMost = 32;
 
 // First place whose row is not below `key` (between lo and hi), by the whole wave: 64 probes a step.
 __device__ __forceinline__ int64_t wave_lower_bound(const uint32_t* __restrict__ keys, int64_t lo, int64_t hi, uint32_t key) {
@@ -477,9 +479,10 @@ __global__ __launch_bounds__(256) void embedding_chains_kernel(EmbSums a, const 
   }
 }
 
-// Tokens of a chunk: 64, fewer where there would not be a thousand chunks.
+// Tokens of a chunk: 32 (147456 tokens: sums 147 us and chains 23; 64: 155 and 21; 16: 141 and 38), fewer where there would
+// not be a thousand chunks (8192 tokens: 8, sums 10 us, with 16 15).
 static int emb_chunk(int64_t n) {
-  int c = 16;
+  int c = 8;
   while (c < kChunkMost && c * 1024 < n) c *= 2;
   return c;
 }
@@ -540,14 +543,15 @@ extern "C" int mx_embedding(const void* ids, int ids_i64, int64_t n, const void*
   if (!ids || (rows > 0 && !weight) || !out) return MX_ERR_INVALID_ARG;
   const uintptr_t w_odd = weight_f32 ? 3 : 1, o_odd = out_f32 ? 3 : 1;
   if (((uintptr_t)ids & (ids_i64 ? 7 : 3)) || ((uintptr_t)weight & w_odd) || ((uintptr_t)out & o_odd)) return MX_ERR_ALIGNMENT;
-  const int64_t groups = (n + kEmbWaves - 1) / kEmbWaves;
+  const int64_t slabs = (cols + kEmbSlab - 1) / kEmbSlab;
+  const int64_t groups = slabs > kEmbGroups * kEmbWaves / n ? kEmbGroups + 1 : (n * slabs + kEmbWaves - 1) / kEmbWaves;
   if (rows >= 0x7FFFFFFF || groups > kEmbGroups) return MX_ERR_UNSUPPORTED;
   const EmbIds e{ids, ids_i64 != 0, first, rows, 0};
   of_type(weight_f32, [&](auto w) {
     of_type(out_f32, [&](auto o) {
       hipLaunchKernelGGL((embedding_kernel<decltype(w), decltype(o)>), dim3((unsigned)groups), dim3(kEmbThreads), 0,
                          (hipStream_t)stream, e, n, (const decltype(w)*)weight, cols, ldw, scale,
-                         emb_past(n * cols * (out_f32 ? 4 : 2)), (decltype(o)*)out);
+                         emb_past(n * cols * (out_f32 ? 4 : 2)), (uint32_t)slabs, (decltype(o)*)out);
     });
   });
   return hipGetLastError() == hipSuccess ? MX_OK : MX_ERR_LAUNCH;

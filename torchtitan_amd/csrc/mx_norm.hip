@@ -149,11 +149,13 @@ __device__ __forceinline__ float lanes_sum(float v, float* part) {
   return v;
 }
 
-// 1 / sqrt(x), x >= 0, within a few units in the last place: the hardware's, which takes no denormals.
+// 1 / sqrt(x), x >= 0: the hardware's, which takes no denormals, and a Newton step on its remainder, which brings it to
+// within an ulp (none for 0 and infinity, whose remainder is NaN).
 __device__ __forceinline__ float norm_rsqrt(float x) {
   const bool tiny = x < 0x1p-100f;
-  const float s = __builtin_amdgcn_rsqf(tiny ? x * 0x1p100f : x);
-  return tiny ? s * 0x1p50f : s;
+  const float y = tiny ? x * 0x1p100f : x, s = __builtin_amdgcn_rsqf(y), rest = __builtin_fmaf(-y * s, s, 1.f);
+  const float best = rest == rest ? __builtin_fmaf(0.5f * s, rest, s) : s;
+  return tiny ? best * 0x1p50f : best;
 }
 
 // Sum of a * b over a lane's pieces of a row; `ragged`: the width is no multiple of kV, and elements may be another
