@@ -169,6 +169,25 @@ def test_many_rows_share_and_own_gates(device):
     check(*make(device, (35000, 2), 8, (True, True, True), gate_shape=(35000, 1, 8)))
 
 
+@pytest.mark.parametrize("dim", [20, 128, 190, 256, 300, 511])
+@pytest.mark.parametrize("rows,gates", [(9000, 9000), (9000, 3000), (10000, 2000), (9003, 1), (4000, 4000), (16390, 8195)])
+@pytest.mark.parametrize("post", [True, False])
+def test_narrow_rows_with_gates_for_a_few_rows_each(device, rows, gates, dim, post):
+    """Rows whose lanes work on their own, and those that share a strip, with all counts of rows left over."""
+    h, r, p, g, w = make(device, rows, dim, (post, True, True), (BF, F32, F32), gate_shape=(gates, dim))
+    gate = g if gates == rows else g.reshape(gates, 1, dim)
+    shape = (rows, dim) if gates == rows else (gates, rows // gates, dim)
+    check(h.reshape(shape), r.reshape(shape), p, gate, w, 0.9)
+
+
+@pytest.mark.parametrize("dim", [513, 1000, 1024, 2050, 4096, 4100])
+@pytest.mark.parametrize("rows,gates", [(2100, 2100), (2100, 1050), (2049, 683), (2048, 512)])
+def test_wide_rows_with_gates_for_a_few_rows_each(device, rows, gates, dim):
+    for types in ((BF, BF, BF), (BF, F32, F32)):
+        h, r, p, g, w = make(device, (gates, rows // gates), dim, (True, True, True), types, gate_shape=(gates, 1, dim))
+        check(h, r, p, g, w, 1.1)
+
+
 def test_strides_and_alignment(device):
     g = torch.Generator(device=device).manual_seed(3)
     for dim, lo in ((512, 1), (2048, 3), (100, 5), (5000, 7)):

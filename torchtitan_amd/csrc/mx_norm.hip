@@ -117,6 +117,30 @@ __device__ __forceinline__ void weight_at(const NormWeight& w, int64_t row, cons
   }
 }
 
+// The same of a vector that is there, as it lies in memory: nothing waits for it yet.
+struct RawWeight {
+  uint32_t w[kV];
+};
+__device__ __forceinline__ RawWeight raw_weight(const NormWeight& w, int64_t row, const NormPlace& p) {
+  RawWeight raw{};
+  if (w.f32) {
+    Piece<float, kV> q;
+    load_at<false>((const float*)w.p + row, p, q);
+#pragma unroll
+    for (int i = 0; i < kV; ++i) raw.w[i] = q.w[i];
+  } else {
+    Piece<uint16_t, kV> q;
+    load_at<false>((const uint16_t*)w.p + row, p, q);
+#pragma unroll
+    for (int i = 0; i < kV / 2; ++i) raw.w[i] = q.w[i];
+  }
+  return raw;
+}
+__device__ __forceinline__ void raw_floats(const NormWeight& w, const RawWeight& raw, float (&f)[kV]) {
+#pragma unroll
+  for (int e = 0; e < kV; ++e) f[e] = __uint_as_float(w.f32 ? raw.w[e] : e & 1 ? raw.w[e / 2] & 0xFFFF0000u : raw.w[e / 2] << 16);
+}
+
 // gate * post: what a row's normalised block output is multiplied with.
 __device__ __forceinline__ void side_at(const NormArgs& a, int64_t g0, const NormPlace& p, float (&f)[kV]) {
   float q[kV];
@@ -398,7 +422,9 @@ __device__ __forceinline__ void rows_joined(float (&acc)[S::kPieces][kV], float*
 // SIDE: the block's side of the sum (norm behind it, gate) as well; else h has the gradient e.  Over the rows of a strip,
 // which share a row of the gate, both weights of that side need the same sum of e h s1: times post it is the gate's
 // gradient, times the gate post's.
-template <class S, bool SIDE, class H, class R>
+// SOLO: the lanes of a row take strips of their own (see norm_solo), of a row of the gate each; the next strip's first row
+// and gate are on their way while one is worked on.
+template <class S, bool SIDE, bool SOLO, class H, class R>
 __global__ __launch_bounds__(S::kThreads) void residual_norm_bwd_kernel(NormArgs a, NormStrips strips,
                                                                         const float* __restrict__ rstd, NormGrads o) {
   constexpr int N = S::kPieces;
@@ -435,19 +461,47 @@ __global__ __launch_bounds__(S::kThreads) void residual_norm_bwd_kernel(NormArgs
   if constexpr (kHeld) pre_at(0, pre1);
   float dpre[N][kV] = {}, dpost[N][kV] = {};
   int turn = 0;
-  for (int64_t strip = blockIdx.x; strip < strips.total; strip += gridDim.x) {
-    const int64_t group = (uint32_t)strip / (uint32_t)strips.strips, first = group * a.gate_each + (strip - group * strips.strips) * S::kRows;
-    const int64_t end = (group + 1) * a.gate_each, hop = strips.strips * S::kRows;
+  constexpr int kTogether = SOLO ? 1 : S::kRows;  // rows that a strip takes at a time
+  constexpr int kStrips = S::kRows / kTogether;   // strips that a workgroup takes at a time
+  const int mine = SOLO ? 0 : sub;
+  Row now, next;
+  bool fetched = false;  // `now` and the gate, by the strip before
+  RawWeight gate_next;
+  float gate1[kV], post1[kV];
+  if constexpr (SOLO) weight_at(a.post, 0, at[0], post1);
+  for (int64_t strip = (int64_t)blockIdx.x * kStrips + (SOLO ? sub : 0); strip < strips.total; strip += (int64_t)gridDim.x * kStrips) {
+    const int64_t group = (uint32_t)strip / (uint32_t)strips.strips, first = group * a.gate_each + (strip - group * strips.strips) * kTogether;
+    const int64_t end = (group + 1) * a.gate_each, hop = strips.strips * kTogether;
     const int64_t g0 = group * a.cols;
     float both[N][kV] = {};
-    Row now, next;
-    int64_t row = first + sub;
-    if (kHeld && row < end) fetch(now, row);
-    if constexpr (kHeld && SIDE) side_at(a, g0, at[0], side1);
+    int64_t row = first + mine;
+    if (kHeld && !fetched && row < end) fetch(now, row);
+    if constexpr (SOLO) {
+      raw_floats(a.gate, fetched ? gate_next : raw_weight(a.gate, g0, at[0]), gate1);
+#pragma unroll
+      for (int e = 0; e < kV; ++e) side1[e] = gate1[e] * post1[e];
+    } else if constexpr (kHeld && SIDE) {
+      side_at(a, g0, at[0], side1);
+    }
+    fetched = false;
     for (; row < end; row += hop, turn ^= 1) {
       if constexpr (!kHeld) fetch(now, row);
-      if (kHeld && row + hop < end) fetch(next, row + hop);
+      if constexpr (kHeld) {
+        if (row + hop < end) fetch(next, row + hop);
+        else if (SOLO && strip + gridDim.x * kStrips < strips.total) {
+          const int64_t strip2 = strip + gridDim.x * kStrips, group2 = (uint32_t)strip2 / (uint32_t)strips.strips;
+          const int64_t row2 = group2 * a.gate_each + (strip2 - group2 * strips.strips) * kTogether + mine;
+          if (row2 < (group2 + 1) * a.gate_each) {
+            fetch(next, row2);
+            gate_next = raw_weight(a.gate, group2 * a.cols, at[0]);
+            fetched = true;
+          }
+        }
+      }
       const float s1 = now.s1, s2 = now.s2;
+      if constexpr (!kHeld)  // (nothing of the weights is kept from row to row: 8192 x 16384 602 us, where what was kept spilled 975)
+#pragma unroll
+        for (int k = 0; k < N; ++k) asm volatile("" : "+v"(at[k].at));
       float hat[N][kV], u[N][kV];
 #pragma unroll
       for (int k = 0; k < N; ++k) {
@@ -511,19 +565,19 @@ __global__ __launch_bounds__(S::kThreads) void residual_norm_bwd_kernel(NormArgs
 #pragma unroll
       for (int k = 0; k < N; ++k) {
         float g[kV];
-        weight_at(a.gate, g0, at[k], g);
+        if constexpr (!SOLO) weight_at(a.gate, g0, at[k], g);
 #pragma unroll
-        for (int e = 0; e < kV; ++e) dpost[k][e] = __builtin_fmaf(g[e], both[k][e], dpost[k][e]);
+        for (int e = 0; e < kV; ++e) dpost[k][e] = __builtin_fmaf(SOLO ? gate1[e] : g[e], both[k][e], dpost[k][e]);
       }
       if (o.dgate) {
-        rows_joined<S>(both, lds);
-        if (sub == 0) {
+        if constexpr (!SOLO) rows_joined<S>(both, lds);
+        if (SOLO || sub == 0) {
 #pragma unroll
           for (int k = 0; k < N; ++k) {
             float p[kV];
-            weight_at(a.post, 0, at[k], p);
+            if constexpr (!SOLO) weight_at(a.post, 0, at[k], p);
 #pragma unroll
-            for (int e = 0; e < kV; ++e) p[e] *= both[k][e];
+            for (int e = 0; e < kV; ++e) p[e] = (SOLO ? post1[e] : p[e]) * both[k][e];
             if (strips.strips > 1) store_at(o.gate_part + strip * a.cols, at[k], p);
             else if (o.dgate_f32) store_at((float*)o.dgate + g0, at[k], p);
             else store_at((uint16_t*)o.dgate + g0, at[k], p);
@@ -609,11 +663,6 @@ static int64_t norm_fwd_groups(const NormArgs& a) {
 // for narrow rows (147456 x 2048: 702 us, with four 788; 16384 x 4096 135 and 132).
 static int64_t norm_bwd_groups(int64_t cols, bool side) { return norm_groups(cols, side ? 8 : cols <= 2048 ? 12 : 16); }
 
-static NormStrips norm_strips(int64_t rows, int64_t gate_rows, int64_t groups) {
-  const int64_t strips = std::max<int64_t>(1, std::min(groups / gate_rows, rows / gate_rows));
-  return {strips, strips * gate_rows};
-}
-
 // Calls f(shape) with the smallest shape that holds a row, or f(0) for rows that none does.
 template <class F>
 static void norm_shape(int64_t cols, F&& f) {
@@ -627,6 +676,39 @@ static void norm_shape(int64_t cols, F&& f) {
   else if (cols <= NormShape<1024, 1>::kCols) f(NormShape<1024, 1>());
   else if (cols <= NormShape<1024, 2>::kCols) f(NormShape<1024, 2>());
   else f(0);
+}
+
+// Strips for each row's lanes, for rows of the gate that have few rows themselves.  Where a workgroup takes several rows at
+// a time: if they work through their rows sooner so than together.  Where it takes one: up to 4 rows of one gate.  us
+// shared / so: 65536 x 512 with a gate for every row 394 / 108, x 1024 309 / 227, 16384 x 4096 277 / 216 and for every 4 rows
+// 170 / 169.  Rows of 1024 lanes have no registers for it (8192 x 8192 392 / 466).
+template <class S>
+constexpr bool norm_solo_shape() {
+  return S::kPieces == 1 && S::kLanes < 1024;
+}
+static bool norm_solo(int64_t rows, int64_t gate_rows, int64_t groups, int64_t together) {
+  auto up = [](int64_t x, int64_t y) { return (x + y - 1) / y; };
+  const int64_t each = rows / gate_rows;
+  if (together == 1) return each <= 4;
+  return up(gate_rows, groups * together) * each < up(gate_rows, groups) * up(each, together);
+}
+
+struct NormBwdPlan {
+  NormStrips strips;
+  int64_t groups;
+  bool solo;
+};
+static NormBwdPlan norm_bwd_plan(int64_t rows, int64_t cols, int64_t gate_rows, bool side, bool gate) {
+  int64_t together = 0;
+  norm_shape(cols, [&](auto shape) {
+    if constexpr (!std::is_same_v<decltype(shape), int>) {
+      if (norm_solo_shape<decltype(shape)>()) together = decltype(shape)::kRows;
+    }
+  });
+  const int64_t groups = norm_bwd_groups(cols, side), strips = std::max<int64_t>(1, std::min(groups, rows) / gate_rows);
+  const bool solo = gate && strips == 1 && together > 0 && norm_solo(rows, gate_rows, groups, together);
+  const int64_t total = strips * gate_rows, units = solo ? (total + together - 1) / together : total;
+  return {{strips, total}, std::min(units, groups), solo};
 }
 
 template <class F>
@@ -686,8 +768,8 @@ extern "C" int64_t mx_residual_norm_workspace(int64_t rows, int64_t cols, int64_
   if (rows <= 0 || cols <= 0 || gate_rows < 1 || rows % gate_rows) return 0;
   int64_t most = 0;
   for (bool side : {false, true}) {
-    const NormStrips s = norm_strips(rows, gate_rows, norm_bwd_groups(cols, side));
-    most = std::max(most, 3 * std::min(s.total, norm_bwd_groups(cols, side)) + (s.strips > 1 ? s.total : 0));
+    const NormBwdPlan p = norm_bwd_plan(rows, cols, gate_rows, side, false);  // (with a gate: no more workgroups)
+    most = std::max(most, 3 * p.groups + (p.strips.strips > 1 ? p.strips.total : 0));
   }
   return 4 * cols * most;
 }
@@ -708,8 +790,9 @@ extern "C" int mx_residual_norm_bwd(const void* h, int h_f32, const void* r, int
     return MX_ERR_ALIGNMENT;
   const NormArgs a{h, r, rows, cols, ldh, ldr, {post, weights_f32 & 1}, {gate, weights_f32 & 2}, {pre, weights_f32 & 4},
                    rows / gate_rows, scale, 0.f, norm_past(rows * cols, h_f32, r_f32)};
-  const NormStrips s = norm_strips(rows, gate_rows, norm_bwd_groups(cols, post || gate));
-  const int64_t groups = std::min(s.total, norm_bwd_groups(cols, post || gate));
+  const NormBwdPlan plan = norm_bwd_plan(rows, cols, gate_rows, post || gate, gate);
+  const NormStrips s = plan.strips;
+  const int64_t groups = plan.groups;
   float* rows_part = (float*)workspace;
   float* gate_part = rows_part + 3 * groups * cols;
   const NormGrads o{dstream, dnormed, dh, dr, rows_part, gate_part, dgate, weights_f32 & 2};
@@ -721,12 +804,12 @@ extern "C" int mx_residual_norm_bwd(const void* h, int h_f32, const void* r, int
       using S = decltype(shape);
       if constexpr (std::is_same_v<S, int>)
         hipLaunchKernelGGL((residual_norm_bwd_any_kernel<H, R>), dim3((unsigned)groups), dim3(kNormThreads), 0, st, a, s, rstd, o);
-      else if (post || gate)
-        hipLaunchKernelGGL((residual_norm_bwd_kernel<S, true, H, R>), dim3((unsigned)groups), dim3(S::kThreads), 0, st, a, s,
-                           rstd, o);
-      else
-        hipLaunchKernelGGL((residual_norm_bwd_kernel<S, false, H, R>), dim3((unsigned)groups), dim3(S::kThreads), 0, st, a, s,
-                           rstd, o);
+      else {
+        auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(S::kThreads), 0, st, a, s, rstd, o); };
+        if (!post && !gate) launch(residual_norm_bwd_kernel<S, false, false, H, R>);
+        else if (!plan.solo) launch(residual_norm_bwd_kernel<S, true, false, H, R>);
+        else if constexpr (norm_solo_shape<S>()) launch(residual_norm_bwd_kernel<S, true, true, H, R>);
+      }
     });
   });
   const int64_t gates = dgate && s.strips > 1 ? gate_rows : 0;  // (fewer than workgroups)
