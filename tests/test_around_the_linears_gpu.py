@@ -299,3 +299,106 @@ def test_more_elements_than_32_bits_count(device):
     ops.grad_scale_([h], norm, float(norm) / 4)
     factor = (float(norm) / 4) / (float(norm) + 1e-6)
     assert ((h[-last:].double() - before.double() * factor).abs() <= before.double().abs() * 2.0 ** -8).all()
+
+
+def test_negated_views(device):
+    """Views whose memory holds the negated values: read as the values that they stand for, or refused."""
+    neg = torch._neg_view
+    operands = [t.detach() for t in _operands(device, seed=5)]
+    dense = [(-t).requires_grad_(True) for t in operands]
+    views = [neg(t).requires_grad_(True) for t in operands]
+    g = torch.randn(operands[0].shape, device=device).to(BF)
+    ids = torch.randint(0, 3, (40,), device=device)
+    d = torch.randn((40, 320), device=device).to(BF)
+    for into, of in ((lambda t: t, lambda t: t), (lambda t: -t, neg)):
+        want = torch.autograd.grad(_norm(dense), dense, [into(g), into(g)])
+        for got in (torch.autograd.grad(_norm(dense), dense, [of(g), of(g)]), torch.autograd.grad(_norm(views), views, [of(g), of(g)])):
+            assert all((a - b).abs().max() <= 2.0 ** -7 * b.abs().max() for a, b in zip(got, want))  # (torch operations round alike)
+        table, seen = dense[0][0].detach().requires_grad_(True), neg(operands[0][0]).requires_grad_(True)
+        a, b = scaled_embedding(ids, table, 2.0), scaled_embedding(ids, seen, 2.0)
+        assert torch.equal(a, b)
+        assert torch.equal(torch.autograd.grad(a, table, into(d))[0], torch.autograd.grad(scaled_embedding(ids, table, 2.0), table, of(d))[0])
+    assert torch.equal(ops.embedding_fwd(ids, neg(operands[0][0])), -ops.embedding_fwd(ids, operands[0][0]))
+    with pytest.raises(ValueError):
+        ops.grad_norm([neg(operands[0])])
+    p = nn.Parameter(torch.zeros(8, device=device))
+    p.grad = neg(torch.ones(8, device=device))
+    with pytest.raises(RuntimeError):
+        clip_grad_norm_([p], 0.1)
+
+
+def test_batched_gradients_are_refused(device):
+    operands = _operands(device, seed=6)
+    stream, normed = _norm(operands)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(stream, operands[0], torch.ones((2, *stream.shape), dtype=BF, device=device), is_grads_batched=True)
+    weight = torch.randn((9, 16), device=device, requires_grad=True)
+    out = scaled_embedding(torch.zeros(5, dtype=torch.int64, device=device), weight)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(out, weight, torch.ones((2, *out.shape), device=device), is_grads_batched=True)
+
+
+def test_nothing_outlives_its_graph(device):
+    operands = _operands(device, (4, 512, 1024), seed=7)
+    ids = torch.randint(0, 100, (4, 512), device=device)
+    weight = torch.randn((100, 1024), device=device).to(BF).requires_grad_(True)
+    for _ in range(3):
+        before = torch.cuda.memory_allocated()
+        out = [*_norm(operands), scaled_embedding(ids, weight)]
+        torch.autograd.grad([t.sum() for t in out], [*operands, weight])
+        out = [*_norm(operands), scaled_embedding(ids, weight)]  # (and one without a backward)
+        del out
+        assert torch.cuda.memory_allocated() == before
+
+
+def test_two_graphs_and_two_streams(device):
+    """Two captured passes replayed in turn and out of turn, and two streams at work at once: no shared workspace."""
+    sets = []
+    for seed in (8, 9):
+        operands = _operands(device, (5, 700, 512), seed=seed)
+        ids = torch.randint(0, 3000, (9000,), device=device, generator=torch.Generator(device=device).manual_seed(seed))
+        d = torch.randn((9000, 96), device=device).to(BF)
+        sets.append(([t.detach() for t in operands], ids, d))
+
+    def work(s):
+        (h, r, post, gate, pre), ids, d = s
+        h2, r2 = h.view(-1, 512), r.view(-1, 512)
+        stream, normed, rstd = ops.residual_norm(h2, r2, post, gate.view(-1, 512), pre, 0.5, 1e-5, True)
+        grads = ops.residual_norm_bwd(h2, r2, post, gate.view(-1, 512), pre, 0.5, rstd, stream, normed)
+        table = ops.embedding_bwd(ids, d, 3000)
+        scaled = [g.clone() for g in grads]
+        norm = ops.grad_norm(scaled)
+        ops.grad_scale_(scaled, norm, 0.1)
+        return [stream, normed, *grads, table, norm, *scaled]
+
+    want = [[t.clone() for t in work(s)] for s in sets]
+    graphs, outs = [], []
+    for s in sets:
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            work(s)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(work(s))
+        graphs.append(graph)
+    for order in ((0, 1), (1, 0), (0, 0, 1, 1)):
+        for k in order:
+            graphs[k].replay()
+        torch.cuda.synchronize()
+        assert torch.randn(1 << 20, device=device).sum().isfinite()
+        for got, expected in zip(outs, want):
+            assert all(torch.equal(a, b) for a, b in zip(got, expected))
+    streams = [torch.cuda.Stream() for _ in sets]
+    for st in streams:
+        st.wait_stream(torch.cuda.current_stream())
+    got = []
+    for _ in range(5):
+        got = []
+        for st, s in zip(streams, sets):
+            with torch.cuda.stream(st):
+                got.append(work(s))
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))

@@ -799,9 +799,9 @@ std::optional<std::vector<Tensor>> dequant_many(const std::vector<Tensor>& codes
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
-// bf16 or float32 on the GPU, no subclass that sees its operations
+// bf16 or float32 values in GPU memory as they are, no subclass that sees its operations
 bool row_tensor(const Tensor& t) {
-  return t.is_cuda() && t.layout() == at::kStrided && (t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kFloat) &&
+  return t.is_cuda() && !t.is_neg() && t.layout() == at::kStrided && (t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kFloat) &&
          !t.unsafeGetTensorImpl()->is_python_dispatch();
 }
 int is_f32(const Tensor& t) { return t.scalar_type() == at::kFloat; }
@@ -863,6 +863,7 @@ struct EmbeddingNode : torch::autograd::Function<EmbeddingNode> {
     const int64_t n = ids.numel(), cols = dout.size(-1), rows = ctx->saved_data["rows"].toInt();
     TORCH_CHECK(dout.numel() == n * cols, "the saved ids came back as ", ids.sizes(), " for a gradient of ", dout.sizes());
     const bool f32 = ctx->saved_data["f32"].toBool();
+    dout = dout.resolve_neg();
     if (!row_pitch(dout, cols)) dout = dout.contiguous();
     const Tensor grad = at::empty({rows, cols}, dout.options().dtype(f32 ? at::kFloat : at::kBFloat16));
     const Tensor work = at::empty({lib.embedding_grad_workspace(n, rows, cols)}, dout.options().dtype(at::kByte));
@@ -950,8 +951,8 @@ struct ResidualNormNode : torch::autograd::Function<ResidualNormNode> {
     for (const Tensor& w : weights)
       TORCH_CHECK(!w.defined() || (row_tensor(w) && w.device() == h.device() && w.size(-1) == cols),
                   "a saved weight came back with another type or size");
-    if (dstream.defined()) dstream = dstream.contiguous();
-    if (dnormed.defined()) dnormed = dnormed.contiguous();
+    if (dstream.defined()) dstream = dstream.resolve_neg().contiguous();
+    if (dnormed.defined()) dnormed = dnormed.resolve_neg().contiguous();
     const int64_t wanted = ctx->saved_data["wanted"].toInt();
     const std::array<const Tensor*, 5> of = {&h, &r, &post, &gate, &pre};
     for (size_t i = 0; i < 5; ++i)

@@ -985,14 +985,15 @@ def plain_rows(*operands) -> bool:
     """The kernels below take these tensors (None among them: no operand): plain ones on the GPU, bf16 or float32,
     outside function transforms."""
     return not _transformed() and all(
-        t is None or (type(t) in (torch.Tensor, torch.nn.Parameter) and t.is_cuda and t.dtype in ROW_TYPES) for t in operands)
+        t is None or (type(t) in (torch.Tensor, torch.nn.Parameter) and t.is_cuda and t.dtype in ROW_TYPES and not t.is_neg())
+        for t in operands)
 
 
 def _rows_as_they_lie(t: torch.Tensor) -> torch.Tensor:
     """[rows, cols] with unit inner stride and rows that do not overlap (a copy where they do)."""
     if (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
-        return t.contiguous()
-    return t
+        t = t.contiguous()
+    return t.resolve_neg()
 
 
 def _row_type(t: torch.Tensor, what: str) -> int:
@@ -1060,7 +1061,7 @@ def _norm_operands(h, residual, post, gate, pre):
                     raise ValueError(f"gate must be [n, {cols}] with n dividing {rows}, got {tuple(w.shape)}")
             elif w.shape != (cols,):
                 raise ValueError(f"{name} must be [{cols}], got {tuple(w.shape)}")
-            w = w.contiguous()
+            w = w.resolve_neg().contiguous()
         weights.append(w)
     if residual.device != h.device:
         raise ValueError(f"residual on {residual.device}, h on {h.device}")
@@ -1100,7 +1101,7 @@ def residual_norm_bwd(h: torch.Tensor, residual: torch.Tensor, post: torch.Tenso
     for d, like in ((dstream, r), (dnormed, h)):
         if d is not None and (d.shape != like.shape or d.dtype != like.dtype or d.device != dev):
             raise TypeError("gradients must have their outputs' shape, type and device")
-    dstream, dnormed = (None if d is None else d.contiguous() for d in (dstream, dnormed))
+    dstream, dnormed = (None if d is None else d.resolve_neg().contiguous() for d in (dstream, dnormed))
     rstd = rstd.contiguous()
     grads = [torch.empty(t.shape, dtype=t.dtype, device=dev) if need and t is not None else None
              for need, t in zip(needs, (h, r, *weights))]
@@ -1122,8 +1123,8 @@ def _grad_lists(grads):
         _row_type(t, "gradients")
         if t.device != dev:
             raise ValueError(f"gradients on {dev} and {t.device}: one device a call")
-        if not is_dense(t):
-            raise ValueError(f"a gradient of shape {tuple(t.shape)} with strides {t.stride()} is not one run of memory")
+        if not is_dense(t) or t.is_neg():
+            raise ValueError(f"a gradient of shape {tuple(t.shape)} with strides {t.stride()} is not one run of memory as it is")
     return (len(grads), _host_table([_ptr(t) for t in grads], c_int64), _host_table([t.numel() for t in grads], c_int64),
             _host_table([int(t.dtype == torch.float32) for t in grads], c_int32))
 
