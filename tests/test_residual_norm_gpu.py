@@ -188,6 +188,13 @@ def test_wide_rows_with_gates_for_a_few_rows_each(device, rows, gates, dim):
         check(h, r, p, g, w, 1.1)
 
 
+@pytest.mark.parametrize("types", [(BF, BF, BF), (F32, F32, F32), (BF, F32, BF)], ids=["bf16", "f32", "mixed"])
+@pytest.mark.parametrize("dim", [4104, 5119, 5120, 5121, 6143, 6144, 6150, 7168])
+def test_rows_of_some_thousands(device, dim, types):
+    check(*make(device, (2, 300), dim, (True, True, True), types, gate_shape=(2, 1, dim)), 0.7)
+    check(*make(device, 515, dim, (False, False, True), types))
+
+
 def test_strides_and_alignment(device):
     g = torch.Generator(device=device).manual_seed(3)
     for dim, lo in ((512, 1), (2048, 3), (100, 5), (5000, 7)):

@@ -280,35 +280,36 @@ __global__ __launch_bounds__(S::kThreads) void residual_norm_kernel(NormArgs a, 
   }
 }
 
-// Rows of any width, one workgroup a row, element by element; what a later step needs of an earlier one is formed again.
-template <class H, class R>
-__global__ __launch_bounds__(kNormThreads) void residual_norm_any_kernel(NormArgs a, R* __restrict__ stream,
+// Rows of any width (below 8 and above 16384 columns), one workgroup a row, element by element; what a later step needs of an
+// earlier one is formed again: 2048 x 20000 231 us forward and 1355 backward, limited by the instructions of the repeated work.
+template <int THREADS, class H, class R>
+__global__ __launch_bounds__(THREADS) void residual_norm_any_kernel(NormArgs a, R* __restrict__ stream,
                                                                          H* __restrict__ normed, float* __restrict__ rstd) {
-  __shared__ float part[kNormThreads / 64];
+  __shared__ float part[THREADS / 64];
   const int64_t row = blockIdx.x;
   const H* h = (const H*)a.h + row * a.ldh;
   const R* r = (const R*)a.r + row * a.ldr;
   const int64_t g0 = row / a.gate_each * a.cols;
   float s1 = 1.f, s2 = 1.f, sum = 0.f;
   if (a.post.p) {
-    for (int64_t c = threadIdx.x; c < a.cols; c += kNormThreads) {
+    for (int64_t c = threadIdx.x; c < a.cols; c += THREADS) {
       const float x = norm_element(h + c);
       sum += x * x;
     }
-    s1 = 1.f / sqrtf(group_sum<kNormThreads>(sum, part) / (float)a.cols + a.eps);
+    s1 = 1.f / sqrtf(group_sum<THREADS>(sum, part) / (float)a.cols + a.eps);
   }
   auto total = [&](int64_t c) {
     return a.scale * norm_element(r + c) + a.gate.at(g0 + c) * (norm_element(h + c) * s1 * a.post.at(c));
   };
   sum = 0.f;
-  for (int64_t c = threadIdx.x; c < a.cols; c += kNormThreads) {
+  for (int64_t c = threadIdx.x; c < a.cols; c += THREADS) {
     const float t = total(c);
     stream[row * a.cols + c] = norm_rounded<R>(t);
     sum += t * t;
   }
   if (a.pre.p) {
-    s2 = 1.f / sqrtf(group_sum<kNormThreads>(sum, part) / (float)a.cols + a.eps);
-    for (int64_t c = threadIdx.x; c < a.cols; c += kNormThreads)
+    s2 = 1.f / sqrtf(group_sum<THREADS>(sum, part) / (float)a.cols + a.eps);
+    for (int64_t c = threadIdx.x; c < a.cols; c += THREADS)
       normed[row * a.cols + c] = norm_rounded<H>(total(c) * s2 * a.pre.at(c));
   }
   if (rstd && threadIdx.x == 0) {
@@ -335,20 +336,20 @@ struct NormGrads {
   int dgate_f32;
 };
 
-template <class H, class R>
-__global__ __launch_bounds__(kNormThreads) void residual_norm_bwd_any_kernel(NormArgs a, NormStrips strips,
+template <int THREADS, class H, class R>
+__global__ __launch_bounds__(THREADS) void residual_norm_bwd_any_kernel(NormArgs a, NormStrips strips,
                                                                              const float* __restrict__ rstd, NormGrads o) {
-  __shared__ float part[kNormThreads / 64];
+  __shared__ float part[THREADS / 64];
   float* dpost = o.rows_part + (int64_t)blockIdx.x * 3 * a.cols;
   float* dpre = dpost + a.cols;
   float* dgate = o.dgate ? dpre + a.cols : nullptr;
-  for (int64_t c = threadIdx.x; c < a.cols; c += kNormThreads) dpost[c] = dpre[c] = 0.f;
+  for (int64_t c = threadIdx.x; c < a.cols; c += THREADS) dpost[c] = dpre[c] = 0.f;
   const float width = (float)a.cols;
   for (int64_t strip = blockIdx.x; strip < strips.total; strip += gridDim.x) {
     const int64_t group = strip / strips.strips, first = group * a.gate_each + strip - group * strips.strips;
     const int64_t g0 = group * a.cols;
     if (dgate)
-      for (int64_t c = threadIdx.x; c < a.cols; c += kNormThreads) dgate[c] = 0.f;
+      for (int64_t c = threadIdx.x; c < a.cols; c += THREADS) dgate[c] = 0.f;
     for (int64_t row = first; row < (group + 1) * a.gate_each; row += strips.strips) {
       const H* h = (const H*)a.h + row * a.ldh;
       const R* r = (const R*)a.r + row * a.ldr;
@@ -359,15 +360,15 @@ __global__ __launch_bounds__(kNormThreads) void residual_norm_bwd_any_kernel(Nor
       auto hat = [&](int64_t c) { return (a.scale * norm_element(r + c) + a.gate.at(g0 + c) * branch(c)) * s2; };
       float mean = 0.f;
       if (dy) {
-        for (int64_t c = threadIdx.x; c < a.cols; c += kNormThreads) mean += norm_element(dy + c) * a.pre.at(c) * hat(c);
-        mean = group_sum<kNormThreads>(mean, part) / width;
+        for (int64_t c = threadIdx.x; c < a.cols; c += THREADS) mean += norm_element(dy + c) * a.pre.at(c) * hat(c);
+        mean = group_sum<THREADS>(mean, part) / width;
       }
       auto inner = [&](int64_t c) {
         const float e = ds ? norm_element(ds + c) : 0.f;
         return dy ? e + s2 * (norm_element(dy + c) * a.pre.at(c) - hat(c) * mean) : e;
       };
       float sum = 0.f;
-      for (int64_t c = threadIdx.x; c < a.cols; c += kNormThreads) {
+      for (int64_t c = threadIdx.x; c < a.cols; c += THREADS) {
         const float e = inner(c), q = e * a.gate.at(g0 + c), hs = norm_element(h + c) * s1;
         if (o.dr) ((R*)o.dr)[row * a.cols + c] = norm_rounded<R>(a.scale * e);
         if (dy) dpre[c] += norm_element(dy + c) * hat(c);
@@ -376,8 +377,8 @@ __global__ __launch_bounds__(kNormThreads) void residual_norm_bwd_any_kernel(Nor
         sum += q * a.post.at(c) * hs;
       }
       if (o.dh) {
-        if (a.post.p) sum = group_sum<kNormThreads>(sum, part) / width;
-        for (int64_t c = threadIdx.x; c < a.cols; c += kNormThreads) {
+        if (a.post.p) sum = group_sum<THREADS>(sum, part) / width;
+        for (int64_t c = threadIdx.x; c < a.cols; c += THREADS) {
           const float q = inner(c) * a.gate.at(g0 + c);
           const float d = a.post.p ? s1 * (q * a.post.at(c) - norm_element(h + c) * s1 * sum) : q;
           ((H*)o.dh)[row * a.cols + c] = norm_rounded<H>(d);
@@ -385,7 +386,7 @@ __global__ __launch_bounds__(kNormThreads) void residual_norm_bwd_any_kernel(Nor
       }
     }
     if (dgate)
-      for (int64_t c = threadIdx.x; c < a.cols; c += kNormThreads) {
+      for (int64_t c = threadIdx.x; c < a.cols; c += THREADS) {
         if (strips.strips > 1) o.gate_part[strip * a.cols + c] = dgate[c];
         else if (o.dgate_f32) ((float*)o.dgate)[group * a.cols + c] = dgate[c];
         else ((uint16_t*)o.dgate)[group * a.cols + c] = norm_rounded<uint16_t>(dgate[c]);
@@ -499,7 +500,7 @@ __global__ __launch_bounds__(S::kThreads) void residual_norm_bwd_kernel(NormArgs
         }
       }
       const float s1 = now.s1, s2 = now.s2;
-      if constexpr (!kHeld)  // (nothing of the weights is kept from row to row: 8192 x 16384 602 us, where what was kept spilled 975)
+      if constexpr (!kHeld)  // (nothing of the weights is kept from row to row: 8192 x 16384 412 us, where what was kept spilled 975)
 #pragma unroll
         for (int k = 0; k < N; ++k) asm volatile("" : "+v"(at[k].at));
       float hat[N][kV], u[N][kV];
@@ -645,46 +646,62 @@ __global__ __launch_bounds__(kNormThreads) void residual_norm_join_kernel(NormJo
 // 212 + 339; 147456 x 2048 424 + 663 / 445 + 704.
 static bool norm_past(int64_t elements, int h_f32, int r_f32) { return elements * (2 * (2 + !!h_f32 + !!r_f32)) > (384 << 20); }
 
-// Workgroups of `waves` waves for every CU.
-static int64_t norm_groups(int64_t cols, int waves) {
-  return 256 * 64 * waves / (cols <= 512 ? 256 : cols <= 1024 ? 128 : cols <= 2048 ? 256 : cols <= 4096 ? 512 : 1024);
-}
-// Forward: as many workgroups as stay resident come back for more rows; matrices that the last cache does not hold are
-// gone through in order, two rows a workgroup, up to 2048 columns.  us in turn / two rows: 147456 x 2048 461 / 419, 65536 x
-// 1024 (past no cache) 83 / 92, 73728 x 4096 448 / 460, 16384 x 8192 218 / 238.
-static int norm_pair(const NormArgs& a) { return a.past && a.cols <= 2048 ? 2 : 0; }
+// Calls f(shape) with the smallest shape that holds a row (640 and 768 lanes: 16384 x 5120 265 -> 192 us backward, x 6144 274 ->
+// 229, some of it by a workgroup for every CU; 896 lanes gain nothing over 1024), or f(threads) for rows that none does.
 template <class S>
-static int64_t norm_fwd_groups(const NormArgs& a) {
-  if (const int64_t pair = norm_pair(a)) return (a.rows + S::kRows * pair - 1) / (S::kRows * pair);
-  return std::min<int64_t>((a.rows + S::kRows - 1) / S::kRows, norm_groups(a.cols, 16));
-}
-
-// The backward pass has the waves that its registers let a CU hold: two a SIMD with the block's side; four without, three
-// for narrow rows (147456 x 2048: 702 us, with four 788; 16384 x 4096 135 and 132).
-static int64_t norm_bwd_groups(int64_t cols, bool side) { return norm_groups(cols, side ? 8 : cols <= 2048 ? 12 : 16); }
-
-// Calls f(shape) with the smallest shape that holds a row, or f(0) for rows that none does.
+constexpr bool norm_shaped = false;
+template <int LANES, int N>
+constexpr bool norm_shaped<NormShape<LANES, N>> = true;
 template <class F>
 static void norm_shape(int64_t cols, F&& f) {
-  if (cols < kV) f(0);
+  if (cols < kV) f(std::integral_constant<int, 64>());
   else if (cols <= NormShape<16, 1>::kCols) f(NormShape<16, 1>());
   else if (cols <= NormShape<32, 1>::kCols) f(NormShape<32, 1>());
   else if (cols <= NormShape<64, 1>::kCols) f(NormShape<64, 1>());
   else if (cols <= NormShape<128, 1>::kCols) f(NormShape<128, 1>());
   else if (cols <= NormShape<256, 1>::kCols) f(NormShape<256, 1>());
   else if (cols <= NormShape<512, 1>::kCols) f(NormShape<512, 1>());
+  else if (cols <= NormShape<640, 1>::kCols) f(NormShape<640, 1>());
+  else if (cols <= NormShape<768, 1>::kCols) f(NormShape<768, 1>());
   else if (cols <= NormShape<1024, 1>::kCols) f(NormShape<1024, 1>());
   else if (cols <= NormShape<1024, 2>::kCols) f(NormShape<1024, 2>());
-  else f(0);
+  else f(std::integral_constant<int, 1024>());
 }
+
+// Workgroups of `waves` waves for every CU, one at least (16384 x 8192 with the block's side 297 us, with one for two CUs 322; 8192 x
+// 16384 412 and 603).
+static int64_t norm_groups(int64_t cols, int waves) {
+  int threads = 0;
+  norm_shape(cols, [&](auto shape) {
+    using S = decltype(shape);
+    if constexpr (norm_shaped<S>) threads = S::kThreads;
+    else threads = S::value;
+  });
+  return 256 * std::max(1, 64 * waves / threads);
+}
+// Forward: as many workgroups as stay resident come back for more rows; matrices that the last cache does not hold are
+// gone through in order, two rows a workgroup, up to 2048 columns.  us in turn / two rows: 147456 x 2048 461 / 419, 65536 x
+// 1024 (past no cache) 83 / 92, 73728 x 4096 448 / 460, 16384 x 8192 218 / 238.  16 waves a CU stay, of workgroups of more than
+// 512 lanes two: 16384 x 5120 136 us with one, 123 with two, 141 with three; x 6144 164 and 149; x 4096 83, with twice as
+// many 93.
+static int norm_pair(const NormArgs& a) { return a.past && a.cols <= 2048 ? 2 : 0; }
+template <class S>
+static int64_t norm_fwd_groups(const NormArgs& a) {
+  if (const int64_t pair = norm_pair(a)) return (a.rows + S::kRows * pair - 1) / (S::kRows * pair);
+  return std::min<int64_t>((a.rows + S::kRows - 1) / S::kRows, norm_groups(a.cols, S::kThreads > 512 ? S::kThreads / 32 : 16));
+}
+
+// The backward pass has the waves that its registers let a CU hold: two a SIMD with the block's side; four without, three
+// for narrow rows (147456 x 2048: 702 us, with four 788; 16384 x 4096 135 and 132).
+static int64_t norm_bwd_groups(int64_t cols, bool side) { return norm_groups(cols, side ? 8 : cols <= 2048 ? 12 : 16); }
 
 // Strips for each row's lanes, for rows of the gate that have few rows themselves.  Where a workgroup takes several rows at
 // a time: if they work through their rows sooner so than together.  Where it takes one: up to 4 rows of one gate.  us
 // shared / so: 65536 x 512 with a gate for every row 394 / 108, x 1024 309 / 227, 16384 x 4096 277 / 216 and for every 4 rows
-// 170 / 169.  Rows of 1024 lanes have no registers for it (8192 x 8192 392 / 466).
+// 170 / 169.  Rows of more lanes have no registers for it (8192 x 8192 392 / 466).
 template <class S>
 constexpr bool norm_solo_shape() {
-  return S::kPieces == 1 && S::kLanes < 1024;
+  return S::kPieces == 1 && S::kLanes <= 512;
 }
 static bool norm_solo(int64_t rows, int64_t gate_rows, int64_t groups, int64_t together) {
   auto up = [](int64_t x, int64_t y) { return (x + y - 1) / y; };
@@ -701,7 +718,7 @@ struct NormBwdPlan {
 static NormBwdPlan norm_bwd_plan(int64_t rows, int64_t cols, int64_t gate_rows, bool side, bool gate) {
   int64_t together = 0;
   norm_shape(cols, [&](auto shape) {
-    if constexpr (!std::is_same_v<decltype(shape), int>) {
+    if constexpr (norm_shaped<decltype(shape)>) {
       if (norm_solo_shape<decltype(shape)>()) together = decltype(shape)::kRows;
     }
   });
@@ -729,7 +746,7 @@ static int norm_check(const void* h, int h_f32, const void* r, int r_f32, int64_
     return MX_ERR_ALIGNMENT;
   // (a launch has fewer than 2^32 lanes: rows with a workgroup each)
   const bool any = cols < kV || cols > NormShape<1024, 2>::kCols;
-  if (rows > (any ? 0xFFFFFF : 0x7FFFFFFF) || cols > 0x7FFFFFFF) return MX_ERR_UNSUPPORTED;
+  if (rows > (any ? 0x3FFFFF : 0x7FFFFFFF) || cols > 0x7FFFFFFF) return MX_ERR_UNSUPPORTED;
   return MX_OK;
 }
 
@@ -753,9 +770,9 @@ extern "C" int mx_residual_norm(const void* h, int h_f32, const void* r, int r_f
     using R = decltype(rt);
     norm_shape(cols, [&](auto shape) {
       using S = decltype(shape);
-      if constexpr (std::is_same_v<S, int>)
-        hipLaunchKernelGGL((residual_norm_any_kernel<H, R>), dim3((unsigned)rows), dim3(kNormThreads), 0, (hipStream_t)stream,
-                           a, (R*)stream_out, (H*)normed, rstd);
+      if constexpr (!norm_shaped<S>)
+        hipLaunchKernelGGL((residual_norm_any_kernel<S::value, H, R>), dim3((unsigned)rows), dim3(S::value), 0,
+                           (hipStream_t)stream, a, (R*)stream_out, (H*)normed, rstd);
       else
         hipLaunchKernelGGL((residual_norm_kernel<S, H, R>), dim3((unsigned)norm_fwd_groups<S>(a)), dim3(S::kThreads), 0,
                            (hipStream_t)stream, a, norm_pair(a), (R*)stream_out, (H*)normed, rstd);
@@ -802,8 +819,8 @@ extern "C" int mx_residual_norm_bwd(const void* h, int h_f32, const void* r, int
     using R = decltype(rt);
     norm_shape(cols, [&](auto shape) {
       using S = decltype(shape);
-      if constexpr (std::is_same_v<S, int>)
-        hipLaunchKernelGGL((residual_norm_bwd_any_kernel<H, R>), dim3((unsigned)groups), dim3(kNormThreads), 0, st, a, s, rstd, o);
+      if constexpr (!norm_shaped<S>)
+        hipLaunchKernelGGL((residual_norm_bwd_any_kernel<S::value, H, R>), dim3((unsigned)groups), dim3(S::value), 0, st, a, s, rstd, o);
       else {
         auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(S::kThreads), 0, st, a, s, rstd, o); };
         if (!post && !gate) launch(residual_norm_bwd_kernel<S, false, false, H, R>);
