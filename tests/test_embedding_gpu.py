@@ -236,3 +236,18 @@ def test_tables_around_a_digit_of_the_sort(device, rows):
     ids, weight, dout = make(device, 10007, rows, 8, torch.bfloat16, torch.bfloat16, rows)
     ids[:3] = torch.tensor([0, rows - 1, rows], device=device)
     check(ids, weight, 1.0, None, 0, torch.bfloat16, dout)
+
+
+@pytest.mark.parametrize("cols", [5, 63, 64, 65, 128, 200, 256, 257, 300, 511, 512, 513, 1024, 1030])
+@pytest.mark.parametrize("w_type,o_type", TYPES)
+def test_forward_of_every_width(device, cols, w_type, o_type):
+    """Every result is one product in float32 and its rounding: equal bits.  The table's rows are apart, ids lie on both sides of it."""
+    g = torch.Generator(device=device).manual_seed(cols)
+    weight = torch.randn((40, cols + 3), generator=g, device=device).to(w_type)[:, 1:cols + 1]
+    for n in (1, 3, 515):
+        ids = torch.randint(95, 145, (n,), generator=g, device=device)
+        out = scaled_embedding(ids, weight, 1.7, first_row=100, dtype=o_type)
+        row = ids - 100
+        inside = (row >= 0) & (row < 40)
+        want = torch.where(inside[:, None], weight.float()[row.clamp(0, 39)] * torch.tensor(1.7, device=device), 0.0).to(o_type)
+        assert torch.equal(out, want)

@@ -34,7 +34,7 @@ struct EmbIds {
   }
 };
 
-// One wave for 1024 columns of a token, all asked for before the first is stored: 147456 x 2048 151 us (604 MB written and
+// Wider rows: one wave for 1024 columns of a token, all asked for before the first is stored: 147456 x 2048 151 us (604 MB written and
 // as many read, most of them from the caches; with 2048 columns a wave 156), 8192 x 4096 of a shard 18 (with a wave for the
 // whole row 24).
 constexpr int kEmbPieces = 2, kEmbSlab = 64 * 8 * kEmbPieces;
@@ -68,6 +68,36 @@ __global__ __launch_bounds__(kEmbThreads) void embedding_kernel(EmbIds ids, int6
     const Piece<O, V> q = from_floats<O>(f);
     if (past) store_piece<true>(dst + c, cols - c, q);
     else store_piece<false>(dst + c, cols - c, q);
+  }
+}
+
+// Rows of up to 512 columns: 8 to 64 lanes (1 << shift) a token, a piece each, two tokens a lane.  us for a million tokens, with a
+// wave for each / so: 512 columns 290 / 272, 256 254 / 134, 64 259 / 34.
+constexpr int kEmbTokens = 2;
+template <class W, class O>
+__global__ __launch_bounds__(kEmbThreads) void embedding_narrow_kernel(EmbIds ids, int64_t n, const W* __restrict__ weight,
+                                                                       int64_t cols, int64_t ldw, float scale, bool past, int shift,
+                                                                       O* __restrict__ out) {
+  constexpr int V = 8;
+  const int64_t c = (int64_t)(threadIdx.x & ((1 << shift) - 1)) * V, left = cols - c;
+  const int64_t step = kEmbThreads >> shift, t0 = (int64_t)blockIdx.x * step * kEmbTokens + (threadIdx.x >> shift);
+  uint32_t r[kEmbTokens];
+#pragma unroll
+  for (int k = 0; k < kEmbTokens; ++k) r[k] = t0 + k * step < n ? ids.row(t0 + k * step) : (uint32_t)ids.rows;
+  Piece<W, V> p[kEmbTokens];
+#pragma unroll
+  for (int k = 0; k < kEmbTokens; ++k) load_piece<false>(weight + (int64_t)r[k] * ldw + c, r[k] < (uint32_t)ids.rows ? left : 0, p[k]);
+#pragma unroll
+  for (int k = 0; k < kEmbTokens; ++k) {
+    if (t0 + k * step >= n) break;
+    float f[V];
+    to_floats(p[k], f);
+#pragma unroll
+    for (int e = 0; e < V; ++e) f[e] = r[k] < (uint32_t)ids.rows ? f[e] * scale : 0.f;
+    const Piece<O, V> q = from_floats<O>(f);
+    O* dst = out + (t0 + k * step) * cols + c;
+    if (past) store_piece<true>(dst, left, q);
+    else store_piece<false>(dst, left, q);
   }
 }
 
@@ -549,6 +579,14 @@ extern "C" int mx_embedding(const void* ids, int ids_i64, int64_t n, const void*
   const EmbIds e{ids, ids_i64 != 0, first, rows, 0};
   of_type(weight_f32, [&](auto w) {
     of_type(out_f32, [&](auto o) {
+      if (cols <= 512) {
+        const int shift = cols <= 64 ? 3 : cols <= 128 ? 4 : cols <= 256 ? 5 : 6;
+        const int64_t per = (int64_t)(kEmbThreads >> shift) * kEmbTokens;
+        hipLaunchKernelGGL((embedding_narrow_kernel<decltype(w), decltype(o)>), dim3((unsigned)((n + per - 1) / per)), dim3(kEmbThreads), 0,
+                           (hipStream_t)stream, e, n, (const decltype(w)*)weight, cols, ldw, scale,
+                           emb_past(n * cols * (out_f32 ? 4 : 2)), shift, (decltype(o)*)out);
+        return;
+      }
       hipLaunchKernelGGL((embedding_kernel<decltype(w), decltype(o)>), dim3((unsigned)groups), dim3(kEmbThreads), 0,
                          (hipStream_t)stream, e, n, (const decltype(w)*)weight, cols, ldw, scale,
                          emb_past(n * cols * (out_f32 ? 4 : 2)), (uint32_t)slabs, (decltype(o)*)out);
