@@ -195,6 +195,17 @@ def test_rows_of_some_thousands(device, dim, types):
     check(*make(device, 515, dim, (False, False, True), types))
 
 
+@pytest.mark.parametrize("shape,dim,kind", [((16, 3200), 2048, (True, True, True)), ((1, 51201), 2047, (True, True, True)),
+                                            ((51200,), 2048, (False, False, True)), ((25603,), 4096, (True, False, True)),
+                                            ((10, 10241), 1000, (True, True, True)), ((40, 5121), 512, (False, True, True)),
+                                            ((400, 256), 1024, (True, True, True)), ((205000,), 505, (True, True, True)),
+                                            ((51200, 1), 2048, (True, True, True))])
+def test_matrices_that_no_cache_holds(device, shape, dim, kind):
+    gate_shape = (shape[0], *[1] * (len(shape) - 1), dim) if len(shape) > 1 else None
+    check(*make(device, shape, dim, kind, gate_shape=gate_shape), 0.8)
+    torch.cuda.empty_cache()
+
+
 def test_strides_and_alignment(device):
     g = torch.Generator(device=device).manual_seed(3)
     for dim, lo in ((512, 1), (2048, 3), (100, 5), (5000, 7)):

@@ -319,10 +319,17 @@ __global__ __launch_bounds__(THREADS) void residual_norm_any_kernel(NormArgs a, 
 }
 
 // How the rows are dealt out in the backward pass: `strips` workgroups' worth to every row of the gate, which take its
-// rows in turn, so that the chip works its way through memory in order (16384 x 4096: 139 us, with strips of rows that
+// rows in turn, so that the chip works its way through memory in order (16384 x 4096: 133 us, with strips of rows that
 // lie together 150); a workgroup takes every gridDim.x-th strip.
+// `run`: workgroup b, which runs on XCD b mod 8, takes the strips as if `run` of them were dealt to one XCD after the
+// other; 1: in the order of b.
 struct NormStrips {
   int64_t strips, total;
+  unsigned run;
+  __device__ __forceinline__ int64_t mine() const {
+    const unsigned b = blockIdx.x;
+    return (int64_t)(b / (8 * run)) * (8 * run) + b % 8 * run + b / 8 % run;
+  }
 };
 
 struct NormGrads {
@@ -470,7 +477,7 @@ __global__ __launch_bounds__(S::kThreads) void residual_norm_bwd_kernel(NormArgs
   RawWeight gate_next;
   float gate1[kV], post1[kV];
   if constexpr (SOLO) weight_at(a.post, 0, at[0], post1);
-  for (int64_t strip = (int64_t)blockIdx.x * kStrips + (SOLO ? sub : 0); strip < strips.total; strip += (int64_t)gridDim.x * kStrips) {
+  for (int64_t strip = strips.mine() * kStrips + (SOLO ? sub : 0); strip < strips.total; strip += (int64_t)gridDim.x * kStrips) {
     const int64_t group = (uint32_t)strip / (uint32_t)strips.strips, first = group * a.gate_each + (strip - group * strips.strips) * kTogether;
     const int64_t end = (group + 1) * a.gate_each, hop = strips.strips * kTogether;
     const int64_t g0 = group * a.cols;
@@ -691,9 +698,19 @@ static int64_t norm_fwd_groups(const NormArgs& a) {
   return std::min<int64_t>((a.rows + S::kRows - 1) / S::kRows, norm_groups(a.cols, S::kThreads > 512 ? S::kThreads / 32 : 16));
 }
 
-// The backward pass has the waves that its registers let a CU hold: two a SIMD with the block's side; four without, three
-// for narrow rows (147456 x 2048: 702 us, with four 788; 16384 x 4096 135 and 132).
-static int64_t norm_bwd_groups(int64_t cols, bool side) { return norm_groups(cols, side ? 8 : cols <= 2048 ? 12 : 16); }
+// The backward pass, waves a CU: with the block's side the 8 that its registers allow, without it 16, or 8 for narrow rows.  With
+// the block's side and matrices that the last cache does not hold as many workgroups as bring 6 waves' worth of columns, one at least: the
+// fewer are on their way, the better they stay in the order of memory (147456 x 2048 768 -> 649 us, x 1024 358 -> 332, 300000 x 512
+// 367 -> 327; 32768 x 2048, which it nearly holds, 138 -> 150).
+static int64_t norm_bwd_groups(int64_t cols, bool side, bool past) {
+  if (!side) return norm_groups(cols, cols <= 2048 ? 8 : 16);
+  if (!past) return norm_groups(cols, 8);
+  int64_t together = 1;
+  norm_shape(cols, [&](auto shape) {
+    if constexpr (norm_shaped<decltype(shape)>) together = decltype(shape)::kRows;
+  });
+  return 256 * std::max<int64_t>(1, 6 * 64 * kV / (cols * together));
+}
 
 // Strips for each row's lanes, for rows of the gate that have few rows themselves.  Where a workgroup takes several rows at
 // a time: if they work through their rows sooner so than together.  Where it takes one: up to 4 rows of one gate.  us
@@ -715,17 +732,22 @@ struct NormBwdPlan {
   int64_t groups;
   bool solo;
 };
-static NormBwdPlan norm_bwd_plan(int64_t rows, int64_t cols, int64_t gate_rows, bool side, bool gate) {
+static NormBwdPlan norm_bwd_plan(int64_t rows, int64_t cols, int64_t gate_rows, bool side, bool gate, bool past) {
   int64_t together = 0;
   norm_shape(cols, [&](auto shape) {
     if constexpr (norm_shaped<decltype(shape)>) {
       if (norm_solo_shape<decltype(shape)>()) together = decltype(shape)::kRows;
     }
   });
-  const int64_t groups = norm_bwd_groups(cols, side), strips = std::max<int64_t>(1, std::min(groups, rows) / gate_rows);
+  // (with more gates than CUs the rows are in no such order: 147456 x 2048 with a gate each 1422 -> 929 us)
+  const int64_t groups = norm_bwd_groups(cols, side, past && gate_rows <= 256), strips = std::max<int64_t>(1, std::min(groups, rows) / gate_rows);
   const bool solo = gate && strips == 1 && together > 0 && norm_solo(rows, gate_rows, groups, together);
   const int64_t total = strips * gate_rows, units = solo ? (total + together - 1) / together : total;
-  return {{strips, total}, std::min(units, groups), solo};
+  // Matrices that the last cache does not hold: an XCD's strips lie together, an eighth of them all, with the block's side and one
+  // gate eight.  us in the order of b / by eighths / by eights: 147456 x 2048 with 16 gates 707 / 696 / 726, without the block's side 690 /
+  // 687 / 707, 73728 x 4096 without it 716 / 673 / 704, with it 804 / 796 / 717, 16384 x 8192 298 / 296 / 288.
+  const int64_t used = std::min(units, groups), run = !past ? 1 : side && gate_rows == 1 ? 8 : used / 8;
+  return {{strips, total, (unsigned)(run > 0 && used % (8 * run) == 0 ? run : 1)}, used, solo};
 }
 
 template <class F>
@@ -784,8 +806,8 @@ extern "C" int mx_residual_norm(const void* h, int h_f32, const void* r, int r_f
 extern "C" int64_t mx_residual_norm_workspace(int64_t rows, int64_t cols, int64_t gate_rows) {
   if (rows <= 0 || cols <= 0 || gate_rows < 1 || rows % gate_rows) return 0;
   int64_t most = 0;
-  for (bool side : {false, true}) {
-    const NormBwdPlan p = norm_bwd_plan(rows, cols, gate_rows, side, false);  // (with a gate: no more workgroups)
+  for (int form = 0; form < 4; ++form) {
+    const NormBwdPlan p = norm_bwd_plan(rows, cols, gate_rows, form & 1, false, form & 2);  // (with a gate: no more workgroups)
     most = std::max(most, 3 * p.groups + (p.strips.strips > 1 ? p.strips.total : 0));
   }
   return 4 * cols * most;
@@ -807,7 +829,7 @@ extern "C" int mx_residual_norm_bwd(const void* h, int h_f32, const void* r, int
     return MX_ERR_ALIGNMENT;
   const NormArgs a{h, r, rows, cols, ldh, ldr, {post, weights_f32 & 1}, {gate, weights_f32 & 2}, {pre, weights_f32 & 4},
                    rows / gate_rows, scale, 0.f, norm_past(rows * cols, h_f32, r_f32)};
-  const NormBwdPlan plan = norm_bwd_plan(rows, cols, gate_rows, post || gate, gate);
+  const NormBwdPlan plan = norm_bwd_plan(rows, cols, gate_rows, post || gate, gate, a.past);
   const NormStrips s = plan.strips;
   const int64_t groups = plan.groups;
   float* rows_part = (float*)workspace;
