@@ -704,12 +704,13 @@ static int64_t norm_fwd_groups(const NormArgs& a) {
 // 367 -> 327; 32768 x 2048, which it nearly holds, 138 -> 150).
 static int64_t norm_bwd_groups(int64_t cols, bool side, bool past) {
   if (!side) return norm_groups(cols, cols <= 2048 ? 8 : 16);
-  if (!past) return norm_groups(cols, 8);
+  const int64_t most = norm_groups(cols, 8);
+  if (!past) return most;
   int64_t together = 1;
   norm_shape(cols, [&](auto shape) {
     if constexpr (norm_shaped<decltype(shape)>) together = decltype(shape)::kRows;
   });
-  return 256 * std::max<int64_t>(1, 6 * 64 * kV / (cols * together));
+  return std::min(most, 256 * std::max<int64_t>(1, 6 * 64 * kV / (cols * together)));
 }
 
 // Strips for each row's lanes, for rows of the gate that have few rows themselves.  Where a workgroup takes several rows at
