@@ -161,6 +161,22 @@ def test_entry_points_check_their_arguments_before_any_launch():
     assert lib.mx_grad_norm_workspace(0) == 0 and lib.mx_grad_norm_workspace(161) == 2 * lib.mx_grad_norm_workspace(160)
 
 
+def test_entry_points_refuse_what_no_launch_holds():
+    """A launch has fewer than 2^32 lanes, and rows are counted in 32 bits: status 4, before any launch."""
+    lib, a = _lib.load(), c_void_p(0x1000)
+    assert lib.mx_embedding(a, 1, 1 << 26, a, 0, 10, 8, 8, 0, 1.0, a, 0, None) == 4
+    assert lib.mx_embedding(a, 1, 1 << 20, a, 0, 10, 1 << 17, 1 << 17, 0, 1.0, a, 0, None) == 4
+    assert lib.mx_embedding(a, 1, 5, a, 0, 10, 1 << 40, 1 << 40, 0, 1.0, a, 0, None) == 4
+    assert lib.mx_embedding_grad(a, 1, 4, a, 0, 1 << 28, 9, 1 << 28, 0, -1, 1.0, a, 0, a, None) == 4
+    assert lib.mx_embedding_grad(a, 1, 4, a, 0, 4096, 1 << 24, 4096, 0, -1, 1.0, a, 0, a, None) == 4
+    assert lib.mx_embedding_grad(a, 1, 1 << 30, a, 0, 8, 9, 8, 0, -1, 1.0, a, 0, a, None) == 4
+    norm = lambda rows, cols: lib.mx_residual_norm(a, 0, a, 0, rows, cols, cols, cols, None, None, None, 0, 1, 1.0, 1e-5, a, None, None, None)
+    assert norm(1 << 22, 5) == 4 and norm(1 << 22, 20000) == 4 and norm(1, 1 << 31) == 4
+    ptrs, sizes, kinds = (c_void_p * 2)(0x1000, 0x2000), (_lib._I * 2)(1 << 36, 1 << 36), (c_int32 * 2)(1, 0)
+    assert lib.mx_grad_norm(2, ptrs, sizes, kinds, 0, a, a, None) == 4
+    assert lib.mx_grad_clip(2, ptrs, sizes, kinds, 0, a, 1.0, a, None) == 4
+
+
 def test_embedding_and_norms_trace_without_a_break():
     """Off the GPU their formulas are traced, one graph; on it (fake tensors) one operator each."""
     class Two(torch.nn.Module):
@@ -178,6 +194,7 @@ def test_embedding_and_norms_trace_without_a_break():
     traced = torch.compile(module, backend=lambda graph, example: graphs.append(graph) or graph.forward, fullgraph=True)
     assert all(torch.equal(a, b) for a, b in zip(traced(ids), module(ids))) and len(graphs) == 1
     torch._dynamo.reset()
+    import torchtitan_amd.compiled  # noqa: F401
     from torch._subclasses.fake_tensor import FakeTensorMode
 
     with FakeTensorMode():
