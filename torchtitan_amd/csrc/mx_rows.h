@@ -10,10 +10,9 @@
 namespace mx {
 
 typedef uint32_t u32x4_el2 __attribute__((ext_vector_type(4), aligned(2)));
-typedef uint32_t u32x2_el2 __attribute__((ext_vector_type(2), aligned(2)));
 typedef uint32_t u32x4_el4 __attribute__((ext_vector_type(4), aligned(4)));
 
-// V elements of T as they lie in memory.
+// V elements of T as they lie in memory: 16 bytes or 32.
 template <class T, int V>
 struct Piece {
   static constexpr int kWords = V * (int)sizeof(T) / 4;
@@ -22,34 +21,22 @@ struct Piece {
 
 template <bool NT, class T, int V>
 __device__ __forceinline__ void load_words(const T* p, Piece<T, V>& q) {
-  if constexpr (Piece<T, V>::kWords == 2) {
-    const u32x2_el2* s = reinterpret_cast<const u32x2_el2*>(p);
-    const u32x2_el2 v = NT ? __builtin_nontemporal_load(s) : *s;
-    q.w[0] = v.x, q.w[1] = v.y;
-  } else {
-    using W = std::conditional_t<sizeof(T) == 4, u32x4_el4, u32x4_el2>;
+  using W = std::conditional_t<sizeof(T) == 4, u32x4_el4, u32x4_el2>;
 #pragma unroll
-    for (int k = 0; k < Piece<T, V>::kWords / 4; ++k) {
-      const W* s = reinterpret_cast<const W*>(p) + k;
-      const W v = NT ? __builtin_nontemporal_load(s) : *s;
-      q.w[4 * k] = v.x, q.w[4 * k + 1] = v.y, q.w[4 * k + 2] = v.z, q.w[4 * k + 3] = v.w;
-    }
+  for (int k = 0; k < Piece<T, V>::kWords / 4; ++k) {
+    const W* s = reinterpret_cast<const W*>(p) + k;
+    const W v = NT ? __builtin_nontemporal_load(s) : *s;
+    q.w[4 * k] = v.x, q.w[4 * k + 1] = v.y, q.w[4 * k + 2] = v.z, q.w[4 * k + 3] = v.w;
   }
 }
 template <bool NT, class T, int V>
 __device__ __forceinline__ void store_words(T* p, const Piece<T, V>& q) {
-  if constexpr (Piece<T, V>::kWords == 2) {
-    u32x2_el2* d = reinterpret_cast<u32x2_el2*>(p);
-    const u32x2_el2 v = {q.w[0], q.w[1]};
-    if (NT) __builtin_nontemporal_store(v, d); else *d = v;
-  } else {
-    using W = std::conditional_t<sizeof(T) == 4, u32x4_el4, u32x4_el2>;
+  using W = std::conditional_t<sizeof(T) == 4, u32x4_el4, u32x4_el2>;
 #pragma unroll
-    for (int k = 0; k < Piece<T, V>::kWords / 4; ++k) {
-      W* d = reinterpret_cast<W*>(p) + k;
-      const W v = {q.w[4 * k], q.w[4 * k + 1], q.w[4 * k + 2], q.w[4 * k + 3]};
-      if (NT) __builtin_nontemporal_store(v, d); else *d = v;
-    }
+  for (int k = 0; k < Piece<T, V>::kWords / 4; ++k) {
+    W* d = reinterpret_cast<W*>(p) + k;
+    const W v = {q.w[4 * k], q.w[4 * k + 1], q.w[4 * k + 2], q.w[4 * k + 3]};
+    if (NT) __builtin_nontemporal_store(v, d); else *d = v;
   }
 }
 
