@@ -432,7 +432,9 @@ __device__ __forceinline__ void rows_joined(float (&acc)[S::kPieces][kV], float*
 // gradient, times the gate post's.
 // SOLO: the lanes of a row take strips of their own (see norm_solo), of a row of the gate each; the next strip's first row
 // and gate are on their way while one is worked on.
-template <class S, bool SIDE, bool SOLO, class H, class R>
+// NORMED: normed has a gradient.  Without one e is dstream as it is: nothing of t, which may be infinite, is in the
+// result, and neither residual nor a sum over the row is needed for it.
+template <class S, bool SIDE, bool SOLO, bool NORMED, class H, class R>
 __global__ __launch_bounds__(S::kThreads) void residual_norm_bwd_kernel(NormArgs a, NormStrips strips,
                                                                         const float* __restrict__ rstd, NormGrads o) {
   constexpr int N = S::kPieces;
@@ -444,7 +446,7 @@ __global__ __launch_bounds__(S::kThreads) void residual_norm_bwd_kernel(NormArgs
   struct Row {
     Piece<H, kV> h[N], dy[N];
     Piece<R, kV> r[N], ds[N];
-    float s1, s2;
+    float s1 = 1.f, s2 = 1.f;
   };
   NormPlace at[N];
 #pragma unroll
@@ -452,21 +454,22 @@ __global__ __launch_bounds__(S::kThreads) void residual_norm_bwd_kernel(NormArgs
   auto fetch = [&](Row& q, int64_t i) {
 #pragma unroll
     for (int k = 0; k < N; ++k) {
-      load_at<true>((const H*)a.h + i * a.ldh, at[k], q.h[k]);
-      load_at<true>((const R*)a.r + i * a.ldr, at[k], q.r[k]);
-      q.dy[k] = Piece<H, kV>{};
+      if constexpr (SIDE || NORMED) load_at<true>((const H*)a.h + i * a.ldh, at[k], q.h[k]);
+      if constexpr (NORMED) {
+        load_at<true>((const R*)a.r + i * a.ldr, at[k], q.r[k]);
+        load_at<true>((const H*)o.dnormed + i * a.cols, at[k], q.dy[k]);
+      }
       q.ds[k] = Piece<R, kV>{};
-      if (o.dnormed) load_at<true>((const H*)o.dnormed + i * a.cols, at[k], q.dy[k]);
       if (o.dstream) load_at<true>((const R*)o.dstream + i * a.cols, at[k], q.ds[k]);
     }
-    q.s1 = rstd[i];
-    q.s2 = rstd[a.rows + i];
+    if constexpr (SIDE || NORMED) q.s1 = rstd[i];
+    if constexpr (NORMED) q.s2 = rstd[a.rows + i];
   };
   // pre, and gate * post of the strip, of piece k
   float pre1[kV], side1[kV];
   auto pre_at = [&](int k, float (&f)[kV]) { weight_at(a.pre, 0, at[k], f); };
   const bool ragged = a.cols % kV != 0;
-  if constexpr (kHeld) pre_at(0, pre1);
+  if constexpr (kHeld && NORMED) pre_at(0, pre1);
   float dpre[N][kV] = {}, dpost[N][kV] = {};
   int turn = 0;
   constexpr int kTogether = SOLO ? 1 : S::kRows;  // rows that a strip takes at a time
@@ -510,27 +513,29 @@ __global__ __launch_bounds__(S::kThreads) void residual_norm_bwd_kernel(NormArgs
       if constexpr (!kHeld)  // (nothing of the weights is kept from row to row: 8192 x 16384 412 us, where what was kept spilled 975)
 #pragma unroll
         for (int k = 0; k < N; ++k) asm volatile("" : "+v"(at[k].at));
-      float hat[N][kV], u[N][kV];
+      float hat[N][kV], u[N][kV], mean = 0.f;
+      if constexpr (NORMED) {
 #pragma unroll
-      for (int k = 0; k < N; ++k) {
-        float x[kV], y[kV], d[kV], w[kV];
-        to_floats(now.h[k], x);
-        to_floats(now.r[k], y);
-        to_floats(now.dy[k], d);
-        if constexpr (SIDE) {
-          if constexpr (!kHeld) side_at(a, g0, at[k], w);
+        for (int k = 0; k < N; ++k) {
+          float x[kV], y[kV], d[kV], w[kV];
+          to_floats(now.h[k], x);
+          to_floats(now.r[k], y);
+          to_floats(now.dy[k], d);
+          if constexpr (SIDE) {
+            if constexpr (!kHeld) side_at(a, g0, at[k], w);
 #pragma unroll
-          for (int e = 0; e < kV; ++e) x[e] = x[e] * s1 * (kHeld ? side1[e] : w[e]);
+            for (int e = 0; e < kV; ++e) x[e] = x[e] * s1 * (kHeld ? side1[e] : w[e]);
+          }
+          if constexpr (!kHeld) pre_at(k, w);
+#pragma unroll
+          for (int e = 0; e < kV; ++e) {
+            hat[k][e] = __builtin_fmaf(a.scale, y[e], x[e]) * s2;
+            dpre[k][e] = __builtin_fmaf(d[e], hat[k][e], dpre[k][e]);
+            u[k][e] = d[e] * (kHeld ? pre1[e] : w[e]);
+          }
         }
-        if constexpr (!kHeld) pre_at(k, w);
-#pragma unroll
-        for (int e = 0; e < kV; ++e) {
-          hat[k][e] = __builtin_fmaf(a.scale, y[e], x[e]) * s2;
-          dpre[k][e] = __builtin_fmaf(d[e], hat[k][e], dpre[k][e]);
-          u[k][e] = d[e] * (kHeld ? pre1[e] : w[e]);
-        }
+        mean = lanes_sum<S::kLanes>(own_products(u, hat, at, ragged), part[turn][0]) * per;
       }
-      const float mean = lanes_sum<S::kLanes>(own_products(u, hat, at, ragged), part[turn][0]) * per;
       float (&q)[N][kV] = u;  // (in place: what h's gradient is formed from)
 #pragma unroll
       for (int k = 0; k < N; ++k) {
@@ -538,7 +543,7 @@ __global__ __launch_bounds__(S::kThreads) void residual_norm_bwd_kernel(NormArgs
         to_floats(now.ds[k], e1);
 #pragma unroll
         for (int e = 0; e < kV; ++e) {
-          e1[e] = __builtin_fmaf(s2, __builtin_fmaf(-hat[k][e], mean, u[k][e]), e1[e]);
+          if constexpr (NORMED) e1[e] = __builtin_fmaf(s2, __builtin_fmaf(-hat[k][e], mean, u[k][e]), e1[e]);
           dr[e] = a.scale * e1[e];
         }
         if (o.dr) store_at((R*)o.dr + row * a.cols, at[k], dr, a.past);
@@ -846,9 +851,14 @@ extern "C" int mx_residual_norm_bwd(const void* h, int h_f32, const void* r, int
         hipLaunchKernelGGL((residual_norm_bwd_any_kernel<S::value, H, R>), dim3((unsigned)groups), dim3(S::value), 0, st, a, s, rstd, o);
       else {
         auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(S::kThreads), 0, st, a, s, rstd, o); };
-        if (!post && !gate) launch(residual_norm_bwd_kernel<S, false, false, H, R>);
-        else if (!plan.solo) launch(residual_norm_bwd_kernel<S, true, false, H, R>);
-        else if constexpr (norm_solo_shape<S>()) launch(residual_norm_bwd_kernel<S, true, true, H, R>);
+        auto form = [&](auto normed) {
+          constexpr bool kNormed = decltype(normed)::value;
+          if (!post && !gate) launch(residual_norm_bwd_kernel<S, false, false, kNormed, H, R>);
+          else if (!plan.solo) launch(residual_norm_bwd_kernel<S, true, false, kNormed, H, R>);
+          else if constexpr (norm_solo_shape<S>()) launch(residual_norm_bwd_kernel<S, true, true, kNormed, H, R>);
+        };
+        if (dnormed) form(std::true_type());
+        else form(std::false_type());
       }
     });
   });
