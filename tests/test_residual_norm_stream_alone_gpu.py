@@ -83,3 +83,37 @@ def test_what_is_not_finite_in_the_block_output(device, dim, kind):
     for types in TYPES:
         for value in (INF, NAN, -INF):
             check(device, dim, kind, types, [("h", value)])
+
+
+@pytest.mark.parametrize("pre", [False, True])
+@pytest.mark.parametrize("dim", [5, 12, 640, 4096, 9001, 16400])
+def test_what_is_not_finite_behind_a_gate(device, dim, pre):
+    """A gate without a norm in front of it: the block's gradient has nothing of the block's output in it."""
+    for types in TYPES:
+        for value in (INF, NAN, -INF):
+            check(device, dim, (False, True, pre), types, [("h", value)])
+
+
+@pytest.mark.parametrize("dim", [640, 2048])
+def test_a_gate_for_every_row(device, dim):
+    """The lanes of a row take gates of their own."""
+    rows = 4099
+    g = torch.Generator(device=device).manual_seed(dim)
+    h, r, ds, gate = (torch.randn((rows, dim), generator=g, device=device) for _ in range(4))
+    post = 1 + 0.3 * torch.randn(dim, generator=g, device=device)
+    h[5, 7], r[9, 3], r[4000, dim - 1] = INF, INF, NAN
+    for weight in (None, post):
+        leaves = [t.detach().requires_grad_(True) for t in (h, r, gate)]
+        stream, _ = residual_rms_norm(leaves[0], leaves[1], gate=leaves[2], post_weight=weight, residual_scale=0.5)
+        got = torch.autograd.grad(stream, leaves, ds)
+        k = h.double()
+        s = torch.ones((rows, 1), dtype=torch.float64, device=device) if weight is None else torch.rsqrt(k.square().mean(1, keepdim=True) + EPS)
+        n, p = k * s, 1.0 if weight is None else weight.double()
+        q = ds.double() * gate.double() * p
+        mean = 0.0 if weight is None else (q * n).mean(1, keepdim=True)
+        dh = q if weight is None else s * (q - n * mean)
+        room = s * (q.abs() + (0.0 if weight is None else n.abs() * (q * n).abs().mean(1, keepdim=True)))
+        assert torch.equal(got[1], 0.5 * ds)
+        for a, b, absolute in ((got[0].double(), dh, room), (got[2].double(), ds.double() * n * p, (ds.double() * n * p).abs())):
+            assert torch.equal(a.isnan(), b.isnan()) and torch.equal(a[b.isinf()], b[b.isinf()])
+            assert ((a - b).abs() <= 170 * U * absolute)[b.isfinite()].all()

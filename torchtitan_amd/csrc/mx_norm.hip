@@ -562,14 +562,16 @@ __global__ __launch_bounds__(S::kThreads) void residual_norm_bwd_kernel(NormArgs
         }
       }
       if constexpr (SIDE) {
-        const float mean1 = a.post.p ? lanes_sum<S::kLanes>(own_products(q, hat, at, ragged), part[turn][1]) * per : 0.f;
-        if (o.dh) {
+        if (a.post.p) {  // (else q is the gradient: h, which may be infinite, is not in it)
+          const float mean1 = lanes_sum<S::kLanes>(own_products(q, hat, at, ragged), part[turn][1]) * per;
 #pragma unroll
-          for (int k = 0; k < N; ++k) {
+          for (int k = 0; k < N; ++k)
 #pragma unroll
             for (int e = 0; e < kV; ++e) q[k][e] = s1 * __builtin_fmaf(-hat[k][e], mean1, q[k][e]);
-            store_at((H*)o.dh + row * a.cols, at[k], q[k], a.past);
-          }
+        }
+        if (o.dh) {
+#pragma unroll
+          for (int k = 0; k < N; ++k) store_at((H*)o.dh + row * a.cols, at[k], q[k], a.past);
         }
       }
       if constexpr (kHeld) now = next;
