@@ -402,3 +402,20 @@ def test_two_graphs_and_two_streams(device):
     torch.cuda.synchronize()
     for a, b in zip(got, want):
         assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_more_rows_than_two_a_workgroup_reach(device):
+    """2^29 rows of 16 lanes each, two a lane: 2^32 lanes, one more than a launch has.  The first and last rows against the
+    operator on them alone."""
+    rows, dim, few = (1 << 29) + 5, 8, 4099
+    h, r = (torch.zeros((rows, dim), dtype=BF, device=device) for _ in range(2))
+    post, pre = (1 + torch.rand(dim, device=device).to(BF) for _ in range(2))
+    for part in (slice(0, few), slice(rows - few, rows)):
+        h[part], r[part] = (torch.randn((few, dim), device=device).to(BF) for _ in range(2))
+    stream, normed, rstd = ops.residual_norm(h, r, post, None, pre, 0.5, 1e-5, want_rstd=True)
+    for part in (slice(0, few), slice(rows - few, rows)):
+        alone = ops.residual_norm(h[part], r[part], post, None, pre, 0.5, 1e-5, want_rstd=True)
+        assert torch.equal(stream[part], alone[0]) and torch.equal(normed[part], alone[1]) and torch.equal(rstd[:, part], alone[2])
+    assert not stream[few:-few:4097].any()
+    del h, r, stream, normed, rstd
+    torch.cuda.empty_cache()

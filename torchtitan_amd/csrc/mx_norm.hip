@@ -698,10 +698,17 @@ static int64_t norm_groups(int64_t cols, int waves) {
 // 1024 (past no cache) 83 / 92, 73728 x 4096 448 / 460, 16384 x 8192 218 / 238.  16 waves a CU stay, of workgroups of more than
 // 512 lanes two: 16384 x 5120 136 us with one, 123 with two, 141 with three; x 6144 164 and 149; x 4096 83, with twice as
 // many 93.
-static int norm_pair(const NormArgs& a) { return a.past && a.cols <= 2048 ? 2 : 0; }
+// A launch has fewer than 2^32 lanes: more rows than two a workgroup reach by that (2^29 of 128 columns) are taken in turn.
+constexpr int kNormPair = 2;
+template <class S>
+static int64_t norm_pairs(const NormArgs& a) { return (a.rows + S::kRows * kNormPair - 1) / (S::kRows * kNormPair); }
+template <class S>
+static int norm_pair(const NormArgs& a) {
+  return a.past && a.cols <= 2048 && norm_pairs<S>(a) * S::kThreads < (int64_t{1} << 32) ? kNormPair : 0;
+}
 template <class S>
 static int64_t norm_fwd_groups(const NormArgs& a) {
-  if (const int64_t pair = norm_pair(a)) return (a.rows + S::kRows * pair - 1) / (S::kRows * pair);
+  if (norm_pair<S>(a)) return norm_pairs<S>(a);
   return std::min<int64_t>((a.rows + S::kRows - 1) / S::kRows, norm_groups(a.cols, S::kThreads > 512 ? S::kThreads / 32 : 16));
 }
 
@@ -805,7 +812,7 @@ extern "C" int mx_residual_norm(const void* h, int h_f32, const void* r, int r_f
                            (hipStream_t)stream, a, (R*)stream_out, (H*)normed, rstd);
       else
         hipLaunchKernelGGL((residual_norm_kernel<S, H, R>), dim3((unsigned)norm_fwd_groups<S>(a)), dim3(S::kThreads), 0,
-                           (hipStream_t)stream, a, norm_pair(a), (R*)stream_out, (H*)normed, rstd);
+                           (hipStream_t)stream, a, norm_pair<S>(a), (R*)stream_out, (H*)normed, rstd);
     });
   });
   return hipGetLastError() == hipSuccess ? MX_OK : MX_ERR_LAUNCH;
