@@ -13,6 +13,7 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/python_variable.h>
 #include <torch/extension.h>
 
 #include <array>
@@ -804,6 +805,12 @@ bool row_tensor(const Tensor& t) {
   return t.is_cuda() && !t.is_neg() && t.layout() == at::kStrided && (t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kFloat) &&
          !t.unsafeGetTensorImpl()->is_python_dispatch();
 }
+// No more than its values: a subclass in Python keeps its type, and may want to see its operations, even where it has no
+// dispatch of its own.  (With the GIL held.  A tensor that Python has not met yet is none.)
+bool no_subclass(const Tensor& t) {
+  PyObject* object = t.defined() ? t.unsafeGetTensorImpl()->pyobj_slot()->load_pyobj() : nullptr;
+  return !object || THPVariable_CheckExact(object);
+}
 int is_f32(const Tensor& t) { return t.scalar_type() == at::kFloat; }
 // Elements between the rows of [..., cols], 0 where they do not lie one after the other at one distance
 int64_t row_pitch(const Tensor& t, int64_t cols) {
@@ -880,7 +887,7 @@ std::optional<Tensor> scaled_embedding(const Tensor& ids, const Tensor& weight, 
                                        int64_t first, bool out_f32) {
   if (!row_tensor(weight) || weight.dim() != 2 || !on_current_device(weight) || ids.device() != weight.device() ||
       (ids.scalar_type() != at::kLong && ids.scalar_type() != at::kInt) || !ids.is_contiguous() || weight.numel() == 0 ||
-      ids.unsafeGetTensorImpl()->is_python_dispatch() || !row_pitch(weight, weight.size(1)))
+      ids.unsafeGetTensorImpl()->is_python_dispatch() || !row_pitch(weight, weight.size(1)) || !no_subclass(weight) || !no_subclass(ids))
     return std::nullopt;
   Unlocked unlocked(std::in_place);
   if (at::GradMode::is_enabled() && weight.requires_grad())
@@ -976,6 +983,7 @@ py::object residual_rms_norm(const Tensor& h, const Tensor& r, const std::option
   if (!row_tensor(h) || !row_tensor(r) || h.dim() == 0 || h.sizes() != r.sizes() || h.numel() == 0 || (is_f32(h) && !is_f32(r)) ||
       r.device() != h.device() || !on_current_device(h))
     return py::none();
+  if (!no_subclass(h) || !no_subclass(r) || !no_subclass(post) || !no_subclass(gate) || !no_subclass(pre)) return py::none();
   const int64_t cols = h.size(-1);
   if (!row_pitch(h, cols) || !row_pitch(r, cols)) return py::none();
   auto weight = [&](const Tensor& w) { return row_tensor(w) && w.device() == h.device() && w.is_contiguous(); };
@@ -1009,7 +1017,7 @@ std::optional<Tensor> clip_gradients(const std::vector<Tensor>& parameters, doub
   for (const Tensor& p : parameters) {
     const Tensor& g = p.grad();
     if (!g.defined()) continue;
-    if (!row_tensor(g) || !g.is_non_overlapping_and_dense() || g.device() != (grads.empty() ? g : grads[0]).device())
+    if (!row_tensor(g) || !no_subclass(g) || !g.is_non_overlapping_and_dense() || g.device() != (grads.empty() ? g : grads[0]).device())
       return std::nullopt;
     grads.push_back(g);
   }
