@@ -344,3 +344,10 @@ def test_module(device):
     assert (stream.double() - t).abs().max() <= 200 * U * t.abs().max()
     assert (normed.double() - torch.nn.functional.rms_norm(t, (96,), eps=1e-5)).abs().max() <= 400 * U * 10
     assert [n for n, _ in seam.named_parameters()] == ["post_weight", "gate", "pre_weight"]
+
+
+def test_a_gate_without_dimensions_is_refused_as_others_are(device):
+    h = torch.randn((3, 64), device=device)
+    for gate in (torch.ones((), device=device), torch.ones((3, 1), device=device), torch.ones((2, 64), device=device)):
+        with pytest.raises(ValueError, match="gate must be"):
+            residual_rms_norm(h, h, gate=gate)

@@ -990,7 +990,7 @@ py::object residual_rms_norm(const Tensor& h, const Tensor& r, const std::option
   for (const Tensor& w : {post, pre})
     if (w.defined() && (!weight(w) || w.dim() != 1 || w.size(0) != cols)) return py::none();
   if (gate.defined()) {
-    if (!weight(gate) || gate.size(-1) != cols || (gate.dim() != 1 && gate.dim() != h.dim())) return py::none();
+    if (!weight(gate) || gate.dim() == 0 || gate.size(-1) != cols || (gate.dim() != 1 && gate.dim() != h.dim())) return py::none();
     bool shared = false;  // h's leading dimensions up to one, ones behind it
     for (int64_t i = 0; i + 1 < gate.dim(); ++i) {
       if (gate.size(i) != h.size(i)) shared = true;
