@@ -973,6 +973,7 @@ def swiglu_bwd_to_mx_dim0_dim1(dg: torch.Tensor, a: torch.Tensor, b: torch.Tenso
 
 # --------------------------------------------------------------------------- around the linears
 ROW_TYPES = (torch.bfloat16, torch.float32)  # of the embedding, the norms around a block and the gradients
+PLAIN_TYPES = (torch.Tensor, torch.nn.Parameter)
 
 
 def native_rows(t: torch.Tensor) -> bool:
@@ -985,8 +986,7 @@ def plain_rows(*operands) -> bool:
     """The kernels below take these tensors (None among them: no operand): plain ones on the GPU, bf16 or float32,
     outside function transforms."""
     return not _transformed() and all(
-        t is None or (type(t) in (torch.Tensor, torch.nn.Parameter) and t.is_cuda and t.dtype in ROW_TYPES and not t.is_neg())
-        for t in operands)
+        t is None or (type(t) in PLAIN_TYPES and t.is_cuda and t.dtype in ROW_TYPES and not t.is_neg()) for t in operands)
 
 
 def _rows_as_they_lie(t: torch.Tensor) -> torch.Tensor:
