@@ -198,3 +198,32 @@ def test_refusals(device):
         ops.grad_norm([t], 3.0)
     with pytest.raises(TypeError):
         ops.grad_scale_([t], torch.zeros((), device=device, dtype=torch.float64), 1.0)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_every_place_in_the_list_scales(device, dtype):
+    """A column slice listed twice, a part of it a third time through a view of its own and its frame once: every element times the factor
+    as often as it is listed."""
+    frame = torch.randn((64, 100), device=device).to(dtype)
+    other = torch.randn(33, device=device).to(dtype)
+    lists = ([frame[:, 3:40]] * 2 + [other], [frame[:, 3:40], frame[:32, 10:90], other, frame], [frame[:, ::2], frame[:, 1::2], other],
+             [frame.t()[2:50], frame, frame.t()[2:50]])
+    half = 0.0 if dtype == torch.float32 else torch.finfo(dtype).eps / 2
+    for grads in lists:
+        before, before_other = frame.double(), other.double()
+        places = torch.zeros((64, 100), device=device)
+        mirror = lambda t: places.as_strided(t.shape, t.stride(), t.storage_offset())
+        for t in grads:
+            if t is not other:
+                mirror(t).add_(1)
+        exact = float(sum(t.double().square().sum() for t in grads)) ** 0.5
+        norm = clip_grad_norm_(parameters_of(grads), exact / 2)
+        assert abs(float(norm) - exact) <= 2 * U * exact
+        factor = exact / 2 / (exact + 1e-6)
+        listed = torch.full((33,), float(any(t is other for t in grads)), dtype=torch.float64, device=device)
+        for now, was, times in ((frame, before, places.double()), (other, before_other, listed)):
+            want = was * factor ** times
+            # the factor to 6 U and a rounding to the type for every place in the list
+            assert ((now.double() - want).abs() <= want.abs() * (times * (half + 7 * U) * 1.01) + 1e-30).all()
+        clip_grads_with_norm_(parameters_of(grads), 1e9, norm)  # a factor of 1: nothing changes
+        assert ((frame.double() - before * factor ** places).abs() <= before.abs() * (places * (half + 7 * U) * 1.01) + 1e-30).all()

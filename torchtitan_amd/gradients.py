@@ -38,6 +38,13 @@ def _grads(parameters):
     return [p.grad for p in parameters if p.grad is not None]
 
 
+def _apart(tensors) -> bool:
+    """No element of one lies between the first and the last of another."""
+    spans = sorted((t.data_ptr(), t.data_ptr() + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))))
+                   for t in tensors if t.numel())
+    return all(end <= start for (_, end), (start, _) in zip(spans, spans[1:]))
+
+
 def clip_grads_with_norm_(parameters, max_norm: float, total_norm: torch.Tensor, foreach: bool | None = None) -> None:
     """Scales the parameters' gradients in place by min(1, max_norm / (total_norm + 1e-6)), as
     ``torch.nn.utils.clip_grads_with_norm_``; nothing is read or written where that is exactly 1."""
@@ -50,11 +57,14 @@ def clip_grads_with_norm_(parameters, max_norm: float, total_norm: torch.Tensor,
         return
     with torch.no_grad():
         total_norm = total_norm.to(device=grads[0].device, dtype=torch.float32)
-        runs = [t if ops.is_dense(t) else t.contiguous() for t in grads]
-        ops.grad_scale_(runs, total_norm, float(max_norm))
-        for t, run in zip(grads, runs):
-            if run is not t:
-                t.copy_(run)
+        # copies that share memory with another gradient are written back before the next one is read
+        together = [grads] if all(ops.is_dense(t) for t in grads) or _apart(grads) else [[t] for t in grads]
+        for some in together:
+            runs = [t if ops.is_dense(t) else t.contiguous() for t in some]
+            ops.grad_scale_(runs, total_norm, float(max_norm))
+            for t, run in zip(some, runs):
+                if run is not t:
+                    t.copy_(run)
 
 
 def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_if_nonfinite: bool = False,
