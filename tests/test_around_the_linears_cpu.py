@@ -209,3 +209,24 @@ def test_embedding_and_norms_trace_without_a_break():
         grads = torch.ops.torchtitan_amd.residual_norm_bwd(h, r, w[0], None, w[1], 1.0, rstd, stream, None,
                                                            [True, False, True, True, True])
         assert [tuple(g.shape) for g in grads] == [(6, 32), (0,), (32,), (0,), (32,)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_gradients_of_equal_ids_are_added_up_in_float32(dtype):
+    """In a table's own type the sum of ones ends where a one is less than half a step: at 256 in bf16, 2048 in fp16."""
+    ids = torch.cat([torch.full((5001,), 2), torch.tensor([0, 9])])
+    ones = torch.ones((5003, 8), dtype=dtype)
+    want = torch.tensor([[1.0], [0.0], [5001.0], [0.0]]).to(dtype).expand(4, 8)
+    weight = torch.randn((4, 8)).to(dtype)
+    leaf = weight.clone().requires_grad_(True)
+    scaled_embedding(ids, leaf).backward(ones)
+    assert leaf.grad.dtype == dtype and torch.equal(leaf.grad, want)
+    leaf = weight.clone().requires_grad_(True)
+    scaled_embedding(ids, leaf, padding_idx=2).backward(ones)
+    assert torch.equal(leaf.grad, torch.where(want > 1, 0, want))
+    assert torch.equal(torch.func.grad(lambda t: (scaled_embedding(ids, t, dtype=torch.float32)).sum())(weight), want)
+    module = Embedding.Config().build(num_embeddings=4, embedding_dim=8).to(dtype)
+    torch._dynamo.reset()
+    torch.compile(module, backend="aot_eager", fullgraph=True)(ids).backward(ones)
+    torch._dynamo.reset()
+    assert torch.equal(module.weight.grad, want)

@@ -37,6 +37,8 @@ def _in_torch_ops(ids, weight, scale, padding_idx, first_row, dtype):
     inside = (row >= 0) & (row < weight.shape[0])
     if weight.shape[0] == 0:
         return weight.new_zeros((*ids.shape, weight.shape[1]), dtype=dtype)
+    if torch.is_grad_enabled() and weight.requires_grad:  # equal ids' gradients are added up in the table's type
+        weight = weight.to(wide)
     values = weight[torch.where(inside, row, 0)].to(wide) * scale
     if padding_idx is not None:
         values = torch.where((ids == padding_idx)[..., None], values.detach(), values)
