@@ -230,3 +230,13 @@ def test_gradients_of_equal_ids_are_added_up_in_float32(dtype):
     torch.compile(module, backend="aot_eager", fullgraph=True)(ids).backward(ones)
     torch._dynamo.reset()
     assert torch.equal(module.weight.grad, want)
+
+
+def test_a_table_without_rows_has_a_gradient_without_rows():
+    """A shard of no rows: zeros for every token, as part of the graph."""
+    none = torch.empty((0, 6), dtype=torch.bfloat16, requires_grad=True)
+    out = scaled_embedding(torch.arange(4).view(2, 2), none, dtype=torch.float32)
+    assert out.shape == (2, 2, 6) and out.dtype == torch.float32 and not out.any()
+    (grad,) = torch.autograd.grad(out.sum(), none)
+    assert grad.shape == (0, 6) and grad.dtype == torch.bfloat16
+    assert scaled_embedding(torch.zeros((0, 3), dtype=torch.int32), none).shape == (0, 3, 6)

@@ -35,8 +35,8 @@ def _in_torch_ops(ids, weight, scale, padding_idx, first_row, dtype):
     wide = torch.promote_types(weight.dtype, torch.float32)
     row = ids.long() - first_row
     inside = (row >= 0) & (row < weight.shape[0])
-    if weight.shape[0] == 0:
-        return weight.new_zeros((*ids.shape, weight.shape[1]), dtype=dtype)
+    if weight.shape[0] == 0:  # (the sum of no rows: zeros with a gradient of no rows)
+        return weight.sum(0).to(dtype).expand(*ids.shape, weight.shape[1]).clone()
     if torch.is_grad_enabled() and weight.requires_grad:  # equal ids' gradients are added up in the table's type
         weight = weight.to(wide)
     values = weight[torch.where(inside, row, 0)].to(wide) * scale
