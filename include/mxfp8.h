@@ -360,8 +360,9 @@ int mx_token_logprob_bwd_any(const void* logits, int64_t rows, int64_t vocab, in
  * padding; an id outside the table: no padding), every row written, zeros where there is no such t; dout [n, cols]
  * (row stride ldd), grad [rows, cols] dense.  Sums are float32, in the order of t within parts that depend on the ids
  * alone: the same bits on every run.  workspace: mx_embedding_grad_workspace bytes, 16-byte aligned.
- * Element-aligned tensors; any cols; rows below 2^31 - 1, n up to 2^26 - 4 (forward) and 2^29 (gradient), and
- * a gradient's rows of ceil(bytes / 16) pieces each fewer than 15 * 2^28 pieces in all, else MX_ERR_UNSUPPORTED. */
+ * Element-aligned tensors; any cols.  MX_ERR_UNSUPPORTED, before any launch, for 2^31 - 1 rows and more; forward for n times
+ * ceil(cols / 1024) above 2^26 - 4; for a gradient of n above 2^29 - 32, of rows of 2^31 bytes and more, or of more
+ * pieces of 16 bytes than a launch has lanes (every row begins one; up to 15 * 2^28 are taken whatever n). */
 int mx_embedding(const void* ids, int ids_i64, int64_t n, const void* weight, int weight_f32, int64_t rows, int64_t cols,
                  int64_t ldw, int64_t first, float scale, void* out, int out_f32, void* stream);
 int64_t mx_embedding_grad_workspace(int64_t n, int64_t rows, int64_t cols);
@@ -379,7 +380,8 @@ int mx_embedding_grad(const void* ids, int ids_i64, int64_t n, const void* dout,
  * bf16.  rstd (float32 [2, rows], may be NULL): both 1 / sqrt(...), which the backward needs.
  * mx_residual_norm_bwd: from the gradients of stream_out and normed (dense; NULL: zero) those of h, r, post, gate and pre
  * (NULL: not wanted), each in its operand's type; sums over rows in float32, in an order that depends on the sizes alone.
- * workspace: mx_residual_norm_workspace bytes, 16-byte aligned.  Element-aligned tensors; any cols. */
+ * workspace: mx_residual_norm_workspace bytes, 16-byte aligned.  Element-aligned tensors; any cols.  MX_ERR_UNSUPPORTED, before any
+ * launch, for more than 2^31 - 1 rows (2^22 - 1 of fewer than 8 or more than 16384 columns) or columns. */
 int mx_residual_norm(const void* h, int h_f32, const void* r, int r_f32, int64_t rows, int64_t cols, int64_t ldh, int64_t ldr,
                      const void* post, const void* gate, const void* pre, int weights_f32, int64_t gate_rows, float scale,
                      float eps, void* stream_out, void* normed, float* rstd, void* stream);
@@ -394,7 +396,8 @@ int mx_residual_norm_bwd(const void* h, int h_f32, const void* r, int r_f32, int
  * x^2), 1: sum |x|, 2: max |x|; sums in float64, norm: one float32 on the device.  workspace: mx_grad_norm_workspace(n)
  * bytes, 8-byte aligned.
  * mx_grad_scale (mx_grad_clip: the norm and then this): every value times min(1, limit / (*norm + 1e-6)), in float32, rounded to its type, in place; nothing
- * is touched where that is exactly 1.  Tensors that share memory are scaled one after the other. */
+ * is touched where that is exactly 1.  Tensors that share memory are scaled one after the other.  MX_ERR_UNSUPPORTED, before any
+ * launch, for more than 2^24 - 1 chunks of 16 KB in all, of which every tensor that is not empty begins one. */
 int64_t mx_grad_norm_workspace(int64_t n);
 int mx_grad_norm(int64_t n, void* const* grads, const int64_t* elems, const int32_t* is_f32, int kind, float* norm,
                  void* workspace, void* stream);

@@ -240,3 +240,30 @@ def test_a_table_without_rows_has_a_gradient_without_rows():
     (grad,) = torch.autograd.grad(out.sum(), none)
     assert grad.shape == (0, 6) and grad.dtype == torch.bfloat16
     assert scaled_embedding(torch.zeros((0, 3), dtype=torch.int32), none).shape == (0, 3, 6)
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="what is taken would be launched on addresses that are none")
+def test_the_last_sizes_that_are_taken_and_the_first_that_are_refused():
+    """Without a GPU a call that is taken ends at its launch, status 3; one that is refused never gets there, status 4."""
+    lib, a = _lib.load(), c_void_p(0x1000)
+    forward = lambda n, cols: lib.mx_embedding(a, 1, n, a, 0, 10, cols, cols, 0, 1.0, a, 0, None)
+    for cols, most in ((8, 2 ** 26 - 4), (512, 2 ** 26 - 4), (1024, 2 ** 26 - 4), (1025, 2 ** 25 - 2), (2048, 2 ** 25 - 2), (4096, 2 ** 24 - 1)):
+        assert (forward(most, cols), forward(most + 1, cols)) == (3, 4), cols
+    gradient = lambda n, rows, cols: lib.mx_embedding_grad(a, 1, n, a, 0, cols, rows, cols, 0, -1, 1.0, a, 0, a, None)
+    assert (gradient(2 ** 29 - 32, 9, 8), gradient(2 ** 29 - 31, 9, 8)) == (3, 4)
+    assert (gradient(4, 9, 2 ** 27 - 2048), gradient(4, 9, 2 ** 27)) == (3, 4)  # slabs of 2048 columns
+    assert (gradient(2 ** 29 - 32, 15 * 2 ** 18, 2 ** 13), gradient(4, 2 ** 22, 2 ** 13)) == (3, 4)  # 2^10 pieces a row
+    assert (gradient(4, 2 ** 31 - 2, 1), gradient(4, 2 ** 31 - 1, 1)) == (3, 4)
+    norm = lambda rows, cols: lib.mx_residual_norm(a, 0, a, 0, rows, cols, cols, cols, None, None, None, 0, 1, 1.0, 1e-5, a, None, None, None)
+    back = lambda rows, cols: lib.mx_residual_norm_bwd(a, 0, a, 0, rows, cols, cols, cols, None, None, None, 0, 1, 1.0, a, a, None, a, a,
+                                                       None, None, None, a, None)
+    for call in (norm, back):
+        for cols, most in ((1, 2 ** 22 - 1), (7, 2 ** 22 - 1), (8, 2 ** 31 - 1), (128, 2 ** 31 - 1), (16384, 2 ** 31 - 1), (16385, 2 ** 22 - 1)):
+            assert (call(most, cols), call(most + 1, cols)) == (3, 4), cols
+        assert (call(1, 2 ** 31 - 1), call(1, 2 ** 31)) == (3, 4)
+    ptrs, sizes, kinds = (c_void_p * 2)(0x1000, 0x2000), (_lib._I * 2)(), (c_int32 * 2)(1, 0)
+    for second, status in ((8192, 3), (8193, 4)):  # behind 2^24 - 2 chunks of float32 one of bf16, or two
+        sizes[0], sizes[1] = (2 ** 24 - 2) * 4096, second
+        assert lib.mx_grad_norm(2, ptrs, sizes, kinds, 0, a, a, None) == status
+        assert lib.mx_grad_scale(2, ptrs, sizes, kinds, a, 1.0, None) == status
+        assert lib.mx_grad_clip(2, ptrs, sizes, kinds, 0, a, 1.0, a, None) == status
