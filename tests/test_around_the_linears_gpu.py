@@ -419,3 +419,26 @@ def test_more_rows_than_two_a_workgroup_reach(device):
     assert not stream[few:-few:4097].any()
     del h, r, stream, normed, rstd
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_a_penalty_on_a_gradient_is_refused_whatever_it_is_formed_from(device, native, monkeypatch):
+    """The norms' operands are in their gradients: a penalty beside a loss is an error, not left out, where the outputs'
+    gradients are constants too.  A plain sum has none of them in its gradients, and no penalty to lose."""
+    if not native:
+        monkeypatch.setattr(ops, "native_rows", lambda t: False)
+    h, r, post, gate, pre = _operands(device, seed=10)
+    for weights, out in ((dict(pre_weight=pre), 1), (dict(post_weight=post), 0), (dict(gate=gate), 0), (dict(post_weight=post, pre_weight=pre), 0)):
+        loss = residual_rms_norm(h, r, **weights)[out].float().sum()
+        grads = torch.autograd.grad(loss, [h, *weights.values()], create_graph=True, allow_unused=True)
+        for g in grads:
+            with pytest.raises(RuntimeError, match="differentia"):
+                (loss + g.float().square().sum()).backward(retain_graph=True)
+    stream, _ = residual_rms_norm(h, r, residual_scale=0.5)
+    dh, dr = torch.autograd.grad(stream.float().sum(), [h, r], create_graph=True)
+    assert not dh.requires_grad and (dr == 0.5).all()
+    for use in (dict(create_graph=True), dict()):  # and a backward that nobody differentiates goes through
+        h.grad = None
+        residual_rms_norm(h, r, pre_weight=pre)[1].float().sum().backward(**use)
+        assert h.grad.isfinite().all() and h.grad.requires_grad == bool(use)
+    h.grad = None

@@ -828,9 +828,9 @@ Tensor saved_rows(const Tensor& t, const Tensor& like, at::IntArrayRef sizes) {
   return row_pitch(t, sizes.back()) ? t : t.contiguous();
 }
 
-// Gradients that cannot be differentiated again: asking for it is an error.
-variable_list once(const variable_list& from, variable_list grads) {
-  bool again = false;
+// Gradients that cannot be differentiated again: asking for it is an error.  `again`: the operands that they were formed
+// from, which take gradients themselves, are in them, and not only the gradients `from`.
+variable_list once(const variable_list& from, variable_list grads, bool again = false) {
   for (const Tensor& t : from) again |= t.defined() && t.requires_grad();
   if (!again || !at::GradMode::is_enabled()) return grads;
   for (Tensor& t : grads)
@@ -971,7 +971,8 @@ struct ResidualNormNode : torch::autograd::Function<ResidualNormNode> {
                                   pointer(dstream), pointer(dnormed), pointer(out[0]), pointer(out[1]), pointer(out[2]),
                                   pointer(out[3]), pointer(out[4]), work.data_ptr(), stream_of(h)),
             "mx_residual_norm_bwd");
-    return once(grads, std::move(out));
+    // (of a plain sum the operands are not in the gradients)
+    return once(grads, std::move(out), post.defined() || gate.defined() || dnormed.defined());
   }
 };
 

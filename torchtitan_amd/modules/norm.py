@@ -16,7 +16,6 @@ from dataclasses import dataclass, field
 
 import torch
 import torch.nn as nn
-from torch.autograd.function import once_differentiable
 
 from .. import _lib, ops
 from ..protocols import Module
@@ -34,13 +33,29 @@ class _ResidualRMSNorm(torch.autograd.Function):
         return stream, normed
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dstream, dnormed):
         if dstream is None and dnormed is None:
             return None, None, None, None, None, None, None
         *operands, rstd = ctx.saved_tensors
-        grads = ops.residual_norm_bwd(*operands, ctx.scale, rstd, dstream, dnormed, ctx.needs_input_grad[:5])
+        with torch.no_grad():
+            grads = ops.residual_norm_bwd(*operands, ctx.scale, rstd, dstream, dnormed, ctx.needs_input_grad[:5])
+        # The operands are in the gradients too (but for a plain sum), whether or not the outputs' gradients have gradients.
+        inside = operands[2] is not None or operands[3] is not None or dnormed is not None
+        if torch.is_grad_enabled() and (inside or any(d is not None and d.requires_grad for d in (dstream, dnormed))):
+            grads = [None if g is None else _Refusing.apply(g, torch.empty(0, requires_grad=True)) for g in grads]
         return *grads, None, None
+
+
+class _Refusing(torch.autograd.Function):
+    """Gradients that cannot be differentiated again: asking for it is an error."""
+
+    @staticmethod
+    def forward(ctx, grad, _):
+        return grad.view_as(grad)
+
+    @staticmethod
+    def backward(ctx, _):
+        raise RuntimeError("this operator's gradients cannot be differentiated again")
 
 
 def _in_torch_ops(h, residual, post, gate, pre, scale, eps):
