@@ -267,3 +267,25 @@ def test_the_last_sizes_that_are_taken_and_the_first_that_are_refused():
         assert lib.mx_grad_norm(2, ptrs, sizes, kinds, 0, a, a, None) == status
         assert lib.mx_grad_scale(2, ptrs, sizes, kinds, a, 1.0, None) == status
         assert lib.mx_grad_clip(2, ptrs, sizes, kinds, 0, a, 1.0, a, None) == status
+
+
+@pytest.mark.parametrize("strict", [False, True])
+def test_embedding_and_norms_export_as_operators(strict):
+    """On the GPU (fake tensors, which torch.export's default way runs the module on) one operator each."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    class Two(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.tokens = Embedding.Config(scale=2.0).build(num_embeddings=9, embedding_dim=32)
+            self.seam = ResidualRMSNorm.Config(post_norm=True, gate=True).build(dim=32)
+
+        def forward(self, ids):
+            x = self.tokens(ids)
+            return self.seam(x, x)
+
+    with FakeTensorMode(), torch.device("cuda"):
+        module, ids = Two(), torch.zeros((2, 3), dtype=torch.int64)
+    targets = [str(n.target) for n in torch.export.export(module, (ids,), strict=strict).graph.nodes if n.op == "call_function"]
+    assert [t for t in targets if "torchtitan_amd" in t] == ["torchtitan_amd.embedding_fwd.default", "torchtitan_amd.residual_norm_fwd.default"]
+    assert not any("rsqrt" in t or "index" in t for t in targets)

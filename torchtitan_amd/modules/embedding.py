@@ -68,7 +68,7 @@ def scaled_embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0
         raise ValueError(f"ids on {ids.device}, weight on {weight.device}")
     dtype = dtype or weight.dtype
     if (tracing and weight.is_cuda and weight.dtype in ops.ROW_TYPES and dtype in ops.ROW_TYPES
-            and type(weight) in ops.PLAIN_TYPES and type(ids) in ops.PLAIN_TYPES):
+            and not ops.wrapped(weight, ids)):
         from .. import compiled  # noqa: F401  (the same launches as nodes of the graph)
 
         return torch.ops.torchtitan_amd.embedding_fwd(ids, weight, float(scale), padding_idx, first_row, dtype)

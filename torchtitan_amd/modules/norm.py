@@ -113,7 +113,7 @@ def residual_rms_norm(h: torch.Tensor, residual: torch.Tensor, *, post_weight: t
         if w is not None and w.shape != (dim,):
             raise ValueError(f"{name} must be [{dim}], got {tuple(w.shape)}")
     rows = None if gate is None else _gate_as_matrix(gate, h.shape)
-    ours = all(type(t) in ops.PLAIN_TYPES and t.is_cuda and t.dtype in ops.ROW_TYPES for t in operands) and (
+    ours = not ops.wrapped(*operands) and all(t.is_cuda and t.dtype in ops.ROW_TYPES for t in operands) and (
         h.dtype == torch.bfloat16 or residual.dtype == torch.float32)
     if not ours or h.numel() == 0 or not (tracing or ops.plain_rows(*operands)):
         return _in_torch_ops(h, residual, post_weight, gate, pre_weight, residual_scale, eps)

@@ -973,7 +973,6 @@ def swiglu_bwd_to_mx_dim0_dim1(dg: torch.Tensor, a: torch.Tensor, b: torch.Tenso
 
 # --------------------------------------------------------------------------- around the linears
 ROW_TYPES = (torch.bfloat16, torch.float32)  # of the embedding, the norms around a block and the gradients
-PLAIN_TYPES = (torch.Tensor, torch.nn.Parameter)
 
 
 def native_rows(t: torch.Tensor) -> bool:
@@ -986,7 +985,15 @@ def plain_rows(*operands) -> bool:
     """The kernels below take these tensors (None among them: no operand): plain ones on the GPU, bf16 or float32,
     outside function transforms."""
     return not _transformed() and all(
-        t is None or (type(t) in PLAIN_TYPES and t.is_cuda and t.dtype in ROW_TYPES and not t.is_neg()) for t in operands)
+        t is None or (type(t) in (torch.Tensor, torch.nn.Parameter) and t.is_cuda and t.dtype in ROW_TYPES and not t.is_neg())
+        for t in operands)
+
+
+def wrapped(*operands) -> bool:
+    """One of the tensors holds others (a distributed tensor its shard), which an operator of this package would have to be
+    taken apart for.  (Asked while a graph is traced: by torch's protocol of such types, since plain tensors may be fake
+    ones there.)"""
+    return any(hasattr(type(t), "__tensor_flatten__") for t in operands)
 
 
 def _rows_as_they_lie(t: torch.Tensor) -> torch.Tensor:
