@@ -4,12 +4,16 @@
 //   t = scale r + g n                                    (g n = n without a gate)
 //   stream = t,  normed = t s2 pre,  s2 = 1 / sqrt(mean t^2 + eps)
 //
-// `normed` comes from t before t is rounded to the stream's type.  Backward, from the same h and r (t is formed again:
-// as many bytes as reading the stream, without its rounding), with u = normed's gradient times pre:
+// `normed` comes from t before t is rounded to the stream's type.  Backward, from the same h and r, with u = normed's
+// gradient times pre:
 //
 //   e  = dstream + s2 (u - t s2 mean(u t s2)),   dr = scale e,   dpre = sum of rows dnormed t s2
 //   dg = sum over the gate's rows of e n,        q = e g
-//   dpost = sum of rows q h s1,                  dh = s1 (q post - h s1 mean(q post h s1))
+//   dpost = sum of rows q h s1,                  dh = s1 (q post - h s1 mean(q post h s1)); without post dh = q
+//
+// t is formed again, without the rounding that the stream has.  With post or gate, whose gradients need h, that reads as
+// much as the stream would be; for a plain sum it reads one matrix more, and both stay in memory until then.  Without a
+// gradient of normed e = dstream and t is not needed.
 //
 // Sums over rows are float32 parts of one workgroup's rows each, joined in order by a second launch: the same result
 // on every run.  Row r of T uses row r / (T / G) of a gate of G rows.
@@ -205,8 +209,8 @@ __device__ __forceinline__ float own_products(const float (&a)[N][kV], const flo
 
 // A workgroup takes every gridDim.x-th row, or `pair` rows that lie together (kRows times as many); the next row is on its
 // way while one is worked on, and the weights stay in registers (with two pieces a lane they are read for every row).
-// Bound by memory: 16384 x 4096 with both norms and a gate 83 us (6.5 TB/s of the 6.5 of a copy that the last cache helps),
-// 147456 x 2048 419 us (5.8 of the 6.2 that two matrices read and two written reach without any arithmetic).
+// Bound by memory: 16384 x 4096 with both norms and a gate 97 us (5.5 TB/s; 83 where the last cache has h and r already),
+// 147456 x 2048 419 to 440 (5.5 to 5.8, of the 6.2 that two matrices read and two written reach without any arithmetic).
 template <class S, class H, class R>
 __global__ __launch_bounds__(S::kThreads) void residual_norm_kernel(NormArgs a, int pair, R* __restrict__ stream,
                                                                     H* __restrict__ normed, float* __restrict__ rstd) {
@@ -433,7 +437,8 @@ __device__ __forceinline__ void rows_joined(float (&acc)[S::kPieces][kV], float*
 // SOLO: the lanes of a row take strips of their own (see norm_solo), of a row of the gate each; the next strip's first row
 // and gate are on their way while one is worked on.
 // NORMED: normed has a gradient.  Without one e is dstream as it is: nothing of t, which may be infinite, is in the
-// result, and neither residual nor a sum over the row is needed for it.
+// result, and neither residual nor a sum over the row is needed for it.  us with one / without, 16384 x 4096: norm and gate
+// 139 / 90 (5.8 and 6.0 TB/s), the norm alone 89, the plain sum 63; 147456 x 2048 708 / 546; 8192 x 16384 428 / 225.
 template <class S, bool SIDE, bool SOLO, bool NORMED, class H, class R>
 __global__ __launch_bounds__(S::kThreads) void residual_norm_bwd_kernel(NormArgs a, NormStrips strips,
                                                                         const float* __restrict__ rstd, NormGrads o) {

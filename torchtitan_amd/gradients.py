@@ -47,7 +47,8 @@ def _apart(tensors) -> bool:
 
 def clip_grads_with_norm_(parameters, max_norm: float, total_norm: torch.Tensor, foreach: bool | None = None) -> None:
     """Scales the parameters' gradients in place by min(1, max_norm / (total_norm + 1e-6)), as
-    ``torch.nn.utils.clip_grads_with_norm_``; nothing is read or written where that is exactly 1."""
+    ``torch.nn.utils.clip_grads_with_norm_``; nothing is read or written where that is exactly 1 (a gradient that is not one
+    run of memory is copied and written back either way)."""
     parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
     grads = _grads(parameters)
     if not grads:
