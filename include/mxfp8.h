@@ -406,6 +406,30 @@ int mx_grad_clip(int64_t n, void* const* grads, const int64_t* elems, const int3
 int mx_grad_scale(int64_t n, void* const* grads, const int64_t* elems, const int32_t* is_f32, const float* norm, float limit,
                   void* stream);
 
+/* The AdamW step over n parameters (the optimizer behind torchtitan/components/optimizer.py).  table (host memory): n
+ * times MX_ADAMW_FIELDS numbers -- parameter, whether it and its gradient are float32 (else bf16), gradient, first moment, second
+ * moment, their scales (8 bits only), float32 master weight (or 0), number of values, step that this one is (from 1), the
+ * parameter's number.  In float32 for every value, each tensor one run of memory:
+ *     g = f gradient (- with maximize);  m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2
+ *     w = (1 - lr weight_decay) w - lr / (1 - beta1^step) m / (sqrt(v) / sqrt(1 - beta2^step) + eps)
+ * w: the master weight where there is one, and the parameter its rounding; else the parameter.  f = min(1, limit / (*norm +
+ * 1e-6)) for a float32 norm on the device, 1 for NULL.  Moments are float32, or with `eight` codes in blocks of 32 values (the last one
+ * filled up: whole blocks of codes, 8-byte aligned) with a scale byte b = 2^(b - 127) each, 255 = NaN: first moment e4m3 as
+ * above, second moment e5m3 without a sign (bias 15, max 122880), rounded up or down by chance so that the value is the mean,
+ * by a hash of seed, step, the parameter's number and the value's place; a second moment above 0 keeps a code above 0.
+ * steps (or NULL): float32 step counters on the device by the parameters' numbers, in place of the table's; they are raised by the
+ * call, which can be captured into a graph; corrections: 16 bytes for each of them, 16-byte aligned; lr_device (or NULL):
+ * float32 in place of lr.  Parameters that share memory are updated one after the other.  MX_ERR_UNSUPPORTED, before any
+ * launch, for a parameter of 2^33 values and more. */
+#define MX_ADAMW_FIELDS 11
+int mx_adamw(int64_t n, const int64_t* table, int eight, double lr, double beta1, double beta2, double eps, double weight_decay,
+             int maximize, const float* norm, float limit, uint64_t seed, float* steps, const float* lr_device, void* corrections,
+             void* stream);
+/* The values of n moments that mx_adamw holds in 8 bits: kinds 0 first, 1 second moment, + 2 for float32 out, else bf16 (which
+ * holds every code exactly but for values below its range). */
+int mx_adamw_moments(int64_t n, const uint8_t* const* codes, const uint8_t* const* scales, const int64_t* elems,
+                     const int32_t* kinds, void* const* out, void* stream);
+
 /* Re-order a row-major [rows, nblk] scale matrix into MX_SCALES_MFMA order
  * (the "blocked layout" step the reference leaves to torch._scaled_mm, docs/mxfp8.md:36). */
 int mx_scale_layout(const uint8_t* scales, int64_t rows, int64_t nblk, uint8_t* out, void* stream);

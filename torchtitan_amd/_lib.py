@@ -78,6 +78,9 @@ SIGNATURES = {
     "mx_grad_norm": (c_int, [_I, _P, _P, _P, c_int, _P, _P, _P]),
     "mx_grad_clip": (c_int, [_I, _P, _P, _P, c_int, _P, ctypes.c_float, _P, _P]),
     "mx_grad_scale": (c_int, [_I, _P, _P, _P, _P, ctypes.c_float, _P]),
+    "mx_adamw": (c_int, [_I, _P, c_int, ctypes.c_double, ctypes.c_double, ctypes.c_double, ctypes.c_double, ctypes.c_double,
+                         c_int, _P, ctypes.c_float, ctypes.c_uint64, _P, _P, _P, _P]),
+    "mx_adamw_moments": (c_int, [_I, _P, _P, _P, _P, _P, _P]),
     "mx_scale_layout": (c_int, [_P, _I, _I, _P, _P]),
     "mx_scale_unlayout": (c_int, [_P, _I, _I, _P, _P]),
     "mx_gemm_nt": (c_int, [_P, _P, _P, _P, _P, _I, _I, _I, _I, _P]),

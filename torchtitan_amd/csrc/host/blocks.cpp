@@ -70,6 +70,7 @@ struct Library {
   decltype(&mx_residual_norm_bwd) residual_norm_bwd = nullptr;
   decltype(&mx_grad_norm_workspace) grad_norm_workspace = nullptr;
   decltype(&mx_grad_clip) grad_clip = nullptr;
+  decltype(&mx_adamw) adamw = nullptr;
 } lib;
 PyObject* check_status = nullptr;  // _lib.check, never released
 
@@ -119,6 +120,7 @@ void bind(const py::dict& addresses, const py::object& check) {
   set("mx_residual_norm_bwd", lib.residual_norm_bwd);
   set("mx_grad_norm_workspace", lib.grad_norm_workspace);
   set("mx_grad_clip", lib.grad_clip);
+  set("mx_adamw", lib.adamw);
   check_status = check.ptr();
   Py_INCREF(check_status);
 }
@@ -1042,6 +1044,111 @@ std::optional<Tensor> clip_gradients(const std::vector<Tensor>& parameters, doub
   return norm;
 }
 
+// t's elements are one run of memory in p's order
+bool same_order(const Tensor& t, const Tensor& p) {
+  if (t.is_contiguous()) return p.is_contiguous() && t.numel() == p.numel();
+  return t.sizes() == p.sizes() && t.strides() == p.strides();
+}
+
+// The AdamW step of a group: parameters that have a gradient, with their states (a dict of tensors and the step so far, as
+// torchtitan_amd/optimizers.py makes them) updated.  False, with nothing done, where one of them is not the plain case: state not
+// made yet, a type, device or layout of its own.
+bool adamw(const py::list& parameters, const py::list& states, int64_t first, bool eight, double lr, double b1, double b2,
+           double eps, double decay, bool maximize, const std::optional<Tensor>& total_norm, double limit, uint64_t seed) {
+  static PyObject* const names[] = {PyUnicode_InternFromString("exp_avg"), PyUnicode_InternFromString("exp_avg_sq"),
+                                    PyUnicode_InternFromString("exp_avg_scale"), PyUnicode_InternFromString("exp_avg_sq_scale"),
+                                    PyUnicode_InternFromString("master"), PyUnicode_InternFromString("step")};
+  struct One {
+    Tensor p, g;
+    std::array<Tensor, 5> state;  // in the order of the names
+    PyObject* dict;
+    int64_t step;
+  };
+  const size_t count = parameters.size();
+  if (states.size() != count) return false;
+  std::vector<One> all;
+  std::vector<int64_t> table;
+  all.reserve(count);
+  for (size_t i = 0; i < count; ++i) {
+    PyObject* object = PyList_GET_ITEM(parameters.ptr(), i);
+    if (!THPVariable_Check(object)) return false;
+    One one;
+    one.p = THPVariable_Unpack(object);
+    one.g = one.p.grad();
+    if (!one.g.defined()) continue;
+    const Tensor &p = one.p, &g = one.g;
+    if (!row_tensor(p) || !row_tensor(g) || !no_subclass(g) || g.scalar_type() != p.scalar_type() || g.sizes() != p.sizes() ||
+        !p.is_non_overlapping_and_dense() || !same_order(g, p) || p.device() != (all.empty() ? p : all[0].p).device() ||
+        g.device() != p.device())
+      return false;
+    one.dict = PyList_GET_ITEM(states.ptr(), i);
+    if (!PyDict_Check(one.dict)) return false;
+    const int64_t blocks = (p.numel() + 31) / 32;
+    for (int k = 0; k < 5; ++k) {
+      const bool moment = k < 2, scale = k == 2 || k == 3;
+      PyObject* value = PyDict_GetItemWithError(one.dict, names[k]);
+      if (!value) {
+        if (PyErr_Occurred()) throw py::error_already_set();
+        if (moment || (scale && eight)) return false;
+        continue;
+      }
+      if (scale && !eight) continue;
+      if (!THPVariable_CheckExact(value)) return false;
+      const Tensor& t = one.state[k] = THPVariable_Unpack(value);
+      const bool bytes = eight && k < 4;
+      if (!t.is_cuda() || t.device() != p.device() || t.layout() != at::kStrided || t.is_neg() ||
+          t.scalar_type() != (bytes ? at::kByte : at::kFloat))
+        return false;
+      if (bytes ? !p.is_contiguous() || !t.is_contiguous() || t.numel() != (scale ? blocks : 32 * blocks)
+                : t.numel() != p.numel() || !same_order(t, p))
+        return false;
+    }
+    PyObject* step = PyDict_GetItemWithError(one.dict, names[5]);
+    if (!step || !PyLong_CheckExact(step)) return false;
+    one.step = PyLong_AsLongLong(step);
+    if (one.step < 0) {
+      PyErr_Clear();
+      return false;
+    }
+    const auto& [m, v, ms, vs, master] = one.state;
+    auto at = [](const Tensor& t) { return reinterpret_cast<int64_t>(pointer(t)); };
+    for (const int64_t field : {at(p), int64_t{is_f32(p)}, at(g), at(m), at(v), at(ms), at(vs), at(master), p.numel(),
+                                one.step + 1, first + static_cast<int64_t>(i)})
+      table.push_back(field);
+    all.push_back(std::move(one));
+  }
+  if (all.empty()) return true;
+  const Tensor& like = all[0].p;
+  Tensor norm;
+  if (total_norm) {
+    norm = *total_norm;
+    if (!no_subclass(norm) || norm.device() != like.device() || norm.scalar_type() != at::kFloat || norm.numel() != 1 || norm.is_neg())
+      return false;
+  }
+  if (!on_current_device(like)) return false;
+  const hipStream_t st = stream_of(like);
+  hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing(st, &capture) != hipSuccess || capture != hipStreamCaptureStatusNone) return false;
+  for (const One& one : all) {
+    auto wrote = [](const Tensor& t) {
+      if (t.defined() && !t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+    };
+    wrote(one.p);
+    for (const Tensor& t : one.state) wrote(t);
+  }
+  {
+    Unlocked unlocked(std::in_place);
+    checked(lib.adamw(static_cast<int64_t>(all.size()), table.data(), eight, lr, b1, b2, eps, decay, maximize,
+                      static_cast<const float*>(pointer(norm)), static_cast<float>(limit), seed, nullptr, nullptr, nullptr, st),
+            "mx_adamw");
+  }
+  for (const One& one : all) {
+    const py::object next = py::reinterpret_steal<py::object>(PyLong_FromLongLong(one.step + 1));
+    if (!next || PyDict_SetItem(one.dict, names[5], next.ptr())) throw py::error_already_set();
+  }
+  return true;
+}
+
 // The capture that `stream` is part of, a number of its own for every capture (0: none).
 unsigned long long capture_id(uintptr_t stream) {
   hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
@@ -1076,4 +1183,5 @@ PYBIND11_MODULE(_blocks, m) {
   m.def("scaled_embedding", torch::wrap_pybind_function(scaled_embedding));
   m.def("residual_rms_norm", torch::wrap_pybind_function(residual_rms_norm));
   m.def("clip_gradients", torch::wrap_pybind_function(clip_gradients));
+  m.def("adamw", torch::wrap_pybind_function(adamw));
 }

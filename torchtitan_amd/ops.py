@@ -1170,6 +1170,53 @@ def grad_scale_(grads, norm: torch.Tensor, limit: float) -> None:
     _call("mx_grad_scale", "grad_scale", grads[0].device, *lists, _ptr(norm), limit, _stream(norm))
 
 
+ADAMW_FIELDS = 11  # of the table that `mx_adamw` reads
+
+
+def adamw_(operands, eight: bool, lr: float, betas, eps: float, weight_decay: float, maximize: bool,
+           norm: torch.Tensor | None = None, limit: float = 0.0, seed: int = 0, steps: torch.Tensor | None = None,
+           lr_device: torch.Tensor | None = None, corrections: torch.Tensor | None = None) -> None:
+    """One AdamW step in place.  operands: (parameter, gradient, moments, master or None, step, number) each, on one GPU;
+    moments: two float32 tensors, or with `eight` codes and scales of the first and of the second.  Tensors of one parameter
+    lie in memory alike, each in one run; steps: float32 step counters by number, which the call raises, with 16 bytes each of
+    `corrections`."""
+    table, written = [], []
+    for p, g, moments, master, step, number in operands:
+        codes = [moments[0], moments[2]] if eight else moments
+        scales = [_ptr(moments[1]), _ptr(moments[3])] if eight else [0, 0]
+        table += [_ptr(p), int(p.dtype == torch.float32), _ptr(g), *map(_ptr, codes), *scales,
+                  0 if master is None else _ptr(master), p.numel(), step, number]
+        written += [p, *moments] + ([] if master is None else [master])
+    dev = operands[0][0].device
+    if norm is not None:
+        if norm.numel() != 1:
+            raise ValueError(f"the norm must be one number, got {tuple(norm.shape)}")
+        norm = norm.detach().to(device=dev, dtype=torch.float32)
+    if lr_device is not None and (lr_device.dtype != torch.float32 or lr_device.device != dev):
+        raise TypeError(f"a tensor lr must be float32 on {dev}, got {lr_device.dtype} on {lr_device.device}")
+    torch.autograd.graph.increment_version(written)
+    _call("mx_adamw", "adamw", dev, len(operands), _host_table(table, c_int64), int(eight), lr, *betas, eps, weight_decay,
+          int(maximize), _optional_ptr(norm), limit, seed, _optional_ptr(steps), _optional_ptr(lr_device),
+          _optional_ptr(corrections), _stream(operands[0][0]))
+
+
+def adamw_moments(asked) -> None:
+    """Writes the values of 8-bit moments: (codes [blocks, 32], scales [blocks], 1 for a second moment, out) each, on one GPU,
+    out bf16 or float32, contiguous."""
+    asked = list(asked)
+    dev = asked[0][3].device
+    for codes, scales, _, out in asked:
+        blocks = -(-out.numel() // BLOCK)
+        for t, n in ((codes, blocks * BLOCK), (scales, blocks)):
+            if t.dtype != torch.uint8 or t.numel() != n or t.device != dev or not t.is_contiguous():
+                raise ValueError(f"a moment of {out.numel()} values wants {n} contiguous bytes on {dev}, got {tuple(t.shape)} "
+                                 f"{t.dtype} on {t.device}")
+    _call("mx_adamw_moments", "adamw_moments", dev, len(asked), _host_table([_ptr(a[0]) for a in asked], c_int64),
+          _host_table([_ptr(a[1]) for a in asked], c_int64), _host_table([a[3].numel() for a in asked], c_int64),
+          _host_table([a[2] + 2 * _row_type(a[3], "moments") for a in asked], c_int32),
+          _host_table([_ptr(a[3]) for a in asked], c_int64), _stream(asked[0][3]))
+
+
 def scale_layout(scales: torch.Tensor) -> torch.Tensor:
     """Row-major [rows, nblk] scales -> flat buffer in MFMA order."""
     rows, nblk = scales.shape

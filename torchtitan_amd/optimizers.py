@@ -1,0 +1,371 @@
+"""AdamW over all parameters of a model in a few launches, with moments in float32 or in 8 bits.
+
+Counterpart of the optimizer that the reference's container builds (torchtitan/components/optimizer.py), with torch's own
+signature.  bf16 and float32 parameters on a GPU, converted weights among them, run as HIP kernels; everything else runs
+the same formula in torch operations.  The gradients' clipping (``gradients.py``) can be applied as they are read.
+"""
+from __future__ import annotations
+
+import math
+
+import torch
+
+from . import _lib, ops
+from .mx_tensor import MXFP8TrainingWeight, _capture, _unwrap
+
+_TYPES = (torch.Tensor, torch.nn.Parameter, MXFP8TrainingWeight)
+_MOMENTS = {32: ("exp_avg", "exp_avg_sq"), 8: ("exp_avg", "exp_avg_scale", "exp_avg_sq", "exp_avg_sq_scale")}
+
+
+# ------------------------------------------------------------------------------ moments in 8 bits, in torch operations
+# (exponent bias, largest code, its exponent, what carries a float32's mantissa above the largest code's, has a sign): the
+# first moment in e4m3, the second in e5m3 without a sign; blocks of 32 values with an E8M0 scale.
+_FIRST, _SECOND = (7, 0x7E, 8, 0x1FFFFF, True), (15, 0xFF, 16, 0x0FFFFF, False)
+
+
+def _mixed(x):
+    x = ((x ^ (x >> 16)) * 0x6A09E667) & 0xFFFFFFFF
+    x = ((x ^ (x >> 15)) * 0xBB67AE85) & 0xFFFFFFFF
+    return x ^ (x >> 16)
+
+
+def _random_bits(n: int, seed: int, step: int, number: int, device) -> torch.Tensor:
+    """16 random bits for each of n values, the kernel's."""
+    key = 0
+    for word in (seed & 0xFFFFFFFF, seed >> 32, step, number):
+        key = _mixed((key + word + 0x9E3779B9) & 0xFFFFFFFF)
+    pair = torch.arange(-(-n // 2), dtype=torch.int64, device=device)
+    bits = _mixed((pair * 0x9E3779B9 + key) & 0xFFFFFFFF)
+    return torch.stack((bits & 0xFFFF, bits >> 16), 1).reshape(-1)[:n]
+
+
+def _blocks(x: torch.Tensor) -> torch.Tensor:
+    x = x.reshape(-1)
+    return torch.nn.functional.pad(x, (0, -x.numel() % ops.BLOCK)).view(-1, ops.BLOCK)
+
+
+def _encode(x: torch.Tensor, form, random: torch.Tensor):
+    """(codes [blocks, 32], scales [blocks]) of float32 values."""
+    bias, most, top, up, signed = form
+    x, random = _blocks(x), _blocks(random)
+    bits = x.abs().view(torch.int32).long()
+    amax = bits.amax(1) if bits.shape[0] else bits.new_zeros(0)
+    scale = torch.where(amax > 0, ((amax + up) >> 23) - top, 0).clamp(0, 254)
+    scale = torch.where(amax >= 0x7F800000, 255, scale)
+    size = torch.ldexp(x.abs().double(), (bias - scale).double()[:, None]).float().view(torch.int32).long()
+    code = torch.where(x == 0, 0, ((size + (random << 4) + 8) >> 20).clamp(max=most))
+    if not signed:
+        code = torch.where(x > 0, code.clamp(min=1), code)
+    code = torch.where(scale[:, None] == 255, most, code)
+    if signed:
+        code = code | (x.signbit().long() << 7)
+    return code.to(torch.uint8), scale.to(torch.uint8)
+
+
+def _decode(codes: torch.Tensor, scales: torch.Tensor, form, n: int) -> torch.Tensor:
+    """The n float32 values of codes."""
+    bias, _, _, _, signed = form
+    code, scale = codes.long(), scales.long()
+    size = ((code & 127 if signed else code) << 20).to(torch.int32).view(torch.float32)
+    value = torch.ldexp(size.double(), (scale - bias).double()[:, None]).float()
+    value = torch.where(scale[:, None] == 255, math.nan, value)
+    return (torch.where(code >= 128, -value, value) if signed else value).reshape(-1)[:n]
+
+
+def _in_torch_ops(p, g, state, group, factor, step, number):
+    (b1, b2), lr, eps = group["betas"], float(group["lr"]), group["eps"]
+    wide = torch.promote_types(p.dtype, torch.float32)
+    g = g.to(wide)
+    if factor is not None:
+        g = g * factor.to(g.device)
+    if group["maximize"]:
+        g = -g
+    if group["state_bits"] == 8:
+        m = _decode(state["exp_avg"], state["exp_avg_scale"], _FIRST, p.numel()).view(p.shape)
+        v = _decode(state["exp_avg_sq"], state["exp_avg_sq_scale"], _SECOND, p.numel()).view(p.shape)
+    else:
+        m, v = state["exp_avg"], state["exp_avg_sq"]
+    m_new, v_new = m * b1 + g * (1 - b1), v * b2 + g * g * (1 - b2)
+    below = v_new.sqrt() * (1 / math.sqrt(1 - b2 ** step)) + eps
+    w = state.get("master", p)
+    new = w.to(wide) * (1 - lr * group["weight_decay"]) - (m_new / below) * (lr / (1 - b1 ** step))
+    if w is not p:
+        w.copy_(new)
+    p.copy_(new)
+    if group["state_bits"] == 8:
+        random = _random_bits(p.numel(), group["seed"], step, number, p.device)
+        for name, x, form in (("exp_avg", m_new, _FIRST), ("exp_avg_sq", v_new, _SECOND)):
+            codes, scales = _encode(x, form, random)
+            state[name].copy_(codes)
+            state[name + "_scale"].copy_(scales)
+    else:
+        m.copy_(m_new)
+        v.copy_(v_new)
+
+
+def _kernel_takes(p: torch.Tensor) -> bool:
+    return (type(p) in _TYPES and p.is_cuda and p.dtype in ops.ROW_TYPES and p.layout == torch.strided and not p.is_neg()
+            and ops.is_dense(p))
+
+
+class AdamW(torch.optim.Optimizer):
+    """``torch.optim.AdamW``, whose arguments these are, with moments in `state_bits` bits whatever the parameters' type.
+
+        g = f * gradient               (its sign turned with `maximize`)
+        m = b1 m + (1 - b1) g          v = b2 v + (1 - b2) g^2
+        p = (1 - lr * weight_decay) p - lr / (1 - b1^t) * m / (sqrt(v / (1 - b2^t)) + eps)
+
+    in float32, p rounded once to its type.  `master_weights`: parameters narrower than float32 keep a float32 weight in
+    their state, which the step updates; the parameter is its rounding.  ``state_bits=8``: the first moment is held in e4m3, the
+    second in e5m3 without a sign, 32 values in the order of memory with a power of two between them (``exp_avg`` uint8
+    [blocks, 32] and ``exp_avg_scale`` [blocks]; likewise ``exp_avg_sq``), rounded up or down by chance so that
+    their mean is the exact one; `seed` decides about that chance, the same seed gives the same bits.  A block whose gradients
+    hold an infinity or a NaN becomes NaN.  Such parameters must be contiguous.
+
+    ``step(total_norm=..., max_norm=...)`` scales the gradients by min(1, max_norm / (total_norm + 1e-6)) as they are read:
+    ``clip_grads_with_norm_`` without its pass over memory (the gradients stay as they are, and of bf16 ones no scaled rounding).
+
+    With `capturable` the step counters are on the device and `lr` may be a float32 tensor there: a step can be captured into a
+    graph once a step has run outside of one."""
+
+    def __init__(self, params, lr: float | torch.Tensor = 1e-3, betas: tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
+                 weight_decay: float = 1e-2, *, state_bits: int = 32, master_weights: bool = False, maximize: bool = False,
+                 capturable: bool = False, seed: int = 0):
+        if isinstance(lr, torch.Tensor) and lr.numel() != 1:
+            raise ValueError("a tensor lr must have one element")
+        if not float(lr) >= 0:
+            raise ValueError(f"lr must not be negative, got {lr}")
+        if not all(0 <= b < 1 for b in betas):
+            raise ValueError(f"betas must be in [0, 1), got {betas}")
+        if not eps >= 0 or not weight_decay >= 0:
+            raise ValueError(f"eps and weight_decay must not be negative, got {eps} and {weight_decay}")
+        if state_bits not in _MOMENTS:
+            raise ValueError(f"state_bits must be 32 or 8, got {state_bits}")
+        if not 0 <= seed < 1 << 64:
+            raise ValueError("seed must fit 64 bits without a sign")
+        self._counters = {}  # group -> (float32 step counters by the parameters' numbers, what follows from them)
+        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay, state_bits=state_bits,
+                                      master_weights=master_weights, maximize=maximize, capturable=capturable, seed=seed))
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        self._counters = {}
+
+    # -------------------------------------------------------------------------------- state
+    def _new_state(self, p: torch.Tensor, group) -> None:
+        if p.is_cuda and type(p) in _TYPES and _capture(p):
+            raise RuntimeError("AdamW: the state of a parameter is made by its first step, which cannot be captured into a "
+                               "graph: run one step outside")
+        plain, state = _unwrap(p.detach()), {}
+        if plain.is_complex():
+            raise TypeError(f"AdamW: complex parameters are not supported, got {p.dtype}")
+        wide = torch.promote_types(p.dtype, torch.float32)
+        if group["state_bits"] == 8:
+            if hasattr(type(p), "__tensor_flatten__") or not p.is_contiguous() or wide != torch.float32:
+                raise ValueError(f"AdamW: moments in 8 bits want plain contiguous parameters of up to 32 bits, got "
+                                 f"{type(p).__name__} {p.dtype} {tuple(p.shape)} with strides {p.stride()}")
+            blocks = -(-p.numel() // ops.BLOCK)
+            for name in ("exp_avg", "exp_avg_sq"):
+                state[name] = torch.zeros((blocks, ops.BLOCK), dtype=torch.uint8, device=p.device)
+                state[name + "_scale"] = torch.zeros(blocks, dtype=torch.uint8, device=p.device)
+        else:
+            for name in ("exp_avg", "exp_avg_sq"):
+                state[name] = torch.zeros_like(plain, dtype=wide, memory_format=torch.preserve_format)
+        if group["master_weights"] and p.dtype != wide:
+            state["master"] = plain.to(wide, copy=True)
+        state["step"] = 0
+        self.state[p] = state
+
+    def load_state_dict(self, state_dict) -> None:
+        """As torch's, but moments keep their own types, and `state_bits`, `master_weights` and `capturable` stay this
+        optimizer's: a state that ``torch.optim.AdamW`` or this optimizer with others of them has saved is converted."""
+        held = [{key: group[key] for key in ("state_bits", "master_weights", "capturable")} for group in self.param_groups]
+        super().load_state_dict(state_dict)
+        self._counters = {}
+        for group, own in zip(self.param_groups, held):
+            group.update(own)
+            for key, value in self.defaults.items():
+                group.setdefault(key, value)
+        saved_ids = [i for group in state_dict["param_groups"] for i in group["params"]]
+        number = -1
+        for group in self.param_groups:
+            for p in group["params"]:
+                number += 1
+                saved = state_dict["state"].get(saved_ids[number])
+                if not saved:
+                    self.state.pop(p, None)
+                    continue
+                self._load_one(p, group, saved, number)
+
+    @torch.no_grad()
+    def _load_one(self, p, group, saved, number: int) -> None:
+        self._new_state(p, group)
+        state = self.state[p]
+        state["step"] = int(saved["step"])
+        wide = torch.promote_types(p.dtype, torch.float32)
+        eight = saved["exp_avg"].dtype == torch.uint8
+        if eight and group["state_bits"] == 8:
+            moves = {name: saved[name] for name in _MOMENTS[8]}
+        elif eight:
+            moves = {name: _decode(saved[name].to(p.device), saved[name + "_scale"].to(p.device), form, p.numel()).view(p.shape)
+                     for name, form in (("exp_avg", _FIRST), ("exp_avg_sq", _SECOND))}
+        elif group["state_bits"] == 8:
+            moves, random = {}, _random_bits(p.numel(), group["seed"], state["step"], number, p.device)
+            for name, form in (("exp_avg", _FIRST), ("exp_avg_sq", _SECOND)):
+                values = saved[name].to(p.device, torch.float32)
+                if values.shape != p.shape:
+                    raise ValueError(f"AdamW: a saved {name} has shape {tuple(values.shape)}, its parameter {tuple(p.shape)}")
+                moves[name], moves[name + "_scale"] = _encode(values, form, random)
+        else:
+            moves = {name: saved[name] for name in _MOMENTS[32]}
+        if "master" in state and "master" in saved:
+            moves["master"] = saved["master"]
+        for name, value in moves.items():
+            if value.shape != state[name].shape:
+                raise ValueError(f"AdamW: a saved {name} has shape {tuple(value.shape)}, expected {tuple(state[name].shape)}")
+            state[name].copy_(value.to(state[name].dtype) if state[name].dtype == wide else value)
+
+    def _counter(self, index: int, first: int):
+        """The device's step counters of a group whose parameters have the numbers from `first` on, and their corrections; the
+        states' steps are its elements."""
+        group = self.param_groups[index]
+        device = next((p.device for p in group["params"] if p.is_cuda), None)
+        if device is None:
+            raise RuntimeError("AdamW: capturable wants parameters on a GPU")
+        steps, corrections = self._counters.get(index) or (None, None)
+        here = [self.state[p]["step"] for p in group["params"] if p in self.state]
+        places = [first + i for i, p in enumerate(group["params"]) if p in self.state]
+        if steps is None or any(not isinstance(s, torch.Tensor) or s.data_ptr() != steps.data_ptr() + 4 * i
+                                for s, i in zip(here, places)):
+            if device.type == "cuda" and _capture(torch.empty(0, device=device)):
+                raise RuntimeError("AdamW: step counters are laid out by a step outside of a capture")
+            values = [float(s) for s in here]
+            if steps is None or steps.device != device:
+                size = first + len(group["params"])
+                steps = torch.zeros(size, dtype=torch.float32, device=device)
+                corrections = torch.zeros((size, 4), dtype=torch.float32, device=device)
+                self._counters[index] = (steps, corrections)
+            for value, i, p in zip(values, places, (p for p in group["params"] if p in self.state)):
+                steps[i] = value
+                self.state[p]["step"] = steps[i]
+        return steps, corrections
+
+    # -------------------------------------------------------------------------------- step
+    def step(self, closure=None, *, total_norm: torch.Tensor | None = None, max_norm: float | None = None):
+        """One update of every parameter with a gradient; the closure's value, if there is one."""
+        if (total_norm is None) != (max_norm is None):
+            raise ValueError("total_norm and max_norm come together")
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        first = 0
+        with torch.no_grad():
+            for index, group in enumerate(self.param_groups):
+                self._step_group(index, group, first, total_norm, 0.0 if max_norm is None else float(max_norm))
+                first += len(group["params"])
+        return loss
+
+    def _step_group(self, index: int, group, first: int, norm, limit: float) -> None:
+        params = group["params"]
+        if not group["capturable"] and all(type(p) in _TYPES for p in params) and params and ops.native_rows(_unwrap(params[0])):
+            states = [self.state.get(p) for p in params]
+            b1, b2 = group["betas"]
+            if _lib.blocks().adamw(params, states, first, group["state_bits"] == 8, float(group["lr"]), b1, b2, group["eps"],
+                                   group["weight_decay"], group["maximize"], norm, limit, group["seed"]):
+                return
+        with_grad = [(first + i, p) for i, p in enumerate(params) if p.grad is not None]
+        for _, p in with_grad:
+            if p.grad.is_sparse:
+                raise RuntimeError("AdamW: sparse gradients are not supported")
+            if p not in self.state or not self.state[p]:
+                self._new_state(p, group)
+        if not with_grad:
+            return
+        if group["capturable"]:
+            if not all(_kernel_takes(p) and p.device == with_grad[0][1].device for _, p in with_grad):
+                raise RuntimeError("AdamW: capturable wants bf16 or float32 parameters on one GPU")
+            self._launch(with_grad, group, norm, limit, *self._counter(index, first))
+            return
+        by_device: dict = {}
+        for number, p in with_grad:
+            if _kernel_takes(p):
+                by_device.setdefault(p.device, []).append((number, p))
+                continue
+            state, factor = self.state[p], None
+            if norm is not None:
+                factor = torch.full_like(norm, limit, dtype=torch.float32).div(norm.float() + 1e-6).clamp(max=1.0)
+            step = int(state["step"]) + 1
+            _in_torch_ops(_unwrap(p), _unwrap(p.grad), state, group, factor, step, number)
+            state["step"] = step
+        for some in by_device.values():
+            self._launch(some, group, norm, limit)
+
+    def _launch(self, numbered, group, norm, limit: float, counters=None, corrections=None) -> None:
+        eight = group["state_bits"] == 8
+        device = numbered[0][1].device
+        if counters is None and _capture(_unwrap(numbered[0][1])):
+            raise RuntimeError("AdamW: a step that is captured into a graph wants capturable=True")
+        operands = []
+        for number, p in numbered:
+            p, g, state = _unwrap(p), _unwrap(p.grad), self.state[p]
+            if g.device != device or g.shape != p.shape:
+                raise ValueError(f"AdamW: a gradient of shape {tuple(g.shape)} on {g.device} for a parameter of {tuple(p.shape)} on {device}")
+            if g.dtype != p.dtype or g.is_neg() or type(g) is not torch.Tensor or not _same_order(g, p):
+                g = torch.empty_like(p).copy_(g)
+            moments = [state[name] for name in _MOMENTS[group["state_bits"]]]
+            master = state.get("master")
+            _check_state(p, moments, master, eight)
+            operands.append((p, g, moments, master, 0 if counters is not None else int(state["step"]) + 1, number))
+        on_device = counters is not None and isinstance(group["lr"], torch.Tensor) and group["lr"].is_cuda
+        ops.adamw_(operands, eight, 0.0 if on_device else float(group["lr"]), group["betas"], group["eps"], group["weight_decay"],
+                   group["maximize"], norm, limit, group["seed"], counters, group["lr"] if on_device else None, corrections)
+        if counters is None:  # (a refused step has not been one)
+            for _, p in numbered:
+                self.state[p]["step"] = int(self.state[p]["step"]) + 1
+
+    @torch.no_grad()
+    def moments(self, dtype: torch.dtype = torch.bfloat16) -> list:
+        """(first moment, second moment) of every parameter in order, None for one without a state.  Moments in 32 bits are the state's own
+        tensors; those in 8 bits are written out in `dtype`, bfloat16 or float32, of which the first holds their codes as they
+        are (but for values below its range)."""
+        if dtype not in ops.ROW_TYPES:
+            raise TypeError(f"moments are written in bfloat16 or float32, got {dtype}")
+        out, asked = [], []
+        for group in self.param_groups:
+            for p in group["params"]:
+                state = self.state.get(p)
+                if not state:
+                    out.append(None)
+                elif group["state_bits"] == 32:
+                    out.append((state["exp_avg"], state["exp_avg_sq"]))
+                else:
+                    pair = tuple(torch.empty(p.shape, dtype=dtype, device=p.device) for _ in range(2))
+                    if p.is_cuda:
+                        for second, (name, t) in enumerate(zip(("exp_avg", "exp_avg_sq"), pair)):
+                            asked.append((state[name], state[name + "_scale"], second, t))
+                    else:
+                        for name, form, t in zip(("exp_avg", "exp_avg_sq"), (_FIRST, _SECOND), pair):
+                            t.copy_(_decode(state[name], state[name + "_scale"], form, p.numel()).view(p.shape))
+                    out.append(pair)
+        for device in {t.device for *_, t in asked}:
+            ops.adamw_moments([a for a in asked if a[3].device == device])
+        return out
+
+
+def _same_order(t: torch.Tensor, p: torch.Tensor) -> bool:
+    """t's elements lie in memory as p's do."""
+    return (t.is_contiguous() and p.is_contiguous()) or (t.shape == p.shape and t.stride() == p.stride())
+
+
+def _check_state(p, moments, master, eight: bool) -> None:
+    blocks = -(-p.numel() // ops.BLOCK)
+    want = [(blocks * ops.BLOCK, torch.uint8), (blocks, torch.uint8)] * 2 if eight else [(p.numel(), torch.float32)] * 2
+    want.append((p.numel(), torch.float32))
+    for t, (n, dtype) in zip((*moments, master), want):
+        if t is None:
+            continue
+        fits = t.is_contiguous() if dtype == torch.uint8 else _same_order(t, p)
+        if t.numel() != n or t.dtype != dtype or t.device != p.device or not fits:
+            raise ValueError(f"AdamW: a state of {tuple(t.shape)} {t.dtype} on {t.device} with strides {t.stride()} does not fit a "
+                             f"parameter of {tuple(p.shape)} on {p.device} with strides {p.stride()}: {n} x {dtype} wanted")
