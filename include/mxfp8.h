@@ -406,6 +406,54 @@ int mx_grad_clip(int64_t n, void* const* grads, const int64_t* elems, const int3
 int mx_grad_scale(int64_t n, void* const* grads, const int64_t* elems, const int32_t* is_f32, const float* norm, float limit,
                   void* stream);
 
+/* Losses over the tokens of many sequences (the policy loss of torchtitan/experiments/rl/unified/actors/utils.py:51-147 and
+ * its token-wise relatives; the preference loss of paired sequences).  Tokens lie in one array; sequence s has those from offsets[s] to
+ * offsets[s + 1] (int64, or int32 with offsets_i64 = 0; NULL: `length` each, and tokens = sequences * length), of which the ones
+ * count whose mask byte is not 0 (NULL: all).  Whatever a token that does not count holds, its gradient is 0 and it adds
+ * nothing; a sequence without tokens that count is left out of every mean.  Log-probabilities are float32 or bf16, each array for itself,
+ * element-aligned.  Terms and sums are in float64, in an order that depends on the sizes and offsets alone.
+ *
+ * mx_policy_loss: r = exp(log_probs - old) of a token, or with ratio_per_sequence exp(mean of that) of a sequence (old NULL: r = 1,
+ * whose gradient is that of old = log_probs); A: advantages float32, of every sequence or with advantage_per_token of every token.
+ *     objective = -min(r A, clip(r, ratio_low, ratio_high) A)         loss = pg + kl_coef KL - entropy_coef entropy
+ * pg and KL: means over all tokens, or with mean_per_sequence over sequences of the means over their tokens, of the objective and of the
+ * estimator at x = log_probs - ref (ref NULL: 0): kl 0 x, 1 x^2 / 2, 2 exp(-x) - 1 + x, 3 exp(x) - 1 - x; entropy: minus the mean of
+ * log_probs over all tokens.  metrics [5]: pg, KL, entropy, mean of the ratios, share of them that clip() changes by more than 1e-6
+ * (over tokens, or sequences with ratio_per_sequence).
+ * each (2 * sequences + 2 doubles, or NULL without a backward): what the backward needs of every sequence.
+ * mx_policy_loss_bwd: grad [tokens] in log_probs' type = *dloss times the gradient of the loss in log_probs.
+ *
+ * mx_preference_loss: sequences is even; pair p is sequence p, preferred to sequence sequences / 2 + p.  h = sum (or with `mean` mean)
+ * of log_probs - ref (ref NULL: of log_probs); z = h of the one - h of the other; the loss of a pair, averaged over pairs
+ * with a token that counts: kind 0 -(1 - smoothing) log sigmoid(beta z) - smoothing log sigmoid(-beta z), 1 max(0, 1 - beta z), 2 (z - 1 /
+ * (2 beta))^2.  rewards [sequences]: beta h.  each: sequences + 1 doubles, as above.
+ * workspace: mx_sequence_loss_workspace bytes, 8-byte aligned.  MX_ERR_UNSUPPORTED, before any launch, for 2^32 - 255 tokens and
+ * more or 2^30 sequences and more. */
+typedef struct {
+  const void *log_probs, *old_log_probs, *ref_log_probs;
+  int log_probs_f32, old_f32, ref_f32;
+  const float* advantages;
+  const void* offsets;
+  const uint8_t* mask;
+  int64_t sequences, tokens, length;
+  int offsets_i64, advantage_per_token, ratio_per_sequence, mean_per_sequence, kl;
+  double ratio_low, ratio_high, kl_coef, entropy_coef;
+} mx_policy_loss_t;
+typedef struct {
+  const void *log_probs, *ref_log_probs;
+  int log_probs_f32, ref_f32;
+  const void* offsets;
+  const uint8_t* mask;
+  int64_t sequences, tokens, length;
+  int offsets_i64, kind, mean;
+  double beta, smoothing;
+} mx_preference_loss_t;
+int64_t mx_sequence_loss_workspace(int64_t tokens, int64_t sequences);
+int mx_policy_loss(const mx_policy_loss_t* args, float* loss, float* metrics, double* each, void* workspace, void* stream);
+int mx_policy_loss_bwd(const mx_policy_loss_t* args, const double* each, const float* dloss, void* grad, void* stream);
+int mx_preference_loss(const mx_preference_loss_t* args, float* loss, float* rewards, double* each, void* workspace, void* stream);
+int mx_preference_loss_bwd(const mx_preference_loss_t* args, const double* each, const float* dloss, void* grad, void* stream);
+
 /* The AdamW step over n parameters (the optimizer behind torchtitan/components/optimizer.py).  table (host memory): n
  * times MX_ADAMW_FIELDS numbers -- parameter, whether it and its gradient are float32 (else bf16), gradient, first moment, second
  * moment, their scales (8 bits only), float32 master weight (or 0), number of values, step that this one is (from 1), the

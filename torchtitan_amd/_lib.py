@@ -78,6 +78,11 @@ SIGNATURES = {
     "mx_grad_norm": (c_int, [_I, _P, _P, _P, c_int, _P, _P, _P]),
     "mx_grad_clip": (c_int, [_I, _P, _P, _P, c_int, _P, ctypes.c_float, _P, _P]),
     "mx_grad_scale": (c_int, [_I, _P, _P, _P, _P, ctypes.c_float, _P]),
+    "mx_sequence_loss_workspace": (_I, [_I, _I]),
+    "mx_policy_loss": (c_int, [_P, _P, _P, _P, _P, _P]),
+    "mx_policy_loss_bwd": (c_int, [_P, _P, _P, _P, _P]),
+    "mx_preference_loss": (c_int, [_P, _P, _P, _P, _P, _P]),
+    "mx_preference_loss_bwd": (c_int, [_P, _P, _P, _P, _P]),
     "mx_adamw": (c_int, [_I, _P, c_int, ctypes.c_double, ctypes.c_double, ctypes.c_double, ctypes.c_double, ctypes.c_double,
                          c_int, _P, ctypes.c_float, ctypes.c_uint64, _P, _P, _P, _P]),
     "mx_adamw_moments": (c_int, [_I, _P, _P, _P, _P, _P, _P]),

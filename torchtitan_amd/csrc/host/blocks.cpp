@@ -71,6 +71,11 @@ struct Library {
   decltype(&mx_grad_norm_workspace) grad_norm_workspace = nullptr;
   decltype(&mx_grad_clip) grad_clip = nullptr;
   decltype(&mx_adamw) adamw = nullptr;
+  decltype(&mx_sequence_loss_workspace) sequence_loss_workspace = nullptr;
+  decltype(&mx_policy_loss) policy_loss = nullptr;
+  decltype(&mx_policy_loss_bwd) policy_loss_bwd = nullptr;
+  decltype(&mx_preference_loss) preference_loss = nullptr;
+  decltype(&mx_preference_loss_bwd) preference_loss_bwd = nullptr;
 } lib;
 PyObject* check_status = nullptr;  // _lib.check, never released
 
@@ -121,6 +126,11 @@ void bind(const py::dict& addresses, const py::object& check) {
   set("mx_grad_norm_workspace", lib.grad_norm_workspace);
   set("mx_grad_clip", lib.grad_clip);
   set("mx_adamw", lib.adamw);
+  set("mx_sequence_loss_workspace", lib.sequence_loss_workspace);
+  set("mx_policy_loss", lib.policy_loss);
+  set("mx_policy_loss_bwd", lib.policy_loss_bwd);
+  set("mx_preference_loss", lib.preference_loss);
+  set("mx_preference_loss_bwd", lib.preference_loss_bwd);
   check_status = check.ptr();
   Py_INCREF(check_status);
 }
@@ -1044,6 +1054,175 @@ std::optional<Tensor> clip_gradients(const std::vector<Tensor>& parameters, doub
   return norm;
 }
 
+// Losses over the tokens of sequences: the tensors of a call, in the order in which they are saved for the backward
+struct LossOperands {
+  Tensor log_probs, old, ref, advantages, offsets, mask;
+  int64_t sequences;
+};
+template <class Args>
+void loss_operands(Args& a, const LossOperands& o) {
+  a.log_probs = pointer(o.log_probs);
+  a.log_probs_f32 = is_f32(o.log_probs);
+  a.ref_log_probs = pointer(o.ref);
+  a.ref_f32 = o.ref.defined() && is_f32(o.ref);
+  a.offsets = pointer(o.offsets);
+  a.offsets_i64 = o.offsets.defined() && o.offsets.scalar_type() == at::kLong;
+  a.mask = static_cast<const uint8_t*>(pointer(o.mask));
+  a.sequences = o.sequences;
+  a.tokens = o.log_probs.numel();
+  a.length = o.offsets.defined() || o.sequences == 0 ? 0 : a.tokens / o.sequences;
+}
+// The plain case: dense tensors of the types that the kernels read, on the current GPU.
+bool loss_plain(const LossOperands& o) {
+  const Tensor& lp = o.log_probs;
+  if (!row_tensor(lp) || !lp.is_contiguous() || !no_subclass(lp) || !on_current_device(lp)) return false;
+  auto like = [&](const Tensor& t) { return t.device() == lp.device() && t.is_contiguous() && no_subclass(t) && !t.is_neg(); };
+  for (const Tensor& t : {o.old, o.ref})
+    if (t.defined() && (!row_tensor(t) || !like(t) || t.sizes() != lp.sizes())) return false;
+  if (o.advantages.defined() && (o.advantages.scalar_type() != at::kFloat || !like(o.advantages))) return false;
+  if (o.mask.defined() && (o.mask.scalar_type() != at::kBool || !like(o.mask) || o.mask.sizes() != lp.sizes())) return false;
+  if (o.offsets.defined())
+    return (o.offsets.scalar_type() == at::kLong || o.offsets.scalar_type() == at::kInt) && like(o.offsets) && lp.dim() == 1 &&
+           o.offsets.dim() == 1 && o.offsets.numel() == o.sequences + 1;
+  return lp.dim() == 2 && lp.size(0) == o.sequences;
+}
+
+struct PolicyNumbers {
+  int64_t advantage_per_token, ratio_per_sequence, mean_per_sequence, kl;
+  double low, high, kl_coef, entropy_coef;
+  mx_policy_loss_t args(const LossOperands& o) const {
+    mx_policy_loss_t a = {};
+    loss_operands(a, o);
+    a.old_log_probs = pointer(o.old);
+    a.old_f32 = o.old.defined() && is_f32(o.old);
+    a.advantages = static_cast<const float*>(pointer(o.advantages));
+    a.advantage_per_token = static_cast<int>(advantage_per_token);
+    a.ratio_per_sequence = static_cast<int>(ratio_per_sequence);
+    a.mean_per_sequence = static_cast<int>(mean_per_sequence);
+    a.kl = static_cast<int>(kl);
+    a.ratio_low = low, a.ratio_high = high, a.kl_coef = kl_coef, a.entropy_coef = entropy_coef;
+    return a;
+  }
+  int64_t more(const LossOperands&) const { return 5; }
+  int64_t each(const LossOperands& o) const { return 2 * o.sequences + 2; }
+  int forward(const LossOperands& o, float* loss, float* out, double* each, void* work, hipStream_t st) const {
+    const mx_policy_loss_t a = args(o);
+    return lib.policy_loss(&a, loss, out, each, work, st);
+  }
+  int backward(const LossOperands& o, const double* each, const float* dloss, void* grad, hipStream_t st) const {
+    const mx_policy_loss_t a = args(o);
+    return lib.policy_loss_bwd(&a, each, dloss, grad, st);
+  }
+  std::vector<double> pack() const {
+    return {double(advantage_per_token), double(ratio_per_sequence), double(mean_per_sequence), double(kl), low, high, kl_coef, entropy_coef};
+  }
+  static PolicyNumbers unpack(const std::vector<double>& v) {
+    return {int64_t(v[0]), int64_t(v[1]), int64_t(v[2]), int64_t(v[3]), v[4], v[5], v[6], v[7]};
+  }
+  static constexpr const char* name = "mx_policy_loss";
+};
+struct PreferenceNumbers {
+  int64_t kind, mean;
+  double beta, smoothing;
+  mx_preference_loss_t args(const LossOperands& o) const {
+    mx_preference_loss_t a = {};
+    loss_operands(a, o);
+    a.kind = static_cast<int>(kind);
+    a.mean = static_cast<int>(mean);
+    a.beta = beta, a.smoothing = smoothing;
+    return a;
+  }
+  int64_t more(const LossOperands& o) const { return o.sequences; }
+  int64_t each(const LossOperands& o) const { return o.sequences + 1; }
+  int forward(const LossOperands& o, float* loss, float* out, double* each, void* work, hipStream_t st) const {
+    const mx_preference_loss_t a = args(o);
+    return lib.preference_loss(&a, loss, out, each, work, st);
+  }
+  int backward(const LossOperands& o, const double* each, const float* dloss, void* grad, hipStream_t st) const {
+    const mx_preference_loss_t a = args(o);
+    return lib.preference_loss_bwd(&a, each, dloss, grad, st);
+  }
+  std::vector<double> pack() const { return {double(kind), double(mean), beta, smoothing}; }
+  static PreferenceNumbers unpack(const std::vector<double>& v) { return {int64_t(v[0]), int64_t(v[1]), v[2], v[3]}; }
+  static constexpr const char* name = "mx_preference_loss";
+};
+
+// (loss, metrics or rewards); `each`, where it is given, becomes what the backward needs
+template <class Numbers>
+std::array<Tensor, 2> loss_launch(const LossOperands& o, const Numbers& numbers, Tensor* each) {
+  const auto options = o.log_probs.options();
+  const Tensor loss = at::empty({}, options.dtype(at::kFloat)), more = at::empty({numbers.more(o)}, options.dtype(at::kFloat)),
+               work = at::empty({lib.sequence_loss_workspace(o.log_probs.numel(), o.sequences)}, options.dtype(at::kByte));
+  if (each) *each = at::empty({numbers.each(o)}, options.dtype(at::kDouble));
+  checked(numbers.forward(o, loss.data_ptr<float>(), more.data_ptr<float>(), each ? each->data_ptr<double>() : nullptr,
+                          work.data_ptr(), stream_of(o.log_probs)),
+          Numbers::name);
+  return {loss, more};
+}
+
+template <class Numbers>
+struct LossNode : torch::autograd::Function<LossNode<Numbers>> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& log_probs, const LossOperands& o, const Numbers& numbers) {
+    Tensor each;
+    const auto [loss, more] = loss_launch(o, numbers, &each);
+    ctx->save_for_backward({log_probs, o.old, o.ref, o.advantages, o.offsets, o.mask, each});
+    ctx->saved_data["numbers"] = numbers.pack();
+    ctx->saved_data["sequences"] = o.sequences;
+    ctx->set_materialize_grads(false);
+    ctx->mark_non_differentiable({more});
+    return {loss, more};
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    variable_list out(3);
+    if (!grads[0].defined()) return out;
+    const variable_list saved = ctx->get_saved_variables();
+    const auto dense = [](const Tensor& t) { return t.defined() ? t.contiguous() : t; };
+    const LossOperands o = {dense(saved[0]), dense(saved[1]), dense(saved[2]), dense(saved[3]), dense(saved[4]), dense(saved[5]),
+                            ctx->saved_data["sequences"].toInt()};
+    const Tensor each = saved[6].contiguous();
+    const Numbers numbers = Numbers::unpack(ctx->saved_data["numbers"].toDoubleVector());
+    const c10::DeviceGuard guard(grads[0].device());
+    // (hooks on saved tensors may have replaced them)
+    TORCH_CHECK(loss_plain(o) && each.device() == grads[0].device() && each.scalar_type() == at::kDouble &&
+                    each.numel() == numbers.each(o) && o.log_probs.device() == grads[0].device(),
+                "a saved tensor came back with another type, size or device");
+    const Tensor dloss = grads[0].resolve_neg().to(at::kFloat).contiguous(), grad = at::empty(o.log_probs.sizes(), o.log_probs.options());
+    checked(numbers.backward(o, each.data_ptr<double>(), dloss.data_ptr<float>(), grad.data_ptr(), stream_of(grad)), Numbers::name);
+    out[0] = grad;
+    return once(grads, std::move(out), true);
+  }
+};
+
+template <class Numbers>
+py::object loss_of(const LossOperands& o, const Numbers& numbers) {
+  if (!loss_plain(o)) return py::none();
+  Unlocked unlocked(std::in_place);
+  Tensor loss, more;
+  if (at::GradMode::is_enabled() && o.log_probs.requires_grad()) {
+    const variable_list out = LossNode<Numbers>::apply(o.log_probs, o, numbers);
+    loss = out[0], more = out[1];
+  } else {
+    const auto out = loss_launch(o, numbers, nullptr);
+    loss = out[0], more = out[1];
+  }
+  unlocked.reset();
+  return py::make_tuple(loss, more);
+}
+
+py::object policy_loss(const Tensor& log_probs, const Tensor& advantages, const std::optional<Tensor>& old,
+                       const std::optional<Tensor>& ref, const std::optional<Tensor>& offsets, const std::optional<Tensor>& mask,
+                       int64_t sequences, bool advantage_per_token, bool ratio_per_sequence, bool mean_per_sequence, int64_t kl,
+                       double low, double high, double kl_coef, double entropy_coef) {
+  return loss_of(LossOperands{log_probs, or_none(old), or_none(ref), advantages, or_none(offsets), or_none(mask), sequences},
+                 PolicyNumbers{advantage_per_token, ratio_per_sequence, mean_per_sequence, kl, low, high, kl_coef, entropy_coef});
+}
+py::object preference_loss(const Tensor& log_probs, const std::optional<Tensor>& ref, const std::optional<Tensor>& offsets,
+                           const std::optional<Tensor>& mask, int64_t sequences, int64_t kind, bool mean, double beta,
+                           double smoothing) {
+  return loss_of(LossOperands{log_probs, Tensor(), or_none(ref), Tensor(), or_none(offsets), or_none(mask), sequences},
+                 PreferenceNumbers{kind, mean, beta, smoothing});
+}
+
 // t's elements are one run of memory in p's order
 bool same_order(const Tensor& t, const Tensor& p) {
   if (t.is_contiguous()) return p.is_contiguous() && t.numel() == p.numel();
@@ -1183,5 +1362,7 @@ PYBIND11_MODULE(_blocks, m) {
   m.def("scaled_embedding", torch::wrap_pybind_function(scaled_embedding));
   m.def("residual_rms_norm", torch::wrap_pybind_function(residual_rms_norm));
   m.def("clip_gradients", torch::wrap_pybind_function(clip_gradients));
+  m.def("policy_loss", torch::wrap_pybind_function(policy_loss));
+  m.def("preference_loss", torch::wrap_pybind_function(preference_loss));
   m.def("adamw", torch::wrap_pybind_function(adamw));
 }

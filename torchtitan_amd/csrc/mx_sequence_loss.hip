@@ -1,0 +1,538 @@
+// Losses over the tokens of many sequences, and their gradients: the clipped policy loss with KL and entropy terms, and the
+// preference loss of paired sequences.
+//
+// Tokens lie in one array; sequence s has those from offsets[s] to offsets[s + 1], or every sequence `length` of them, and of
+// these the ones whose mask byte is not 0 count.  What is summed over a sequence (how many count, their log-ratios, the terms of
+// the loss) is summed in three steps, in an order that depends on the sizes alone:
+//   parts    a wave takes a chunk of tokens, whatever sequences they are of, and leaves the sums of each of them: chunk c and
+//            sequence s share the place c + s, and no other pair does, since one of the two grows from pair to pair.  Long and short
+//            sequences are the same work, and nothing has to be cleared.
+//   join     every sequence's parts are added up, the loss formed, and what a token's gradient needs of its sequence
+//   gradient tokens as they lie (backward)
+// A few megabytes at most are read: bound by the three launches' latency.  Terms are formed in float64, which is free here: a
+// ratio's side of a clipping border decides about its whole gradient, and the KL estimators are differences of nearly equal numbers.
+#include "mx_rows.h"
+
+namespace mx {
+
+constexpr int kSeqLanes = 64;
+constexpr int kSeqTokens = 8;  // of a lane and chunk
+constexpr int kSeqChunk = kSeqLanes * kSeqTokens;
+constexpr int kSeqJoin = 256;     // lanes of a workgroup that joins
+constexpr int kSeqJoinGroups = 1024;  // workgroups that join, at most
+constexpr int kSeqGrad = 256, kSeqGradTokens = 4;  // lanes of a workgroup, tokens of a lane
+
+// Log-probabilities, bf16 or float32
+struct SeqValues {
+  const void* p;
+  int f32;
+  __device__ __forceinline__ float at(int64_t i) const {
+    return f32 ? ((const float*)p)[i] : bf16_lo(((const uint16_t*)p)[i]);
+  }
+};
+
+struct Sequences {
+  const void* offsets;  // [count + 1], or null: `length` tokens each
+  int64_t count, tokens, length;
+  const uint8_t* mask;  // or null
+  int wide;             // offsets are int64
+  // (offsets outside the array, or that fall, are not followed out of it)
+  __device__ __forceinline__ int64_t offset(int64_t s) const {
+    if (!offsets) return s * length;
+    const int64_t at = wide ? ((const int64_t*)offsets)[s] : (int64_t)((const int32_t*)offsets)[s];
+    return at < 0 ? 0 : at > tokens ? tokens : at;
+  }
+  // The sequence of token i < tokens, from `first` on: -1 before the first one, `count` behind the last.
+  __device__ __forceinline__ int64_t find(int64_t i, int64_t first = -1) const {
+    if (!offsets) return tokens <= 0xFFFFFFFF ? (int64_t)((uint32_t)i / (uint32_t)length) : i / length;
+    int64_t lo = first, hi = count + 1;  // the last place whose offset is not behind i
+    while (hi - lo > 1) {
+      const int64_t mid = (lo + hi) >> 1;
+      if (offset(mid) <= i) lo = mid; else hi = mid;
+    }
+    return lo;
+  }
+};
+
+struct Policy {
+  SeqValues lp, old, ref;  // p null: none
+  const float* advantages;
+  int advantage_tokens;    // one for every token, else for every sequence
+  int whole;               // one ratio a sequence
+  int by_sequence;         // means over sequences of means over their tokens, else over all tokens
+  int kl;                  // 0 k1, 1 k2, 2 k3, 3 k3 swapped
+  double low, high;        // the ratio's borders
+  double kl_coef, entropy_coef;
+};
+struct Preference {
+  SeqValues lp, ref;
+  int kind;  // 0 sigmoid, 1 hinge, 2 squared
+  int mean;  // means of log-ratios, else sums
+  double beta, smoothing;
+};
+
+// -min(r A, clip(r) A): for A >= 0 the smaller, for A < 0 the larger of r and its border (0 where A is 0, whatever r is)
+__device__ __forceinline__ double seq_objective(const Policy& f, double r, double A) {
+  return A >= 0 ? -A * (r > f.high ? f.high : r) : -A * (r < f.low ? f.low : r);
+}
+__device__ __forceinline__ bool seq_clipped(const Policy& f, double r) {
+  const double c = r > f.high ? f.high : r < f.low ? f.low : r;
+  return fabs(r - c) > 1e-6;
+}
+__device__ __forceinline__ double seq_kl(int kind, double x) {
+  switch (kind) {
+    case 0: return x;
+    case 1: return 0.5 * x * x;
+    case 2: return expm1(-x) + x;
+    default: return expm1(x) - x;
+  }
+}
+__device__ __forceinline__ double seq_kl_slope(int kind, double x) {
+  switch (kind) {
+    case 0: return 1.0;
+    case 1: return x;
+    case 2: return -expm1(-x);
+    default: return expm1(x);
+  }
+}
+
+__device__ __forceinline__ double seq_wave_sum(double v) {
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
+  return v;
+}
+
+// What is read of a token, and what it adds to its sequence's sums.
+struct SeqToken {
+  float lp, old, ref, advantage;
+  bool counts;
+};
+constexpr int kPolicySums = 7;      // tokens, x, lp, kl, objective, ratio, clipped
+constexpr int kPreferenceSums = 2;  // tokens, x
+
+__device__ __forceinline__ SeqToken seq_load(const Policy& f, const Sequences& q, int64_t i) {
+  SeqToken t = {0.f, 0.f, 0.f, 0.f, i < q.tokens};
+  if (t.counts) {
+    t.lp = f.lp.at(i);
+    if (f.old.p) t.old = f.old.at(i);
+    if (f.ref.p) t.ref = f.ref.at(i);
+    if (f.advantage_tokens) t.advantage = f.advantages[i];
+    if (q.mask) t.counts = q.mask[i] != 0;
+  }
+  return t;
+}
+__device__ __forceinline__ SeqToken seq_load(const Preference& f, const Sequences& q, int64_t i) {
+  SeqToken t = {0.f, 0.f, 0.f, 0.f, i < q.tokens};
+  if (t.counts) {
+    t.lp = f.lp.at(i);
+    if (f.ref.p) t.ref = f.ref.at(i);
+    if (q.mask) t.counts = q.mask[i] != 0;
+  }
+  return t;
+}
+__device__ __forceinline__ double seq_advantage(const Policy& f, const SeqToken& t, int64_t s) {
+  return (double)(f.advantage_tokens ? t.advantage : f.advantages[s]);
+}
+__device__ __forceinline__ void seq_add(const Policy& f, const SeqToken& t, int64_t s, double (&sum)[kPolicySums]) {
+  const double lp = (double)t.lp, x = f.old.p ? lp - (double)t.old : 0.0;
+  sum[0] += 1.0;
+  sum[1] += x;
+  sum[2] += lp;
+  if (f.ref.p) sum[3] += seq_kl(f.kl, lp - (double)t.ref);
+  if (!f.whole) {
+    const double r = exp(x);
+    sum[4] += seq_objective(f, r, seq_advantage(f, t, s));
+    sum[5] += r;
+    sum[6] += seq_clipped(f, r) ? 1.0 : 0.0;
+  }
+}
+__device__ __forceinline__ void seq_add(const Preference& f, const SeqToken& t, int64_t, double (&sum)[kPreferenceSums]) {
+  sum[0] += 1.0;
+  sum[1] += f.ref.p ? (double)t.lp - (double)t.ref : (double)t.lp;
+}
+
+// parts: [chunks + count][SUMS].  A wave's chunk is rows of 64 tokens.  Rows inside one sequence are added up lane by lane; in a row
+// that sequences end in, those that lie in it whole are summed among their lanes, and the running one is summed up and left.
+template <class F, int SUMS>
+__global__ __launch_bounds__(kSeqLanes) void seq_parts_kernel(F f, Sequences q, double* __restrict__ parts) {
+  const int64_t chunk = blockIdx.x, begin = chunk * kSeqChunk;
+  const int64_t end = begin + kSeqChunk < q.tokens ? begin + kSeqChunk : q.tokens;
+  const int lane = threadIdx.x;
+  SeqToken t[kSeqTokens];
+#pragma unroll
+  for (int k = 0; k < kSeqTokens; ++k) t[k] = seq_load(f, q, begin + k * kSeqLanes + lane);
+  int64_t s = q.find(begin);
+  int64_t stop = s < 0 || s >= q.count ? begin : q.offset(s + 1);
+  double sum[SUMS];
+  auto clear = [&]() {
+#pragma unroll
+    for (int k = 0; k < SUMS; ++k) sum[k] = 0.0;
+  };
+  auto leave = [&]() {  // the running sequence's sums
+    if (s < 0 || s >= q.count) return;
+#pragma unroll
+    for (int k = 0; k < SUMS; ++k) {
+      const double all = seq_wave_sum(sum[k]);
+      if (lane == k) parts[(chunk + s) * SUMS + k] = all;
+    }
+  };
+  clear();
+#pragma unroll
+  for (int k = 0; k < kSeqTokens; ++k) {
+    const int64_t row = begin + k * kSeqLanes, i = row + lane;
+    if (row >= end) break;
+    if (stop >= (row + kSeqLanes < end ? row + kSeqLanes : end)) {
+      if (t[k].counts) seq_add(f, t[k], s, sum);
+      continue;
+    }
+    const int64_t mine = i < end ? q.find(i, s < q.count ? s : -1) : q.count;
+    double v[SUMS];
+#pragma unroll
+    for (int j = 0; j < SUMS; ++j) v[j] = 0.0;
+    if (mine >= 0 && mine < q.count && t[k].counts) seq_add(f, t[k], mine, v);
+    if (mine == s)
+#pragma unroll
+      for (int j = 0; j < SUMS; ++j) sum[j] += v[j];
+    const int64_t last = __shfl(mine, 63, 64);
+    if (last == s) continue;
+    leave();
+    const bool middle = mine != s && mine != last;
+#pragma unroll
+    for (int j = 0; j < SUMS; ++j) sum[j] = mine == last ? v[j] : 0.0;
+    if (__ballot(middle)) {
+      for (int off = 1; off < 64; off <<= 1) {
+        const int64_t other = __shfl_down(mine, off, 64);
+        const bool same = lane + off < 64 && other == mine;
+#pragma unroll
+        for (int j = 0; j < SUMS; ++j) {
+          const double more = __shfl_down(v[j], off, 64);
+          if (same) v[j] += more;
+        }
+      }
+      const int64_t before = __shfl_up(mine, 1, 64);
+      if (middle && mine >= 0 && mine < q.count && (lane == 0 || before != mine))
+#pragma unroll
+        for (int j = 0; j < SUMS; ++j) parts[(chunk + mine) * SUMS + j] = v[j];
+    }
+    s = last;
+    stop = s < 0 || s >= q.count ? row : q.offset(s + 1);
+  }
+  leave();
+}
+
+// The sums of sequence s from its parts, in the first of `lanes` lanes that take them in turn (others: part of them).
+template <int SUMS>
+__device__ __forceinline__ void seq_joined(const Sequences& q, const double* __restrict__ parts, int64_t s, int lane, int lanes,
+                                           double (&sum)[SUMS]) {
+#pragma unroll
+  for (int k = 0; k < SUMS; ++k) sum[k] = 0.0;
+  const int64_t begin = q.offset(s), end = q.offset(s + 1);
+  if (end > begin) {
+    const int64_t last = (end - 1) / kSeqChunk;
+    for (int64_t c = begin / kSeqChunk + lane; c <= last; c += lanes)
+#pragma unroll
+      for (int k = 0; k < SUMS; ++k) sum[k] += parts[(c + s) * SUMS + k];
+  }
+  for (int off = 1; off < lanes; off <<= 1)
+#pragma unroll
+    for (int k = 0; k < SUMS; ++k) sum[k] += __shfl_xor(sum[k], off, 64);
+}
+
+// Sums over the lanes of the workgroup, in lane 0.
+template <int N>
+__device__ __forceinline__ void seq_group_sum(double (&v)[N]) {
+  __shared__ double shared[kSeqJoin / 64][N];
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    v[k] = seq_wave_sum(v[k]);
+    if ((threadIdx.x & 63) == 0) shared[threadIdx.x >> 6][k] = v[k];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    v[k] = 0.0;
+    for (int w = 0; w < kSeqJoin / 64; ++w) v[k] += shared[w][k];
+  }
+}
+
+// Sums over all sequences.  Policy: tokens, sequences that have some; by token objective, kl, ratio, clipped; by sequence the
+// same; lp.  Preference: losses, pairs.
+constexpr int kPolicyTotals = 11, kPreferenceTotals = 2;
+
+// Of the sequence: for the gradient, each[2 s] tokens, each[2 s + 1] what its ratio adds to a token's gradient.
+__device__ __forceinline__ void seq_take(const Policy& f, const Sequences& q, const double* __restrict__ parts, int64_t s, int lane,
+                                         int lanes, double* __restrict__ each, float*, double (&total)[kPolicyTotals]) {
+  double sum[kPolicySums];
+  seq_joined(q, parts, s, lane, lanes, sum);
+  if (lane) return;
+  const double n = sum[0];
+  double slope = 0.0;
+  if (n > 0.0) {
+    if (f.whole) {
+      const double r = exp(sum[1] / n), A = (double)f.advantages[s];
+      if (A >= 0 ? !(r > f.high) : !(r < f.low)) slope = -A * r;
+      sum[4] = n * seq_objective(f, r, A);
+      sum[5] = n * r;
+      sum[6] = seq_clipped(f, r) ? n : 0.0;
+    }
+    total[0] += n;
+    total[1] += 1.0;
+    total[2] += sum[4], total[3] += sum[3], total[4] += sum[5], total[5] += sum[6];
+    total[6] += sum[4] / n, total[7] += sum[3] / n, total[8] += sum[5] / n, total[9] += sum[6] / n;
+    total[10] += sum[2];
+  }
+  if (each) each[2 * s] = n, each[2 * s + 1] = slope;
+}
+__device__ __forceinline__ void seq_finish(const Policy& f, const Sequences& q, const double (&total)[kPolicyTotals],
+                                           double* __restrict__ each, float* __restrict__ loss, float* __restrict__ metrics) {
+  const double tokens = total[0] > 0 ? total[0] : 1.0, filled = total[1] > 0 ? total[1] : 1.0;
+  const double pg = f.by_sequence ? total[6] / filled : total[2] / tokens, kl = f.by_sequence ? total[7] / filled : total[3] / tokens;
+  const double entropy = -total[10] / tokens;
+  *loss = (float)(pg + f.kl_coef * kl - f.entropy_coef * entropy);
+  metrics[0] = (float)pg;
+  metrics[1] = (float)kl;
+  metrics[2] = (float)entropy;
+  metrics[3] = (float)(f.whole ? total[8] / filled : total[4] / tokens);
+  metrics[4] = (float)(f.whole ? total[9] / filled : total[5] / tokens);
+  if (each) each[2 * q.count] = tokens, each[2 * q.count + 1] = filled;
+}
+
+__device__ __forceinline__ double seq_soft(double y) {  // -log sigmoid(y)
+  return log1p(exp(-fabs(y))) + (y < 0 ? -y : 0.0);
+}
+__device__ __forceinline__ double seq_sigmoid(double y) {
+  const double e = exp(-fabs(y)), p = 1.0 / (1.0 + e);
+  return y < 0 ? e * p : p;
+}
+
+// Of the pair: for the gradient, each[s] that of a token of either sequence (but for the mean over the pairs).
+__device__ __forceinline__ void seq_take(const Preference& f, const Sequences& q, const double* __restrict__ parts, int64_t p, int lane,
+                                         int lanes, double* __restrict__ each, float* __restrict__ rewards,
+                                         double (&total)[kPreferenceTotals]) {
+  const int64_t other = q.count / 2 + p;
+  double one[kPreferenceSums], two[kPreferenceSums];
+  seq_joined(q, parts, p, lane, lanes, one);
+  seq_joined(q, parts, other, lane, lanes, two);
+  if (lane) return;
+  const double of1 = f.mean && one[0] > 0 ? 1.0 / one[0] : 1.0, of2 = f.mean && two[0] > 0 ? 1.0 / two[0] : 1.0;
+  const double h1 = one[1] * of1, h2 = two[1] * of2, z = h1 - h2, y = f.beta * z;
+  double value, slope;
+  if (f.kind == 0) {
+    value = (1.0 - f.smoothing) * seq_soft(y) + f.smoothing * seq_soft(-y);
+    slope = f.beta * (f.smoothing * seq_sigmoid(y) - (1.0 - f.smoothing) * seq_sigmoid(-y));
+  } else if (f.kind == 1) {
+    value = 1.0 - y < 0 ? 0.0 : 1.0 - y;  // (NaN stays)
+    slope = y < 1.0 ? -f.beta : 0.0;
+  } else {
+    const double left = z - 0.5 / f.beta;
+    value = left * left;
+    slope = 2.0 * left;
+  }
+  if (one[0] + two[0] > 0) total[0] += value, total[1] += 1.0;
+  rewards[p] = (float)(f.beta * h1);
+  rewards[other] = (float)(f.beta * h2);
+  if (each) each[p] = slope * of1, each[other] = -slope * of2;
+}
+__device__ __forceinline__ void seq_finish(const Preference&, const Sequences& q, const double (&total)[kPreferenceTotals],
+                                           double* __restrict__ each, float* __restrict__ loss, float*) {
+  const double pairs = total[1] > 0 ? total[1] : 1.0;
+  *loss = (float)(total[0] / pairs);
+  if (each) each[q.count] = pairs;
+}
+
+// `lanes` lanes a sequence (or pair), `items` of them.  One workgroup finishes the loss; several leave their sums in `totals`.
+template <class F, int TOTALS>
+__global__ __launch_bounds__(kSeqJoin) void seq_join_kernel(F f, Sequences q, int64_t items, int lanes,
+                                                            const double* __restrict__ parts, double* __restrict__ totals,
+                                                            double* __restrict__ each, float* __restrict__ loss,
+                                                            float* __restrict__ more) {
+  double total[TOTALS];
+#pragma unroll
+  for (int k = 0; k < TOTALS; ++k) total[k] = 0.0;
+  const int lane = threadIdx.x & (lanes - 1), groups = kSeqJoin / lanes;
+  for (int64_t s = (int64_t)blockIdx.x * groups + threadIdx.x / lanes; s < items; s += (int64_t)gridDim.x * groups)
+    seq_take(f, q, parts, s, lane, lanes, each, more, total);
+  seq_group_sum(total);
+  if (threadIdx.x == 0) {
+    if (gridDim.x == 1) {
+      seq_finish(f, q, total, each, loss, more);
+    } else {
+#pragma unroll
+      for (int k = 0; k < TOTALS; ++k) totals[(int64_t)blockIdx.x * TOTALS + k] = total[k];
+    }
+  }
+}
+template <class F, int TOTALS>
+__global__ __launch_bounds__(kSeqJoin) void seq_finish_kernel(F f, Sequences q, int groups, const double* __restrict__ totals,
+                                                              double* __restrict__ each, float* __restrict__ loss,
+                                                              float* __restrict__ more) {
+  double total[TOTALS];
+#pragma unroll
+  for (int k = 0; k < TOTALS; ++k) total[k] = 0.0;
+  for (int g = threadIdx.x; g < groups; g += kSeqJoin)
+#pragma unroll
+    for (int k = 0; k < TOTALS; ++k) total[k] += totals[(int64_t)g * TOTALS + k];
+  seq_group_sum(total);
+  if (threadIdx.x == 0) seq_finish(f, q, total, each, loss, more);
+}
+
+// The gradient of one token that counts.
+__device__ __forceinline__ double seq_grad(const Policy& f, const double* __restrict__ each, int64_t count, const SeqToken& t,
+                                           int64_t s) {
+  const double lp = (double)t.lp, tokens = each[2 * count], filled = each[2 * count + 1];
+  double g = each[2 * s + 1];
+  if (!f.whole) {
+    const double r = f.old.p ? exp(lp - (double)t.old) : 1.0, A = seq_advantage(f, t, s);
+    if (A >= 0 ? !(r > f.high) : !(r < f.low)) g = -A * r;
+  }
+  if (f.ref.p) g += f.kl_coef * seq_kl_slope(f.kl, lp - (double)t.ref);
+  return g / (f.by_sequence ? filled * each[2 * s] : tokens) + f.entropy_coef / tokens;
+}
+__device__ __forceinline__ double seq_grad(const Preference&, const double* __restrict__ each, int64_t count, const SeqToken&,
+                                           int64_t s) {
+  return each[s] / each[count];
+}
+
+// grad[i] = dloss * (that, where token i counts, else 0)
+template <class F>
+__global__ __launch_bounds__(kSeqGrad) void seq_grad_kernel(F f, Sequences q, const double* __restrict__ each,
+                                                            const float* __restrict__ dloss, void* __restrict__ grad) {
+  const int64_t begin = ((int64_t)blockIdx.x * (kSeqGrad / 64) + (threadIdx.x >> 6)) * (64 * kSeqGradTokens);
+  const int lane = threadIdx.x & 63;
+  if (begin >= q.tokens) return;
+  SeqToken t[kSeqGradTokens];
+#pragma unroll
+  for (int k = 0; k < kSeqGradTokens; ++k) t[k] = seq_load(f, q, begin + k * 64 + lane);
+  const int64_t first = q.find(begin);
+  const int64_t end = begin + 64 * kSeqGradTokens < q.tokens ? begin + 64 * kSeqGradTokens : q.tokens;
+  const bool one = first >= 0 && first < q.count && q.offset(first + 1) >= end;  // all of one sequence
+  const double by = (double)*dloss;
+#pragma unroll
+  for (int k = 0; k < kSeqGradTokens; ++k) {
+    const int64_t i = begin + k * 64 + lane;
+    if (i >= q.tokens) return;
+    const int64_t s = one ? first : q.find(i, first < q.count ? first : -1);
+    double g = 0.0;
+    if (t[k].counts && s >= 0 && s < q.count) g = seq_grad(f, each, q.count, t[k], s) * by;
+    if (f.lp.f32) ((float*)grad)[i] = (float)g;
+    else ((uint16_t*)grad)[i] = (uint16_t)__builtin_bit_cast(uint32_t, __builtin_convertvector(v2f_t{(float)g, 0.f}, v2bf_t));
+  }
+}
+
+static int seq_check(const Sequences& q) {
+  if (q.count < 0 || q.tokens < 0 || (q.count == 0 && !q.offsets && q.tokens > 0)) return MX_ERR_INVALID_ARG;
+  if (!q.offsets && (q.length < 0 || q.length * q.count != q.tokens)) return MX_ERR_INVALID_ARG;
+  if ((uintptr_t)q.offsets & (q.wide ? 7 : 3)) return MX_ERR_ALIGNMENT;
+  // (a wave for every chunk, a lane for every token: launches have fewer than 2^32 lanes)
+  if (q.tokens > 0xFFFFFF00 || q.count > 0x3FFFFFFF) return MX_ERR_UNSUPPORTED;
+  return MX_OK;
+}
+static bool seq_odd(const SeqValues& v) { return (uintptr_t)v.p & (v.f32 ? 3 : 1); }
+
+// Lanes that add up a sequence's parts: about as many as it has of them on average.
+static int seq_lanes(const Sequences& q) {
+  const int64_t each = q.count ? (q.tokens + kSeqChunk - 1) / kSeqChunk / q.count : 0;
+  int lanes = 1;
+  while (lanes < 64 && lanes < each) lanes *= 2;
+  return lanes;
+}
+
+// Two launches, or three where one workgroup would have more than four rounds of sequences to join.
+template <int SUMS, int TOTALS, class F>
+static void seq_loss(const F& f, const Sequences& q, int64_t items, double* parts, double* each, float* loss, float* more,
+                     hipStream_t st) {
+  const int64_t chunks = (q.tokens + kSeqChunk - 1) / kSeqChunk;
+  if (chunks) hipLaunchKernelGGL((seq_parts_kernel<F, SUMS>), dim3((unsigned)chunks), dim3(kSeqLanes), 0, st, f, q, parts);
+  const int lanes = seq_lanes(q);
+  const int64_t rounds = (items * lanes + kSeqJoin - 1) / kSeqJoin;
+  const int groups = rounds <= 4 ? 1 : rounds < kSeqJoinGroups ? (int)rounds : kSeqJoinGroups;
+  double* const totals = parts + (chunks + q.count) * SUMS;
+  hipLaunchKernelGGL((seq_join_kernel<F, TOTALS>), dim3(groups), dim3(kSeqJoin), 0, st, f, q, items, lanes, (const double*)parts,
+                     totals, each, loss, more);
+  if (groups > 1)
+    hipLaunchKernelGGL((seq_finish_kernel<F, TOTALS>), dim3(1), dim3(kSeqJoin), 0, st, f, q, groups, (const double*)totals, each,
+                       loss, more);
+}
+template <class F>
+static void seq_grads(const F& f, const Sequences& q, const double* each, const float* dloss, void* grad, hipStream_t st) {
+  constexpr int64_t per = kSeqGrad * kSeqGradTokens;
+  hipLaunchKernelGGL(seq_grad_kernel<F>, dim3((unsigned)((q.tokens + per - 1) / per)), dim3(kSeqGrad), 0, st, f, q, each, dloss, grad);
+}
+
+static int status() { return hipGetLastError() == hipSuccess ? MX_OK : MX_ERR_LAUNCH; }
+
+}  // namespace mx
+
+using namespace mx;
+
+extern "C" int64_t mx_sequence_loss_workspace(int64_t tokens, int64_t sequences) {
+  if (tokens < 0 || sequences < 0) return 0;
+  return 8 * (kPolicySums * ((tokens + kSeqChunk - 1) / kSeqChunk + sequences) + kPolicyTotals * kSeqJoinGroups);
+}
+
+static int policy_check(const mx_policy_loss_t* a, Policy& f, Sequences& q) {
+  if (!a) return MX_ERR_INVALID_ARG;
+  f = {{a->log_probs, a->log_probs_f32}, {a->old_log_probs, a->old_f32}, {a->ref_log_probs, a->ref_f32}, a->advantages,
+       a->advantage_per_token, a->ratio_per_sequence, a->mean_per_sequence, a->kl, a->ratio_low, a->ratio_high, a->kl_coef,
+       a->entropy_coef};
+  q = {a->offsets, a->sequences, a->tokens, a->length, a->mask, a->offsets_i64};
+  if (const int rc = seq_check(q)) return rc;
+  if ((q.tokens > 0 && !f.lp.p) || (q.count > 0 && q.tokens > 0 && !f.advantages) || f.kl < 0 || f.kl > 3 ||
+      (f.whole && f.advantage_tokens))
+    return MX_ERR_INVALID_ARG;
+  return seq_odd(f.lp) || seq_odd(f.old) || seq_odd(f.ref) || ((uintptr_t)f.advantages & 3) ? MX_ERR_ALIGNMENT : MX_OK;
+}
+
+extern "C" int mx_policy_loss(const mx_policy_loss_t* args, float* loss, float* metrics, double* each, void* workspace,
+                              void* stream) {
+  Policy f;
+  Sequences q;
+  if (const int rc = policy_check(args, f, q)) return rc;
+  if (!loss || !metrics || !workspace) return MX_ERR_INVALID_ARG;
+  if (((uintptr_t)loss & 3) || ((uintptr_t)metrics & 3) || ((uintptr_t)each & 7) || ((uintptr_t)workspace & 7)) return MX_ERR_ALIGNMENT;
+  seq_loss<kPolicySums, kPolicyTotals>(f, q, q.count, (double*)workspace, each, loss, metrics, (hipStream_t)stream);
+  return status();
+}
+
+extern "C" int mx_policy_loss_bwd(const mx_policy_loss_t* args, const double* each, const float* dloss, void* grad, void* stream) {
+  Policy f;
+  Sequences q;
+  if (const int rc = policy_check(args, f, q)) return rc;
+  if (q.tokens == 0) return MX_OK;
+  if (!each || !dloss || !grad) return MX_ERR_INVALID_ARG;
+  if (((uintptr_t)each & 7) || ((uintptr_t)dloss & 3) || ((uintptr_t)grad & (f.lp.f32 ? 3 : 1))) return MX_ERR_ALIGNMENT;
+  seq_grads(f, q, each, dloss, grad, (hipStream_t)stream);
+  return status();
+}
+
+static int preference_check(const mx_preference_loss_t* a, Preference& f, Sequences& q) {
+  if (!a) return MX_ERR_INVALID_ARG;
+  f = {{a->log_probs, a->log_probs_f32}, {a->ref_log_probs, a->ref_f32}, a->kind, a->mean, a->beta, a->smoothing};
+  q = {a->offsets, a->sequences, a->tokens, a->length, a->mask, a->offsets_i64};
+  if (const int rc = seq_check(q)) return rc;
+  if ((q.tokens > 0 && !f.lp.p) || q.count % 2 || f.kind < 0 || f.kind > 2) return MX_ERR_INVALID_ARG;
+  return seq_odd(f.lp) || seq_odd(f.ref) ? MX_ERR_ALIGNMENT : MX_OK;
+}
+
+extern "C" int mx_preference_loss(const mx_preference_loss_t* args, float* loss, float* rewards, double* each, void* workspace,
+                                  void* stream) {
+  Preference f;
+  Sequences q;
+  if (const int rc = preference_check(args, f, q)) return rc;
+  if (!loss || (q.count > 0 && !rewards) || !workspace) return MX_ERR_INVALID_ARG;
+  if (((uintptr_t)loss & 3) || ((uintptr_t)rewards & 3) || ((uintptr_t)each & 7) || ((uintptr_t)workspace & 7)) return MX_ERR_ALIGNMENT;
+  seq_loss<kPreferenceSums, kPreferenceTotals>(f, q, q.count / 2, (double*)workspace, each, loss, rewards, (hipStream_t)stream);
+  return status();
+}
+
+extern "C" int mx_preference_loss_bwd(const mx_preference_loss_t* args, const double* each, const float* dloss, void* grad,
+                                      void* stream) {
+  Preference f;
+  Sequences q;
+  if (const int rc = preference_check(args, f, q)) return rc;
+  if (q.tokens == 0) return MX_OK;
+  if (!each || !dloss || !grad) return MX_ERR_INVALID_ARG;
+  if (((uintptr_t)each & 7) || ((uintptr_t)dloss & 3) || ((uintptr_t)grad & (f.lp.f32 ? 3 : 1))) return MX_ERR_ALIGNMENT;
+  seq_grads(f, q, each, dloss, grad, (hipStream_t)stream);
+  return status();
+}

@@ -5,13 +5,19 @@ Same functions, arguments, return values and formulas as the reference.  The one
 log-softmax over the vocabulary in float32 followed by a gather of the generated tokens, runs
 as one HIP kernel over the bf16 logits (and one more in backward) whenever the logits are a
 bf16 GPU tensor; otherwise the same torch ops as the reference run.
+
+``policy_loss`` is the loss itself over the tokens of a whole batch, packed or padded, with ratios of tokens or of sequences, and
+``preference_loss`` that of pairs of sequences: two launches forward and one backward on the GPU, elsewhere the same
+formula in torch operations.
 """
 from __future__ import annotations
+
+import math
 
 import torch
 import torch.nn.functional as F
 
-from .. import ops
+from .. import _lib, ops
 
 
 class _TokenLogProbs(torch.autograd.Function):
@@ -60,6 +66,13 @@ def compute_policy_gradient_loss(model: torch.nn.Module, vllm_token_ids: list[li
     device = next(model.parameters()).device
     advantages = advantages.to(device)
     batch_lps = [compute_token_log_probs(model, p, g, device) for p, g in zip(prompt_token_ids, vllm_token_ids)]
+    if _one_launch(batch_lps, ref_token_log_probs, advantages):
+        offsets = torch.tensor([0, *(len(g) for g in vllm_token_ids)], dtype=torch.int64).cumsum(0).to(device)
+        ref = torch.cat(list(ref_token_log_probs))
+        total, values = policy_loss(torch.cat(batch_lps), advantages, ref, ref, offsets=offsets, clip_eps=ppo_clip_eps,
+                                    kl_coef=kl_coef, kl="k3_swapped", entropy_coef=entropy_coef, ratio="sequence",
+                                    average="sequence")
+        return total, dict(zip(POLICY_METRICS, values.tolist())), batch_lps
     mean_log_ratio, mean_kl = [], []
     for lps, ref in zip(batch_lps, ref_token_log_probs):
         log_ratio = lps - ref.detach()
@@ -80,3 +93,222 @@ def compute_policy_gradient_loss(model: torch.nn.Module, vllm_token_ids: list[li
         "ratio_clipped_frac": (torch.abs(ratio - clipped_ratio) > 1e-6).float().mean().item(),
     }
     return total, metrics, batch_lps
+
+
+def _one_launch(log_probs, ref, advantages: torch.Tensor) -> bool:
+    """The samples' losses can be formed over all tokens at once: float32 on one GPU, no sample empty."""
+    plain = lambda t: type(t) is torch.Tensor and t.is_cuda and t.dtype == torch.float32 and t.device == advantages.device
+    return (bool(log_probs) and len(log_probs) == len(ref) and plain(advantages) and advantages.shape == (len(log_probs),)
+            and not advantages.requires_grad
+            and all(plain(a) and plain(b) and a.dim() == 1 and a.shape == b.shape and a.numel() > 0 for a, b in zip(log_probs, ref)))
+
+
+POLICY_METRICS = ("pg_loss", "kl_div", "entropy", "ratio_mean", "ratio_clipped_frac")
+_KL = ("k1", "k2", "k3", "k3_swapped")
+_PREFERENCES = ("sigmoid", "hinge", "ipo")
+
+
+def _check_tokens(log_probs, others: dict, offsets, mask) -> int:
+    """How many sequences the tokens are of."""
+    if not log_probs.is_floating_point():
+        raise TypeError(f"log_probs must be floating-point, got {log_probs.dtype}")
+    if log_probs.dim() != (2 if offsets is None else 1):
+        raise ValueError(f"log_probs must be [sequences, length], or [tokens] with offsets; got {tuple(log_probs.shape)}"
+                         f"{'' if offsets is None else ' with offsets'}")
+    for name, t in others.items():
+        if t is not None and not t.is_floating_point():
+            raise TypeError(f"{name} must be floating-point, got {t.dtype}")
+        if t is not None and t.shape != log_probs.shape:
+            raise ValueError(f"{name} must have the shape of log_probs, {tuple(log_probs.shape)}, got {tuple(t.shape)}")
+    if mask is not None and (mask.dtype != torch.bool or mask.shape != log_probs.shape):
+        raise ValueError(f"mask must be bool with the shape of log_probs, {tuple(log_probs.shape)}, got {tuple(mask.shape)} {mask.dtype}")
+    if offsets is not None and (offsets.dtype not in (torch.int64, torch.int32) or offsets.dim() != 1 or offsets.numel() == 0):
+        raise ValueError(f"offsets must be int64 or int32 [sequences + 1], got {tuple(offsets.shape)} {offsets.dtype}")
+    for name, t in (*others.items(), ("offsets", offsets), ("mask", mask)):
+        if t is not None and t.device != log_probs.device:
+            raise ValueError(f"log_probs on {log_probs.device}, {name} on {t.device}")
+    return log_probs.shape[0] if offsets is None else offsets.numel() - 1
+
+
+def _native(log_probs, *others) -> bool:
+    """Worth asking the native module: tensors of the types that the kernels read, eager and untransformed."""
+    return (not torch.compiler.is_compiling() and log_probs.dtype in ops.ROW_TYPES and ops.native_rows(log_probs)
+            and all(t is None or type(t) in (torch.Tensor, torch.nn.Parameter) for t in (log_probs, *others)))
+
+
+def _dense(t):
+    """Without a gradient, as the kernels read it."""
+    if t is None:
+        return None
+    t = t.detach()
+    if t.is_floating_point() and t.dtype not in ops.ROW_TYPES:
+        t = t.float()
+    return t.resolve_neg().contiguous()
+
+
+def _places(log_probs, offsets, mask, sequences: int):
+    """(sequence of every token, whether it counts), flat."""
+    place = torch.arange(log_probs.numel(), device=log_probs.device)
+    if offsets is None:
+        sequence = place // max(1, log_probs.shape[1])
+        counts = torch.ones_like(place, dtype=torch.bool)
+    else:
+        sequence = torch.bucketize(place, offsets.long(), right=True) - 1
+        counts = (sequence >= 0) & (sequence < sequences)
+        sequence = sequence.clamp(0, max(0, sequences - 1))
+    return sequence, counts if mask is None else counts & mask.reshape(-1)
+
+
+def _sums(values, sequence, sequences: int):
+    return values.new_zeros(sequences).index_add(0, sequence, values)
+
+
+def _nothing(log_probs):
+    """The loss of no sequences, with its gradient."""
+    return log_probs[:0].float().sum()
+
+
+def _kl_term(x, kind: int):
+    if _KL[kind] == "k1":
+        return x
+    if _KL[kind] == "k2":
+        return 0.5 * x * x
+    return torch.expm1(-x) + x if _KL[kind] == "k3" else torch.expm1(x) - x
+
+
+def _policy_in_torch_ops(log_probs, advantages, old, ref, offsets, mask, sequences, per_token, whole, by_sequence, kl, low, high,
+                         kl_coef, entropy_coef):
+    if sequences == 0:
+        return _nothing(log_probs), torch.zeros(5, device=log_probs.device)
+    sequence, counts = _places(log_probs, offsets, mask, sequences)
+    flat = lambda t: torch.where(counts, t.reshape(-1).double(), 0.0)
+    lp = flat(log_probs)
+    n = _sums(counts.double(), sequence, sequences)
+    tokens, filled, per_sequence = n.sum().clamp(min=1), (n > 0).sum().clamp(min=1).double(), n.clamp(min=1)
+    each = (1 / (filled * per_sequence))[sequence] if by_sequence else (1 / tokens).expand_as(lp)
+    x = lp - (lp.detach() if old is None else flat(old))
+    A = advantages.detach().double()
+    A = A.reshape(-1) if per_token else A[sequence]
+    if whole:
+        x = (_sums(x, sequence, sequences) / per_sequence)[sequence]
+    A = torch.where(counts, A, 0.0)
+    ratio = torch.exp(torch.where(A >= 0, x.detach(), x))
+    # (where the upper border is behind, nothing that overflows is differentiated)
+    bounded = torch.where(A >= 0, torch.exp(x.clamp(max=math.log(max(high, 1e-300)) + 1.0)).clamp(max=high), ratio.clamp(min=low))
+    objective = -A * bounded
+    mean = lambda values, weight: torch.where(counts, values * weight, 0.0).sum()
+    pg, kl_div = mean(objective, each), lp.new_zeros(())
+    if ref is not None:
+        kl_div = mean(_kl_term(lp - flat(ref), kl), each)
+    entropy = -lp.sum() / tokens
+    total = pg + kl_coef * kl_div - entropy_coef * entropy
+    with torch.no_grad():
+        per = (1 / (filled * per_sequence))[sequence] if whole else (1 / tokens).expand_as(lp)
+        clipped = ((ratio - ratio.clamp(low, high)).abs() > 1e-6).double()
+        metrics = torch.stack([pg.detach(), kl_div.detach(), entropy.detach(), mean(ratio, per), mean(clipped, per)]).float()
+    return total.float(), metrics
+
+
+def policy_loss(log_probs: torch.Tensor, advantages: torch.Tensor, old_log_probs: torch.Tensor | None = None,
+                ref_log_probs: torch.Tensor | None = None, *, offsets: torch.Tensor | None = None, mask: torch.Tensor | None = None,
+                clip_eps: float = 0.2, clip_eps_high: float | None = None, kl_coef: float = 0.0, kl: str = "k3",
+                entropy_coef: float = 0.0, ratio: str = "token", average: str = "token"):
+    """(loss, metrics): the clipped policy loss of many sequences, and float32 [5] metrics named by `POLICY_METRICS`.
+
+        r = exp(log_probs - old_log_probs)       (or ratio="sequence": of the mean of that over a sequence)
+        pg = mean of -min(r A, clip(r, 1 - clip_eps, 1 + clip_eps_high) A)
+        loss = pg + kl_coef * (mean of the KL estimator) - entropy_coef * entropy
+
+    log_probs: of the sampled tokens, [sequences, length], or [tokens] with `offsets` (int64 or int32 [sequences + 1]: sequence s has
+    the tokens from offsets[s] to offsets[s + 1]; rising, not behind the last token).  `mask` (bool) says which of them count.  What a token
+    that does not count holds has no influence, and its gradient is 0; sequences without a token that counts are left out of
+    every mean.  advantages: [sequences], or of every token (ratio="token").  Without `old_log_probs` the policy has not moved: r is
+    1, with its gradient.  kl, at x = log_probs - ref_log_probs: "k1" x, "k2" x^2 / 2, "k3" exp(-x) - 1 + x, "k3_swapped" exp(x) - 1 - x.
+    The entropy is minus the mean of log_probs.  average: means of pg and KL over all tokens, or over sequences of the means
+    over their tokens.  Only log_probs gets a gradient, which on the GPU cannot be differentiated again; terms and sums
+    are in float64."""
+    if ratio not in ("token", "sequence") or average not in ("token", "sequence"):
+        raise ValueError(f"ratio and average must be 'token' or 'sequence', got {ratio!r} and {average!r}")
+    if kl not in _KL:
+        raise ValueError(f"kl must be one of {_KL}, got {kl!r}")
+    if kl_coef and ref_log_probs is None:
+        raise ValueError("kl_coef wants ref_log_probs")
+    low, high = 1.0 - clip_eps, 1.0 + (clip_eps if clip_eps_high is None else clip_eps_high)
+    if not low <= high:
+        raise ValueError(f"clip_eps {clip_eps} and clip_eps_high {clip_eps_high} leave nothing between them")
+    sequences = _check_tokens(log_probs, dict(old_log_probs=old_log_probs, ref_log_probs=ref_log_probs), offsets, mask)
+    per_token = advantages.shape != (sequences,)
+    if (per_token and (advantages.shape != log_probs.shape or ratio == "sequence")) or not advantages.is_floating_point():
+        raise ValueError(f"advantages must be floating-point [{sequences}]{'' if ratio == 'sequence' else f' or {tuple(log_probs.shape)}'}, "
+                         f"got {tuple(advantages.shape)} {advantages.dtype}")
+    if advantages.device != log_probs.device:
+        raise ValueError(f"log_probs on {log_probs.device}, advantages on {advantages.device}")
+    numbers = (sequences, per_token, ratio == "sequence", average == "sequence", _KL.index(kl), low, high, kl_coef, entropy_coef)
+    if _native(log_probs, advantages, old_log_probs, ref_log_probs, offsets, mask):
+        call = _lib.blocks().policy_loss
+        out = call(log_probs, advantages, old_log_probs, ref_log_probs, offsets, mask, *numbers)
+        if out is None:
+            with torch.cuda.device(log_probs.device):
+                out = call(log_probs.contiguous(), _dense(advantages).float(), _dense(old_log_probs), _dense(ref_log_probs),
+                           _dense(offsets), _dense(mask), *numbers)
+        if out is not None:
+            return out
+    return _policy_in_torch_ops(log_probs, advantages, old_log_probs if old_log_probs is None else old_log_probs.detach(),
+                                ref_log_probs if ref_log_probs is None else ref_log_probs.detach(), offsets, mask, *numbers)
+
+
+def _preference_in_torch_ops(log_probs, ref, offsets, mask, sequences, kind, mean, beta, smoothing):
+    if sequences == 0:
+        return _nothing(log_probs), torch.zeros(0, device=log_probs.device)
+    sequence, counts = _places(log_probs, offsets, mask, sequences)
+    flat = lambda t: torch.where(counts, t.reshape(-1).double(), 0.0)
+    x = flat(log_probs) if ref is None else flat(log_probs) - flat(ref)
+    n = _sums(counts.double(), sequence, sequences)
+    h = _sums(x, sequence, sequences)
+    if mean:
+        h = h / n.clamp(min=1)
+    z, pairs = h[:sequences // 2] - h[sequences // 2:], n[:sequences // 2] + n[sequences // 2:] > 0
+    if _PREFERENCES[kind] == "sigmoid":
+        losses = -(1 - smoothing) * F.logsigmoid(beta * z) - smoothing * F.logsigmoid(-beta * z)
+    elif _PREFERENCES[kind] == "hinge":
+        losses = F.relu(1 - beta * z)
+    else:
+        losses = (z - 0.5 / beta) ** 2
+    loss = torch.where(pairs, losses, 0.0).sum() / pairs.sum().clamp(min=1)
+    return loss.float(), (beta * h.detach()).float()
+
+
+def preference_loss(log_probs: torch.Tensor, ref_log_probs: torch.Tensor | None = None, *, offsets: torch.Tensor | None = None,
+                    mask: torch.Tensor | None = None, beta: float = 0.1, kind: str = "sigmoid", label_smoothing: float = 0.0,
+                    average_log_probs: bool = False):
+    """(loss, rewards): the preference loss of pairs of sequences, and float32 [sequences] rewards beta * h.
+
+        h = sum over a sequence's tokens of log_probs - ref_log_probs     (their mean with `average_log_probs`)
+        z = h of the preferred sequence - h of the other
+        "sigmoid": -(1 - label_smoothing) log sigmoid(beta z) - label_smoothing log sigmoid(-beta z)
+        "hinge":   max(0, 1 - beta z)              "ipo": (z - 1 / (2 beta))^2
+
+    averaged over the pairs.  The first half of the sequences are the preferred ones, the second half the others, in the same
+    order.  Tokens, `offsets` and `mask` as for ``policy_loss``; a pair without a token that counts is left out.  Without
+    `ref_log_probs` h is of log_probs alone.  Only log_probs gets a gradient, which on the GPU cannot be differentiated
+    again; terms and sums are in float64."""
+    if kind not in _PREFERENCES:
+        raise ValueError(f"kind must be one of {_PREFERENCES}, got {kind!r}")
+    if not beta > 0:
+        raise ValueError(f"beta must be positive, got {beta}")
+    if not 0 <= label_smoothing <= 0.5 or (label_smoothing and kind != "sigmoid"):
+        raise ValueError(f"label_smoothing is of the sigmoid loss, from 0 to 0.5; got {label_smoothing} with {kind!r}")
+    sequences = _check_tokens(log_probs, dict(ref_log_probs=ref_log_probs), offsets, mask)
+    if sequences % 2:
+        raise ValueError(f"pairs want an even number of sequences, got {sequences}")
+    numbers = (sequences, _PREFERENCES.index(kind), average_log_probs, beta, label_smoothing)
+    if _native(log_probs, ref_log_probs, offsets, mask):
+        call = _lib.blocks().preference_loss
+        out = call(log_probs, ref_log_probs, offsets, mask, *numbers)
+        if out is None:
+            with torch.cuda.device(log_probs.device):
+                out = call(log_probs.contiguous(), _dense(ref_log_probs), _dense(offsets), _dense(mask), *numbers)
+        if out is not None:
+            return out
+    return _preference_in_torch_ops(log_probs, ref_log_probs if ref_log_probs is None else ref_log_probs.detach(), offsets, mask,
+                                    *numbers)
