@@ -32,7 +32,9 @@ def step_bounds(p, g, m, v, step, lr, betas, eps, decay, factor=1.0, half=0.0):
     m_off, v_off = 7 * U * m_size, 13 * U * v_new
     below = (v_new / (1 - b2 ** step)).sqrt() + eps
     scale = lr / (1 - b1 ** step)
-    update_off = scale * m_off / below + scale * m_size / below * (7 + 6) * U
+    # (half of v_off under the root; the root and the reciprocal within an ulp, 2 roundings, each; root's factor, its product, the
+    # sum, the quotient's product, the step and its product)
+    update_off = scale * m_off / below + scale * m_size / below * (6.5 + 2 * 2 + 6) * U
     p_off = 3 * U * p + update_off + (half + U) * (p + scale * m_size / below)
     return p_off + 1e-44, m_off + 1e-44, v_off + 1e-44  # (denormal results: half of 2^-149)
 

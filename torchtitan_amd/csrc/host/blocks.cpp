@@ -71,6 +71,7 @@ struct Library {
   decltype(&mx_grad_norm_workspace) grad_norm_workspace = nullptr;
   decltype(&mx_grad_clip) grad_clip = nullptr;
   decltype(&mx_adamw) adamw = nullptr;
+  decltype(&mx_adamw_moments) adamw_moments = nullptr;
   decltype(&mx_sequence_loss_workspace) sequence_loss_workspace = nullptr;
   decltype(&mx_policy_loss) policy_loss = nullptr;
   decltype(&mx_policy_loss_bwd) policy_loss_bwd = nullptr;
@@ -126,6 +127,7 @@ void bind(const py::dict& addresses, const py::object& check) {
   set("mx_grad_norm_workspace", lib.grad_norm_workspace);
   set("mx_grad_clip", lib.grad_clip);
   set("mx_adamw", lib.adamw);
+  set("mx_adamw_moments", lib.adamw_moments);
   set("mx_sequence_loss_workspace", lib.sequence_loss_workspace);
   set("mx_policy_loss", lib.policy_loss);
   set("mx_policy_loss_bwd", lib.policy_loss_bwd);
@@ -1229,14 +1231,19 @@ bool same_order(const Tensor& t, const Tensor& p) {
   return t.sizes() == p.sizes() && t.strides() == p.strides();
 }
 
+// The names of a state's entries.
+PyObject* state_name(int k) {
+  static PyObject* const names[] = {PyUnicode_InternFromString("exp_avg"), PyUnicode_InternFromString("exp_avg_sq"),
+                                    PyUnicode_InternFromString("exp_avg_scale"), PyUnicode_InternFromString("exp_avg_sq_scale"),
+                                    PyUnicode_InternFromString("master"), PyUnicode_InternFromString("step")};
+  return names[k];
+}
+
 // The AdamW step of a group: parameters that have a gradient, with their states (a dict of tensors and the step so far, as
 // torchtitan_amd/optimizers.py makes them) updated.  False, with nothing done, where one of them is not the plain case: state not
 // made yet, a type, device or layout of its own.
 bool adamw(const py::list& parameters, const py::list& states, int64_t first, bool eight, double lr, double b1, double b2,
            double eps, double decay, bool maximize, const std::optional<Tensor>& total_norm, double limit, uint64_t seed) {
-  static PyObject* const names[] = {PyUnicode_InternFromString("exp_avg"), PyUnicode_InternFromString("exp_avg_sq"),
-                                    PyUnicode_InternFromString("exp_avg_scale"), PyUnicode_InternFromString("exp_avg_sq_scale"),
-                                    PyUnicode_InternFromString("master"), PyUnicode_InternFromString("step")};
   struct One {
     Tensor p, g;
     std::array<Tensor, 5> state;  // in the order of the names
@@ -1265,7 +1272,7 @@ bool adamw(const py::list& parameters, const py::list& states, int64_t first, bo
     const int64_t blocks = (p.numel() + 31) / 32;
     for (int k = 0; k < 5; ++k) {
       const bool moment = k < 2, scale = k == 2 || k == 3;
-      PyObject* value = PyDict_GetItemWithError(one.dict, names[k]);
+      PyObject* value = PyDict_GetItemWithError(one.dict, state_name(k));
       if (!value) {
         if (PyErr_Occurred()) throw py::error_already_set();
         if (moment || (scale && eight)) return false;
@@ -1282,7 +1289,7 @@ bool adamw(const py::list& parameters, const py::list& states, int64_t first, bo
                 : t.numel() != p.numel() || !same_order(t, p))
         return false;
     }
-    PyObject* step = PyDict_GetItemWithError(one.dict, names[5]);
+    PyObject* step = PyDict_GetItemWithError(one.dict, state_name(5));
     if (!step || !PyLong_CheckExact(step)) return false;
     one.step = PyLong_AsLongLong(step);
     if (one.step < 0) {
@@ -1323,9 +1330,56 @@ bool adamw(const py::list& parameters, const py::list& states, int64_t first, bo
   }
   for (const One& one : all) {
     const py::object next = py::reinterpret_steal<py::object>(PyLong_FromLongLong(one.step + 1));
-    if (!next || PyDict_SetItem(one.dict, names[5], next.ptr())) throw py::error_already_set();
+    if (!next || PyDict_SetItem(one.dict, state_name(5), next.ptr())) throw py::error_already_set();
   }
   return true;
+}
+
+// (first moment, second moment) of every parameter of a group with moments in 8 bits, written out; None where one of them is
+// not the plain case.
+py::object adamw_moments(const py::list& parameters, const py::list& states, bool f32) {
+  const size_t count = parameters.size();
+  std::vector<Tensor> out, held;  // (held: the codes and scales, until the launch)
+  std::vector<const uint8_t*> codes, scales;
+  std::vector<int64_t> elems;
+  std::vector<int32_t> kinds;
+  std::vector<void*> to;
+  for (size_t i = 0; i < count; ++i) {
+    PyObject *object = PyList_GET_ITEM(parameters.ptr(), i), *dict = PyList_GET_ITEM(states.ptr(), i);
+    if (!THPVariable_Check(object) || !PyDict_Check(dict)) return py::none();
+    const Tensor& p = THPVariable_Unpack(object);
+    if (!row_tensor(p) || !on_current_device(p)) return py::none();
+    const int64_t blocks = (p.numel() + 31) / 32;
+    std::array<Tensor, 4> state;
+    for (int k = 0; k < 4; ++k) {
+      PyObject* value = PyDict_GetItemWithError(dict, state_name(k));
+      if (!value || !THPVariable_CheckExact(value)) return py::none();
+      state[k] = THPVariable_Unpack(value);
+      if (state[k].device() != p.device() || state[k].scalar_type() != at::kByte || !state[k].is_contiguous() ||
+          state[k].numel() != (k < 2 ? 32 * blocks : blocks))
+        return py::none();
+    }
+    for (int k = 0; k < 2; ++k) {
+      out.push_back(at::empty(p.sizes(), state[k].options().dtype(f32 ? at::kFloat : at::kBFloat16)));
+      codes.push_back(state[k].data_ptr<uint8_t>());
+      scales.push_back(state[k + 2].data_ptr<uint8_t>());
+      elems.push_back(p.numel());
+      kinds.push_back(k + 2 * f32);
+      to.push_back(out.back().data_ptr());
+      held.push_back(state[k]);
+      held.push_back(state[k + 2]);
+    }
+  }
+  if (out.empty()) return py::list();
+  {
+    Unlocked unlocked(std::in_place);
+    checked(lib.adamw_moments(static_cast<int64_t>(out.size()), codes.data(), scales.data(), elems.data(), kinds.data(), to.data(),
+                              stream_of(out[0])),
+            "mx_adamw_moments");
+  }
+  py::list pairs(count);
+  for (size_t i = 0; i < count; ++i) pairs[i] = py::make_tuple(out[2 * i], out[2 * i + 1]);
+  return pairs;
 }
 
 // The capture that `stream` is part of, a number of its own for every capture (0: none).
@@ -1365,4 +1419,5 @@ PYBIND11_MODULE(_blocks, m) {
   m.def("policy_loss", torch::wrap_pybind_function(policy_loss));
   m.def("preference_loss", torch::wrap_pybind_function(preference_loss));
   m.def("adamw", torch::wrap_pybind_function(adamw));
+  m.def("adamw_moments", torch::wrap_pybind_function(adamw_moments));
 }

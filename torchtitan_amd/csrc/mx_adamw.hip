@@ -28,8 +28,9 @@ namespace mx {
 
 constexpr int kAdamThreads = 256;
 constexpr int kAdamTensors = 44;  // of one launch
-constexpr int kAdamPieces = 2;    // pieces a lane and chunk
-constexpr int kAdamValues = 4, kAdam8Values = 8;  // values a piece: 16 bytes of float32; a quarter of a block of 32
+constexpr int kAdamPieces = 4;  // pieces a lane and chunk
+constexpr int kAdamValues = 4;  // values a piece: 16 bytes of float32
+constexpr int kAdam8Values = 8;  // values a lane and chunk of a parameter with moments in 8 bits
 
 struct AdamEntry {
   void* p;
@@ -73,12 +74,12 @@ __device__ __forceinline__ int adam_find(const AdamTable& t, int n, uint32_t chu
   return lo;
 }
 
-// V values at p, of which `left` exist (the others: 0), from any element on.
-template <int V, class T>
+// V values at p, from any element on; ALL: they exist, else `left` of them do (the others: 0).
+template <bool ALL, int V, class T>
 __device__ __forceinline__ void adam_load(const T* p, int64_t left, float (&f)[V]) {
   constexpr int W = V * (int)sizeof(T) / 4;
   typedef uint32_t words __attribute__((ext_vector_type(W > 4 ? 4 : W), aligned(sizeof(T))));
-  if (left >= V) {
+  if (ALL || left >= V) {
     uint32_t w[W];
 #pragma unroll
     for (int k = 0; k < W; k += 4) {
@@ -102,7 +103,7 @@ __device__ __forceinline__ void adam_load(const T* p, int64_t left, float (&f)[V
     }
   }
 }
-template <int V, class T>
+template <bool ALL, int V, class T>
 __device__ __forceinline__ void adam_store(T* p, int64_t left, const float (&f)[V]) {
   constexpr int W = V * (int)sizeof(T) / 4;
   typedef uint32_t words __attribute__((ext_vector_type(W > 4 ? 4 : W), aligned(sizeof(T))));
@@ -115,7 +116,7 @@ __device__ __forceinline__ void adam_store(T* p, int64_t left, const float (&f)[
     for (int e = 0; e < V; e += 2)
       w[e / 2] = __builtin_bit_cast(uint32_t, __builtin_convertvector(v2f_t{f[e], f[e + 1]}, v2bf_t));
   }
-  if (left >= V) {
+  if (ALL || left >= V) {
 #pragma unroll
     for (int k = 0; k < W; k += 4) {
       words q;
@@ -135,17 +136,26 @@ __device__ __forceinline__ void adam_store(T* p, int64_t left, const float (&f)[
 
 // The new moments and weight of one value.  Products and sums are rounded one by one, as separate operations on tensors
 // round them: the same bits as the formula in torch operations.
+// ROUGH: the hardware's root and reciprocal, each within an ulp, for an eps (from 1e-9 on) that covers what they lose of a
+// denormal second moment; the sequences around them that round right took 7 to 15 % of the time of a bf16 parameter with moments
+// in 8 bits (673 million 1336 us with them, 1245 without), and nothing elsewhere.
+template <bool ROUGH>
 __device__ __forceinline__ void adam_update(const AdamHyper& h, float f, float step, float root, float decay, float g, float& m,
                                             float& v, float& w) {
 #pragma clang fp contract(off)
   g = g * f;
   m = m * h.b1 + g * h.c1;
   v = v * h.b2 + g * g * h.c2;
-  const float below = __builtin_sqrtf(v) * root + h.eps;
-  w = w * decay - step * (m / below);
+  if constexpr (ROUGH) {
+    const float below = __builtin_amdgcn_sqrtf(v) * root + h.eps;
+    w = w * decay - step * (m * __builtin_amdgcn_rcpf(below));
+  } else {
+    const float below = __builtin_sqrtf(v) * root + h.eps;
+    w = w * decay - step * (m / below);
+  }
 }
 
-template <class T>
+template <bool ALL, class T>
 __device__ __forceinline__ void adam_chunk(const AdamEntry& e, const AdamHyper& h, float f, float step, float root, float decay,
                                            int64_t at) {
   constexpr int V = kAdamValues;
@@ -153,57 +163,33 @@ __device__ __forceinline__ void adam_chunk(const AdamEntry& e, const AdamHyper& 
   T* p = (T*)e.p;
   float *m = (float*)e.m, *v = (float*)e.v;
   float qg[kAdamPieces][V], qm[kAdamPieces][V], qv[kAdamPieces][V], qw[kAdamPieces][V];
+  auto pieces = [&](auto&& piece) {
 #pragma unroll
-  for (int k = 0; k < kAdamPieces; ++k) {
-    const int64_t i = at + (k * kAdamThreads + threadIdx.x) * V, left = e.elems - i;
-    adam_load(g + i, left, qg[k]);
-    adam_load(m + i, left, qm[k]);
-    adam_load(v + i, left, qv[k]);
-    if (e.master) adam_load(e.master + i, left, qw[k]);
-    else adam_load((const T*)p + i, left, qw[k]);
-  }
+    for (int k = 0; k < kAdamPieces; ++k) {
+      const int64_t i = at + (k * kAdamThreads + threadIdx.x) * V;
+      piece(k, i, e.elems - i);
+    }
+  };
+  // one array after the other
+  pieces([&](int k, int64_t i, int64_t left) { adam_load<ALL>(g + i, left, qg[k]); });
+  pieces([&](int k, int64_t i, int64_t left) { adam_load<ALL>(m + i, left, qm[k]); });
+  pieces([&](int k, int64_t i, int64_t left) { adam_load<ALL>(v + i, left, qv[k]); });
+  if (e.master) pieces([&](int k, int64_t i, int64_t left) { adam_load<ALL>(e.master + i, left, qw[k]); });
+  else pieces([&](int k, int64_t i, int64_t left) { adam_load<ALL>((const T*)p + i, left, qw[k]); });
 #pragma unroll
-  for (int k = 0; k < kAdamPieces; ++k) {
-    const int64_t i = at + (k * kAdamThreads + threadIdx.x) * V, left = e.elems - i;
+  for (int k = 0; k < kAdamPieces; ++k)
 #pragma unroll
-    for (int j = 0; j < V; ++j) adam_update(h, f, step, root, decay, qg[k][j], qm[k][j], qv[k][j], qw[k][j]);
-    adam_store(m + i, left, qm[k]);
-    adam_store(v + i, left, qv[k]);
-    if (e.master) adam_store(e.master + i, left, qw[k]);
-    adam_store(p + i, left, qw[k]);
-  }
+    for (int j = 0; j < V; ++j) adam_update<false>(h, f, step, root, decay, qg[k][j], qm[k][j], qv[k][j], qw[k][j]);
+  pieces([&](int k, int64_t i, int64_t left) { adam_store<ALL>(m + i, left, qm[k]); });
+  pieces([&](int k, int64_t i, int64_t left) { adam_store<ALL>(v + i, left, qv[k]); });
+  if (e.master) pieces([&](int k, int64_t i, int64_t left) { adam_store<ALL>(e.master + i, left, qw[k]); });
+  pieces([&](int k, int64_t i, int64_t left) { adam_store<ALL>(p + i, left, qw[k]); });
 }
 
 __device__ __forceinline__ float adam_factor(const AdamHyper& h) {
   if (!h.norm) return h.sign;
-  const float f = h.limit / (*h.norm + 1e-6f);
+  const float f = (1.f / (*h.norm + 1e-6f)) * h.limit;  // (a reciprocal and a product, as torch divides a number by a tensor)
   return h.sign * (f > 1.f ? 1.f : f);  // (NaN stays)
-}
-
-template <class T>
-__device__ __forceinline__ void adam8_chunk(const AdamEntry& e, const AdamHyper& h, float f, float step, float root, float decay,
-                                            uint32_t key, int64_t at);
-
-template <bool EIGHT>
-__global__ __launch_bounds__(kAdamThreads) void adamw_kernel(AdamTable table, int n, AdamHyper h) {
-  const uint32_t chunk = blockIdx.x;
-  const AdamEntry& e = table.e[adam_find(table, n, chunk)];
-  float step = e.step, root = e.root, decay = h.decay;
-  uint32_t key = e.key;
-  if (h.corrections) {
-    const float4 c = h.corrections[key];
-    step = c.x, root = c.y, decay = c.z, key = __float_as_uint(c.w);
-  }
-  const float f = adam_factor(h);
-  if constexpr (EIGHT) {
-    const int64_t at = (int64_t)(chunk - e.first) * (kAdamThreads * kAdamPieces * kAdam8Values);
-    if (e.f32) adam8_chunk<float>(e, h, f, step, root, decay, key, at);
-    else adam8_chunk<uint16_t>(e, h, f, step, root, decay, key, at);
-  } else {
-    const int64_t at = (int64_t)(chunk - e.first) * (kAdamThreads * kAdamPieces * kAdamValues);
-    if (e.f32) adam_chunk<float>(e, h, f, step, root, decay, at);
-    else adam_chunk<uint16_t>(e, h, f, step, root, decay, at);
-  }
 }
 
 // ---- 8 bits.  A code's bits are the topmost bits of a float32 whose exponent is the code's: a value times 2^(bias - b), b the
@@ -227,93 +213,139 @@ __device__ __forceinline__ int adam_scale(uint32_t amax, uint32_t up, int top) {
   const int b = (int)((amax + up) >> 23) - top;
   return amax == 0 || b < 0 ? 0 : b;  // (at most 255 - 8, which is below 255)
 }
-// Largest magnitude bits of a block: 8 values here, 4 lanes.
-__device__ __forceinline__ uint32_t adam_block_max(const float (&x)[kAdam8Values]) {
+// Largest magnitude bits of a block: V values here, 32 / V lanes.
+template <int V>
+__device__ __forceinline__ uint32_t adam_block_max(const float (&x)[V]) {
   uint32_t a = 0;
 #pragma unroll
-  for (int j = 0; j < kAdam8Values; ++j) a = max(a, __float_as_uint(x[j]) & 0x7FFFFFFFu);
+  for (int j = 0; j < V; ++j) a = max(a, __float_as_uint(x[j]) & 0x7FFFFFFFu);
   a = max(a, dpp<kQuadXor1>(a));
-  return max(a, dpp<kQuadXor2>(a));
+  a = max(a, dpp<kQuadXor2>(a));
+  return V == 8 ? a : max(a, dpp<kRowHalfMirror>(a));
 }
 
-template <class T>
+// Four codes of a first moment as values of scale 1.
+__device__ __forceinline__ void adam_decode_first(uint32_t codes, float* x) {
+  const v2f_t lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes, true);
+  x[0] = lo.x, x[1] = lo.y, x[2] = hi.x, x[3] = hi.y;
+}
+
+// V values a piece: 8 of a bf16 parameter, 4 of a float32 one, so that either is 16 bytes (float32, 8 / 4: 50 million 167 / 138 us,
+// 673 million 2.06 / 2.12 ms).
+template <bool ALL, bool ROUGH, int V, class T>
 __device__ __forceinline__ void adam8_chunk(const AdamEntry& e, const AdamHyper& h, float f, float step, float root, float decay,
                                             uint32_t key, int64_t at) {
-  constexpr int V = kAdam8Values;
+  constexpr int kPieces = kAdam8Values / V, kWords = V / 4;
+  typedef uint32_t Codes __attribute__((ext_vector_type(kWords)));
   const T* g = (const T*)e.g;
   T* p = (T*)e.p;
   uint8_t *m = (uint8_t*)e.m, *v = (uint8_t*)e.v;
   const int64_t whole = (e.elems + 31) & ~int64_t{31};  // codes are whole blocks
-  float qg[kAdamPieces][V], qw[kAdamPieces][V];
-  u32x2 cm[kAdamPieces], cv[kAdamPieces];
-  uint32_t sm[kAdamPieces], sv[kAdamPieces];
+  float qg[kPieces][V], qw[kPieces][V];
+  Codes cm[kPieces], cv[kPieces];
+  int sm[kPieces], sv[kPieces];
 #pragma unroll
-  for (int k = 0; k < kAdamPieces; ++k) {
+  for (int k = 0; k < kPieces; ++k) {
     const int64_t i = at + (k * kAdamThreads + threadIdx.x) * V, left = e.elems - i;
-    adam_load(g + i, left, qg[k]);
-    if (e.master) adam_load(e.master + i, left, qw[k]);
-    else adam_load((const T*)p + i, left, qw[k]);
-    cm[k] = cv[k] = u32x2{0, 0};
+    adam_load<ALL>(g + i, left, qg[k]);
+    if (e.master) adam_load<ALL>(e.master + i, left, qw[k]);
+    else adam_load<ALL>((const T*)p + i, left, qw[k]);
+    cm[k] = cv[k] = Codes(0);
     sm[k] = sv[k] = 0;
-    if (i < whole) {
-      cm[k] = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(m + i));
-      cv[k] = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(v + i));
+    if (ALL || i < whole) {
+      cm[k] = __builtin_nontemporal_load(reinterpret_cast<const Codes*>(m + i));
+      cv[k] = __builtin_nontemporal_load(reinterpret_cast<const Codes*>(v + i));
       sm[k] = e.ms[i >> 5];
       sv[k] = e.vs[i >> 5];
     }
   }
 #pragma unroll
-  for (int k = 0; k < kAdamPieces; ++k) {
+  for (int k = 0; k < kPieces; ++k) {
     const int64_t i = at + (k * kAdamThreads + threadIdx.x) * V, left = e.elems - i;
     float fm[V], fv[V];
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      fm[j] = adam_decode1(cm[k][j / 4] >> (8 * (j & 3)) & 255u, (int)sm[k]);
-      fv[j] = adam_decode2(cv[k][j / 4] >> (8 * (j & 3)) & 255u, (int)sv[k]);
-    }
-    if (sm[k] == 255)
-#pragma unroll
-      for (int j = 0; j < V; ++j) fm[j] = __builtin_nanf("");
-    if (sv[k] == 255)
-#pragma unroll
-      for (int j = 0; j < V; ++j) fv[j] = __builtin_nanf("");
+    for (int j = 0; j < kWords; ++j) adam_decode_first(cm[k][j], fm + 4 * j);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      adam_update(h, f, step, root, decay, qg[k][j], fm[j], fv[j], qw[k][j]);
-      if (j >= left) fm[j] = fv[j] = 0.f;  // (values that the last block does not have)
+      fm[j] = __builtin_amdgcn_ldexpf(fm[j], sm[k] - 127);
+      fv[j] = adam_decode2(cv[k][j / 4] >> (8 * (j & 3)) & 255u, sv[k]);
     }
-    if (e.master) adam_store(e.master + i, left, qw[k]);
-    adam_store(p + i, left, qw[k]);
+    if (sm[k] == 255 || sv[k] == 255) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        if (sm[k] == 255) fm[j] = __builtin_nanf("");
+        if (sv[k] == 255) fv[j] = __builtin_nanf("");
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      adam_update<ROUGH>(h, f, step, root, decay, qg[k][j], fm[j], fv[j], qw[k][j]);
+      if (!ALL && j >= left) fm[j] = fv[j] = 0.f;  // (values that the last block does not have)
+    }
+    if (e.master) adam_store<ALL>(e.master + i, left, qw[k]);
+    adam_store<ALL>(p + i, left, qw[k]);
     const int s1 = adam_scale(adam_block_max(fm), kFirstUp, kFirstTop), s2 = adam_scale(adam_block_max(fv), kSecondUp, kSecondTop);
-    u32x2 o1 = {0, 0}, o2 = {0, 0};
+    Codes o1 = Codes(0), o2 = Codes(0);
 #pragma unroll
     for (int j = 0; j < V; j += 2) {
       const uint32_t random = adam_mix((uint32_t)((i + j) >> 1) * 0x9E3779B9u + key);
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
-        const uint32_t up = (q ? random >> 16 : random & 0xFFFFu) << 4 | 8u;
-        const float x = fm[j + q], y = fv[j + q];
-        const uint32_t xb = __float_as_uint(x), size = xb & 0x7FFFFFFFu;
-        uint32_t a = (__float_as_uint(__builtin_amdgcn_ldexpf(__uint_as_float(size), kFirstBias - s1)) + up) >> 20;
-        uint32_t b = (__float_as_uint(__builtin_amdgcn_ldexpf(y, kSecondBias - s2)) + up) >> 20;
-        a = size == 0 ? 0 : min(a, kFirstMost);
-        b = y > 0.f ? max(min(b, kSecondMost), 1u) : 0u;
-        if (s1 == 255) a = kFirstMost;
-        if (s2 == 255) b = kSecondMost;
-        a |= xb >> 31 << 7;
-        o1[j / 4] |= a << (8 * ((j + q) & 3));
-        o2[j / 4] |= b << (8 * ((j + q) & 3));
+        // (0 stays 0: what is added is less than a code)
+        const uint32_t up = (q ? random >> 16 << 4 : (random & 0xFFFFu) << 4) | 8u;
+        const uint32_t x = __float_as_uint(fm[j + q]);
+        const uint32_t a = __float_as_uint(__builtin_amdgcn_ldexpf(__builtin_fabsf(fm[j + q]), kFirstBias - s1)) + up;
+        const uint32_t b = __float_as_uint(__builtin_amdgcn_ldexpf(fv[j + q], kSecondBias - s2)) + up;
+        const uint32_t code1 = min(a >> 20, kFirstMost) | (x >> 31 << 7);
+        const uint32_t code2 = min(max(b >> 20, min(__float_as_uint(fv[j + q]), 1u)), kSecondMost);
+        o1[j / 4] |= code1 << (8 * ((j + q) & 3));
+        o2[j / 4] |= code2 << (8 * ((j + q) & 3));
       }
     }
-    if (i < whole) {
-      __builtin_nontemporal_store(o1, reinterpret_cast<u32x2*>(m + i));
-      __builtin_nontemporal_store(o2, reinterpret_cast<u32x2*>(v + i));
-      if ((threadIdx.x & 3) == 0) {
+    if (s1 == 255) o1 = (o1 & 0x80808080u) | 0x7E7E7E7Eu;
+    if (s2 == 255) o2 = Codes(0xFFFFFFFFu);
+    if (ALL || i < whole) {
+      __builtin_nontemporal_store(o1, reinterpret_cast<Codes*>(m + i));
+      __builtin_nontemporal_store(o2, reinterpret_cast<Codes*>(v + i));
+      if ((threadIdx.x & (32 / V - 1)) == 0) {
         e.ms[i >> 5] = (uint8_t)s1;
         e.vs[i >> 5] = (uint8_t)s2;
       }
     }
   }
+}
+
+template <bool EIGHT>
+__global__ __launch_bounds__(kAdamThreads) void adamw_kernel(AdamTable table, int n, AdamHyper h) {
+  const uint32_t chunk = blockIdx.x;
+  const AdamEntry& e = table.e[adam_find(table, n, chunk)];
+  float step = e.step, root = e.root, decay = h.decay;
+  uint32_t key = e.key;
+  if (h.corrections) {
+    const float4 c = h.corrections[key];
+    step = c.x, root = c.y, decay = c.z, key = __float_as_uint(c.w);
+  }
+  const float f = adam_factor(h);
+  constexpr int kValues = kAdamThreads * (EIGHT ? kAdam8Values : kAdamPieces * kAdamValues);
+  const int64_t at = (int64_t)(chunk - e.first) * kValues;
+  const bool all = e.elems - at >= kValues;
+  auto types = [&](auto whole) {
+    constexpr bool ALL = decltype(whole)::value;
+    if constexpr (EIGHT) {
+      if (!ALL || h.eps < 1e-9f) {
+        if (e.f32) adam8_chunk<ALL, false, 4, float>(e, h, f, step, root, decay, key, at);
+        else adam8_chunk<ALL, false, 8, uint16_t>(e, h, f, step, root, decay, key, at);
+      } else {
+        if (e.f32) adam8_chunk<ALL, true, 4, float>(e, h, f, step, root, decay, key, at);
+        else adam8_chunk<ALL, true, 8, uint16_t>(e, h, f, step, root, decay, key, at);
+      }
+    } else {
+      if (e.f32) adam_chunk<ALL, float>(e, h, f, step, root, decay, at);
+      else adam_chunk<ALL, uint16_t>(e, h, f, step, root, decay, at);
+    }
+  };
+  if (all) types(std::true_type());
+  else types(std::false_type());
 }
 
 // Step counters on the device: one more, and what follows from it, for every tensor of the table.
@@ -375,8 +407,8 @@ __global__ __launch_bounds__(kAdamThreads) void adamw_moments_kernel(MomentTable
       x[j] = e.kind & 1 ? adam_decode2(code, s[k]) : adam_decode1(code, s[k]);
       if (s[k] == 255) x[j] = __builtin_nanf("");
     }
-    if (e.kind & 2) adam_store((float*)e.out + i, left, x);
-    else adam_store((uint16_t*)e.out + i, left, x);
+    if (e.kind & 2) adam_store<false>((float*)e.out + i, left, x);
+    else adam_store<false>((uint16_t*)e.out + i, left, x);
   }
 }
 
@@ -407,7 +439,7 @@ extern "C" int mx_adamw(int64_t n, const int64_t* table, int eight, double lr, d
   if (((uintptr_t)norm & 3) || ((uintptr_t)steps & 3) || ((uintptr_t)lr_device & 3) || ((uintptr_t)corrections & 15))
     return MX_ERR_ALIGNMENT;
   if ((steps != nullptr) != (corrections != nullptr) || (lr_device && !steps)) return MX_ERR_INVALID_ARG;
-  const int64_t per = kAdamThreads * kAdamPieces * (eight ? kAdam8Values : kAdamValues);
+  const int64_t per = kAdamThreads * (eight ? kAdam8Values : kAdamPieces * kAdamValues);
   for (int64_t i = 0; i < n; ++i) {
     const int64_t* t = table + i * MX_ADAMW_FIELDS;
     const int64_t elems = t[8], number = t[10];

@@ -294,7 +294,7 @@ class AdamW(torch.optim.Optimizer):
                 continue
             state, factor = self.state[p], None
             if norm is not None:
-                factor = torch.full_like(norm, limit, dtype=torch.float32).div(norm.float() + 1e-6).clamp(max=1.0)
+                factor = (limit / (norm.float() + 1e-6)).clamp(max=1.0)
             step = int(state["step"]) + 1
             _in_torch_ops(_unwrap(p), _unwrap(p.grad), state, group, factor, step, number)
             state["step"] = step
@@ -333,7 +333,13 @@ class AdamW(torch.optim.Optimizer):
             raise TypeError(f"moments are written in bfloat16 or float32, got {dtype}")
         out, asked = [], []
         for group in self.param_groups:
-            for p in group["params"]:
+            params = group["params"]
+            if group["state_bits"] == 8 and params and all(type(p) in _TYPES for p in params) and ops.native_rows(_unwrap(params[0])):
+                pairs = _lib.blocks().adamw_moments(params, [self.state.get(p) for p in params], dtype == torch.float32)
+                if pairs is not None:
+                    out += pairs
+                    continue
+            for p in params:
                 state = self.state.get(p)
                 if not state:
                     out.append(None)
