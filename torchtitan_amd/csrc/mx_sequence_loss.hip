@@ -9,18 +9,26 @@
 //            sequences are the same work, and nothing has to be cleared.
 //   join     every sequence's parts are added up, the loss formed, and what a token's gradient needs of its sequence
 //   gradient tokens as they lie (backward)
-// A few megabytes at most are read: bound by the three launches' latency.  Terms are formed in float64, which is free here: a
-// ratio's side of a clipping border decides about its whole gradient, and the KL estimators are differences of nearly equal numbers.
+// Some tens of megabytes at most are read.  Up to 100 000 tokens bound by the latency of two launches forward (10 to 16 us) and one
+// backward (3), so that a wave has a single row of 64 tokens until there are enough for every CU; 4.2 million tokens (89 MB) take 43 and 23
+// us, half of it float64 arithmetic.  Terms are formed in float64: a ratio's side of a clipping border decides about its whole
+// gradient, and the KL estimators are differences of nearly equal numbers.
 #include "mx_rows.h"
 
 namespace mx {
 
-constexpr int kSeqLanes = 64;
-constexpr int kSeqTokens = 8;  // of a lane and chunk
-constexpr int kSeqChunk = kSeqLanes * kSeqTokens;
-constexpr int kSeqJoin = 256;     // lanes of a workgroup that joins
-constexpr int kSeqJoinGroups = 1024;  // workgroups that join, at most
-constexpr int kSeqGrad = 256, kSeqGradTokens = 4;  // lanes of a workgroup, tokens of a lane
+constexpr int kSeqGrad = 256;          // lanes of a workgroup of the gradient
+constexpr int kSeqFew = 1024;          // lanes of the workgroup that joins alone
+constexpr int kSeqMany = 256;          // lanes of a workgroup where several join
+constexpr int kSeqManyGroups = 1024;   // of which there are at most
+// Tokens from which on a wave takes 8 rows of 64 (us forward, 1 / 8 rows: one sequence of 147 456 20.4 / 16.0, 64 of 600 13.8 / 15.5),
+// and 4 of them in the gradient (us, 1 / 4 rows: packed, 524 672 8.3 / 11.1, 4.2 million 46 / 31).
+constexpr int64_t kSeqLong = 65536, kSeqGradLong = 1 << 20;
+__host__ __device__ __forceinline__ int seq_rows(int64_t tokens) { return tokens < kSeqLong ? 1 : 8; }
+__host__ __device__ __forceinline__ int64_t seq_chunks(int64_t tokens) {
+  const int64_t chunk = 64 * seq_rows(tokens);
+  return (tokens + chunk - 1) / chunk;
+}
 
 // Log-probabilities, bf16 or float32
 struct SeqValues {
@@ -79,27 +87,48 @@ __device__ __forceinline__ bool seq_clipped(const Policy& f, double r) {
   const double c = r > f.high ? f.high : r < f.low ? f.low : r;
   return fabs(r - c) > 1e-6;
 }
+// e^x, e^x - 1 and e^x - 1 - x to 1e-14 of each: x = k ln 2 + t, |t| <= ln 2 / 2, and e^t - 1 - t = t^2 (1/2! + t/3! + ...) up to t^12 / 12!.
+struct SeqExp {
+  double e, minus, rest;
+};
+__device__ __forceinline__ SeqExp seq_exp(double x) {
+  const double bounded = x > 750.0 ? 750.0 : x < -750.0 ? -750.0 : x;  // (NaN stays)
+  const double k = __builtin_rint(bounded * 1.4426950408889634);
+  const double t = __builtin_fma(-k, 2.3190468138462996e-17, __builtin_fma(-k, 0.6931471805599453, bounded));
+  double q = 1.0 / 479001600;
+  constexpr double kBelow[10] = {1.0 / 39916800, 1.0 / 3628800, 1.0 / 362880, 1.0 / 40320, 1.0 / 5040,
+                                 1.0 / 720,      1.0 / 120,     1.0 / 24,     1.0 / 6,     1.0 / 2};
+#pragma unroll
+  for (int n = 0; n < 10; ++n) q = __builtin_fma(q, t, kBelow[n]);
+  const double rest = t * t * q, minus = t + rest;
+  const double e = ldexp(1.0 + minus, (int)k);
+  return k == 0.0 ? SeqExp{e, minus, rest} : SeqExp{e, e - 1.0, e - 1.0 - x};
+}
 __device__ __forceinline__ double seq_kl(int kind, double x) {
-  switch (kind) {
-    case 0: return x;
-    case 1: return 0.5 * x * x;
-    case 2: return expm1(-x) + x;
-    default: return expm1(x) - x;
-  }
+  if (kind == 0) return x;
+  if (kind == 1) return 0.5 * x * x;
+  return seq_exp(kind == 2 ? -x : x).rest;
 }
 __device__ __forceinline__ double seq_kl_slope(int kind, double x) {
-  switch (kind) {
-    case 0: return 1.0;
-    case 1: return x;
-    case 2: return -expm1(-x);
-    default: return expm1(x);
-  }
+  if (kind == 0) return 1.0;
+  if (kind == 1) return x;
+  const double minus = seq_exp(kind == 2 ? -x : x).minus;
+  return kind == 2 ? -minus : minus;
 }
 
+// Sums over a wave, in every lane: 16 lanes by moves between lanes, then two steps through the LDS crossbar.
+template <int CTRL>
+__device__ __forceinline__ double seq_moved(double v) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  return __builtin_bit_cast(double, (uint64_t)dpp<CTRL>((uint32_t)b) | (uint64_t)dpp<CTRL>((uint32_t)(b >> 32)) << 32);
+}
 __device__ __forceinline__ double seq_wave_sum(double v) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
-  return v;
+  v += seq_moved<kQuadXor1>(v);
+  v += seq_moved<kQuadXor2>(v);
+  v += seq_moved<kRowHalfMirror>(v);
+  v += seq_moved<kRowMirror>(v);
+  v += __shfl_xor(v, 16, 64);
+  return v + __shfl_xor(v, 32, 64);
 }
 
 // What is read of a token, and what it adds to its sequence's sums.
@@ -140,7 +169,7 @@ __device__ __forceinline__ void seq_add(const Policy& f, const SeqToken& t, int6
   sum[2] += lp;
   if (f.ref.p) sum[3] += seq_kl(f.kl, lp - (double)t.ref);
   if (!f.whole) {
-    const double r = exp(x);
+    const double r = seq_exp(x).e;
     sum[4] += seq_objective(f, r, seq_advantage(f, t, s));
     sum[5] += r;
     sum[6] += seq_clipped(f, r) ? 1.0 : 0.0;
@@ -151,16 +180,15 @@ __device__ __forceinline__ void seq_add(const Preference& f, const SeqToken& t, 
   sum[1] += f.ref.p ? (double)t.lp - (double)t.ref : (double)t.lp;
 }
 
-// parts: [chunks + count][SUMS].  A wave's chunk is rows of 64 tokens.  Rows inside one sequence are added up lane by lane; in a row
+// parts: [chunks + count][SUMS].  A wave's chunk is ROWS rows of 64 tokens.  Rows inside one sequence are added up lane by lane; in a row
 // that sequences end in, those that lie in it whole are summed among their lanes, and the running one is summed up and left.
-template <class F, int SUMS>
-__global__ __launch_bounds__(kSeqLanes) void seq_parts_kernel(F f, Sequences q, double* __restrict__ parts) {
-  const int64_t chunk = blockIdx.x, begin = chunk * kSeqChunk;
-  const int64_t end = begin + kSeqChunk < q.tokens ? begin + kSeqChunk : q.tokens;
-  const int lane = threadIdx.x;
-  SeqToken t[kSeqTokens];
+template <int SUMS, int ROWS, class F>
+__device__ __forceinline__ void seq_parts(const F& f, const Sequences& q, int64_t chunk, int lane, double* parts) {
+  constexpr int kChunk = 64 * ROWS;
+  const int64_t begin = chunk * kChunk, end = begin + kChunk < q.tokens ? begin + kChunk : q.tokens;
+  SeqToken t[ROWS];
 #pragma unroll
-  for (int k = 0; k < kSeqTokens; ++k) t[k] = seq_load(f, q, begin + k * kSeqLanes + lane);
+  for (int k = 0; k < ROWS; ++k) t[k] = seq_load(f, q, begin + k * 64 + lane);
   int64_t s = q.find(begin);
   int64_t stop = s < 0 || s >= q.count ? begin : q.offset(s + 1);
   double sum[SUMS];
@@ -178,10 +206,10 @@ __global__ __launch_bounds__(kSeqLanes) void seq_parts_kernel(F f, Sequences q, 
   };
   clear();
 #pragma unroll
-  for (int k = 0; k < kSeqTokens; ++k) {
-    const int64_t row = begin + k * kSeqLanes, i = row + lane;
+  for (int k = 0; k < ROWS; ++k) {
+    const int64_t row = begin + k * 64, i = row + lane;
     if (row >= end) break;
-    if (stop >= (row + kSeqLanes < end ? row + kSeqLanes : end)) {
+    if (stop >= (row + 64 < end ? row + 64 : end)) {
       if (t[k].counts) seq_add(f, t[k], s, sum);
       continue;
     }
@@ -220,16 +248,23 @@ __global__ __launch_bounds__(kSeqLanes) void seq_parts_kernel(F f, Sequences q, 
   leave();
 }
 
+template <int SUMS, int ROWS, class F>
+__global__ __launch_bounds__(64) void seq_parts_kernel(F f, Sequences q, double* __restrict__ parts) {
+  seq_parts<SUMS, ROWS>(f, q, blockIdx.x, threadIdx.x, parts);
+}
+
 // The sums of sequence s from its parts, in the first of `lanes` lanes that take them in turn (others: part of them).
 template <int SUMS>
-__device__ __forceinline__ void seq_joined(const Sequences& q, const double* __restrict__ parts, int64_t s, int lane, int lanes,
+__device__ __forceinline__ void seq_joined(const Sequences& q, const double* parts, int64_t s, int lane, int lanes,
                                            double (&sum)[SUMS]) {
 #pragma unroll
   for (int k = 0; k < SUMS; ++k) sum[k] = 0.0;
   const int64_t begin = q.offset(s), end = q.offset(s + 1);
+  const int chunk = seq_rows(q.tokens) == 1 ? 6 : 9;  // (tokens of a chunk, as a power of two)
   if (end > begin) {
-    const int64_t last = (end - 1) / kSeqChunk;
-    for (int64_t c = begin / kSeqChunk + lane; c <= last; c += lanes)
+    const int64_t last = (end - 1) >> chunk;
+#pragma unroll 4
+    for (int64_t c = (begin >> chunk) + lane; c <= last; c += lanes)
 #pragma unroll
       for (int k = 0; k < SUMS; ++k) sum[k] += parts[(c + s) * SUMS + k];
   }
@@ -239,20 +274,19 @@ __device__ __forceinline__ void seq_joined(const Sequences& q, const double* __r
 }
 
 // Sums over the lanes of the workgroup, in lane 0.
-template <int N>
+template <int LANES, int N>
 __device__ __forceinline__ void seq_group_sum(double (&v)[N]) {
-  __shared__ double shared[kSeqJoin / 64][N];
+  constexpr int kWaves = LANES / 64;
+  __shared__ double shared[kWaves][N];
 #pragma unroll
   for (int k = 0; k < N; ++k) {
     v[k] = seq_wave_sum(v[k]);
     if ((threadIdx.x & 63) == 0) shared[threadIdx.x >> 6][k] = v[k];
   }
   __syncthreads();
+  if (threadIdx.x >= 64) return;
 #pragma unroll
-  for (int k = 0; k < N; ++k) {
-    v[k] = 0.0;
-    for (int w = 0; w < kSeqJoin / 64; ++w) v[k] += shared[w][k];
-  }
+  for (int k = 0; k < N; ++k) v[k] = seq_wave_sum(threadIdx.x < kWaves ? shared[threadIdx.x][k] : 0.0);
 }
 
 // Sums over all sequences.  Policy: tokens, sequences that have some; by token objective, kl, ratio, clipped; by sequence the
@@ -260,7 +294,7 @@ __device__ __forceinline__ void seq_group_sum(double (&v)[N]) {
 constexpr int kPolicyTotals = 11, kPreferenceTotals = 2;
 
 // Of the sequence: for the gradient, each[2 s] tokens, each[2 s + 1] what its ratio adds to a token's gradient.
-__device__ __forceinline__ void seq_take(const Policy& f, const Sequences& q, const double* __restrict__ parts, int64_t s, int lane,
+__device__ __forceinline__ void seq_take(const Policy& f, const Sequences& q, const double* parts, int64_t s, int lane,
                                          int lanes, double* __restrict__ each, float*, double (&total)[kPolicyTotals]) {
   double sum[kPolicySums];
   seq_joined(q, parts, s, lane, lanes, sum);
@@ -269,7 +303,7 @@ __device__ __forceinline__ void seq_take(const Policy& f, const Sequences& q, co
   double slope = 0.0;
   if (n > 0.0) {
     if (f.whole) {
-      const double r = exp(sum[1] / n), A = (double)f.advantages[s];
+      const double r = seq_exp(sum[1] / n).e, A = (double)f.advantages[s];
       if (A >= 0 ? !(r > f.high) : !(r < f.low)) slope = -A * r;
       sum[4] = n * seq_objective(f, r, A);
       sum[5] = n * r;
@@ -306,7 +340,7 @@ __device__ __forceinline__ double seq_sigmoid(double y) {
 }
 
 // Of the pair: for the gradient, each[s] that of a token of either sequence (but for the mean over the pairs).
-__device__ __forceinline__ void seq_take(const Preference& f, const Sequences& q, const double* __restrict__ parts, int64_t p, int lane,
+__device__ __forceinline__ void seq_take(const Preference& f, const Sequences& q, const double* parts, int64_t p, int lane,
                                          int lanes, double* __restrict__ each, float* __restrict__ rewards,
                                          double (&total)[kPreferenceTotals]) {
   const int64_t other = q.count / 2 + p;
@@ -340,80 +374,105 @@ __device__ __forceinline__ void seq_finish(const Preference&, const Sequences& q
   if (each) each[q.count] = pairs;
 }
 
+template <class F> struct SeqOf;
+template <> struct SeqOf<Policy> { static constexpr int kSums = kPolicySums, kTotals = kPolicyTotals; };
+template <> struct SeqOf<Preference> { static constexpr int kSums = kPreferenceSums, kTotals = kPreferenceTotals; };
+
 // `lanes` lanes a sequence (or pair), `items` of them.  One workgroup finishes the loss; several leave their sums in `totals`.
-template <class F, int TOTALS>
-__global__ __launch_bounds__(kSeqJoin) void seq_join_kernel(F f, Sequences q, int64_t items, int lanes,
-                                                            const double* __restrict__ parts, double* __restrict__ totals,
-                                                            double* __restrict__ each, float* __restrict__ loss,
-                                                            float* __restrict__ more) {
-  double total[TOTALS];
+template <int LANES, class F>
+__device__ __forceinline__ void seq_join(const F& f, const Sequences& q, int64_t items, int lanes, const double* parts, double* totals,
+                                         double* __restrict__ each, float* __restrict__ loss, float* __restrict__ more) {
+  constexpr int kTotals = SeqOf<F>::kTotals;
+  double total[kTotals];
 #pragma unroll
-  for (int k = 0; k < TOTALS; ++k) total[k] = 0.0;
-  const int lane = threadIdx.x & (lanes - 1), groups = kSeqJoin / lanes;
+  for (int k = 0; k < kTotals; ++k) total[k] = 0.0;
+  const int lane = threadIdx.x & (lanes - 1), groups = LANES / lanes;
   for (int64_t s = (int64_t)blockIdx.x * groups + threadIdx.x / lanes; s < items; s += (int64_t)gridDim.x * groups)
     seq_take(f, q, parts, s, lane, lanes, each, more, total);
-  seq_group_sum(total);
+  seq_group_sum<LANES>(total);
   if (threadIdx.x == 0) {
     if (gridDim.x == 1) {
       seq_finish(f, q, total, each, loss, more);
     } else {
 #pragma unroll
-      for (int k = 0; k < TOTALS; ++k) totals[(int64_t)blockIdx.x * TOTALS + k] = total[k];
+      for (int k = 0; k < kTotals; ++k) totals[(int64_t)blockIdx.x * kTotals + k] = total[k];
     }
   }
 }
-template <class F, int TOTALS>
-__global__ __launch_bounds__(kSeqJoin) void seq_finish_kernel(F f, Sequences q, int groups, const double* __restrict__ totals,
+template <int LANES, class F>
+__global__ __launch_bounds__(LANES) void seq_join_kernel(F f, Sequences q, int64_t items, int lanes, const double* __restrict__ parts,
+                                                         double* __restrict__ totals, double* __restrict__ each,
+                                                         float* __restrict__ loss, float* __restrict__ more) {
+  seq_join<LANES>(f, q, items, lanes, parts, totals, each, loss, more);
+}
+template <class F>
+__global__ __launch_bounds__(kSeqMany) void seq_finish_kernel(F f, Sequences q, int groups, const double* __restrict__ totals,
                                                               double* __restrict__ each, float* __restrict__ loss,
                                                               float* __restrict__ more) {
-  double total[TOTALS];
+  constexpr int kTotals = SeqOf<F>::kTotals;
+  double total[kTotals];
 #pragma unroll
-  for (int k = 0; k < TOTALS; ++k) total[k] = 0.0;
-  for (int g = threadIdx.x; g < groups; g += kSeqJoin)
+  for (int k = 0; k < kTotals; ++k) total[k] = 0.0;
+  for (int g = threadIdx.x; g < groups; g += kSeqMany)
 #pragma unroll
-    for (int k = 0; k < TOTALS; ++k) total[k] += totals[(int64_t)g * TOTALS + k];
-  seq_group_sum(total);
+    for (int k = 0; k < kTotals; ++k) total[k] += totals[(int64_t)g * kTotals + k];
+  seq_group_sum<kSeqMany>(total);
   if (threadIdx.x == 0) seq_finish(f, q, total, each, loss, more);
 }
-
 // The gradient of one token that counts.
-__device__ __forceinline__ double seq_grad(const Policy& f, const double* __restrict__ each, int64_t count, const SeqToken& t,
-                                           int64_t s) {
-  const double lp = (double)t.lp, tokens = each[2 * count], filled = each[2 * count + 1];
-  double g = each[2 * s + 1];
+__device__ __forceinline__ double seq_grad(const Policy& f, double share, double entropy, double slope, const SeqToken& t, int64_t s) {
+  const double lp = (double)t.lp;
+  double g = slope;
   if (!f.whole) {
-    const double r = f.old.p ? exp(lp - (double)t.old) : 1.0, A = seq_advantage(f, t, s);
+    const double r = f.old.p ? seq_exp(lp - (double)t.old).e : 1.0, A = seq_advantage(f, t, s);
     if (A >= 0 ? !(r > f.high) : !(r < f.low)) g = -A * r;
   }
-  if (f.ref.p) g += f.kl_coef * seq_kl_slope(f.kl, lp - (double)t.ref);
-  return g / (f.by_sequence ? filled * each[2 * s] : tokens) + f.entropy_coef / tokens;
+  if (f.ref.p && f.kl_coef != 0.0) g += f.kl_coef * seq_kl_slope(f.kl, lp - (double)t.ref);
+  return g * share + entropy;
 }
-__device__ __forceinline__ double seq_grad(const Preference&, const double* __restrict__ each, int64_t count, const SeqToken&,
-                                           int64_t s) {
-  return each[s] / each[count];
+__device__ __forceinline__ double seq_grad(const Preference&, double share, double, double slope, const SeqToken&, int64_t) {
+  return slope * share;
+}
+// What the tokens of sequence s have in common: the share of each in the means, the entropy's gradient, what the sequence adds.
+__device__ __forceinline__ void seq_common(const Policy& f, const double* __restrict__ each, int64_t count, int64_t s, double& share,
+                                           double& entropy, double& slope) {
+  const double tokens = 1.0 / each[2 * count];
+  share = f.by_sequence ? 1.0 / (each[2 * count + 1] * each[2 * s]) : tokens;
+  entropy = f.entropy_coef * tokens;
+  slope = each[2 * s + 1];
+}
+__device__ __forceinline__ void seq_common(const Preference&, const double* __restrict__ each, int64_t count, int64_t s, double& share,
+                                           double&, double& slope) {
+  share = 1.0 / each[count];
+  slope = each[s];
 }
 
 // grad[i] = dloss * (that, where token i counts, else 0)
-template <class F>
+template <int ROWS, class F>
 __global__ __launch_bounds__(kSeqGrad) void seq_grad_kernel(F f, Sequences q, const double* __restrict__ each,
                                                             const float* __restrict__ dloss, void* __restrict__ grad) {
-  const int64_t begin = ((int64_t)blockIdx.x * (kSeqGrad / 64) + (threadIdx.x >> 6)) * (64 * kSeqGradTokens);
+  const int64_t begin = ((int64_t)blockIdx.x * (kSeqGrad / 64) + (threadIdx.x >> 6)) * (64 * ROWS);
   const int lane = threadIdx.x & 63;
   if (begin >= q.tokens) return;
-  SeqToken t[kSeqGradTokens];
+  SeqToken t[ROWS];
 #pragma unroll
-  for (int k = 0; k < kSeqGradTokens; ++k) t[k] = seq_load(f, q, begin + k * 64 + lane);
-  const int64_t first = q.find(begin);
-  const int64_t end = begin + 64 * kSeqGradTokens < q.tokens ? begin + 64 * kSeqGradTokens : q.tokens;
-  const bool one = first >= 0 && first < q.count && q.offset(first + 1) >= end;  // all of one sequence
+  for (int k = 0; k < ROWS; ++k) t[k] = seq_load(f, q, begin + k * 64 + lane);
   const double by = (double)*dloss;
+  const int64_t first = q.find(begin), end = begin + 64 * ROWS < q.tokens ? begin + 64 * ROWS : q.tokens;
+  const bool one = first >= 0 && first < q.count && q.offset(first + 1) >= end;  // all of one sequence
+  double share = 0.0, entropy = 0.0, slope = 0.0;
+  if (one) seq_common(f, each, q.count, first, share, entropy, slope);
 #pragma unroll
-  for (int k = 0; k < kSeqGradTokens; ++k) {
+  for (int k = 0; k < ROWS; ++k) {
     const int64_t i = begin + k * 64 + lane;
     if (i >= q.tokens) return;
-    const int64_t s = one ? first : q.find(i, first < q.count ? first : -1);
+    int64_t s = first;
     double g = 0.0;
-    if (t[k].counts && s >= 0 && s < q.count) g = seq_grad(f, each, q.count, t[k], s) * by;
+    if (!one) s = q.find(i, first < q.count ? first : -1);
+    if (t[k].counts && s >= 0 && s < q.count) {
+      if (!one) seq_common(f, each, q.count, s, share, entropy, slope);
+      g = seq_grad(f, share, entropy, slope, t[k], s) * by;
+    }
     if (f.lp.f32) ((float*)grad)[i] = (float)g;
     else ((uint16_t*)grad)[i] = (uint16_t)__builtin_bit_cast(uint32_t, __builtin_convertvector(v2f_t{(float)g, 0.f}, v2bf_t));
   }
@@ -431,32 +490,44 @@ static bool seq_odd(const SeqValues& v) { return (uintptr_t)v.p & (v.f32 ? 3 : 1
 
 // Lanes that add up a sequence's parts: about as many as it has of them on average.
 static int seq_lanes(const Sequences& q) {
-  const int64_t each = q.count ? (q.tokens + kSeqChunk - 1) / kSeqChunk / q.count : 0;
+  const int64_t each = q.count ? seq_chunks(q.tokens) / q.count : 0;
   int lanes = 1;
   while (lanes < 64 && lanes < each) lanes *= 2;
   return lanes;
 }
 
-// Two launches, or three where one workgroup would have more than four rounds of sequences to join.
-template <int SUMS, int TOTALS, class F>
+// Two launches, or three where one workgroup would have more than four rounds of sequences to join.  (One workgroup for parts and
+// join of few tokens: 976 of 16 sequences 11.4 us forward, in two launches 10.1.)
+template <class F>
 static void seq_loss(const F& f, const Sequences& q, int64_t items, double* parts, double* each, float* loss, float* more,
                      hipStream_t st) {
-  const int64_t chunks = (q.tokens + kSeqChunk - 1) / kSeqChunk;
-  if (chunks) hipLaunchKernelGGL((seq_parts_kernel<F, SUMS>), dim3((unsigned)chunks), dim3(kSeqLanes), 0, st, f, q, parts);
+  constexpr int kSums = SeqOf<F>::kSums;
+  const int64_t chunks = seq_chunks(q.tokens);
   const int lanes = seq_lanes(q);
-  const int64_t rounds = (items * lanes + kSeqJoin - 1) / kSeqJoin;
-  const int groups = rounds <= 4 ? 1 : rounds < kSeqJoinGroups ? (int)rounds : kSeqJoinGroups;
-  double* const totals = parts + (chunks + q.count) * SUMS;
-  hipLaunchKernelGGL((seq_join_kernel<F, TOTALS>), dim3(groups), dim3(kSeqJoin), 0, st, f, q, items, lanes, (const double*)parts,
+  const bool alone = items * lanes <= 4 * kSeqFew;
+  if (chunks) {
+    if (seq_rows(q.tokens) == 1) hipLaunchKernelGGL((seq_parts_kernel<kSums, 1, F>), dim3((unsigned)chunks), dim3(64), 0, st, f, q, parts);
+    else hipLaunchKernelGGL((seq_parts_kernel<kSums, 8, F>), dim3((unsigned)chunks), dim3(64), 0, st, f, q, parts);
+  }
+  if (alone) {
+    hipLaunchKernelGGL((seq_join_kernel<kSeqFew, F>), dim3(1), dim3(kSeqFew), 0, st, f, q, items, lanes, (const double*)parts,
+                       (double*)nullptr, each, loss, more);
+    return;
+  }
+  const int64_t rounds = (items * lanes + kSeqMany - 1) / kSeqMany;
+  const int groups = rounds < kSeqManyGroups ? (int)rounds : kSeqManyGroups;
+  double* const totals = parts + (chunks + q.count) * kSums;
+  hipLaunchKernelGGL((seq_join_kernel<kSeqMany, F>), dim3(groups), dim3(kSeqMany), 0, st, f, q, items, lanes, (const double*)parts,
                      totals, each, loss, more);
-  if (groups > 1)
-    hipLaunchKernelGGL((seq_finish_kernel<F, TOTALS>), dim3(1), dim3(kSeqJoin), 0, st, f, q, groups, (const double*)totals, each,
-                       loss, more);
+  hipLaunchKernelGGL(seq_finish_kernel<F>, dim3(1), dim3(kSeqMany), 0, st, f, q, groups, (const double*)totals, each, loss, more);
 }
 template <class F>
 static void seq_grads(const F& f, const Sequences& q, const double* each, const float* dloss, void* grad, hipStream_t st) {
-  constexpr int64_t per = kSeqGrad * kSeqGradTokens;
-  hipLaunchKernelGGL(seq_grad_kernel<F>, dim3((unsigned)((q.tokens + per - 1) / per)), dim3(kSeqGrad), 0, st, f, q, each, dloss, grad);
+  const int rows = q.tokens < kSeqGradLong ? 1 : 4;
+  const int64_t per = kSeqGrad * rows;
+  const dim3 grid((unsigned)((q.tokens + per - 1) / per));
+  if (rows == 1) hipLaunchKernelGGL((seq_grad_kernel<1, F>), grid, dim3(kSeqGrad), 0, st, f, q, each, dloss, grad);
+  else hipLaunchKernelGGL((seq_grad_kernel<4, F>), grid, dim3(kSeqGrad), 0, st, f, q, each, dloss, grad);
 }
 
 static int status() { return hipGetLastError() == hipSuccess ? MX_OK : MX_ERR_LAUNCH; }
@@ -467,7 +538,7 @@ using namespace mx;
 
 extern "C" int64_t mx_sequence_loss_workspace(int64_t tokens, int64_t sequences) {
   if (tokens < 0 || sequences < 0) return 0;
-  return 8 * (kPolicySums * ((tokens + kSeqChunk - 1) / kSeqChunk + sequences) + kPolicyTotals * kSeqJoinGroups);
+  return 8 * (kPolicySums * (seq_chunks(tokens) + sequences) + kPolicyTotals * kSeqManyGroups);
 }
 
 static int policy_check(const mx_policy_loss_t* a, Policy& f, Sequences& q) {
@@ -490,7 +561,7 @@ extern "C" int mx_policy_loss(const mx_policy_loss_t* args, float* loss, float* 
   if (const int rc = policy_check(args, f, q)) return rc;
   if (!loss || !metrics || !workspace) return MX_ERR_INVALID_ARG;
   if (((uintptr_t)loss & 3) || ((uintptr_t)metrics & 3) || ((uintptr_t)each & 7) || ((uintptr_t)workspace & 7)) return MX_ERR_ALIGNMENT;
-  seq_loss<kPolicySums, kPolicyTotals>(f, q, q.count, (double*)workspace, each, loss, metrics, (hipStream_t)stream);
+  seq_loss(f, q, q.count, (double*)workspace, each, loss, metrics, (hipStream_t)stream);
   return status();
 }
 
@@ -521,7 +592,7 @@ extern "C" int mx_preference_loss(const mx_preference_loss_t* args, float* loss,
   if (const int rc = preference_check(args, f, q)) return rc;
   if (!loss || (q.count > 0 && !rewards) || !workspace) return MX_ERR_INVALID_ARG;
   if (((uintptr_t)loss & 3) || ((uintptr_t)rewards & 3) || ((uintptr_t)each & 7) || ((uintptr_t)workspace & 7)) return MX_ERR_ALIGNMENT;
-  seq_loss<kPreferenceSums, kPreferenceTotals>(f, q, q.count / 2, (double*)workspace, each, loss, rewards, (hipStream_t)stream);
+  seq_loss(f, q, q.count / 2, (double*)workspace, each, loss, rewards, (hipStream_t)stream);
   return status();
 }
 
