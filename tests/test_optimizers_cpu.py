@@ -232,6 +232,62 @@ def test_state_dicts_keep_their_types_and_are_converted():
     assert isinstance(twin, AdamW) and len(twin.state) == 2
 
 
+@pytest.fixture
+def mesh():
+    """One rank; nothing is sent."""
+    import torch.distributed as dist
+    from torch.distributed.device_mesh import DeviceMesh
+
+    dist.init_process_group("gloo", store=dist.HashStore(), rank=0, world_size=1)
+    try:
+        yield DeviceMesh("cpu", [0])
+    finally:
+        dist.destroy_process_group()
+
+
+def test_distributed_parameters_are_updated_shard_by_shard(mesh):
+    from torch.distributed.tensor import DTensor, Replicate, Shard
+
+    plain = torch.nn.Parameter(torch.randn(8, 6, generator=torch.Generator().manual_seed(0)))
+    spread = torch.nn.Parameter(DTensor.from_local(plain.detach().clone(), mesh, [Shard(0)], run_check=False))
+    a, b = AdamW([plain]), AdamW([spread])
+    for step in range(3):
+        plain.grad = torch.randn(8, 6, generator=torch.Generator().manual_seed(step))
+        spread.grad = DTensor.from_local(plain.grad.clone(), mesh, [Shard(0) if step < 2 else Replicate()], run_check=False)
+        norm = torch.tensor(3.0)
+        a.step(total_norm=norm, max_norm=1.0)
+        b.step(total_norm=DTensor.from_local(norm, mesh, [Replicate()], run_check=False), max_norm=1.0)
+    assert isinstance(spread.data, DTensor) and torch.equal(spread.to_local(), plain)
+    assert isinstance(b.state[spread]["exp_avg"], DTensor) and torch.equal(b.state[spread]["exp_avg"].to_local(), a.state[plain]["exp_avg"])
+    c = AdamW([spread])
+    c.load_state_dict(b.state_dict())
+    assert c.state[spread]["step"] == 3 and torch.equal(c.state[spread]["exp_avg_sq"].to_local(), a.state[plain]["exp_avg_sq"])
+    with pytest.raises(ValueError, match="plain contiguous"):
+        AdamW([spread], state_bits=8).step()
+
+
+def test_hooks_schedulers_and_a_compiled_caller():
+    p = torch.nn.Parameter(torch.ones(10))
+    opt = AdamW([p], lr=0.1, weight_decay=0.0)
+    seen = []
+    opt.register_step_post_hook(lambda *a: seen.append(float(p[0])))
+    schedule = torch.optim.lr_scheduler.LambdaLR(opt, lambda step: 0.5 ** step)
+
+    @torch.compile(backend="eager")
+    def update(g):
+        p.grad = g
+        opt.step()
+
+    try:
+        for _ in range(2):
+            update(torch.ones(10))
+            schedule.step()
+    finally:
+        torch._dynamo.reset()
+    # (a constant gradient moves by the learning rate, 0.1 and 0.05, but for eps and some roundings)
+    assert len(seen) == 2 and abs(seen[0] - 0.9) < 1e-6 and abs(seen[1] - 0.85) < 1e-6
+
+
 def test_refusals():
     p = torch.nn.Parameter(torch.ones(4, 4))
     for bad in (dict(lr=-1.0), dict(betas=(1.0, 0.9)), dict(eps=-1e-8), dict(weight_decay=-0.1), dict(state_bits=16), dict(seed=-1),

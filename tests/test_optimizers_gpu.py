@@ -323,3 +323,62 @@ def test_the_timer_and_other_types_take_their_paths(device):
     assert all(torch.equal(p, q) for p, q in zip(params, twins))
     others = parameters_of(device, [(40, 3), (9,)], (torch.float16, torch.float64))
     check_steps(AdamW(others, **HYPER, weight_decay=0.1), others)
+
+
+def test_distributed_parameters_run_on_their_shards(device):
+    import torch.distributed as dist
+    from torch.distributed.device_mesh import DeviceMesh
+    from torch.distributed.tensor import DTensor, Shard
+
+    dist.init_process_group("gloo", store=dist.HashStore(), rank=0, world_size=1)
+    try:
+        mesh = DeviceMesh("cuda", [0])
+        plain = torch.nn.Parameter(torch.randn(300, 70, device=device).bfloat16())
+        spread = torch.nn.Parameter(DTensor.from_local(plain.detach().clone(), mesh, [Shard(0)], run_check=False))
+        a, b = AdamW([plain], master_weights=True), AdamW([spread], master_weights=True)
+        timer = ops.KernelTimer()
+        for step in range(2):
+            set_gradients([plain], step)
+            spread.grad = DTensor.from_local(plain.grad.clone(), mesh, [Shard(0)], run_check=False)
+            a.step()
+            ops.set_kernel_timer(timer)
+            try:
+                b.step()
+            finally:
+                ops.set_kernel_timer(None)
+        assert timer.summary()["adamw"][0] == 2
+        assert torch.equal(spread.to_local(), plain) and isinstance(b.state[spread]["master"], DTensor)
+    finally:
+        dist.destroy_process_group()
+
+
+def test_other_types_are_not_captured_either(device):
+    p = torch.nn.Parameter(torch.randn(10, device=device).half())
+    p.grad = torch.ones_like(p)
+    opt = AdamW([p])
+    opt.step()
+    with pytest.raises(RuntimeError, match="capturable=True"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            opt.step()
+    with pytest.raises(RuntimeError, match="one GPU"):
+        AdamW([p], capturable=True).step()
+
+
+def test_a_compiled_caller(device):
+    params = parameters_of(device, [(64, 33)], (torch.float32,))
+    twins = [torch.nn.Parameter(p.detach().clone()) for p in params]
+    a, b = AdamW(params, state_bits=8), AdamW(twins, state_bits=8)
+
+    @torch.compile(backend="eager")
+    def update(g):
+        twins[0].grad = g * 2
+        b.step()
+
+    try:
+        for step in range(3):
+            set_gradients(params, step)
+            update(params[0].grad / 2)
+            a.step()
+    finally:
+        torch._dynamo.reset()
+    assert torch.equal(params[0], twins[0]) and a.state[params[0]]["step"] == b.state[twins[0]]["step"] == 3

@@ -480,7 +480,8 @@ __global__ __launch_bounds__(kSeqGrad) void seq_grad_kernel(F f, Sequences q, co
 
 static int seq_check(const Sequences& q) {
   if (q.count < 0 || q.tokens < 0 || (q.count == 0 && !q.offsets && q.tokens > 0)) return MX_ERR_INVALID_ARG;
-  if (!q.offsets && (q.length < 0 || q.length * q.count != q.tokens)) return MX_ERR_INVALID_ARG;
+  if (!q.offsets && (q.length < 0 || (q.length ? q.tokens % q.length || q.tokens / q.length != q.count : q.tokens > 0)))
+    return MX_ERR_INVALID_ARG;
   if ((uintptr_t)q.offsets & (q.wide ? 7 : 3)) return MX_ERR_ALIGNMENT;
   // (a wave for every chunk, a lane for every token: launches have fewer than 2^32 lanes)
   if (q.tokens > 0xFFFFFF00 || q.count > 0x3FFFFFFF) return MX_ERR_UNSUPPORTED;

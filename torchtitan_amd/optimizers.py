@@ -72,12 +72,12 @@ def _decode(codes: torch.Tensor, scales: torch.Tensor, form, n: int) -> torch.Te
     return (torch.where(code >= 128, -value, value) if signed else value).reshape(-1)[:n]
 
 
-def _in_torch_ops(p, g, state, group, factor, step, number):
+def _in_torch_ops(p, g, state, group, norm, limit, step, number):
     (b1, b2), lr, eps = group["betas"], float(group["lr"]), group["eps"]
     wide = torch.promote_types(p.dtype, torch.float32)
     g = g.to(wide)
-    if factor is not None:
-        g = g * factor.to(g.device)
+    if norm is not None:
+        g = g * (limit / (norm.to(g.device, torch.float32) + 1e-6)).clamp(max=1.0)
     if group["maximize"]:
         g = -g
     if group["state_bits"] == 8:
@@ -116,7 +116,8 @@ class AdamW(torch.optim.Optimizer):
         p = (1 - lr * weight_decay) p - lr / (1 - b1^t) * m / (sqrt(v / (1 - b2^t)) + eps)
 
     in float32, p rounded once to its type.  `master_weights`: parameters narrower than float32 keep a float32 weight in
-    their state, which the step updates; the parameter is its rounding.  ``state_bits=8``: the first moment is held in e4m3, the
+    their state, which the step updates; the parameter is its rounding (a value that is written into the parameter from outside
+    wants a new state).  ``state_bits=8``: the first moment is held in e4m3, the
     second in e5m3 without a sign, 32 values in the order of memory with a power of two between them (``exp_avg`` uint8
     [blocks, 32] and ``exp_avg_scale`` [blocks]; likewise ``exp_avg_sq``), rounded up or down by chance so that
     their mean is the exact one; `seed` decides about that chance, the same seed gives the same bits.  A block whose gradients
@@ -278,51 +279,48 @@ class AdamW(torch.optim.Optimizer):
         for _, p in with_grad:
             if p.grad.is_sparse:
                 raise RuntimeError("AdamW: sparse gradients are not supported")
-            if p not in self.state or not self.state[p]:
+            if not self.state.get(p):
                 self._new_state(p, group)
-        if not with_grad:
-            return
-        if group["capturable"]:
-            if not all(_kernel_takes(p) and p.device == with_grad[0][1].device for _, p in with_grad):
+        if norm is not None:
+            norm = (norm.full_tensor() if hasattr(norm, "full_tensor") else norm).detach().reshape(())
+        work = [_Work(number, p, self.state[p]) for number, p in with_grad]
+        if group["capturable"] and work:
+            if not all(w.kernel and w.p.device == work[0].p.device for w in work):
                 raise RuntimeError("AdamW: capturable wants bf16 or float32 parameters on one GPU")
-            self._launch(with_grad, group, norm, limit, *self._counter(index, first))
+            self._launch(work, group, norm, limit, *self._counter(index, first))
             return
+        if any(_capture(w.p) for w in work):
+            raise RuntimeError("AdamW: a step that is captured into a graph wants capturable=True")
         by_device: dict = {}
-        for number, p in with_grad:
-            if _kernel_takes(p):
-                by_device.setdefault(p.device, []).append((number, p))
+        for w in work:
+            if w.kernel:
+                by_device.setdefault(w.p.device, []).append(w)
                 continue
-            state, factor = self.state[p], None
-            if norm is not None:
-                factor = (limit / (norm.float() + 1e-6)).clamp(max=1.0)
-            step = int(state["step"]) + 1
-            _in_torch_ops(_unwrap(p), _unwrap(p.grad), state, group, factor, step, number)
-            state["step"] = step
+            step = int(w.state["step"]) + 1
+            _in_torch_ops(w.p, w.g, w.held, group, norm, limit, step, w.number)
+            w.state["step"] = step
         for some in by_device.values():
             self._launch(some, group, norm, limit)
 
-    def _launch(self, numbered, group, norm, limit: float, counters=None, corrections=None) -> None:
+    def _launch(self, work, group, norm, limit: float, counters=None, corrections=None) -> None:
         eight = group["state_bits"] == 8
-        device = numbered[0][1].device
-        if counters is None and _capture(_unwrap(numbered[0][1])):
-            raise RuntimeError("AdamW: a step that is captured into a graph wants capturable=True")
         operands = []
-        for number, p in numbered:
-            p, g, state = _unwrap(p), _unwrap(p.grad), self.state[p]
-            if g.device != device or g.shape != p.shape:
-                raise ValueError(f"AdamW: a gradient of shape {tuple(g.shape)} on {g.device} for a parameter of {tuple(p.shape)} on {device}")
+        for w in work:
+            p, g = w.p, w.g
+            if g.device != p.device or g.shape != p.shape:
+                raise ValueError(f"AdamW: a gradient of shape {tuple(g.shape)} on {g.device} for a parameter of {tuple(p.shape)} on {p.device}")
             if g.dtype != p.dtype or g.is_neg() or type(g) is not torch.Tensor or not _same_order(g, p):
                 g = torch.empty_like(p).copy_(g)
-            moments = [state[name] for name in _MOMENTS[group["state_bits"]]]
-            master = state.get("master")
+            moments = [w.held[name] for name in _MOMENTS[group["state_bits"]]]
+            master = w.held.get("master")
             _check_state(p, moments, master, eight)
-            operands.append((p, g, moments, master, 0 if counters is not None else int(state["step"]) + 1, number))
+            operands.append((p, g, moments, master, 0 if counters is not None else int(w.state["step"]) + 1, w.number))
         on_device = counters is not None and isinstance(group["lr"], torch.Tensor) and group["lr"].is_cuda
         ops.adamw_(operands, eight, 0.0 if on_device else float(group["lr"]), group["betas"], group["eps"], group["weight_decay"],
                    group["maximize"], norm, limit, group["seed"], counters, group["lr"] if on_device else None, corrections)
         if counters is None:  # (a refused step has not been one)
-            for _, p in numbered:
-                self.state[p]["step"] = int(self.state[p]["step"]) + 1
+            for w in work:
+                w.state["step"] = int(w.state["step"]) + 1
 
     @torch.no_grad()
     def moments(self, dtype: torch.dtype = torch.bfloat16) -> list:
@@ -357,6 +355,27 @@ class AdamW(torch.optim.Optimizer):
         for device in {t.device for *_, t in asked}:
             ops.adamw_moments([a for a in asked if a[3].device == device])
         return out
+
+
+def _local(t: torch.Tensor) -> torch.Tensor:
+    """A plain tensor: of a converted weight its values, of a distributed tensor this rank's shard."""
+    t = _unwrap(t)
+    return t.to_local() if hasattr(t, "to_local") else t
+
+
+class _Work:
+    """What a step reads and writes of one parameter: plain tensors (every value is updated by itself, so that a distributed
+    parameter is updated shard by shard)."""
+
+    __slots__ = ("number", "p", "g", "held", "state", "kernel")
+
+    def __init__(self, number: int, p: torch.Tensor, state: dict):
+        g = p.grad
+        if hasattr(p, "placements") and hasattr(g, "placements") and g.placements != p.placements:
+            g = g.redistribute(placements=p.placements)
+        self.number, self.p, self.g, self.state = number, _local(p.detach()), _local(g), state
+        self.held = {name: _local(t) for name, t in state.items() if name != "step"}
+        self.kernel = _kernel_takes(self.p)
 
 
 def _same_order(t: torch.Tensor, p: torch.Tensor) -> bool:
