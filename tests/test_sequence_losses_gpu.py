@@ -117,6 +117,10 @@ def test_saved_tensors_that_hooks_replace(device):
         loss = call()
     with pytest.raises(RuntimeError, match="saved tensor"):
         torch.autograd.grad(loss, case["log_probs"])
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t[:3] if t.shape == (16,) else t):  # (too few advantages)
+        loss = call()
+    with pytest.raises(RuntimeError, match="saved tensor"):
+        torch.autograd.grad(loss, case["log_probs"])
 
 
 def test_streams_and_a_captured_step(device):
@@ -152,15 +156,62 @@ def test_streams_and_a_captured_step(device):
         assert all(torch.equal(a, b) for a, b in zip(captured, want))
 
 
-def test_traced_in_torch_operations(device):
-    """Under torch.compile the formula enters the graph whole."""
-    case = tokens_of((8, 40), device, mask=0.7)
-    call = lambda lp: policy_loss(lp, case["advantages"], case["old"], case["ref"], mask=case["mask"], kl_coef=0.1)[0]
-    loss = torch.compile(call, fullgraph=True, backend="aot_eager")(case["log_probs"])
-    want = call(case["log_probs"])
-    assert torch.allclose(loss, want, rtol=1e-6)
-    a, b = (torch.autograd.grad(t, case["log_probs"])[0] for t in (loss, want))
-    assert torch.allclose(a, b, rtol=1e-6, atol=1e-12)
+@pytest.mark.parametrize("dynamic", [False, True])
+def test_traced_as_nodes_of_the_graph(device, dynamic):
+    """Under torch.compile the losses are operators of the graph: the eager bits, without a break."""
+    torch._dynamo.reset()
+    try:
+        for shape in ((8, 40), (6, 50)):
+            case = tokens_of(shape, device, mask=0.7)
+
+            def call(lp):
+                loss, metrics = policy_loss(lp * 1.0, case["advantages"], case["old"], case["ref"], mask=case["mask"], kl_coef=0.1)
+                other, rewards = preference_loss(lp * 1.0, case["ref"], mask=case["mask"], kind="ipo")
+                return loss, metrics, other, rewards
+
+            compiled = torch.compile(call, fullgraph=True, backend="aot_eager", dynamic=dynamic)
+            got, want = compiled(case["log_probs"]), call(case["log_probs"])
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+            a, b = (torch.autograd.grad(x[0] + x[2], case["log_probs"])[0] for x in (got, want))
+            assert torch.equal(a, b)
+            with torch.no_grad():
+                assert torch.equal(compiled(case["log_probs"])[0], want[0])
+        packed = tokens_of((300,), device, offsets=[0, 100, 100, 290], dtype=torch.bfloat16)
+        call = lambda lp: policy_loss(lp, packed["advantages"].double(), packed["old"].float(), offsets=packed["offsets"])[0]
+        got, want = torch.compile(call, fullgraph=True, backend="aot_eager")(packed["log_probs"]), call(packed["log_probs"])
+        assert torch.equal(got, want)
+        assert torch.equal(*(torch.autograd.grad(x, packed["log_probs"])[0] for x in (got, want)))
+    finally:
+        torch._dynamo.reset()
+
+
+def test_under_a_timer_and_in_transforms(device):
+    """The launches one by one under a kernel timer give the same bits; function transforms take the formula in torch operations."""
+    case, pair = tokens_of((8, 40), device, mask=0.7), tokens_of((8, 40), device, mask=0.7, seed=2, dtype=torch.bfloat16)
+
+    def call():
+        loss, metrics = policy_loss(case["log_probs"], case["advantages"], case["old"], case["ref"], mask=case["mask"], kl_coef=0.1)
+        other, rewards = preference_loss(pair["log_probs"], pair["ref"], mask=pair["mask"])
+        return (loss, metrics, other, rewards, *torch.autograd.grad(loss, case["log_probs"], retain_graph=True),
+                *torch.autograd.grad(other, pair["log_probs"], retain_graph=True))
+
+    want, timer = call(), ops.KernelTimer()
+    ops.set_kernel_timer(timer)
+    try:
+        got = call()
+        with torch.no_grad():
+            assert torch.equal(policy_loss(case["log_probs"], case["advantages"], case["old"], mask=case["mask"])[0].isnan(),
+                               torch.tensor(False, device=device))
+        (g,) = torch.autograd.grad(got[0], case["log_probs"], create_graph=True)
+        with pytest.raises(RuntimeError, match="cannot be differentiated again"):
+            g.sum().backward()
+    finally:
+        ops.set_kernel_timer(None)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert {"policy_loss", "policy_loss_bwd", "preference_loss", "preference_loss_bwd"} <= set(timer.summary())
+    grad = torch.func.grad(lambda lp: policy_loss(lp, case["advantages"], case["old"], case["ref"], mask=case["mask"], kl_coef=0.1)[0])(
+        case["log_probs"].detach())
+    assert torch.allclose(grad, want[4], rtol=1e-6, atol=1e-12)  # (64 bits there too; one rounding)
 
 
 class _TwoLayers(torch.nn.Module):
@@ -236,6 +287,55 @@ def test_a_training_step_from_logits_to_weights(device):
         want = torch.stack(terms).mean()
         assert abs(float(loss) - float(want)) <= 1e-6 * max(1.0, abs(float(want)))
         weight.grad = None
+
+
+def test_a_policy_step_of_a_converted_model(device):
+    """Linears in MXFP8, the sample loss, the gradients' norm, an update with 8-bit moments that clips as it reads, and the hand-over: the
+    casts that were kept are made anew from the updated weights."""
+    from torchtitan_amd.modules import Linear
+    from torchtitan_amd.mx_tensor import MXFP8TrainingWeight
+    from torchtitan_amd.protocols import ModelConvertersContainer
+    from torchtitan_amd.quantization.mx import MXFP8Converter, export_mxfp8_state_dict
+
+    class Model(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            linear = lambda k, n: Linear.Config().build(in_features=k, out_features=n)
+            self.emb = torch.nn.Embedding(512, 128)
+            self.up, self.down, self.out = linear(128, 256), linear(256, 128), linear(128, 512)
+
+        def forward(self, tokens, attention_masks=None):
+            h = self.emb(tokens)
+            return self.out(h + self.down(torch.nn.functional.silu(self.up(h))))
+
+    torch.manual_seed(0)
+    model = Model().to(device).bfloat16()
+    box = ModelConvertersContainer.Config(converters=[MXFP8Converter.Config(fqns=["up", "down"], cache_weight_casts=True)]).build(
+        parallel_dims=None, model_compile_enabled=False)
+    box.convert(model)
+    opt = AdamW(model.parameters(), lr=1e-2, state_bits=8, master_weights=True)
+    rng = torch.Generator().manual_seed(1)
+    ids = lambda n: torch.randint(0, 512, (n,), generator=rng).tolist()
+    prompts, answers = [ids(n) for n in (5, 9)], [ids(n) for n in (27, 55)]
+    ref = [torch.full((len(a),), -6.0, device=device) for a in answers]
+    for step in range(2):
+        total, metrics, _ = compute_policy_gradient_loss(model, answers, prompts, torch.tensor([1.0, -0.5]), ref)
+        total.backward()
+        before = {n: p.detach().as_subclass(torch.Tensor).clone() for n, p in model.named_parameters()}
+        norm = get_total_norm([p.grad for p in model.parameters()])
+        opt.step(total_norm=norm, max_norm=1.0)
+        box.post_optimizer_hook(model)
+        payload = export_mxfp8_state_dict(model)
+        converted = 0
+        for name, p in model.named_parameters():
+            plain = p.detach().as_subclass(torch.Tensor)
+            assert torch.isfinite(plain).all() and not torch.equal(plain, before[name])
+            assert torch.equal(plain, opt.state[p]["master"].bfloat16())
+            if isinstance(p, MXFP8TrainingWeight):
+                converted += 1
+                assert torch.equal(payload[name]["codes"], ops.to_mx_dim0(plain, "rceil").codes)
+        assert converted == 2
+        opt.zero_grad()
 
 
 def test_the_launches_are_the_librarys(device):

@@ -918,3 +918,77 @@ def residual_norm_traced(h, residual, post, gate, pre, scale: float, eps: float)
     """(stream, normed or None) of matrices while a graph is being traced."""
     stream, normed, _ = torch.ops.torchtitan_amd.residual_norm_fwd(h, residual, post, gate, pre, scale, eps)
     return stream, None if pre is None else normed
+
+
+# ----------------------------------------------------------------------------- losses over sequences
+@torch.library.custom_op("torchtitan_amd::policy_loss_fwd", mutates_args=())
+def policy_loss_fwd(log_probs: torch.Tensor, advantages: torch.Tensor, old: torch.Tensor | None, ref: torch.Tensor | None,
+                    offsets: torch.Tensor | None, mask: torch.Tensor | None, sequences: int, per_token: bool, whole: bool,
+                    by_sequence: bool, kl: int, low: float, high: float, kl_coef: float,
+                    entropy_coef: float) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """`ops.policy_loss_fwd` as a node of the graph."""
+    return ops.policy_loss_fwd(log_probs, advantages, old, ref, offsets, mask, sequences, per_token, whole, by_sequence, kl, low,
+                               high, kl_coef, entropy_coef)
+
+
+@policy_loss_fwd.register_fake
+def _(log_probs, advantages, old, ref, offsets, mask, sequences, per_token, whole, by_sequence, kl, low, high, kl_coef, entropy_coef):
+    new = lambda shape, dtype: log_probs.new_empty(shape, dtype=dtype)
+    return new((), torch.float32), new((5,), torch.float32), new((2 * sequences + 2,), torch.float64)
+
+
+@torch.library.custom_op("torchtitan_amd::policy_loss_bwd", mutates_args=())
+def policy_loss_bwd(log_probs: torch.Tensor, advantages: torch.Tensor, old: torch.Tensor | None, ref: torch.Tensor | None,
+                    offsets: torch.Tensor | None, mask: torch.Tensor | None, each: torch.Tensor, dloss: torch.Tensor, sequences: int,
+                    per_token: bool, whole: bool, by_sequence: bool, kl: int, low: float, high: float, kl_coef: float,
+                    entropy_coef: float) -> torch.Tensor:
+    return ops.policy_loss_bwd(log_probs, advantages, old, ref, offsets, mask, each, dloss, sequences, per_token, whole, by_sequence,
+                               kl, low, high, kl_coef, entropy_coef)
+
+
+@policy_loss_bwd.register_fake
+def _(log_probs, *others):
+    return log_probs.new_empty(log_probs.shape)
+
+
+@torch.library.custom_op("torchtitan_amd::preference_loss_fwd", mutates_args=())
+def preference_loss_fwd(log_probs: torch.Tensor, ref: torch.Tensor | None, offsets: torch.Tensor | None, mask: torch.Tensor | None,
+                        sequences: int, kind: int, mean: bool, beta: float,
+                        smoothing: float) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """`ops.preference_loss_fwd` as a node of the graph."""
+    return ops.preference_loss_fwd(log_probs, ref, offsets, mask, sequences, kind, mean, beta, smoothing)
+
+
+@preference_loss_fwd.register_fake
+def _(log_probs, ref, offsets, mask, sequences, kind, mean, beta, smoothing):
+    new = lambda shape, dtype: log_probs.new_empty(shape, dtype=dtype)
+    return new((), torch.float32), new((sequences,), torch.float32), new((sequences + 1,), torch.float64)
+
+
+@torch.library.custom_op("torchtitan_amd::preference_loss_bwd", mutates_args=())
+def preference_loss_bwd(log_probs: torch.Tensor, ref: torch.Tensor | None, offsets: torch.Tensor | None, mask: torch.Tensor | None,
+                        each: torch.Tensor, dloss: torch.Tensor, sequences: int, kind: int, mean: bool, beta: float,
+                        smoothing: float) -> torch.Tensor:
+    return ops.preference_loss_bwd(log_probs, ref, offsets, mask, each, dloss, sequences, kind, mean, beta, smoothing)
+
+
+@preference_loss_bwd.register_fake
+def _(log_probs, *others):
+    return log_probs.new_empty(log_probs.shape)
+
+
+def _loss_autograd(forward, backward, tensors: int):
+    def setup(ctx, inputs, output):
+        ctx.numbers = inputs[tensors:]
+        ctx.save_for_backward(*inputs[:tensors], output[2])
+        ctx.set_materialize_grads(False)
+
+    def back(ctx, dloss, dmore, deach):
+        none = (None,) * (tensors - 1 + len(ctx.numbers))
+        return (None if dloss is None else backward(*ctx.saved_tensors, dloss, *ctx.numbers), *none)
+
+    forward.register_autograd(back, setup_context=setup)
+
+
+_loss_autograd(policy_loss_fwd, torch.ops.torchtitan_amd.policy_loss_bwd, 6)
+_loss_autograd(preference_loss_fwd, torch.ops.torchtitan_amd.preference_loss_bwd, 4)

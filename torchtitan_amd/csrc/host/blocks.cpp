@@ -1105,6 +1105,9 @@ struct PolicyNumbers {
     a.ratio_low = low, a.ratio_high = high, a.kl_coef = kl_coef, a.entropy_coef = entropy_coef;
     return a;
   }
+  bool fits(const LossOperands& o) const {
+    return o.advantages.defined() && o.advantages.numel() == (advantage_per_token ? o.log_probs.numel() : o.sequences);
+  }
   int64_t more(const LossOperands&) const { return 5; }
   int64_t each(const LossOperands& o) const { return 2 * o.sequences + 2; }
   int forward(const LossOperands& o, float* loss, float* out, double* each, void* work, hipStream_t st) const {
@@ -1134,6 +1137,7 @@ struct PreferenceNumbers {
     a.beta = beta, a.smoothing = smoothing;
     return a;
   }
+  bool fits(const LossOperands&) const { return true; }
   int64_t more(const LossOperands& o) const { return o.sequences; }
   int64_t each(const LossOperands& o) const { return o.sequences + 1; }
   int forward(const LossOperands& o, float* loss, float* out, double* each, void* work, hipStream_t st) const {
@@ -1185,7 +1189,7 @@ struct LossNode : torch::autograd::Function<LossNode<Numbers>> {
     const Numbers numbers = Numbers::unpack(ctx->saved_data["numbers"].toDoubleVector());
     const c10::DeviceGuard guard(grads[0].device());
     // (hooks on saved tensors may have replaced them)
-    TORCH_CHECK(loss_plain(o) && each.device() == grads[0].device() && each.scalar_type() == at::kDouble &&
+    TORCH_CHECK(loss_plain(o) && numbers.fits(o) && each.device() == grads[0].device() && each.scalar_type() == at::kDouble &&
                     each.numel() == numbers.each(o) && o.log_probs.device() == grads[0].device(),
                 "a saved tensor came back with another type, size or device");
     const Tensor dloss = grads[0].resolve_neg().to(at::kFloat).contiguous(), grad = at::empty(o.log_probs.sizes(), o.log_probs.options());
@@ -1197,7 +1201,7 @@ struct LossNode : torch::autograd::Function<LossNode<Numbers>> {
 
 template <class Numbers>
 py::object loss_of(const LossOperands& o, const Numbers& numbers) {
-  if (!loss_plain(o)) return py::none();
+  if (!loss_plain(o) || !numbers.fits(o)) return py::none();
   Unlocked unlocked(std::in_place);
   Tensor loss, more;
   if (at::GradMode::is_enabled() && o.log_probs.requires_grad()) {

@@ -5,6 +5,7 @@ call into libmxfp8_gfx950.so.  There is no fallback path: CPU tensors are reject
 """
 from __future__ import annotations
 
+import ctypes
 import os
 from ctypes import c_int32, c_int64
 from typing import NamedTuple
@@ -1168,6 +1169,115 @@ def grad_scale_(grads, norm: torch.Tensor, limit: float) -> None:
         raise TypeError("the norm must be one float32 on the gradients' device")
     torch.autograd.graph.increment_version(grads)
     _call("mx_grad_scale", "grad_scale", grads[0].device, *lists, _ptr(norm), limit, _stream(norm))
+
+
+# ------------------------------------------------------------------- losses over the tokens of sequences
+class PolicyArgs(ctypes.Structure):
+    """mx_policy_loss_t"""
+
+    _fields_ = [(n, ctypes.c_void_p) for n in ("log_probs", "old_log_probs", "ref_log_probs")] + [
+        (n, ctypes.c_int) for n in ("log_probs_f32", "old_f32", "ref_f32")] + [
+        (n, ctypes.c_void_p) for n in ("advantages", "offsets", "mask")] + [
+        (n, c_int64) for n in ("sequences", "tokens", "length")] + [
+        (n, ctypes.c_int) for n in ("offsets_i64", "advantage_per_token", "ratio_per_sequence", "mean_per_sequence", "kl")] + [
+        (n, ctypes.c_double) for n in ("ratio_low", "ratio_high", "kl_coef", "entropy_coef")]
+
+
+class PreferenceArgs(ctypes.Structure):
+    """mx_preference_loss_t"""
+
+    _fields_ = [(n, ctypes.c_void_p) for n in ("log_probs", "ref_log_probs")] + [
+        (n, ctypes.c_int) for n in ("log_probs_f32", "ref_f32")] + [
+        (n, ctypes.c_void_p) for n in ("offsets", "mask")] + [
+        (n, c_int64) for n in ("sequences", "tokens", "length")] + [
+        (n, ctypes.c_int) for n in ("offsets_i64", "kind", "mean")] + [
+        (n, ctypes.c_double) for n in ("beta", "smoothing")]
+
+
+def _loss_args(cls, log_probs, ref, offsets, mask, sequences: int, **more):
+    """(the arguments of a loss, the tensors that they point to)."""
+    held = {"log_probs": log_probs, "ref_log_probs": ref, "offsets": offsets, "mask": mask}
+    held.update({k: t for k, t in more.items() if t is None or isinstance(t, torch.Tensor)})
+    types = {"log_probs": ROW_TYPES, "ref_log_probs": ROW_TYPES, "old_log_probs": ROW_TYPES, "offsets": (torch.int64, torch.int32),
+             "mask": (torch.bool,), "advantages": (torch.float32,)}
+    for name, t in held.items():
+        if t is None:
+            continue
+        if not t.is_cuda or t.device != log_probs.device:
+            raise _lib.MXLibraryError(f"{name} on {t.device}: the kernels run on the GPU of log_probs, {log_probs.device}")
+        if t.dtype not in types[name]:
+            raise TypeError(f"{name} must be one of {types[name]}, got {t.dtype}")
+        if name in ("ref_log_probs", "old_log_probs", "mask") and t.shape != log_probs.shape:
+            raise ValueError(f"{name} must have the shape of log_probs, {tuple(log_probs.shape)}, got {tuple(t.shape)}")
+        held[name] = t.detach().resolve_neg().contiguous()
+    if (offsets.shape if offsets is not None else log_probs.shape[:1]) != ((sequences + 1,) if offsets is not None else (sequences,)) or (
+            log_probs.dim() != (2 if offsets is None else 1)):
+        raise ValueError(f"log_probs {tuple(log_probs.shape)} with{'out' if offsets is None else ''} offsets are not of {sequences} sequences")
+    f32 = lambda name: int(held.get(name) is not None and held[name].dtype == torch.float32)
+    tokens = log_probs.numel()
+    values = {name: _optional_ptr(t) for name, t in held.items()}
+    values.update({k: v for k, v in more.items() if k not in held}, log_probs_f32=f32("log_probs"), ref_f32=f32("ref_log_probs"),
+                  sequences=sequences, tokens=tokens, length=0 if offsets is not None or not sequences else tokens // sequences,
+                  offsets_i64=int(offsets is not None and offsets.dtype == torch.int64))
+    if cls is PolicyArgs:
+        values["old_f32"] = f32("old_log_probs")
+    return cls(**values), held
+
+
+def _loss_fwd(name: str, args, held, more: int, each: int | None):
+    log_probs = held["log_probs"]
+    new = lambda shape, dtype: torch.empty(shape, dtype=dtype, device=log_probs.device)
+    loss, out, saved = new((), torch.float32), new((more,), torch.float32), None if each is None else new((each,), torch.float64)
+    work = new((_lib.load().mx_sequence_loss_workspace(args.tokens, args.sequences),), torch.uint8)
+    _call("mx_" + name, name, log_probs.device, ctypes.byref(args), _ptr(loss), _ptr(out), _optional_ptr(saved), _ptr(work),
+          _stream(log_probs))
+    return loss, out, saved
+
+
+def _loss_bwd(name: str, args, held, each: torch.Tensor, count: int, dloss: torch.Tensor):
+    log_probs = held["log_probs"]
+    if each.dtype != torch.float64 or each.numel() != count or each.device != log_probs.device or dloss.device != log_probs.device:
+        raise RuntimeError("what the forward saved came back with another type, size or device")
+    grad, dloss, each = torch.empty_like(log_probs), dloss.detach().resolve_neg().float().contiguous(), each.contiguous()
+    _call(f"mx_{name}_bwd", f"{name}_bwd", log_probs.device, ctypes.byref(args), _ptr(each), _ptr(dloss), _ptr(grad), _stream(grad))
+    return grad
+
+
+def _policy_args(log_probs, advantages, old, ref, offsets, mask, sequences, per_token, whole, by_sequence, kl, low, high, kl_coef,
+                 entropy_coef):
+    if advantages.numel() != (log_probs.numel() if per_token else sequences):
+        raise ValueError(f"{advantages.numel()} advantages for {sequences} sequences of {log_probs.numel()} tokens")
+    return _loss_args(PolicyArgs, log_probs, ref, offsets, mask, sequences, old_log_probs=old, advantages=advantages,
+                      advantage_per_token=int(per_token), ratio_per_sequence=int(whole), mean_per_sequence=int(by_sequence), kl=kl,
+                      ratio_low=low, ratio_high=high, kl_coef=kl_coef, entropy_coef=entropy_coef)
+
+
+def policy_loss_fwd(log_probs, advantages, old, ref, offsets, mask, sequences: int, *numbers, want_each: bool = True):
+    """(loss, metrics [5], what the backward needs or None): `mx_policy_loss` of log_probs [sequences, length], or [tokens] with
+    offsets; numbers: advantage_per_token, ratio_per_sequence, mean_per_sequence, kl, ratio_low, ratio_high, kl_coef,
+    entropy_coef."""
+    args, held = _policy_args(log_probs, advantages, old, ref, offsets, mask, sequences, *numbers)
+    return _loss_fwd("policy_loss", args, held, 5, 2 * sequences + 2 if want_each else None)
+
+
+def policy_loss_bwd(log_probs, advantages, old, ref, offsets, mask, each, dloss, sequences: int, *numbers) -> torch.Tensor:
+    args, held = _policy_args(log_probs, advantages, old, ref, offsets, mask, sequences, *numbers)
+    return _loss_bwd("policy_loss", args, held, each, 2 * sequences + 2, dloss)
+
+
+def _preference_args(log_probs, ref, offsets, mask, sequences, kind, mean, beta, smoothing):
+    return _loss_args(PreferenceArgs, log_probs, ref, offsets, mask, sequences, kind=kind, mean=int(mean), beta=beta, smoothing=smoothing)
+
+
+def preference_loss_fwd(log_probs, ref, offsets, mask, sequences: int, *numbers, want_each: bool = True):
+    """(loss, rewards [sequences], what the backward needs or None): `mx_preference_loss`; numbers: kind, mean, beta, smoothing."""
+    args, held = _preference_args(log_probs, ref, offsets, mask, sequences, *numbers)
+    return _loss_fwd("preference_loss", args, held, sequences, sequences + 1 if want_each else None)
+
+
+def preference_loss_bwd(log_probs, ref, offsets, mask, each, dloss, sequences: int, *numbers) -> torch.Tensor:
+    args, held = _preference_args(log_probs, ref, offsets, mask, sequences, *numbers)
+    return _loss_bwd("preference_loss", args, held, each, sequences + 1, dloss)
 
 
 ADAMW_FIELDS = 11  # of the table that `mx_adamw` reads

@@ -18,6 +18,7 @@ import torch
 import torch.nn.functional as F
 
 from .. import _lib, ops
+from ..modules.norm import _Refusing
 
 
 class _TokenLogProbs(torch.autograd.Function):
@@ -130,20 +131,73 @@ def _check_tokens(log_probs, others: dict, offsets, mask) -> int:
     return log_probs.shape[0] if offsets is None else offsets.numel() - 1
 
 
-def _native(log_probs, *others) -> bool:
-    """Worth asking the native module: tensors of the types that the kernels read, eager and untransformed."""
-    return (not torch.compiler.is_compiling() and log_probs.dtype in ops.ROW_TYPES and ops.native_rows(log_probs)
-            and all(t is None or type(t) in (torch.Tensor, torch.nn.Parameter) for t in (log_probs, *others)))
+def _once(grad):
+    """A gradient that cannot be differentiated again: log_probs is in it."""
+    return _Refusing.apply(grad, torch.empty(0, requires_grad=True)) if torch.is_grad_enabled() else grad
+
+
+class _PolicyLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, log_probs, *rest):
+        loss, metrics, each = ops.policy_loss_fwd(log_probs, *rest)
+        ctx.save_for_backward(log_probs, *rest[:5], each)
+        ctx.numbers = rest[5:]
+        ctx.mark_non_differentiable(metrics)
+        return loss, metrics
+
+    @staticmethod
+    def backward(ctx, dloss, _):
+        return (_once(ops.policy_loss_bwd(*ctx.saved_tensors, dloss, *ctx.numbers)), *(None,) * 14)
+
+
+class _PreferenceLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, log_probs, *rest):
+        loss, rewards, each = ops.preference_loss_fwd(log_probs, *rest)
+        ctx.save_for_backward(log_probs, *rest[:3], each)
+        ctx.numbers = rest[3:]
+        ctx.mark_non_differentiable(rewards)
+        return loss, rewards
+
+    @staticmethod
+    def backward(ctx, dloss, _):
+        return (_once(ops.preference_loss_bwd(*ctx.saved_tensors, dloss, *ctx.numbers)), *(None,) * 8)
+
+
+def _by_kernels(name: str, node, log_probs, tensors: tuple, numbers: tuple):
+    """The loss through the kernels -- one native call, a traced operator, or step by step --, None for tensors that they do
+    not take."""
+    if not log_probs.is_cuda or log_probs.dtype not in ops.ROW_TYPES or ops.wrapped(log_probs, *(t for t in tensors if t is not None)):
+        return None
+    if torch.compiler.is_compiling():
+        from .. import compiled  # noqa: F401  (the same launches as nodes of the graph)
+
+        call = getattr(torch.ops.torchtitan_amd, name + "_fwd")
+        return call(log_probs, *(_narrow(t) for t in tensors), *numbers)[:2]
+    if not ops.plain_rows(log_probs) or not all(t is None or type(t) in (torch.Tensor, torch.nn.Parameter) for t in tensors):
+        return None
+    if ops.native_rows(log_probs):
+        call = getattr(_lib.blocks(), name)
+        out = call(log_probs, *tensors, *numbers)
+        if out is None:
+            with torch.cuda.device(log_probs.device):
+                out = call(log_probs.contiguous(), *(_dense(t) for t in tensors), *numbers)
+        if out is not None:
+            return out
+    tensors = tuple(_dense(t) for t in tensors)
+    if torch.is_grad_enabled() and log_probs.requires_grad:
+        return node.apply(log_probs, *tensors, *numbers)
+    return getattr(ops, name + "_fwd")(log_probs, *tensors, *numbers, want_each=False)[:2]
+
+
+def _narrow(t):
+    """In a type that the kernels read."""
+    return t.float() if t is not None and t.is_floating_point() and t.dtype not in ops.ROW_TYPES else t
 
 
 def _dense(t):
     """Without a gradient, as the kernels read it."""
-    if t is None:
-        return None
-    t = t.detach()
-    if t.is_floating_point() and t.dtype not in ops.ROW_TYPES:
-        t = t.float()
-    return t.resolve_neg().contiguous()
+    return None if t is None else _narrow(t.detach()).resolve_neg().contiguous()
 
 
 def _places(log_probs, offsets, mask, sequences: int):
@@ -233,7 +287,7 @@ def policy_loss(log_probs: torch.Tensor, advantages: torch.Tensor, old_log_probs
         raise ValueError(f"kl must be one of {_KL}, got {kl!r}")
     if kl_coef and ref_log_probs is None:
         raise ValueError("kl_coef wants ref_log_probs")
-    low, high = 1.0 - clip_eps, 1.0 + (clip_eps if clip_eps_high is None else clip_eps_high)
+    low, high = 1.0 - float(clip_eps), 1.0 + float(clip_eps if clip_eps_high is None else clip_eps_high)
     if not low <= high:
         raise ValueError(f"clip_eps {clip_eps} and clip_eps_high {clip_eps_high} leave nothing between them")
     sequences = _check_tokens(log_probs, dict(old_log_probs=old_log_probs, ref_log_probs=ref_log_probs), offsets, mask)
@@ -243,16 +297,14 @@ def policy_loss(log_probs: torch.Tensor, advantages: torch.Tensor, old_log_probs
                          f"got {tuple(advantages.shape)} {advantages.dtype}")
     if advantages.device != log_probs.device:
         raise ValueError(f"log_probs on {log_probs.device}, advantages on {advantages.device}")
-    numbers = (sequences, per_token, ratio == "sequence", average == "sequence", _KL.index(kl), low, high, kl_coef, entropy_coef)
-    if _native(log_probs, advantages, old_log_probs, ref_log_probs, offsets, mask):
-        call = _lib.blocks().policy_loss
-        out = call(log_probs, advantages, old_log_probs, ref_log_probs, offsets, mask, *numbers)
-        if out is None:
-            with torch.cuda.device(log_probs.device):
-                out = call(log_probs.contiguous(), _dense(advantages).float(), _dense(old_log_probs), _dense(ref_log_probs),
-                           _dense(offsets), _dense(mask), *numbers)
-        if out is not None:
-            return out
+    numbers = (sequences, per_token, ratio == "sequence", average == "sequence", _KL.index(kl), low, high, float(kl_coef),
+               float(entropy_coef))
+    # (advantages are read in float32)
+    out = _by_kernels("policy_loss", _PolicyLoss, log_probs,
+                      (advantages if advantages.dtype == torch.float32 else advantages.float(), old_log_probs, ref_log_probs, offsets,
+                       mask), numbers)
+    if out is not None:
+        return out
     return _policy_in_torch_ops(log_probs, advantages, old_log_probs if old_log_probs is None else old_log_probs.detach(),
                                 ref_log_probs if ref_log_probs is None else ref_log_probs.detach(), offsets, mask, *numbers)
 
@@ -301,14 +353,9 @@ def preference_loss(log_probs: torch.Tensor, ref_log_probs: torch.Tensor | None 
     sequences = _check_tokens(log_probs, dict(ref_log_probs=ref_log_probs), offsets, mask)
     if sequences % 2:
         raise ValueError(f"pairs want an even number of sequences, got {sequences}")
-    numbers = (sequences, _PREFERENCES.index(kind), average_log_probs, beta, label_smoothing)
-    if _native(log_probs, ref_log_probs, offsets, mask):
-        call = _lib.blocks().preference_loss
-        out = call(log_probs, ref_log_probs, offsets, mask, *numbers)
-        if out is None:
-            with torch.cuda.device(log_probs.device):
-                out = call(log_probs.contiguous(), _dense(ref_log_probs), _dense(offsets), _dense(mask), *numbers)
-        if out is not None:
-            return out
+    numbers = (sequences, _PREFERENCES.index(kind), bool(average_log_probs), float(beta), float(label_smoothing))
+    out = _by_kernels("preference_loss", _PreferenceLoss, log_probs, (ref_log_probs, offsets, mask), numbers)
+    if out is not None:
+        return out
     return _preference_in_torch_ops(log_probs, ref_log_probs if ref_log_probs is None else ref_log_probs.detach(), offsets, mask,
                                     *numbers)
