@@ -62,6 +62,30 @@ struct Sequences {
   }
 };
 
+// The same for a whole wave with one token i: its lanes look at 64 offsets at a time, two or three rounds where a search by halves
+// takes ten that wait for each other (1024 packed sequences of 2 million tokens: 13.7 us with those, forward parts alone).
+__device__ __forceinline__ int64_t seq_find(const Sequences& q, int64_t i, int lane) {
+  if (!q.offsets) return q.find(i);
+  int64_t lo = -1, hi = q.count + 1;
+  while (hi - lo > 1) {
+    const int64_t step = (hi - lo - 1 + 63) / 64, at = lo + (lane + 1) * step;
+    const int64_t below = __popcll(__ballot(at < hi && q.offset(at) <= i));
+    hi = below < 64 && lo + (below + 1) * step < hi ? lo + (below + 1) * step : hi;
+    lo += below * step;
+  }
+  return lo;
+}
+// The sequence of each lane's token in the row from `row` on, whose first token is of sequence s or a later one.
+__device__ __forceinline__ int64_t seq_of_row(const Sequences& q, int64_t s, int64_t row, int lane) {
+  if (!q.offsets) return q.find(row + lane);
+  const int64_t next = s + 1 + lane <= q.count ? q.offset(s + 1 + lane) : INT64_MAX;
+  const int ends = __popcll(__ballot(next <= row + 63));
+  if (ends > 8) return q.find(row + lane, s);
+  int64_t mine = s;
+  for (int j = 0; j < ends; ++j) mine += row + lane >= __shfl(next, j, 64);
+  return mine;
+}
+
 struct Policy {
   SeqValues lp, old, ref;  // p null: none
   const float* advantages;
@@ -189,7 +213,7 @@ __device__ __forceinline__ void seq_parts(const F& f, const Sequences& q, int64_
   SeqToken t[ROWS];
 #pragma unroll
   for (int k = 0; k < ROWS; ++k) t[k] = seq_load(f, q, begin + k * 64 + lane);
-  int64_t s = q.find(begin);
+  int64_t s = seq_find(q, begin, lane);
   int64_t stop = s < 0 || s >= q.count ? begin : q.offset(s + 1);
   double sum[SUMS];
   auto clear = [&]() {
@@ -213,7 +237,7 @@ __device__ __forceinline__ void seq_parts(const F& f, const Sequences& q, int64_
       if (t[k].counts) seq_add(f, t[k], s, sum);
       continue;
     }
-    const int64_t mine = i < end ? q.find(i, s < q.count ? s : -1) : q.count;
+    const int64_t of = seq_of_row(q, s, row, lane), mine = i < end ? of : q.count;
     double v[SUMS];
 #pragma unroll
     for (int j = 0; j < SUMS; ++j) v[j] = 0.0;
@@ -331,14 +355,6 @@ __device__ __forceinline__ void seq_finish(const Policy& f, const Sequences& q, 
   if (each) each[2 * q.count] = tokens, each[2 * q.count + 1] = filled;
 }
 
-__device__ __forceinline__ double seq_soft(double y) {  // -log sigmoid(y)
-  return log1p(exp(-fabs(y))) + (y < 0 ? -y : 0.0);
-}
-__device__ __forceinline__ double seq_sigmoid(double y) {
-  const double e = exp(-fabs(y)), p = 1.0 / (1.0 + e);
-  return y < 0 ? e * p : p;
-}
-
 // Of the pair: for the gradient, each[s] that of a token of either sequence (but for the mean over the pairs).
 __device__ __forceinline__ void seq_take(const Preference& f, const Sequences& q, const double* parts, int64_t p, int lane,
                                          int lanes, double* __restrict__ each, float* __restrict__ rewards,
@@ -352,8 +368,10 @@ __device__ __forceinline__ void seq_take(const Preference& f, const Sequences& q
   const double h1 = one[1] * of1, h2 = two[1] * of2, z = h1 - h2, y = f.beta * z;
   double value, slope;
   if (f.kind == 0) {
-    value = (1.0 - f.smoothing) * seq_soft(y) + f.smoothing * seq_soft(-y);
-    slope = f.beta * (f.smoothing * seq_sigmoid(y) - (1.0 - f.smoothing) * seq_sigmoid(-y));
+    // -log sigmoid(y) = log(1 + e^-|y|) + max(-y, 0), and the sigmoids of y and -y from the same e^-|y|
+    const double e = seq_exp(-fabs(y)).e, both = log1p(e), large = 1.0 / (1.0 + e), small = e * large;
+    value = both + (y < 0 ? (1.0 - f.smoothing) * -y : f.smoothing * y);
+    slope = f.beta * (y < 0 ? f.smoothing * small - (1.0 - f.smoothing) * large : f.smoothing * large - (1.0 - f.smoothing) * small);
   } else if (f.kind == 1) {
     value = 1.0 - y < 0 ? 0.0 : 1.0 - y;  // (NaN stays)
     slope = y < 1.0 ? -f.beta : 0.0;
@@ -458,21 +476,23 @@ __global__ __launch_bounds__(kSeqGrad) void seq_grad_kernel(F f, Sequences q, co
 #pragma unroll
   for (int k = 0; k < ROWS; ++k) t[k] = seq_load(f, q, begin + k * 64 + lane);
   const double by = (double)*dloss;
-  const int64_t first = q.find(begin), end = begin + 64 * ROWS < q.tokens ? begin + 64 * ROWS : q.tokens;
+  const int64_t first = seq_find(q, begin, lane), end = begin + 64 * ROWS < q.tokens ? begin + 64 * ROWS : q.tokens;
   const bool one = first >= 0 && first < q.count && q.offset(first + 1) >= end;  // all of one sequence
   double share = 0.0, entropy = 0.0, slope = 0.0;
   if (one) seq_common(f, each, q.count, first, share, entropy, slope);
+  int64_t s = first;
 #pragma unroll
   for (int k = 0; k < ROWS; ++k) {
-    const int64_t i = begin + k * 64 + lane;
-    if (i >= q.tokens) return;
-    int64_t s = first;
+    const int64_t row = begin + k * 64, i = row + lane;
+    if (row >= q.tokens) break;
+    if (!one) s = seq_of_row(q, s, row, lane);
     double g = 0.0;
-    if (!one) s = q.find(i, first < q.count ? first : -1);
     if (t[k].counts && s >= 0 && s < q.count) {
       if (!one) seq_common(f, each, q.count, s, share, entropy, slope);
       g = seq_grad(f, share, entropy, slope, t[k], s) * by;
     }
+    if (!one) s = __shfl(s, 63, 64);
+    if (i >= q.tokens) continue;
     if (f.lp.f32) ((float*)grad)[i] = (float)g;
     else ((uint16_t*)grad)[i] = (uint16_t)__builtin_bit_cast(uint32_t, __builtin_convertvector(v2f_t{(float)g, 0.f}, v2bf_t));
   }
