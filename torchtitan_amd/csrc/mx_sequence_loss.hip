@@ -10,8 +10,8 @@
 //   join     every sequence's parts are added up, the loss formed, and what a token's gradient needs of its sequence
 //   gradient tokens as they lie (backward)
 // Some tens of megabytes at most are read.  Up to 100 000 tokens bound by the latency of two launches forward (10 to 16 us) and one
-// backward (3), so that a wave has a single row of 64 tokens until there are enough for every CU; 4.2 million tokens (89 MB) take 43 and 23
-// us, half of it float64 arithmetic.  Terms are formed in float64: a ratio's side of a clipping border decides about its whole
+// backward (3), so that a wave has a single row of 64 tokens until there are enough for every CU; 4.2 million tokens (89 MB) take 38 and 24
+// us, a sixth of it exponentials.  Terms are formed in float64: a ratio's side of a clipping border decides about its whole
 // gradient, and the KL estimators are differences of nearly equal numbers.
 #include "mx_rows.h"
 
@@ -21,10 +21,11 @@ constexpr int kSeqGrad = 256;          // lanes of a workgroup of the gradient
 constexpr int kSeqFew = 1024;          // lanes of the workgroup that joins alone
 constexpr int kSeqMany = 256;          // lanes of a workgroup where several join
 constexpr int kSeqManyGroups = 1024;   // of which there are at most
-// Tokens from which on a wave takes 8 rows of 64 (us forward, 1 / 8 rows: one sequence of 147 456 20.4 / 16.0, 64 of 600 13.8 / 15.5),
-// and 4 of them in the gradient (us, 1 / 4 rows: packed, 524 672 8.3 / 11.1, 4.2 million 46 / 31).
-constexpr int64_t kSeqLong = 65536, kSeqGradLong = 1 << 20;
-__host__ __device__ __forceinline__ int seq_rows(int64_t tokens) { return tokens < kSeqLong ? 1 : 8; }
+// Tokens from which on a wave takes 4 rows of 64 (us forward, 1 / 4 rows: 64 sequences of 600 13.6 / 12.7, one of 147 456 20.7 / 13.9,
+// 1024 of 4099 46.9 / 37.7; 8 rows 43.0 there, 16 63.6), and in the gradient (us, 1 / 4 rows, packed: 128 sequences of 4099 6.0 / 7.4, 1024 of
+// 4099 30.8 / 24.5).
+constexpr int64_t kSeqLong = 32768, kSeqGradLong = 1 << 20;
+__host__ __device__ __forceinline__ int seq_rows(int64_t tokens) { return tokens < kSeqLong ? 1 : 4; }
 __host__ __device__ __forceinline__ int64_t seq_chunks(int64_t tokens) {
   const int64_t chunk = 64 * seq_rows(tokens);
   return (tokens + chunk - 1) / chunk;
@@ -284,7 +285,7 @@ __device__ __forceinline__ void seq_joined(const Sequences& q, const double* par
 #pragma unroll
   for (int k = 0; k < SUMS; ++k) sum[k] = 0.0;
   const int64_t begin = q.offset(s), end = q.offset(s + 1);
-  const int chunk = seq_rows(q.tokens) == 1 ? 6 : 9;  // (tokens of a chunk, as a power of two)
+  const int chunk = seq_rows(q.tokens) == 1 ? 6 : 8;  // (tokens of a chunk, as a power of two)
   if (end > begin) {
     const int64_t last = (end - 1) >> chunk;
 #pragma unroll 4
@@ -528,7 +529,7 @@ static void seq_loss(const F& f, const Sequences& q, int64_t items, double* part
   const bool alone = items * lanes <= 4 * kSeqFew;
   if (chunks) {
     if (seq_rows(q.tokens) == 1) hipLaunchKernelGGL((seq_parts_kernel<kSums, 1, F>), dim3((unsigned)chunks), dim3(64), 0, st, f, q, parts);
-    else hipLaunchKernelGGL((seq_parts_kernel<kSums, 8, F>), dim3((unsigned)chunks), dim3(64), 0, st, f, q, parts);
+    else hipLaunchKernelGGL((seq_parts_kernel<kSums, 4, F>), dim3((unsigned)chunks), dim3(64), 0, st, f, q, parts);
   }
   if (alone) {
     hipLaunchKernelGGL((seq_join_kernel<kSeqFew, F>), dim3(1), dim3(kSeqFew), 0, st, f, q, items, lanes, (const double*)parts,
