@@ -518,15 +518,16 @@ static int seq_lanes(const Sequences& q) {
   return lanes;
 }
 
-// Two launches, or three where one workgroup would have more than four rounds of sequences to join.  (One workgroup for parts and
-// join of few tokens: 976 of 16 sequences 11.4 us forward, in two launches 10.1.)
+// Two launches, or three where one workgroup would have more than two rounds of sequences to join (four rounds of 512 packed pairs 19 us;
+// by several workgroups and one that finishes 6 and 4).  (One workgroup for parts and join of few tokens: 976 of 16 sequences 11.4 us
+// forward, in two launches 10.1.)
 template <class F>
 static void seq_loss(const F& f, const Sequences& q, int64_t items, double* parts, double* each, float* loss, float* more,
                      hipStream_t st) {
   constexpr int kSums = SeqOf<F>::kSums;
   const int64_t chunks = seq_chunks(q.tokens);
   const int lanes = seq_lanes(q);
-  const bool alone = items * lanes <= 4 * kSeqFew;
+  const bool alone = items * lanes <= 2 * kSeqFew;
   if (chunks) {
     if (seq_rows(q.tokens) == 1) hipLaunchKernelGGL((seq_parts_kernel<kSums, 1, F>), dim3((unsigned)chunks), dim3(64), 0, st, f, q, parts);
     else hipLaunchKernelGGL((seq_parts_kernel<kSums, 4, F>), dim3((unsigned)chunks), dim3(64), 0, st, f, q, parts);
