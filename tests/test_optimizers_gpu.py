@@ -382,3 +382,39 @@ def test_a_compiled_caller(device):
     finally:
         torch._dynamo.reset()
     assert torch.equal(params[0], twins[0]) and a.state[params[0]]["step"] == b.state[twins[0]]["step"] == 3
+
+
+def test_more_values_than_31_bits_count(device):
+    """2^31 and some parameters with 8-bit moments: the last ones are updated and rounded as the first."""
+    n = (1 << 31) + (1 << 13) + 5
+    p = torch.nn.Parameter(torch.ones(n, dtype=torch.bfloat16, device=device))
+    p.grad = torch.zeros(n, dtype=torch.bfloat16, device=device)
+    ends = [slice(0, 4096), slice(n - 4096, n)]
+    for i, at in enumerate(ends):
+        g = torch.Generator(device=device).manual_seed(i)
+        p.grad[at] = (torch.randn(4096, generator=g, device=device) * 1e-2).bfloat16()
+    opt = AdamW([p], **HYPER, weight_decay=0.1, state_bits=8)
+    opt.step()
+    ((m, v),) = opt.moments()
+    assert m.shape == (n,) and not m[4096:8192].any() and not opt.state[p]["exp_avg_sq"][1 << 20].any()
+    for at in ends:
+        zero = torch.zeros(4096, device=device)
+        args = (torch.ones(4096, device=device), p.grad[at], zero, zero, 1, *HYPER.values(), 0.1)
+        want, bounds = step64(*args), step_bounds(*args, half=torch.finfo(torch.bfloat16).eps / 2)
+        assert ((p.detach()[at].double().cpu() - want[0]).abs() <= bounds[0]).all()
+        # a code is off by less than an eighth of the value, or by the smallest code
+        for got, w, least in ((m[at], want[1], 2.0 ** -16), (v[at], want[2], 2.0 ** -32)):
+            assert ((got.double().cpu() - w).abs() <= w.abs() / 8 * 1.0001 + w.abs().max() * least).all()
+
+
+def test_states_that_are_there_but_empty(device):
+    """Asking an optimizer for the state of a parameter without one leaves an empty dict."""
+    params = parameters_of(device, [(40,), (50,)])
+    for capturable in (False, True):
+        opt = AdamW(params, capturable=capturable)
+        assert not opt.state[params[0]] and not opt.state[params[1]]
+        set_gradients(params, 1)
+        params[1].grad = None
+        opt.step()
+        opt.step()
+        assert float(opt.state[params[0]]["step"]) == 2 and not opt.state[params[1]]

@@ -343,3 +343,22 @@ def test_the_launches_are_the_librarys(device):
     loss, _ = policy_loss(case["log_probs"], case["advantages"])
     assert "LossNode" in type(loss.grad_fn).__name__ or "LossNode" in loss.grad_fn.name()
     assert ops.native_rows(case["log_probs"])
+
+
+def test_more_tokens_than_31_bits_count(device):
+    """Two sequences on either side of place 2^31 and one behind it: constant log-ratios, the loss in closed form."""
+    tokens = (1 << 31) + 70001
+    offsets = torch.tensor([5, (1 << 31) - 3, (1 << 31) + 1000, tokens - 7], device=device)
+    lp = torch.full((tokens,), -1.0, dtype=torch.bfloat16, device=device).requires_grad_(True)
+    old = torch.full((tokens,), -1.125, dtype=torch.bfloat16, device=device)
+    advantages = torch.tensor([1.0, -2.0, 3.0], device=device)
+    loss, metrics = policy_loss(lp, advantages, old, offsets=offsets, average="sequence", clip_eps=0.2)
+    r = math.exp(0.125)
+    assert abs(loss.item() + r * 2.0 / 3) <= 1e-6 and abs(metrics[3].item() - r) <= 1e-6
+    (grad,) = torch.autograd.grad(loss, lp)
+    ends = offsets.tolist()
+    for s, A in enumerate(advantages.tolist()):
+        want, n = -A * r / 3, ends[s + 1] - ends[s]
+        for i in (ends[s], ends[s + 1] - 1):
+            assert abs(grad[i].item() * n - want) <= abs(want) * 2.0 ** -8
+    assert not grad[:5].any() and not grad[-7:].any()

@@ -109,7 +109,8 @@ def _kernel_takes(p: torch.Tensor) -> bool:
 
 
 class AdamW(torch.optim.Optimizer):
-    """``torch.optim.AdamW``, whose arguments these are, with moments in `state_bits` bits whatever the parameters' type.
+    """``torch.optim.AdamW`` (without its amsgrad, foreach, fused and differentiable) with moments in `state_bits` bits whatever the
+    parameters' type.
 
         g = f * gradient               (its sign turned with `maximize`)
         m = b1 m + (1 - b1) g          v = b2 v + (1 - b2) g^2
@@ -117,11 +118,12 @@ class AdamW(torch.optim.Optimizer):
 
     in float32, p rounded once to its type.  `master_weights`: parameters narrower than float32 keep a float32 weight in
     their state, which the step updates; the parameter is its rounding (a value that is written into the parameter from outside
-    wants a new state).  ``state_bits=8``: the first moment is held in e4m3, the
-    second in e5m3 without a sign, 32 values in the order of memory with a power of two between them (``exp_avg`` uint8
-    [blocks, 32] and ``exp_avg_scale`` [blocks]; likewise ``exp_avg_sq``), rounded up or down by chance so that
-    their mean is the exact one; `seed` decides about that chance, the same seed gives the same bits.  A block whose gradients
-    hold an infinity or a NaN becomes NaN.  Such parameters must be contiguous.
+    wants a new state).
+
+    ``state_bits=8``: the first moment is held in e4m3, the second in e5m3 without a sign, 32 values in the order of memory with a
+    power of two between them (``exp_avg`` uint8 [blocks, 32] and ``exp_avg_scale`` [blocks]; likewise ``exp_avg_sq``), rounded
+    up or down by chance so that their mean is the exact one; `seed` decides about that chance, the same seed gives the same
+    bits.  A block whose gradients hold an infinity or a NaN becomes NaN.  Such parameters must be contiguous.
 
     ``step(total_norm=..., max_norm=...)`` scales the gradients by min(1, max_norm / (total_norm + 1e-6)) as they are read:
     ``clip_grads_with_norm_`` without its pass over memory (the gradients stay as they are, and of bf16 ones no scaled rounding).
@@ -234,21 +236,20 @@ class AdamW(torch.optim.Optimizer):
         if device is None:
             raise RuntimeError("AdamW: capturable wants parameters on a GPU")
         steps, corrections = self._counters.get(index) or (None, None)
-        here = [self.state[p]["step"] for p in group["params"] if p in self.state]
-        places = [first + i for i, p in enumerate(group["params"]) if p in self.state]
-        if steps is None or any(not isinstance(s, torch.Tensor) or s.data_ptr() != steps.data_ptr() + 4 * i
-                                for s, i in zip(here, places)):
-            if device.type == "cuda" and _capture(torch.empty(0, device=device)):
+        here = [(first + i, self.state[p]) for i, p in enumerate(group["params"]) if self.state.get(p)]
+        if steps is None or any(not isinstance(s["step"], torch.Tensor) or s["step"].data_ptr() != steps.data_ptr() + 4 * i
+                                for i, s in here):
+            if _capture(torch.empty(0, device=device)):
                 raise RuntimeError("AdamW: step counters are laid out by a step outside of a capture")
-            values = [float(s) for s in here]
+            values = [float(s["step"]) for _, s in here]
             if steps is None or steps.device != device:
                 size = first + len(group["params"])
                 steps = torch.zeros(size, dtype=torch.float32, device=device)
                 corrections = torch.zeros((size, 4), dtype=torch.float32, device=device)
                 self._counters[index] = (steps, corrections)
-            for value, i, p in zip(values, places, (p for p in group["params"] if p in self.state)):
+            for value, (i, state) in zip(values, here):
                 steps[i] = value
-                self.state[p]["step"] = steps[i]
+                state["step"] = steps[i]
         return steps, corrections
 
     # -------------------------------------------------------------------------------- step
