@@ -418,3 +418,24 @@ def test_states_that_are_there_but_empty(device):
         opt.step()
         opt.step()
         assert float(opt.state[params[0]]["step"]) == 2 and not opt.state[params[1]]
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("eps,std", [(1e-8, 1e-18), (1e-12, 1e-14), (1e-15, 1e-18), (0.0, 1e-15), (1e-8, 1e6)])
+def test_tiny_and_large_gradients_with_any_eps(device, bits, eps, std):
+    """First steps from gradients whose squares are near float32's smallest numbers, or beyond 1e12; whole chunks and a ragged end."""
+    for dtype in (torch.bfloat16, torch.float32):
+        p = torch.nn.Parameter(torch.zeros(2 * 2048 * 4 + 1000, device=device, dtype=dtype))
+        g = torch.randn(p.shape, generator=torch.Generator(device=device).manual_seed(1), device=device)
+        p.grad = ((g + g.sign()) * std).to(dtype)
+        opt = AdamW([p], lr=1e-2, betas=(0.9, 0.95), eps=eps, weight_decay=0.0, state_bits=bits)
+        opt.step()
+        zero = torch.zeros_like(p)
+        args = (zero, p.grad, zero, zero, 1, 1e-2, (0.9, 0.95), eps, 0.0)
+        want, bounds = step64(*args), step_bounds(*args, half=torch.finfo(dtype).eps / 2)
+        # a second moment below 2^-126 is held to 2^-150 of its square's roundings; the root of 3 * 2^-150 where it stands over eps
+        lost = 3 * 2.0 ** -150
+        v = want[2]
+        root = (v / 0.05).sqrt()
+        moved = 1e-2 * (0.1 * p.grad.double().cpu().abs() / 0.1) * (lost / 0.05 / (2 * root.clamp(min=1e-30))) / (root + eps).clamp(min=1e-30) ** 2
+        assert ((p.detach().double().cpu() - want[0]).abs() <= bounds[0] + moved).all()
