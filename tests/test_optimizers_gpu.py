@@ -189,6 +189,25 @@ def test_a_large_tensor_and_groups_with_their_own_numbers(device):
     check_steps(a, params, steps=1, decay=1e-2)
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("master", [False, True])
+def test_odd_sizes_in_a_list_of_more_than_a_million_values(device, bits, master):
+    """Longer lists have larger chunks: the ends of small tensors inside them."""
+    params = parameters_of(device, [*SHAPES, (1200, 1001), (4095,), (4096,), (8191,), (2047, 3)])
+    check_steps(AdamW(params, **HYPER, weight_decay=0.1, state_bits=bits, master_weights=master, seed=3), params, steps=2)
+    if bits == 8 and master:
+        # the same list beside nothing: the same bits in smaller chunks
+        some = parameters_of(device, [(8191,)], (torch.float32,), seed=5)
+        twins = [torch.nn.Parameter(p.detach().clone()) for p in some] + parameters_of(device, [(1200, 1001)], seed=6)
+        a, b = AdamW(some, state_bits=8), AdamW(twins, state_bits=8)
+        set_gradients(some, 1)
+        set_gradients(twins, 1)
+        a.step()
+        b.step()
+        assert torch.equal(a.state[some[0]]["exp_avg"], b.state[twins[0]]["exp_avg"])
+        assert torch.equal(a.state[some[0]]["exp_avg_sq"], b.state[twins[0]]["exp_avg_sq"])
+
+
 def test_converted_weights_are_updated_and_their_versions_counted(device):
     plain = parameters_of(device, [(64, 96)], (torch.bfloat16,))[0]
     twin = torch.nn.Parameter(plain.detach().clone())

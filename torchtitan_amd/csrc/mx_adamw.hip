@@ -33,7 +33,9 @@ constexpr int kAdamTensors = 44;  // of one launch
 constexpr int kAdamPieces = 4;
 constexpr int64_t kAdamFew = 1 << 20;
 constexpr int kAdamValues = 4;  // values a piece: 16 bytes of float32
-constexpr int kAdam8Values = 8;  // values a lane and chunk of a parameter with moments in 8 bits
+// With moments in 8 bits, values a lane and chunk: 16, or 8 for such lists (us with 8 and 16: 673 million bf16 1265 and 1198, float32 2102
+// and 2051, 50 million 94 and 95).
+constexpr int kAdam8Few = 8, kAdam8Values = 16;
 
 struct AdamEntry {
   void* p;
@@ -235,10 +237,10 @@ __device__ __forceinline__ void adam_decode_first(uint32_t codes, float* x) {
 
 // V values a piece: 8 of a bf16 parameter, 4 of a float32 one, so that either is 16 bytes (float32, 8 / 4: 50 million 167 / 138 us,
 // 673 million 2.06 / 2.12 ms).
-template <bool ALL, bool ROUGH, int V, class T>
+template <bool ALL, bool ROUGH, int VALUES, int V, class T>
 __device__ __forceinline__ void adam8_chunk(const AdamEntry& e, const AdamHyper& h, float f, float step, float root, float decay,
                                             uint32_t key, int64_t at) {
-  constexpr int kPieces = kAdam8Values / V, kWords = V / 4;
+  constexpr int kPieces = VALUES / V, kWords = V / 4;
   typedef uint32_t Codes __attribute__((ext_vector_type(kWords)));
   const T* g = (const T*)e.g;
   T* p = (T*)e.p;
@@ -247,21 +249,30 @@ __device__ __forceinline__ void adam8_chunk(const AdamEntry& e, const AdamHyper&
   float qg[kPieces][V], qw[kPieces][V];
   Codes cm[kPieces], cv[kPieces];
   int sm[kPieces], sv[kPieces];
+  auto pieces = [&](auto&& piece) {
 #pragma unroll
-  for (int k = 0; k < kPieces; ++k) {
-    const int64_t i = at + (k * kAdamThreads + threadIdx.x) * V, left = e.elems - i;
-    adam_load<ALL>(g + i, left, qg[k]);
-    if (e.master) adam_load<ALL>(e.master + i, left, qw[k]);
-    else adam_load<ALL>((const T*)p + i, left, qw[k]);
-    cm[k] = cv[k] = Codes(0);
-    sm[k] = sv[k] = 0;
-    if (ALL || i < whole) {
-      cm[k] = __builtin_nontemporal_load(reinterpret_cast<const Codes*>(m + i));
-      cv[k] = __builtin_nontemporal_load(reinterpret_cast<const Codes*>(v + i));
-      sm[k] = e.ms[i >> 5];
-      sv[k] = e.vs[i >> 5];
+    for (int k = 0; k < kPieces; ++k) {
+      const int64_t i = at + (k * kAdamThreads + threadIdx.x) * V;
+      piece(k, i, e.elems - i);
     }
-  }
+  };
+  auto codes = [&](Codes(&c)[kPieces], const uint8_t* from) {
+    pieces([&](int k, int64_t i, int64_t) {
+      c[k] = Codes(0);
+      if (ALL || i < whole) c[k] = __builtin_nontemporal_load(reinterpret_cast<const Codes*>(from + i));
+    });
+  };
+  auto scales = [&](int(&s)[kPieces], const uint8_t* from) {
+    pieces([&](int k, int64_t i, int64_t) { s[k] = ALL || i < whole ? from[i >> 5] : 0; });
+  };
+  // one array after the other
+  pieces([&](int k, int64_t i, int64_t left) { adam_load<ALL>(g + i, left, qg[k]); });
+  if (e.master) pieces([&](int k, int64_t i, int64_t left) { adam_load<ALL>(e.master + i, left, qw[k]); });
+  else pieces([&](int k, int64_t i, int64_t left) { adam_load<ALL>((const T*)p + i, left, qw[k]); });
+  codes(cm, m);
+  codes(cv, v);
+  scales(sm, e.ms);
+  scales(sv, e.vs);
 #pragma unroll
   for (int k = 0; k < kPieces; ++k) {
     const int64_t i = at + (k * kAdamThreads + threadIdx.x) * V, left = e.elems - i;
@@ -318,6 +329,7 @@ __device__ __forceinline__ void adam8_chunk(const AdamEntry& e, const AdamHyper&
   }
 }
 
+// PIECES a lane and chunk; with moments in 8 bits values.
 template <bool EIGHT, int PIECES>
 __global__ __launch_bounds__(kAdamThreads) void adamw_kernel(AdamTable table, int n, AdamHyper h) {
   const uint32_t chunk = blockIdx.x;
@@ -329,18 +341,18 @@ __global__ __launch_bounds__(kAdamThreads) void adamw_kernel(AdamTable table, in
     step = c.x, root = c.y, decay = c.z, key = __float_as_uint(c.w);
   }
   const float f = adam_factor(h);
-  constexpr int kValues = kAdamThreads * (EIGHT ? kAdam8Values : PIECES * kAdamValues);
+  constexpr int kValues = kAdamThreads * PIECES * (EIGHT ? 1 : kAdamValues);
   const int64_t at = (int64_t)(chunk - e.first) * kValues;
   const bool all = e.elems - at >= kValues;
   auto types = [&](auto whole) {
     constexpr bool ALL = decltype(whole)::value;
     if constexpr (EIGHT) {
       if (!ALL || h.eps < 1e-9f) {
-        if (e.f32) adam8_chunk<ALL, false, 4, float>(e, h, f, step, root, decay, key, at);
-        else adam8_chunk<ALL, false, 8, uint16_t>(e, h, f, step, root, decay, key, at);
+        if (e.f32) adam8_chunk<ALL, false, PIECES, 4, float>(e, h, f, step, root, decay, key, at);
+        else adam8_chunk<ALL, false, PIECES, 8, uint16_t>(e, h, f, step, root, decay, key, at);
       } else {
-        if (e.f32) adam8_chunk<ALL, true, 4, float>(e, h, f, step, root, decay, key, at);
-        else adam8_chunk<ALL, true, 8, uint16_t>(e, h, f, step, root, decay, key, at);
+        if (e.f32) adam8_chunk<ALL, true, PIECES, 4, float>(e, h, f, step, root, decay, key, at);
+        else adam8_chunk<ALL, true, PIECES, 8, uint16_t>(e, h, f, step, root, decay, key, at);
       }
     } else {
       if (e.f32) adam_chunk<ALL, PIECES, float>(e, h, f, step, root, decay, at);
@@ -455,7 +467,7 @@ extern "C" int mx_adamw(int64_t n, const int64_t* table, int eight, double lr, d
     values = values > kAdamFew ? values : values + elems;
   }
   const bool few = values <= kAdamFew;
-  const int64_t per = kAdamThreads * (eight ? kAdam8Values : (few ? 1 : kAdamPieces) * kAdamValues);
+  const int64_t per = kAdamThreads * (eight ? (few ? kAdam8Few : kAdam8Values) : (few ? 1 : kAdamPieces) * kAdamValues);
   hipStream_t st = (hipStream_t)stream;
   AdamHyper h = {(float)beta1, (float)(1.0 - beta1), (float)beta2, (float)(1.0 - beta2), (float)eps,
                  (float)(1.0 - lr * weight_decay), maximize ? -1.f : 1.f, limit, norm, (const float4*)corrections};
@@ -471,7 +483,8 @@ extern "C" int mx_adamw(int64_t n, const int64_t* table, int eight, double lr, d
                          weight_decay, seed, (float4*)corrections);
     if (chunks) {
       const dim3 grid((unsigned)chunks), block(kAdamThreads);
-      if (eight) hipLaunchKernelGGL((adamw_kernel<true, 1>), grid, block, 0, st, args, used, h);
+      if (eight && few) hipLaunchKernelGGL((adamw_kernel<true, kAdam8Few>), grid, block, 0, st, args, used, h);
+      else if (eight) hipLaunchKernelGGL((adamw_kernel<true, kAdam8Values>), grid, block, 0, st, args, used, h);
       else if (few) hipLaunchKernelGGL((adamw_kernel<false, 1>), grid, block, 0, st, args, used, h);
       else hipLaunchKernelGGL((adamw_kernel<false, kAdamPieces>), grid, block, 0, st, args, used, h);
     }
