@@ -1,7 +1,7 @@
 // The launches of a converted linear, of the SwiGLU block and of the routed experts, forward and backward, from one
 // native call each; and the single launches around them (gate, routing, log-probabilities, lists of casts), likewise.
-// The embedding and the norms around a block come with their autograd nodes: their launches take 5 us at small sizes, an
-// autograd function in Python around them 60 forward and backward.
+// The embedding, the norms around a block and the losses over sequences come with their autograd nodes: their launches take 5 us at
+// small sizes, an autograd function in Python around them 60 forward and backward.  An AdamW step reads its parameters' states here.
 //
 // On inputs of up to a few thousand tokens these blocks wait for their host side: between two launches
 // (3.3 us each) Python made operands, asked tensors for their pointers and strides and passed them on, 4 to 8 us
