@@ -415,7 +415,7 @@ int mx_grad_scale(int64_t n, void* const* grads, const int64_t* elems, const int
  *
  * mx_policy_loss: r = exp(log_probs - old) of a token, or with ratio_per_sequence exp(mean of that) of a sequence (old NULL: r = 1,
  * whose gradient is that of old = log_probs); A: advantages float32, of every sequence or with advantage_per_token of every token.
- *     objective = -min(r A, clip(r, ratio_low, ratio_high) A)         loss = pg + kl_coef KL - entropy_coef entropy
+ *     objective = -min(r A, clip(r, ratio_low, ratio_high) A)         loss = pg + kl_coef KL - entropy_coef entropy   (0: left out)
  * pg and KL: means over all tokens, or with mean_per_sequence over sequences of the means over their tokens, of the objective and of the
  * estimator at x = log_probs - ref (ref NULL: 0): kl 0 x, 1 x^2 / 2, 2 exp(-x) - 1 + x, 3 exp(x) - 1 - x; entropy: minus the mean of
  * log_probs over all tokens.  metrics [5]: pg, KL, entropy, mean of the ratios, share of them that clip() changes by more than 1e-6

@@ -95,6 +95,21 @@ def test_the_reference_loss_is_a_case_of_it():
     assert torch.allclose(a, b, rtol=1e-5, atol=1e-7)
 
 
+def overflowing_terms(device):
+    """A KL term and an entropy that are infinite, with coefficients of 0 and without."""
+    lp = torch.tensor([[0.0, -1.0, -math.inf]], device=device, requires_grad=True)
+    ref = torch.tensor([[-800.0, -1.0, -math.inf]], device=device)
+    loss, metrics = policy_loss(lp, torch.ones(1, device=device), None, ref, mask=torch.tensor([[True, True, False]], device=device),
+                                kl="k3_swapped")
+    assert loss.item() == -1.0 and math.isinf(metrics[1].item())
+    assert torch.equal(torch.autograd.grad(loss, lp)[0], torch.tensor([[-0.5, -0.5, 0.0]], device=device))
+    assert math.isinf(policy_loss(lp[:, :2], torch.ones(1, device=device), None, ref[:, :2], kl="k3_swapped", kl_coef=0.1)[0].item())
+
+
+def test_terms_without_a_coefficient_are_left_out():
+    overflowing_terms("cpu")
+
+
 def test_refusals():
     lp = torch.zeros(4, 5)
     A = torch.zeros(4)

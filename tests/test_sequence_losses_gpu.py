@@ -5,6 +5,7 @@ import pytest
 import torch
 
 from tests.sequence_losses import check_policy, check_preference, tokens_of
+from tests.test_sequence_losses_cpu import overflowing_terms
 from torchtitan_amd import ops
 from torchtitan_amd.gradients import get_total_norm
 from torchtitan_amd.optimizers import AdamW
@@ -249,6 +250,30 @@ def test_the_sample_loss_runs_through_it(device):
     apart.backward()
     # bf16 gradients of bf16 products: two of their roundings apart at most, summed over the samples in float32
     assert float((first.float() - model.out.weight.grad.float()).norm()) <= 2.0 ** -7 * float(first.float().norm())
+
+
+def test_terms_without_a_coefficient_are_left_out(device):
+    overflowing_terms(device)
+
+
+def test_the_sample_loss_takes_what_it_took(device):
+    """Fewer prompts than answers, a negative clipping width and coefficients that are tensors go through torch operations or
+    the same tokens, as ever."""
+    torch.manual_seed(5)
+    model = _TwoLayers().to(device).bfloat16()
+    rng = torch.Generator().manual_seed(1)
+    ids = lambda n: torch.randint(0, 1000, (n,), generator=rng).tolist()
+    prompts, answers = [ids(n) for n in (5, 9)], [ids(n) for n in (12, 30)]
+    ref = [torch.full((len(a),), -7.0, device=device) for a in answers]
+    A = torch.tensor([0.5, -0.2])
+    want = compute_policy_gradient_loss(model, answers, prompts, A, ref)[0].item()
+    more = compute_policy_gradient_loss(model, answers + [ids(4)], prompts, A, ref)[0].item()
+    assert more == want
+    assert math.isfinite(compute_policy_gradient_loss(model, answers, prompts, A, ref, ppo_clip_eps=-0.1)[0].item())
+    coefficient = torch.tensor(0.1, device=device, requires_grad=True)
+    total, metrics, _ = compute_policy_gradient_loss(model, answers, prompts, A, ref, kl_coef=coefficient)
+    (g,) = torch.autograd.grad(total, coefficient)
+    assert abs(g.item() - metrics["kl_div"]) <= 1e-6 * abs(metrics["kl_div"]) and abs(total.item() - want) <= 1e-4
 
 
 def test_a_training_step_from_logits_to_weights(device):

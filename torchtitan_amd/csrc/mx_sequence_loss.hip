@@ -348,7 +348,8 @@ __device__ __forceinline__ void seq_finish(const Policy& f, const Sequences& q, 
   const double tokens = total[0] > 0 ? total[0] : 1.0, filled = total[1] > 0 ? total[1] : 1.0;
   const double pg = f.by_sequence ? total[6] / filled : total[2] / tokens, kl = f.by_sequence ? total[7] / filled : total[3] / tokens;
   const double entropy = -total[10] / tokens;
-  *loss = (float)(pg + f.kl_coef * kl - f.entropy_coef * entropy);
+  // (a coefficient of 0 leaves out a term that is no number, too)
+  *loss = (float)(pg + (f.kl_coef != 0 ? f.kl_coef * kl : 0.0) - (f.entropy_coef != 0 ? f.entropy_coef * entropy : 0.0));
   metrics[0] = (float)pg;
   metrics[1] = (float)kl;
   metrics[2] = (float)entropy;

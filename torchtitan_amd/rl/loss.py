@@ -67,8 +67,9 @@ def compute_policy_gradient_loss(model: torch.nn.Module, vllm_token_ids: list[li
     device = next(model.parameters()).device
     advantages = advantages.to(device)
     batch_lps = [compute_token_log_probs(model, p, g, device) for p, g in zip(prompt_token_ids, vllm_token_ids)]
-    if _one_launch(batch_lps, ref_token_log_probs, advantages):
-        offsets = torch.tensor([0, *(len(g) for g in vllm_token_ids)], dtype=torch.int64).cumsum(0).to(device)
+    numbers = (kl_coef, ppo_clip_eps, entropy_coef)
+    if all(isinstance(x, (int, float)) for x in numbers) and ppo_clip_eps >= 0 and _one_launch(batch_lps, ref_token_log_probs, advantages):
+        offsets = torch.tensor([0, *(lps.numel() for lps in batch_lps)], dtype=torch.int64).cumsum(0).to(device)
         ref = torch.cat(list(ref_token_log_probs))
         total, values = policy_loss(torch.cat(batch_lps), advantages, ref, ref, offsets=offsets, clip_eps=ppo_clip_eps,
                                     kl_coef=kl_coef, kl="k3_swapped", entropy_coef=entropy_coef, ratio="sequence",
@@ -255,7 +256,7 @@ def _policy_in_torch_ops(log_probs, advantages, old, ref, offsets, mask, sequenc
     if ref is not None:
         kl_div = mean(_kl_term(lp - flat(ref), kl), each)
     entropy = -lp.sum() / tokens
-    total = pg + kl_coef * kl_div - entropy_coef * entropy
+    total = pg + (kl_coef * kl_div if kl_coef else 0.0) - (entropy_coef * entropy if entropy_coef else 0.0)
     with torch.no_grad():
         per = (1 / (filled * per_sequence))[sequence] if whole else (1 / tokens).expand_as(lp)
         clipped = ((ratio - ratio.clamp(low, high)).abs() > 1e-6).double()
@@ -279,7 +280,7 @@ def policy_loss(log_probs: torch.Tensor, advantages: torch.Tensor, old_log_probs
     every mean.  advantages: [sequences], or of every token (ratio="token").  Without `old_log_probs` the policy has not moved: r is
     1, with its gradient.  kl, at x = log_probs - ref_log_probs: "k1" x, "k2" x^2 / 2, "k3" exp(-x) - 1 + x, "k3_swapped" exp(x) - 1 - x.
     The entropy is minus the mean of log_probs.  average: means of pg and KL over all tokens, or over sequences of the means
-    over their tokens.  Only log_probs gets a gradient, which on the GPU cannot be differentiated again; terms and sums
+    over their tokens.  A coefficient of 0 leaves its term out of the loss, whatever it is.  Only log_probs gets a gradient, which on the GPU cannot be differentiated again; terms and sums
     are in float64."""
     if ratio not in ("token", "sequence") or average not in ("token", "sequence"):
         raise ValueError(f"ratio and average must be 'token' or 'sequence', got {ratio!r} and {average!r}")
