@@ -181,24 +181,38 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict) -> None:
         """As torch's, but moments keep their own types, and `state_bits`, `master_weights` and `capturable` stay this
-        optimizer's: a state that ``torch.optim.AdamW`` or this optimizer with others of them has saved is converted."""
+        optimizer's: a state that ``torch.optim.AdamW`` or this optimizer with others of them has saved is converted.  Hooks in front of
+        the loading give the state that is converted, those behind it see the converted one."""
         held = [{key: group[key] for key in ("state_bits", "master_weights", "capturable")} for group in self.param_groups]
-        super().load_state_dict(state_dict)
-        self._counters = {}
-        for group, own in zip(self.param_groups, held):
-            group.update(own)
-            for key, value in self.defaults.items():
-                group.setdefault(key, value)
-        saved_ids = [i for group in state_dict["param_groups"] for i in group["params"]]
-        number = -1
-        for group in self.param_groups:
-            for p in group["params"]:
-                number += 1
-                saved = state_dict["state"].get(saved_ids[number])
-                if not saved:
-                    self.state.pop(p, None)
-                    continue
-                self._load_one(p, group, saved, number)
+        saved, ids = {}, []
+
+        def take(_, hooked):
+            # (torch would round the moments to their parameters' types)
+            ids.extend(i for group in hooked["param_groups"] for i in group["params"])
+            parameters = set(ids)
+            saved.update(hooked["state"])
+            return {**hooked, "state": {i: one for i, one in saved.items() if i not in parameters}}
+
+        def convert(_):
+            self._counters = {}
+            for group, own in zip(self.param_groups, held):
+                group.update(own)
+                for key, value in self.defaults.items():
+                    group.setdefault(key, value)
+            number = -1
+            for group in self.param_groups:
+                for p in group["params"]:
+                    number += 1
+                    if saved.get(ids[number]):
+                        self._load_one(p, group, saved[ids[number]], number)
+
+        # behind the caller's hooks in front of it, before those behind it
+        own_hooks = (self.register_load_state_dict_pre_hook(take), self.register_load_state_dict_post_hook(convert, prepend=True))
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            for hook in own_hooks:
+                hook.remove()
 
     @torch.no_grad()
     def _load_one(self, p, group, saved, number: int) -> None:
