@@ -1,0 +1,32 @@
+"""CPU: the groups that AdamW takes."""
+import pytest
+import torch
+
+from torchtitan_amd.optimizers import AdamW
+
+
+@pytest.mark.parametrize("bad", [dict(lr=-1.0), dict(betas=(1.0, 0.9)), dict(eps=-1e-8), dict(weight_decay=-0.1), dict(state_bits=16),
+                                 dict(seed=-1), dict(seed=1 << 64), dict(lr=torch.ones(2))])
+def test_a_groups_own_numbers_are_checked(bad):
+    """As the constructor's are: when it is made and when a group is added; a refused group is not there."""
+    p, q = torch.nn.Parameter(torch.ones(4)), torch.nn.Parameter(torch.ones(4))
+    with pytest.raises(ValueError):
+        AdamW([dict(params=[p], **bad)])
+    opt = AdamW([p])
+    with pytest.raises(ValueError):
+        opt.add_param_group(dict(params=[q], **bad))
+    assert len(opt.param_groups) == 1
+    opt.add_param_group(dict(params=[q], state_bits=8, lr=0.5))
+    for t in (p, q):
+        t.grad = torch.ones(4)
+    opt.step()
+    assert opt.state[p]["exp_avg"].dtype == torch.float32 and opt.state[q]["exp_avg"].dtype == torch.uint8
+    # (first steps: the learning rate, but for eps, and the decay)
+    assert torch.allclose(p.detach(), torch.full((4,), 1 - 1e-3 - 1e-5)) and torch.allclose(q.detach(), torch.full((4,), 0.5 - 0.005))
+
+
+def test_numbers_without_a_group_of_them():
+    """What every group says for itself need not be right in the defaults, which torch's optimizers check all the same."""
+    p = torch.nn.Parameter(torch.ones(4))
+    with pytest.raises(ValueError):
+        AdamW([dict(params=[p], lr=1e-3)], lr=-1.0)

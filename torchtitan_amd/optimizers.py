@@ -108,6 +108,22 @@ def _kernel_takes(p: torch.Tensor) -> bool:
             and ops.is_dense(p))
 
 
+def _check_numbers(group) -> None:
+    lr, betas, eps, weight_decay = (group[name] for name in ("lr", "betas", "eps", "weight_decay"))
+    if isinstance(lr, torch.Tensor) and lr.numel() != 1:
+        raise ValueError("a tensor lr must have one element")
+    if not float(lr) >= 0:
+        raise ValueError(f"lr must not be negative, got {lr}")
+    if not all(0 <= b < 1 for b in betas):
+        raise ValueError(f"betas must be in [0, 1), got {betas}")
+    if not eps >= 0 or not weight_decay >= 0:
+        raise ValueError(f"eps and weight_decay must not be negative, got {eps} and {weight_decay}")
+    if group["state_bits"] not in _MOMENTS:
+        raise ValueError(f"state_bits must be 32 or 8, got {group['state_bits']}")
+    if not 0 <= group["seed"] < 1 << 64:
+        raise ValueError("seed must fit 64 bits without a sign")
+
+
 class AdamW(torch.optim.Optimizer):
     """``torch.optim.AdamW`` (without its amsgrad, foreach, fused and differentiable) with moments in `state_bits` bits whatever the
     parameters' type.
@@ -134,21 +150,19 @@ class AdamW(torch.optim.Optimizer):
     def __init__(self, params, lr: float | torch.Tensor = 1e-3, betas: tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
                  weight_decay: float = 1e-2, *, state_bits: int = 32, master_weights: bool = False, maximize: bool = False,
                  capturable: bool = False, seed: int = 0):
-        if isinstance(lr, torch.Tensor) and lr.numel() != 1:
-            raise ValueError("a tensor lr must have one element")
-        if not float(lr) >= 0:
-            raise ValueError(f"lr must not be negative, got {lr}")
-        if not all(0 <= b < 1 for b in betas):
-            raise ValueError(f"betas must be in [0, 1), got {betas}")
-        if not eps >= 0 or not weight_decay >= 0:
-            raise ValueError(f"eps and weight_decay must not be negative, got {eps} and {weight_decay}")
-        if state_bits not in _MOMENTS:
-            raise ValueError(f"state_bits must be 32 or 8, got {state_bits}")
-        if not 0 <= seed < 1 << 64:
-            raise ValueError("seed must fit 64 bits without a sign")
         self._counters = {}  # group -> (float32 step counters by the parameters' numbers, what follows from them)
-        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay, state_bits=state_bits,
-                                      master_weights=master_weights, maximize=maximize, capturable=capturable, seed=seed))
+        defaults = dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay, state_bits=state_bits,
+                        master_weights=master_weights, maximize=maximize, capturable=capturable, seed=seed)
+        _check_numbers(defaults)
+        super().__init__(params, defaults)
+
+    def add_param_group(self, param_group) -> None:
+        super().add_param_group(param_group)
+        try:
+            _check_numbers(self.param_groups[-1])
+        except Exception:
+            self.param_groups.pop()
+            raise
 
     def __setstate__(self, state):
         super().__setstate__(state)
