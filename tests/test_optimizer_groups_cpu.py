@@ -30,3 +30,17 @@ def test_numbers_without_a_group_of_them():
     p = torch.nn.Parameter(torch.ones(4))
     with pytest.raises(ValueError):
         AdamW([dict(params=[p], lr=1e-3)], lr=-1.0)
+
+
+@pytest.mark.filterwarnings("ignore:optimizer contains")
+def test_a_parameter_is_in_a_group_once():
+    """Listed twice it would be one state that two entries of a launch update, with one step's correction for both."""
+    p, q = torch.nn.Parameter(torch.ones(4)), torch.nn.Parameter(torch.ones(4))
+    with pytest.raises(ValueError, match="twice"):
+        AdamW([p, q, p])
+    opt = AdamW([p])
+    with pytest.raises(ValueError, match="twice"):
+        opt.add_param_group(dict(params=[q, q]))
+    with pytest.raises(ValueError, match="more than one"):
+        opt.add_param_group(dict(params=[p]))
+    assert len(opt.param_groups) == 1

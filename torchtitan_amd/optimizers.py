@@ -159,7 +159,10 @@ class AdamW(torch.optim.Optimizer):
     def add_param_group(self, param_group) -> None:
         super().add_param_group(param_group)
         try:
-            _check_numbers(self.param_groups[-1])
+            group = self.param_groups[-1]
+            _check_numbers(group)
+            if len(set(group["params"])) != len(group["params"]):
+                raise ValueError("a parameter is listed twice")
         except Exception:
             self.param_groups.pop()
             raise
