@@ -455,7 +455,7 @@ int mx_preference_loss(const mx_preference_loss_t* args, float* loss, float* rew
 int mx_preference_loss_bwd(const mx_preference_loss_t* args, const double* each, const float* dloss, void* grad, void* stream);
 
 /* The AdamW step over n parameters (the optimizer behind torchtitan/components/optimizer.py).  table (host memory): n
- * times MX_ADAMW_FIELDS numbers -- parameter, whether it and its gradient are float32 (else bf16), gradient, first moment, second
+ * times MX_ADAMW_FIELDS numbers -- parameter, its and its gradient's type (0 bf16, 1 float32, 2 bf16 and float32), gradient, first moment, second
  * moment, their scales (8 bits only), float32 master weight (or 0), number of values, step that this one is (from 1), the
  * parameter's number.  In float32 for every value, each tensor one run of memory:
  *     g = f gradient (- with maximize);  m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2

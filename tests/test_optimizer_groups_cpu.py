@@ -44,3 +44,20 @@ def test_a_parameter_is_in_a_group_once():
     with pytest.raises(ValueError, match="more than one"):
         opt.add_param_group(dict(params=[p]))
     assert len(opt.param_groups) == 1
+
+
+def test_types_of_a_table():
+    """Of parameter and gradient: what is none of the three, and a float32 gradient at half of an element, is refused in front of any launch."""
+    import ctypes
+
+    from torchtitan_amd import _lib
+
+    lib = _lib.load()
+
+    def adamw(types, gradient=0x2000, parameter=0x1000):
+        row = [parameter, types, gradient, 0x3000, 0x4000, 0, 0, 0, 10, 1, 0]
+        table = (ctypes.c_int64 * len(row))(*row)
+        return lib.mx_adamw(1, ctypes.cast(table, ctypes.c_void_p), 0, 1e-3, 0.9, 0.95, 1e-8, 0.0, 0, None, 0.0, 0, None, None, None, None)
+
+    assert adamw(3) == 1 and adamw(-1) == 1
+    assert adamw(2, gradient=0x2002) == 2 and adamw(2, parameter=0x1001) == 2 and adamw(1, parameter=0x1002) == 2

@@ -1267,7 +1267,7 @@ bool adamw(const py::list& parameters, const py::list& states, int64_t first, bo
     one.g = one.p.grad();
     if (!one.g.defined()) continue;
     const Tensor &p = one.p, &g = one.g;
-    if (!row_tensor(p) || !row_tensor(g) || !no_subclass(g) || g.scalar_type() != p.scalar_type() || g.sizes() != p.sizes() ||
+    if (!row_tensor(p) || !row_tensor(g) || !no_subclass(g) || (is_f32(p) && !is_f32(g)) || g.sizes() != p.sizes() ||
         !p.is_non_overlapping_and_dense() || !same_order(g, p) || p.device() != (all.empty() ? p : all[0].p).device() ||
         g.device() != p.device())
       return false;
@@ -1302,7 +1302,7 @@ bool adamw(const py::list& parameters, const py::list& states, int64_t first, bo
     }
     const auto& [m, v, ms, vs, master] = one.state;
     auto at = [](const Tensor& t) { return reinterpret_cast<int64_t>(pointer(t)); };
-    for (const int64_t field : {at(p), int64_t{is_f32(p)}, at(g), at(m), at(v), at(ms), at(vs), at(master), p.numel(),
+    for (const int64_t field : {at(p), int64_t{is_f32(p) ? 1 : 2 * is_f32(g)}, at(g), at(m), at(v), at(ms), at(vs), at(master), p.numel(),
                                 one.step + 1, first + static_cast<int64_t>(i)})
       table.push_back(field);
     all.push_back(std::move(one));

@@ -5,8 +5,8 @@
 //   w = (1 - lr decay) w - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
 //
 // Bound by memory: everything is read once and written once, 28 bytes a float32 parameter, 22 a bf16 one, 28 with a float32
-// master weight beside it.  In 8 bits the moments' 16 of these are 4.1.  A table of tensors travels as a kernel argument;
-// a tensor is cut into chunks of one workgroup each.
+// master weight beside it (2 more with float32 gradients of bf16 parameters).  In 8 bits the moments' 16 of these are 4.1.  A table
+// of tensors travels as a kernel argument; a tensor is cut into chunks of one workgroup each.
 //
 // Moments in 8 bits: blocks of 32 in the order of memory, a power of two for each (a byte b: 2^(b - 127), 255: the block is
 // NaN), chosen as the smallest with which the block's largest value is no more than the largest code.
@@ -47,7 +47,7 @@ struct AdamEntry {
   uint32_t first;      // first chunk of this tensor
   uint32_t key;        // of its random bits; its number where the corrections are on the device
   float step, root;    // lr / (1 - b1^t), 1 / sqrt(1 - b2^t)
-  uint32_t f32;
+  uint32_t types;      // of parameter and gradient: 0 bf16, 1 float32, 2 bf16 and float32
 };
 struct AdamTable {
   AdamEntry e[kAdamTensors];
@@ -160,11 +160,12 @@ __device__ __forceinline__ void adam_update(const AdamHyper& h, float f, float s
   }
 }
 
-template <bool ALL, int PIECES, class T>
+// T: the parameter's values, G: its gradient's
+template <bool ALL, int PIECES, class T, class G>
 __device__ __forceinline__ void adam_chunk(const AdamEntry& e, const AdamHyper& h, float f, float step, float root, float decay,
                                            int64_t at) {
   constexpr int V = kAdamValues;
-  const T* g = (const T*)e.g;
+  const G* g = (const G*)e.g;
   T* p = (T*)e.p;
   float *m = (float*)e.m, *v = (float*)e.v;
   float qg[PIECES][V], qm[PIECES][V], qv[PIECES][V], qw[PIECES][V];
@@ -237,12 +238,12 @@ __device__ __forceinline__ void adam_decode_first(uint32_t codes, float* x) {
 
 // V values a piece: 8 of a bf16 parameter, 4 of a float32 one, so that either is 16 bytes (float32, 8 / 4: 50 million 167 / 138 us,
 // 673 million 2.06 / 2.12 ms).
-template <bool ALL, bool ROUGH, int VALUES, int V, class T>
+template <bool ALL, bool ROUGH, int VALUES, int V, class T, class G>
 __device__ __forceinline__ void adam8_chunk(const AdamEntry& e, const AdamHyper& h, float f, float step, float root, float decay,
                                             uint32_t key, int64_t at) {
   constexpr int kPieces = VALUES / V, kWords = V / 4;
   typedef uint32_t Codes __attribute__((ext_vector_type(kWords)));
-  const T* g = (const T*)e.g;
+  const G* g = (const G*)e.g;
   T* p = (T*)e.p;
   uint8_t *m = (uint8_t*)e.m, *v = (uint8_t*)e.v;
   const int64_t whole = (e.elems + 31) & ~int64_t{31};  // codes are whole blocks
@@ -348,15 +349,18 @@ __global__ __launch_bounds__(kAdamThreads) void adamw_kernel(AdamTable table, in
     constexpr bool ALL = decltype(whole)::value;
     if constexpr (EIGHT) {
       if (!ALL || h.eps < 1e-9f) {
-        if (e.f32) adam8_chunk<ALL, false, PIECES, 4, float>(e, h, f, step, root, decay, key, at);
-        else adam8_chunk<ALL, false, PIECES, 8, uint16_t>(e, h, f, step, root, decay, key, at);
+        if (e.types == 1) adam8_chunk<ALL, false, PIECES, 4, float, float>(e, h, f, step, root, decay, key, at);
+        else if (e.types == 0) adam8_chunk<ALL, false, PIECES, 8, uint16_t, uint16_t>(e, h, f, step, root, decay, key, at);
+        else adam8_chunk<ALL, false, PIECES, 8, uint16_t, float>(e, h, f, step, root, decay, key, at);
       } else {
-        if (e.f32) adam8_chunk<ALL, true, PIECES, 4, float>(e, h, f, step, root, decay, key, at);
-        else adam8_chunk<ALL, true, PIECES, 8, uint16_t>(e, h, f, step, root, decay, key, at);
+        if (e.types == 1) adam8_chunk<ALL, true, PIECES, 4, float, float>(e, h, f, step, root, decay, key, at);
+        else if (e.types == 0) adam8_chunk<ALL, true, PIECES, 8, uint16_t, uint16_t>(e, h, f, step, root, decay, key, at);
+        else adam8_chunk<ALL, true, PIECES, 8, uint16_t, float>(e, h, f, step, root, decay, key, at);
       }
     } else {
-      if (e.f32) adam_chunk<ALL, PIECES, float>(e, h, f, step, root, decay, at);
-      else adam_chunk<ALL, PIECES, uint16_t>(e, h, f, step, root, decay, at);
+      if (e.types == 1) adam_chunk<ALL, PIECES, float, float>(e, h, f, step, root, decay, at);
+      else if (e.types == 0) adam_chunk<ALL, PIECES, uint16_t, uint16_t>(e, h, f, step, root, decay, at);
+      else adam_chunk<ALL, PIECES, uint16_t, float>(e, h, f, step, root, decay, at);
     }
   };
   if (all) types(std::true_type());
@@ -433,7 +437,7 @@ static bool adam_overlap(int64_t n, const int64_t* table) try {
   runs.reserve(n);
   for (int64_t i = 0; i < n; ++i) {
     const int64_t* t = table + i * MX_ADAMW_FIELDS;
-    if (t[8]) runs.emplace_back((uintptr_t)t[0], (uintptr_t)t[0] + t[8] * (t[1] ? 4 : 2));
+    if (t[8]) runs.emplace_back((uintptr_t)t[0], (uintptr_t)t[0] + t[8] * (t[1] == 1 ? 4 : 2));
   }
   std::sort(runs.begin(), runs.end());
   for (size_t i = 1; i < runs.size(); ++i)
@@ -458,10 +462,10 @@ extern "C" int mx_adamw(int64_t n, const int64_t* table, int eight, double lr, d
   for (int64_t i = 0; i < n; ++i) {
     const int64_t* t = table + i * MX_ADAMW_FIELDS;
     const int64_t elems = t[8], number = t[10];
-    if (elems < 0 || number < 0 || number > 0x7FFFFFFF || (!steps && t[9] < 1)) return MX_ERR_INVALID_ARG;
+    if (t[1] < 0 || t[1] > 2 || elems < 0 || number < 0 || number > 0x7FFFFFFF || (!steps && t[9] < 1)) return MX_ERR_INVALID_ARG;
     if (elems == 0) continue;
     if (!t[0] || !t[2] || !t[3] || !t[4] || (eight && (!t[5] || !t[6]))) return MX_ERR_INVALID_ARG;
-    if ((t[0] | t[2]) & (t[1] ? 3 : 1) || (t[3] | t[4]) & (eight ? 7 : 3) || t[7] & 3) return MX_ERR_ALIGNMENT;
+    if (t[0] & (t[1] == 1 ? 3 : 1) || t[2] & (t[1] ? 3 : 1) || (t[3] | t[4]) & (eight ? 7 : 3) || t[7] & 3) return MX_ERR_ALIGNMENT;
     // (a place is hashed in 32 bits, two values at a time)
     if (elems >= int64_t{1} << 33) return MX_ERR_UNSUPPORTED;
     values = values > kAdamFew ? values : values + elems;
@@ -501,7 +505,7 @@ extern "C" int mx_adamw(int64_t n, const int64_t* table, int eight, double lr, d
       if (const int rc = flush()) return rc;
     AdamEntry& e = args.e[used++];
     e = {(void*)t[0], (const void*)t[2], (void*)t[3], (void*)t[4], (uint8_t*)t[5], (uint8_t*)t[6], (float*)t[7], elems,
-         (uint32_t)chunks, (uint32_t)t[10], 0.f, 0.f, t[1] != 0};
+         (uint32_t)chunks, (uint32_t)t[10], 0.f, 0.f, (uint32_t)t[1]};
     if (!steps) {
       const double at = (double)t[9];
       e.step = (float)(lr / (1.0 - std::pow(beta1, at)));

@@ -1287,14 +1287,16 @@ def adamw_(operands, eight: bool, lr: float, betas, eps: float, weight_decay: fl
            norm: torch.Tensor | None = None, limit: float = 0.0, seed: int = 0, steps: torch.Tensor | None = None,
            lr_device: torch.Tensor | None = None, corrections: torch.Tensor | None = None) -> None:
     """One AdamW step in place.  operands: (parameter, gradient, moments, master or None, step, number) each, on one GPU;
-    moments: two float32 tensors, or with `eight` codes and scales of the first and of the second.  Tensors of one parameter
+    moments: two float32 tensors, or with `eight` codes and scales of the first and of the second; gradients in their parameter's type or
+    float32.  Tensors of one parameter
     lie in memory alike, each in one run; steps: float32 step counters by number, which the call raises, with 16 bytes each of
     `corrections`."""
     table, written = [], []
     for p, g, moments, master, step, number in operands:
         codes = [moments[0], moments[2]] if eight else moments
         scales = [_ptr(moments[1]), _ptr(moments[3])] if eight else [0, 0]
-        table += [_ptr(p), int(p.dtype == torch.float32), _ptr(g), *map(_ptr, codes), *scales,
+        types = 1 if p.dtype == torch.float32 else 2 * int(g.dtype == torch.float32)
+        table += [_ptr(p), types, _ptr(g), *map(_ptr, codes), *scales,
                   0 if master is None else _ptr(master), p.numel(), step, number]
         written += [p, *moments] + ([] if master is None else [master])
     dev = operands[0][0].device

@@ -341,8 +341,9 @@ class AdamW(torch.optim.Optimizer):
             p, g = w.p, w.g
             if g.device != p.device or g.shape != p.shape:
                 raise ValueError(f"AdamW: a gradient of shape {tuple(g.shape)} on {g.device} for a parameter of {tuple(p.shape)} on {p.device}")
-            if g.dtype != p.dtype or g.is_neg() or type(g) is not torch.Tensor or not _same_order(g, p):
-                g = torch.empty_like(p).copy_(g)
+            kept = p.dtype if g.dtype == p.dtype else torch.float32  # (wider gradients keep float32's bits)
+            if g.dtype != kept or g.is_neg() or type(g) is not torch.Tensor or not _same_order(g, p):
+                g = torch.empty_like(p, dtype=kept).copy_(g)
             moments = [w.held[name] for name in _MOMENTS[group["state_bits"]]]
             master = w.held.get("master")
             _check_state(p, moments, master, eight)
