@@ -464,7 +464,8 @@ int mx_preference_loss_bwd(const mx_preference_loss_t* args, const double* each,
  * 1e-6)) for a float32 norm on the device, 1 for NULL.  Moments are float32, or with `eight` codes in blocks of 32 values (the last one
  * filled up: whole blocks of codes, 8-byte aligned) with a scale byte b = 2^(b - 127) each, 255 = NaN: first moment e4m3 as
  * above, second moment e5m3 without a sign (bias 15, max 122880), rounded up or down by chance so that the value is the mean,
- * by a hash of seed, step, the parameter's number and the value's place; a second moment above 0 keeps a code above 0.
+ * by a hash of seed, step, the parameter's number and the value's place; a second moment above 0 keeps a code above 0.  Everything is
+ * rounded right but, with `eight` and eps of 1e-9 or more, the root (within an ulp) and the quotient (within two) of w.
  * steps (or NULL): float32 step counters on the device by the parameters' numbers, in place of the table's; they are raised by the
  * call, which can be captured into a graph; corrections: 16 bytes for each of them, 16-byte aligned; lr_device (or NULL):
  * float32 in place of lr.  Parameters that share memory are updated one after the other.  MX_ERR_UNSUPPORTED, before any

@@ -142,8 +142,9 @@ __device__ __forceinline__ void adam_store(T* p, int64_t left, const float (&f)[
 // The new moments and weight of one value.  Products and sums are rounded one by one, as separate operations on tensors
 // round them: the same bits as the formula in torch operations.
 // ROUGH: the hardware's root and reciprocal, each within an ulp, for an eps (from 1e-9 on) that covers what they lose of a
-// denormal second moment; the sequences around them that round right took 7 to 15 % of the time of a bf16 parameter with moments
-// in 8 bits (us with them and without: 673 million 1329 and 1251, 50 million 107 and 91), and nothing elsewhere.
+// denormal second moment, and then for every value of the call, whichever chunk it is in; the sequences around them that round right
+// took 7 to 15 % of the time of a bf16 parameter with moments in 8 bits (us with them and without: 673 million 1329 and 1251, 50 million
+// 107 and 91), and nothing elsewhere.
 template <bool ROUGH>
 __device__ __forceinline__ void adam_update(const AdamHyper& h, float f, float step, float root, float decay, float g, float& m,
                                             float& v, float& w) {
@@ -348,7 +349,7 @@ __global__ __launch_bounds__(kAdamThreads) void adamw_kernel(AdamTable table, in
   auto types = [&](auto whole) {
     constexpr bool ALL = decltype(whole)::value;
     if constexpr (EIGHT) {
-      if (!ALL || h.eps < 1e-9f) {
+      if (h.eps < 1e-9f) {
         if (e.types == 1) adam8_chunk<ALL, false, PIECES, 4, float, float>(e, h, f, step, root, decay, key, at);
         else if (e.types == 0) adam8_chunk<ALL, false, PIECES, 8, uint16_t, uint16_t>(e, h, f, step, root, decay, key, at);
         else adam8_chunk<ALL, false, PIECES, 8, uint16_t, float>(e, h, f, step, root, decay, key, at);
