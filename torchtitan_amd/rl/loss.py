@@ -33,7 +33,7 @@ class _TokenLogProbs(torch.autograd.Function):
     @staticmethod
     def backward(ctx, grad):
         logits, target, lse = ctx.saved_tensors
-        return ops.token_logprob_bwd(logits, target, lse, grad), None
+        return _once(ops.token_logprob_bwd(logits, target, lse, grad)), None
 
 
 def token_log_probs(logits: torch.Tensor, target: torch.Tensor) -> torch.Tensor:
@@ -133,7 +133,7 @@ def _check_tokens(log_probs, others: dict, offsets, mask) -> int:
 
 
 def _once(grad):
-    """A gradient that cannot be differentiated again: log_probs is in it."""
+    """A gradient that cannot be differentiated again: what it was formed from is in it."""
     return _Refusing.apply(grad, torch.empty(0, requires_grad=True)) if torch.is_grad_enabled() else grad
 
 
