@@ -71,9 +71,7 @@ def compute_policy_gradient_loss(model: torch.nn.Module, vllm_token_ids: list[li
     if all(isinstance(x, (int, float)) for x in numbers) and ppo_clip_eps >= 0 and _one_launch(batch_lps, ref_token_log_probs, advantages):
         offsets = torch.tensor([0, *(lps.numel() for lps in batch_lps)], dtype=torch.int64).cumsum(0).to(device)
         ref = torch.cat(list(ref_token_log_probs))
-        total, values = policy_loss(torch.cat(batch_lps), advantages, ref, ref, offsets=offsets, clip_eps=ppo_clip_eps,
-                                    kl_coef=kl_coef, kl="k3_swapped", entropy_coef=entropy_coef, ratio="sequence",
-                                    average="sequence")
+        total, values = _sample_loss(torch.cat(batch_lps), advantages, ref, offsets, ppo_clip_eps, kl_coef, entropy_coef)
         return total, dict(zip(POLICY_METRICS, values.tolist())), batch_lps
     mean_log_ratio, mean_kl = [], []
     for lps, ref in zip(batch_lps, ref_token_log_probs):
@@ -98,9 +96,11 @@ def compute_policy_gradient_loss(model: torch.nn.Module, vllm_token_ids: list[li
 
 
 def _one_launch(log_probs, ref, advantages: torch.Tensor) -> bool:
-    """The samples' losses can be formed over all tokens at once: float32 on one GPU, no sample empty."""
+    """The samples' losses can be formed over all tokens at once: float32 on one GPU, no sample empty, outside function transforms."""
+    if not log_probs or not (torch.compiler.is_compiling() or ops.plain_rows(log_probs[0])):
+        return False
     plain = lambda t: type(t) is torch.Tensor and t.is_cuda and t.dtype == torch.float32 and t.device == advantages.device
-    return (bool(log_probs) and len(log_probs) == len(ref) and plain(advantages) and advantages.shape == (len(log_probs),)
+    return (len(log_probs) == len(ref) and plain(advantages) and advantages.shape == (len(log_probs),)
             and not advantages.requires_grad
             and all(plain(a) and plain(b) and a.dim() == 1 and a.shape == b.shape and a.numel() > 0 for a, b in zip(log_probs, ref)))
 
@@ -149,6 +149,27 @@ class _PolicyLoss(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dloss, _):
         return (_once(ops.policy_loss_bwd(*ctx.saved_tensors, dloss, *ctx.numbers)), *(None,) * 14)
+
+
+class _SampleLoss(_PolicyLoss):
+    """The policy loss with a gradient that has one itself: where it is asked for, it is formed in torch operations."""
+
+    @staticmethod
+    def backward(ctx, dloss, _):
+        if not torch.is_grad_enabled():
+            return _PolicyLoss.backward(ctx, dloss, _)
+        tensors = ctx.saved_tensors[:6]
+        loss, _ = _policy_in_torch_ops(*tensors, *ctx.numbers)
+        return (*torch.autograd.grad(loss, tensors[0], dloss, create_graph=True), *(None,) * 14)
+
+
+def _sample_loss(log_probs, advantages, ref, offsets, clip_eps: float, kl_coef: float, entropy_coef: float):
+    """(loss, metrics) with a ratio and a mean for each sample."""
+    if torch.compiler.is_compiling():
+        return policy_loss(log_probs, advantages, ref, ref, offsets=offsets, clip_eps=clip_eps, kl_coef=kl_coef, kl="k3_swapped",
+                           entropy_coef=entropy_coef, ratio="sequence", average="sequence")
+    return _SampleLoss.apply(log_probs, advantages.contiguous(), ref, ref, offsets, None, advantages.shape[0], False, True, True,
+                             _KL.index("k3_swapped"), 1.0 - float(clip_eps), 1.0 + float(clip_eps), float(kl_coef), float(entropy_coef))
 
 
 class _PreferenceLoss(torch.autograd.Function):
