@@ -1,0 +1,36 @@
+"""Infinite values, equal shapes and wide operands in the policy and preference losses, on any device."""
+import math
+
+import torch
+
+from torchtitan_amd.rl import policy_loss
+
+
+def as_many_tokens_as_sequences(device):
+    """Packed, the shape of the advantages does not say what they belong to."""
+    import pytest
+
+    lp = torch.zeros(4, device=device, requires_grad=True)
+    A = torch.tensor([1.0, 2.0, 3.0, 4.0], device=device)
+    for bounds, by_token, by_sequence in (([0, 3, 3, 3, 4], [1.0, 2.0, 3.0, 4.0], [1.0, 1.0, 1.0, 4.0]),
+                                          ([0, 1, 1, 2, 2], [1.0, 2.0, 0.0, 0.0], [1.0, 3.0, 0.0, 0.0]),
+                                          ([0, 1, 2, 3, 4], [1.0, 2.0, 3.0, 4.0], [1.0, 2.0, 3.0, 4.0])):
+        offsets = torch.tensor(bounds, device=device)
+        with pytest.raises(ValueError, match="advantage="):
+            policy_loss(lp, A, offsets=offsets)
+        for advantage, want in (("token", by_token), ("sequence", by_sequence)):
+            loss, _ = policy_loss(lp, A, offsets=offsets, advantage=advantage)
+            n = bounds[-1]
+            assert math.isclose(loss.item(), -sum(want) / n, rel_tol=1e-6)
+            (grad,) = torch.autograd.grad(loss, lp)
+            assert torch.allclose(grad, -torch.tensor(want, device=device) / n, rtol=1e-6)
+        # (a ratio of a sequence has the sequence's advantage)
+        assert math.isclose(policy_loss(lp, A, offsets=offsets, ratio="sequence")[0].item(), -sum(by_sequence) / n, rel_tol=1e-6)
+    one = policy_loss(lp[:1], A[:1], offsets=torch.tensor([0, 1], device=device))[0]
+    assert one.item() == -1.0  # (one token of one sequence: the same)
+    rows = torch.zeros(4, 1, device=device)
+    assert policy_loss(rows, A)[0].item() == policy_loss(rows, A[:, None])[0].item() == -2.5
+    for bad, wrong in ((dict(advantage="row"), A), (dict(advantage="token", ratio="sequence"), A[:, None]), (dict(advantage="token"), A),
+                       (dict(advantage="sequence"), A[:, None])):
+        with pytest.raises(ValueError):
+            policy_loss(rows, wrong, **bad)

@@ -1,0 +1,9 @@
+"""CPU: the losses' edges in torch operations."""
+import pytest
+
+from tests import sequence_loss_edges as edges
+
+
+@pytest.mark.parametrize("case", ["as_many_tokens_as_sequences"])
+def test_edge(case):
+    getattr(edges, case)("cpu")

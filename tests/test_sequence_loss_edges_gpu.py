@@ -1,0 +1,11 @@
+"""GPU: the losses' edges in the kernels."""
+import pytest
+
+from tests import sequence_loss_edges as edges
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("case", ["as_many_tokens_as_sequences"])
+def test_edge(device, case):
+    getattr(edges, case)(device)

@@ -288,7 +288,7 @@ def _policy_in_torch_ops(log_probs, advantages, old, ref, offsets, mask, sequenc
 def policy_loss(log_probs: torch.Tensor, advantages: torch.Tensor, old_log_probs: torch.Tensor | None = None,
                 ref_log_probs: torch.Tensor | None = None, *, offsets: torch.Tensor | None = None, mask: torch.Tensor | None = None,
                 clip_eps: float = 0.2, clip_eps_high: float | None = None, kl_coef: float = 0.0, kl: str = "k3",
-                entropy_coef: float = 0.0, ratio: str = "token", average: str = "token"):
+                entropy_coef: float = 0.0, ratio: str = "token", average: str = "token", advantage: str | None = None):
     """(loss, metrics): the clipped policy loss of many sequences, and float32 [5] metrics named by `POLICY_METRICS`.
 
         r = exp(log_probs - old_log_probs)       (or ratio="sequence": of the mean of that over a sequence)
@@ -298,7 +298,8 @@ def policy_loss(log_probs: torch.Tensor, advantages: torch.Tensor, old_log_probs
     log_probs: of the sampled tokens, [sequences, length], or [tokens] with `offsets` (int64 or int32 [sequences + 1]: sequence s has
     the tokens from offsets[s] to offsets[s + 1]; rising, not behind the last token).  `mask` (bool) says which of them count.  What a token
     that does not count holds has no influence, and its gradient is 0; sequences without a token that counts are left out of
-    every mean.  advantages: [sequences], or of every token (ratio="token").  Without `old_log_probs` the policy has not moved: r is
+    every mean.  advantages: [sequences], or of every token (ratio="token"); their shape says which, but for packed tokens as many as
+    there are sequences, where `advantage`, "sequence" or "token", must.  Without `old_log_probs` the policy has not moved: r is
     1, with its gradient.  kl, at x = log_probs - ref_log_probs: "k1" x, "k2" x^2 / 2, "k3" exp(-x) - 1 + x, "k3_swapped" exp(x) - 1 - x.
     The entropy is minus the mean of log_probs.  average: means of pg and KL over all tokens, or over sequences of the means
     over their tokens.  A coefficient of 0 leaves its term out of the loss, whatever it is.  Only log_probs gets a gradient, which on the GPU cannot be differentiated again; terms and sums
@@ -313,8 +314,14 @@ def policy_loss(log_probs: torch.Tensor, advantages: torch.Tensor, old_log_probs
     if not low <= high:
         raise ValueError(f"clip_eps {clip_eps} and clip_eps_high {clip_eps_high} leave nothing between them")
     sequences = _check_tokens(log_probs, dict(old_log_probs=old_log_probs, ref_log_probs=ref_log_probs), offsets, mask)
-    per_token = advantages.shape != (sequences,)
-    if (per_token and (advantages.shape != log_probs.shape or ratio == "sequence")) or not advantages.is_floating_point():
+    if advantage not in (None, "token", "sequence") or (advantage == "token" and ratio == "sequence"):
+        raise ValueError(f"advantage must be 'sequence', or 'token' with ratio='token', got {advantage!r} with {ratio!r}")
+    per_token = advantages.shape != (sequences,) if advantage is None else advantage == "token"
+    if advantage is None and ratio == "token" and advantages.shape == log_probs.shape == (sequences,) and sequences > 1:
+        raise ValueError(f"{sequences} packed tokens of {sequences} sequences: advantage='sequence' or advantage='token' has to say what "
+                         "the advantages belong to")
+    if (advantages.shape != (log_probs.shape if per_token else (sequences,)) or (per_token and ratio == "sequence")
+            or not advantages.is_floating_point()):
         raise ValueError(f"advantages must be floating-point [{sequences}]{'' if ratio == 'sequence' else f' or {tuple(log_probs.shape)}'}, "
                          f"got {tuple(advantages.shape)} {advantages.dtype}")
     if advantages.device != log_probs.device:
