@@ -286,7 +286,7 @@ def _run_policy(state):
         loss, metrics = policy_loss(log_probs, state["advantages"], state["old"], state["ref"], offsets=state["offsets"],
                                     mask=state["mask"], clip_eps=case["low"], clip_eps_high=case["high"],
                                     kl_coef=case["kl_coef"], kl=case["kl"], entropy_coef=case["entropy_coef"],
-                                    ratio=case["ratio"], average=case["average"])
+                                    ratio=case["ratio"], average=case["average"], advantage=case["advantage"])
         if not case["train"]:
             return dict(metrics=metrics, loss=loss)
         (grad,) = torch.autograd.grad(loss, log_probs, state["dloss"])
