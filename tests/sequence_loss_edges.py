@@ -3,7 +3,22 @@ import math
 
 import torch
 
-from torchtitan_amd.rl import policy_loss
+from torchtitan_amd.rl import policy_loss, preference_loss
+
+
+def a_rejected_answer_without_a_chance(device):
+    """log p of the rejected sequence is minus infinity: nothing is lost on the pair, and it has no gradient."""
+    lp = torch.tensor([[-1.0, -2.0], [-3.0, -1.0], [-math.inf, -1.0], [-1.5, -2.5]], device=device, requires_grad=True)
+    loss, rewards = preference_loss(lp, beta=0.5)
+    z = -4.0 + 4.0
+    assert math.isclose(loss.item(), (0.0 + math.log1p(math.exp(-0.5 * z))) / 2, rel_tol=1e-6)
+    assert rewards.tolist()[2] == -math.inf
+    (grad,) = torch.autograd.grad(loss, lp)
+    assert torch.equal(grad, torch.tensor([[0.0, 0.0], [-0.125, -0.125], [0.0, 0.0], [0.125, 0.125]], device=device))
+    for kind in ("hinge", "sigmoid"):  # (the other way round it is infinite)
+        swapped = torch.cat((lp[2:], lp[:2])).detach().requires_grad_(True)
+        assert preference_loss(swapped, beta=0.5, kind=kind)[0].item() == math.inf
+    assert preference_loss(lp, beta=0.5, label_smoothing=0.1)[0].item() == math.inf
 
 
 def as_many_tokens_as_sequences(device):

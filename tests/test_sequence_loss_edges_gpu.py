@@ -6,6 +6,6 @@ from tests import sequence_loss_edges as edges
 pytestmark = pytest.mark.gpu
 
 
-@pytest.mark.parametrize("case", ["as_many_tokens_as_sequences"])
+@pytest.mark.parametrize("case", ["a_rejected_answer_without_a_chance", "as_many_tokens_as_sequences"])
 def test_edge(device, case):
     getattr(edges, case)(device)

@@ -373,7 +373,7 @@ __device__ __forceinline__ void seq_take(const Preference& f, const Sequences& q
   if (f.kind == 0) {
     // -log sigmoid(y) = log(1 + e^-|y|) + max(-y, 0), and the sigmoids of y and -y from the same e^-|y|
     const double e = seq_exp(-fabs(y)).e, both = log1p(e), large = 1.0 / (1.0 + e), small = e * large;
-    value = both + (y < 0 ? (1.0 - f.smoothing) * -y : f.smoothing * y);
+    value = both + (y < 0 ? (1.0 - f.smoothing) * -y : f.smoothing != 0 ? f.smoothing * y : 0.0);  // (no part of an infinite y)
     slope = f.beta * (y < 0 ? f.smoothing * small - (1.0 - f.smoothing) * large : f.smoothing * large - (1.0 - f.smoothing) * small);
   } else if (f.kind == 1) {
     value = 1.0 - y < 0 ? 0.0 : 1.0 - y;  // (NaN stays)

@@ -350,7 +350,9 @@ def _preference_in_torch_ops(log_probs, ref, offsets, mask, sequences, kind, mea
         h = h / n.clamp(min=1)
     z, pairs = h[:sequences // 2] - h[sequences // 2:], n[:sequences // 2] + n[sequences // 2:] > 0
     if _PREFERENCES[kind] == "sigmoid":
-        losses = -(1 - smoothing) * F.logsigmoid(beta * z) - smoothing * F.logsigmoid(-beta * z)
+        losses = -(1 - smoothing) * F.logsigmoid(beta * z)
+        if smoothing:  # (a part of 0 would be no number where z is infinite)
+            losses = losses - smoothing * F.logsigmoid(-beta * z)
     elif _PREFERENCES[kind] == "hinge":
         losses = F.relu(1 - beta * z)
     else:
