@@ -21,6 +21,21 @@ def a_rejected_answer_without_a_chance(device):
     assert preference_loss(lp, beta=0.5, label_smoothing=0.1)[0].item() == math.inf
 
 
+def a_token_that_the_reference_rules_out(device):
+    """The estimators at x = +inf and -inf: infinite, with the sign of their gradient."""
+    lp = torch.tensor([[-1.0, -2.0]], device=device, requires_grad=True)
+    for kl, value, slope in (("k1", math.inf, 1.0), ("k2", math.inf, math.inf), ("k3", math.inf, 1.0), ("k3_swapped", math.inf, math.inf)):
+        loss, metrics = policy_loss(lp, torch.zeros(1, device=device), None, torch.tensor([[-1.0, -math.inf]], device=device), kl=kl,
+                                    kl_coef=1.0)
+        assert loss.item() == value and metrics[1].item() == value, kl
+        (grad,) = torch.autograd.grad(loss, lp)
+        assert grad[0, 1].item() == slope / 2, kl
+    for kl, value in (("k1", -math.inf), ("k2", math.inf), ("k3", math.inf), ("k3_swapped", math.inf)):
+        _, metrics = policy_loss(torch.tensor([[-1.0, -math.inf]], device=device), torch.zeros(1, device=device),
+                                 torch.zeros(1, 2, device=device), torch.tensor([[-1.0, -1.0]], device=device), kl=kl)
+        assert metrics[1].item() == value, kl
+
+
 def as_many_tokens_as_sequences(device):
     """Packed, the shape of the advantages does not say what they belong to."""
     import pytest

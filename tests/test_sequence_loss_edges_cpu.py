@@ -4,6 +4,7 @@ import pytest
 from tests import sequence_loss_edges as edges
 
 
-@pytest.mark.parametrize("case", ["a_rejected_answer_without_a_chance", "as_many_tokens_as_sequences"])
+@pytest.mark.parametrize("case", ["a_rejected_answer_without_a_chance", "a_token_that_the_reference_rules_out",
+                                  "as_many_tokens_as_sequences"])
 def test_edge(case):
     getattr(edges, case)("cpu")

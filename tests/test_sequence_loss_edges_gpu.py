@@ -6,6 +6,7 @@ from tests import sequence_loss_edges as edges
 pytestmark = pytest.mark.gpu
 
 
-@pytest.mark.parametrize("case", ["a_rejected_answer_without_a_chance", "as_many_tokens_as_sequences"])
+@pytest.mark.parametrize("case", ["a_rejected_answer_without_a_chance", "a_token_that_the_reference_rules_out",
+                                  "as_many_tokens_as_sequences"])
 def test_edge(device, case):
     getattr(edges, case)(device)

@@ -113,7 +113,8 @@ __device__ __forceinline__ bool seq_clipped(const Policy& f, double r) {
   const double c = r > f.high ? f.high : r < f.low ? f.low : r;
   return fabs(r - c) > 1e-6;
 }
-// e^x, e^x - 1 and e^x - 1 - x to 1e-14 of each: x = k ln 2 + t, |t| <= ln 2 / 2, and e^t - 1 - t = t^2 (1/2! + t/3! + ...) up to t^12 / 12!.
+// e^x, e^x - 1 and e^x - 1 - x (infinite where x is) to 1e-14 of each: x = k ln 2 + t, |t| <= ln 2 / 2, and
+// e^t - 1 - t = t^2 (1/2! + t/3! + ...) up to t^12 / 12!.
 struct SeqExp {
   double e, minus, rest;
 };
@@ -128,7 +129,7 @@ __device__ __forceinline__ SeqExp seq_exp(double x) {
   for (int n = 0; n < 10; ++n) q = __builtin_fma(q, t, kBelow[n]);
   const double rest = t * t * q, minus = t + rest;
   const double e = ldexp(1.0 + minus, (int)k);
-  return k == 0.0 ? SeqExp{e, minus, rest} : SeqExp{e, e - 1.0, e - 1.0 - x};
+  return k == 0.0 ? SeqExp{e, minus, rest} : SeqExp{e, e - 1.0, x > 750.0 ? e : e - 1.0 - x};
 }
 __device__ __forceinline__ double seq_kl(int kind, double x) {
   if (kind == 0) return x;

@@ -249,7 +249,9 @@ def _kl_term(x, kind: int):
         return x
     if _KL[kind] == "k2":
         return 0.5 * x * x
-    return torch.expm1(-x) + x if _KL[kind] == "k3" else torch.expm1(x) - x
+    if _KL[kind] == "k3":
+        x = -x
+    return torch.expm1(x) - x.clamp(max=1e300)  # (infinite where x is)
 
 
 def _policy_in_torch_ops(log_probs, advantages, old, ref, offsets, mask, sequences, per_token, whole, by_sequence, kl, low, high,
