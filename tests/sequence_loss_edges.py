@@ -64,3 +64,21 @@ def as_many_tokens_as_sequences(device):
                        (dict(advantage="sequence"), A[:, None])):
         with pytest.raises(ValueError):
             policy_loss(rows, wrong, **bad)
+
+
+def a_border_between_two_float32_numbers(device):
+    """Old log-probabilities in float64: ratios on either side of a border, nearer to it than float32 tells."""
+    border = -math.log(1.2)
+    lp = torch.zeros(1, 2, device=device, requires_grad=True)
+    old = torch.tensor([[border - 1e-10, border + 1e-10]], dtype=torch.float64, device=device)
+    loss, metrics = policy_loss(lp, torch.ones(1, device=device), old, clip_eps=0.2)
+    (grad,) = torch.autograd.grad(loss, lp)
+    assert grad[0, 0].item() == 0.0 and abs(grad[0, 1].item() + 0.6) <= 1e-6
+    # and a reference: 1e-9 between the two of a pair
+    pair = torch.full((2, 1), -2.0, device=device, requires_grad=True)
+    ref = torch.tensor([[-2.0 - 1e-9], [-2.0 + 1e-9]], dtype=torch.float64, device=device)
+    _, rewards = preference_loss(pair, ref, beta=1.0)
+    assert all(abs(a - b) <= 1e-15 for a, b in zip(rewards.tolist(), (1e-9, -1e-9)))
+    x = torch.full((1, 1), 1e-9, dtype=torch.float64, device=device)
+    _, metrics = policy_loss(pair[:1], torch.ones(1, device=device), None, pair[:1].double().detach() - x, kl="k1")
+    assert abs(metrics[1].item() - 1e-9) <= 1e-15

@@ -189,14 +189,17 @@ class _PreferenceLoss(torch.autograd.Function):
 def _by_kernels(name: str, node, log_probs, tensors: tuple, numbers: tuple):
     """The loss through the kernels -- one native call, a traced operator, or step by step --, None for tensors that they do
     not take."""
-    if not log_probs.is_cuda or log_probs.dtype not in ops.ROW_TYPES or ops.wrapped(log_probs, *(t for t in tensors if t is not None)):
+    given = tuple(t for t in tensors if t is not None)
+    if not log_probs.is_cuda or log_probs.dtype not in ops.ROW_TYPES or ops.wrapped(log_probs, *given):
+        return None
+    if any(t.dtype == torch.float64 for t in given):  # (the kernels would read it in float32)
         return None
     if torch.compiler.is_compiling():
         from .. import compiled  # noqa: F401  (the same launches as nodes of the graph)
 
         call = getattr(torch.ops.torchtitan_amd, name + "_fwd")
-        return call(log_probs, *(_narrow(t) for t in tensors), *numbers)[:2]
-    if not ops.plain_rows(log_probs) or not all(t is None or type(t) in (torch.Tensor, torch.nn.Parameter) for t in tensors):
+        return call(log_probs, *(_wide(t) for t in tensors), *numbers)[:2]
+    if not ops.plain_rows(log_probs) or not all(type(t) in (torch.Tensor, torch.nn.Parameter) for t in given):
         return None
     if ops.native_rows(log_probs):
         call = getattr(_lib.blocks(), name)
@@ -212,14 +215,14 @@ def _by_kernels(name: str, node, log_probs, tensors: tuple, numbers: tuple):
     return getattr(ops, name + "_fwd")(log_probs, *tensors, *numbers, want_each=False)[:2]
 
 
-def _narrow(t):
-    """In a type that the kernels read."""
+def _wide(t):
+    """In a type that the kernels read, which holds all of its values."""
     return t.float() if t is not None and t.is_floating_point() and t.dtype not in ops.ROW_TYPES else t
 
 
 def _dense(t):
     """Without a gradient, as the kernels read it."""
-    return None if t is None else _narrow(t.detach()).resolve_neg().contiguous()
+    return None if t is None else _wide(t.detach()).resolve_neg().contiguous()
 
 
 def _places(log_probs, offsets, mask, sequences: int):
@@ -301,7 +304,7 @@ def policy_loss(log_probs: torch.Tensor, advantages: torch.Tensor, old_log_probs
     the tokens from offsets[s] to offsets[s + 1]; rising, not behind the last token).  `mask` (bool) says which of them count.  What a token
     that does not count holds has no influence, and its gradient is 0; sequences without a token that counts are left out of
     every mean.  advantages: [sequences], or of every token (ratio="token"); their shape says which, but for packed tokens as many as
-    there are sequences, where `advantage`, "sequence" or "token", must.  Without `old_log_probs` the policy has not moved: r is
+    there are sequences, where `advantage`, "sequence" or "token", must (on the GPU they are read in float32, whatever their type).  Without `old_log_probs` the policy has not moved: r is
     1, with its gradient.  kl, at x = log_probs - ref_log_probs: "k1" x, "k2" x^2 / 2, "k3" exp(-x) - 1 + x, "k3_swapped" exp(x) - 1 - x.
     The entropy is minus the mean of log_probs.  average: means of pg and KL over all tokens, or over sequences of the means
     over their tokens.  A coefficient of 0 leaves its term out of the loss, whatever it is.  Only log_probs gets a gradient, which on the GPU cannot be differentiated again; terms and sums
@@ -330,7 +333,6 @@ def policy_loss(log_probs: torch.Tensor, advantages: torch.Tensor, old_log_probs
         raise ValueError(f"log_probs on {log_probs.device}, advantages on {advantages.device}")
     numbers = (sequences, per_token, ratio == "sequence", average == "sequence", _KL.index(kl), low, high, float(kl_coef),
                float(entropy_coef))
-    # (advantages are read in float32)
     out = _by_kernels("policy_loss", _PolicyLoss, log_probs,
                       (advantages if advantages.dtype == torch.float32 else advantages.float(), old_log_probs, ref_log_probs, offsets,
                        mask), numbers)
