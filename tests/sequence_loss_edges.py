@@ -82,3 +82,18 @@ def a_border_between_two_float32_numbers(device):
     x = torch.full((1, 1), 1e-9, dtype=torch.float64, device=device)
     _, metrics = policy_loss(pair[:1], torch.ones(1, device=device), None, pair[:1].double().detach() - x, kl="k1")
     assert abs(metrics[1].item() - 1e-9) <= 1e-15
+
+
+def operands_from_inference_mode(device):
+    """What a rollout computed in inference mode is an operand like any other."""
+    lp = torch.full((3, 4), -1.0, device=device, requires_grad=True)
+    with torch.inference_mode():
+        old, ref = (torch.full((3, 4), v, device=device) for v in (-1.25, -1.5))
+        A, mask = torch.ones(3, device=device), torch.ones(3, 4, dtype=torch.bool, device=device)
+    plain = [t.clone() for t in (A, old, ref, mask)]
+    for make in (lambda A, old, ref, mask: policy_loss(lp, A, old, ref, mask=mask, kl_coef=0.1)[0],
+                 lambda A, old, ref, mask: preference_loss(torch.cat((lp, lp * 2)), torch.cat((ref, old)), mask=torch.cat((mask, mask)))[0],
+                 lambda A, old, ref, mask: preference_loss(lp[:2], ref[:2], mask=mask[:2])[0]):
+        got, want = make(A, old, ref, mask), make(*plain)
+        assert torch.equal(got, want)
+        assert torch.equal(torch.autograd.grad(got, lp)[0], torch.autograd.grad(want, lp)[0])

@@ -1202,9 +1202,13 @@ struct LossNode : torch::autograd::Function<LossNode<Numbers>> {
 template <class Numbers>
 py::object loss_of(const LossOperands& o, const Numbers& numbers) {
   if (!loss_plain(o) || !numbers.fits(o)) return py::none();
+  const bool train = at::GradMode::is_enabled() && o.log_probs.requires_grad();
+  if (train)
+    for (const Tensor& t : {o.old, o.ref, o.advantages, o.offsets, o.mask})
+      if (t.defined() && t.is_inference()) return py::none();  // (a node cannot keep it)
   Unlocked unlocked(std::in_place);
   Tensor loss, more;
-  if (at::GradMode::is_enabled() && o.log_probs.requires_grad()) {
+  if (train) {
     const variable_list out = LossNode<Numbers>::apply(o.log_probs, o, numbers);
     loss = out[0], more = out[1];
   } else {

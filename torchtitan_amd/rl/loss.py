@@ -168,7 +168,7 @@ def _sample_loss(log_probs, advantages, ref, offsets, clip_eps: float, kl_coef: 
     if torch.compiler.is_compiling():
         return policy_loss(log_probs, advantages, ref, ref, offsets=offsets, clip_eps=clip_eps, kl_coef=kl_coef, kl="k3_swapped",
                            entropy_coef=entropy_coef, ratio="sequence", average="sequence")
-    return _SampleLoss.apply(log_probs, advantages.contiguous(), ref, ref, offsets, None, advantages.shape[0], False, True, True,
+    return _SampleLoss.apply(log_probs, _dense(advantages), ref, ref, offsets, None, advantages.shape[0], False, True, True,
                              _KL.index("k3_swapped"), 1.0 - float(clip_eps), 1.0 + float(clip_eps), float(kl_coef), float(entropy_coef))
 
 
@@ -221,8 +221,11 @@ def _wide(t):
 
 
 def _dense(t):
-    """Without a gradient, as the kernels read it."""
-    return None if t is None else _wide(t.detach()).resolve_neg().contiguous()
+    """Without a gradient, as the kernels read it and a node keeps it."""
+    if t is None:
+        return None
+    t = _wide(t.detach()).resolve_neg().contiguous()
+    return t.clone() if t.is_inference() else t
 
 
 def _places(log_probs, offsets, mask, sequences: int):
