@@ -198,7 +198,8 @@ def _by_kernels(name: str, node, log_probs, tensors: tuple, numbers: tuple):
         from .. import compiled  # noqa: F401  (the same launches as nodes of the graph)
 
         call = getattr(torch.ops.torchtitan_amd, name + "_fwd")
-        return call(log_probs, *(_wide(t) for t in tensors), *numbers)[:2]
+        loss, more, _ = call(log_probs, *(_wide(t) for t in tensors), *numbers)
+        return loss, more.detach()  # (as the nodes mark it)
     if not ops.plain_rows(log_probs) or not all(type(t) in (torch.Tensor, torch.nn.Parameter) for t in given):
         return None
     if ops.native_rows(log_probs):
