@@ -75,3 +75,20 @@ def test_entries_of_no_parameter_are_kept():
     saved["state"]["note"] = {"run": 7}
     opt.load_state_dict(saved)
     assert opt.state["note"] == {"run": 7}
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("saved_bits", [32, 8])
+def test_a_state_of_other_shapes_leaves_the_optimizer_as_it_was(bits, saved_bits):
+    p, opt = stepped(state_bits=bits)
+    _, other = stepped(state_bits=saved_bits, shape=(8, 9))
+    before, numbers = copy.deepcopy(opt.state[p]), dict(opt.param_groups[0])
+    saved = other.state_dict()
+    saved["param_groups"][0]["lr"] = 0.5
+    with pytest.raises(ValueError, match="shape"):
+        opt.load_state_dict(saved)
+    assert opt.param_groups[0]["lr"] == numbers["lr"] and set(opt.state) == {p}
+    assert all(value == before[name] if name == "step" else torch.equal(value, before[name]) for name, value in opt.state[p].items())
+    p.grad = torch.ones(7, 9)
+    opt.step()
+    assert opt.state[p]["step"] == 4

@@ -203,7 +203,7 @@ class AdamW(torch.optim.Optimizer):
         optimizer's: a state that ``torch.optim.AdamW`` or this optimizer with others of them has saved is converted.  Hooks in front of
         the loading give the state that is converted, those behind it see the converted one."""
         held = [{key: group[key] for key in ("state_bits", "master_weights", "capturable")} for group in self.param_groups]
-        saved, ids = {}, []
+        saved, ids, before = {}, [], (self.state, self.param_groups, self._counters)
 
         def take(_, hooked):
             # (torch would round the moments to their parameters' types)
@@ -219,11 +219,15 @@ class AdamW(torch.optim.Optimizer):
                 for key, value in self.defaults.items():
                     group.setdefault(key, value)
             number = -1
-            for group in self.param_groups:
-                for p in group["params"]:
-                    number += 1
-                    if saved.get(ids[number]):
-                        self._load_one(p, group, saved[ids[number]], number)
+            try:
+                for group in self.param_groups:
+                    for p in group["params"]:
+                        number += 1
+                        if saved.get(ids[number]):
+                            self._load_one(p, group, saved[ids[number]], number)
+            except Exception:  # (a state that does not fit is not loaded by half)
+                self.state, self.param_groups, self._counters = before
+                raise
 
         # behind the caller's hooks in front of it, before those behind it
         own_hooks = (self.register_load_state_dict_pre_hook(take), self.register_load_state_dict_post_hook(convert, prepend=True))
@@ -243,6 +247,9 @@ class AdamW(torch.optim.Optimizer):
         if eight and group["state_bits"] == 8:
             moves = {name: saved[name] for name in _MOMENTS[8]}
         elif eight:
+            blocks = -(-p.numel() // ops.BLOCK)
+            if any(saved[name].shape[0] != blocks for name in _MOMENTS[8]):
+                raise ValueError(f"AdamW: a saved exp_avg has shape {tuple(saved['exp_avg'].shape)}, its parameter {tuple(p.shape)}")
             moves = {name: _decode(saved[name].to(p.device), saved[name + "_scale"].to(p.device), form, p.numel()).view(p.shape)
                      for name, form in (("exp_avg", _FIRST), ("exp_avg_sq", _SECOND))}
         elif group["state_bits"] == 8:
