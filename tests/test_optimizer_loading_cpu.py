@@ -92,3 +92,15 @@ def test_a_state_of_other_shapes_leaves_the_optimizer_as_it_was(bits, saved_bits
     p.grad = torch.ones(7, 9)
     opt.step()
     assert opt.state[p]["step"] == 4
+
+
+def test_a_state_with_the_largest_second_moments_is_refused():
+    """AdamW has no amsgrad: going on without it would be another optimizer."""
+    p, opt = stepped()
+    _, other = stepped(torch.optim.AdamW, amsgrad=True)
+    with pytest.raises(ValueError, match="amsgrad"):
+        opt.load_state_dict(other.state_dict())
+    assert opt.state[p]["step"] == 3 and "amsgrad" not in opt.param_groups[0]
+    _, plain = stepped(torch.optim.AdamW, steps=5)
+    opt.load_state_dict(plain.state_dict())
+    assert opt.state[p]["step"] == 5

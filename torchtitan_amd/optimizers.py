@@ -206,6 +206,8 @@ class AdamW(torch.optim.Optimizer):
         saved, ids, before = {}, [], (self.state, self.param_groups, self._counters)
 
         def take(_, hooked):
+            if any(group.get("amsgrad") for group in hooked["param_groups"]):
+                raise ValueError("AdamW: a state with amsgrad cannot be gone on with here")
             # (torch would round the moments to their parameters' types)
             ids.extend(i for group in hooked["param_groups"] for i in group["params"])
             parameters = set(ids)
