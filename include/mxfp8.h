@@ -425,8 +425,8 @@ int mx_grad_scale(int64_t n, void* const* grads, const int64_t* elems, const int
  *
  * mx_preference_loss: sequences is even; pair p is sequence p, preferred to sequence sequences / 2 + p.  h = sum (or with `mean` mean)
  * of log_probs - ref (ref NULL: of log_probs); z = h of the one - h of the other; the loss of a pair, averaged over pairs
- * with a token that counts: kind 0 -(1 - smoothing) log sigmoid(beta z) - smoothing log sigmoid(-beta z), 1 max(0, 1 - beta z), 2 (z - 1 /
- * (2 beta))^2.  rewards [sequences]: beta h.  each: sequences + 1 doubles, as above.
+ * with a token that counts (in either sequence; one without any has h = 0): kind 0 -(1 - smoothing) log sigmoid(beta z) -
+ * smoothing log sigmoid(-beta z), 1 max(0, 1 - beta z), 2 (z - 1 / (2 beta))^2.  rewards [sequences]: beta h.  each: sequences + 1 doubles, as above.
  * workspace: mx_sequence_loss_workspace bytes, 8-byte aligned.  MX_ERR_UNSUPPORTED, before any launch, for 2^32 - 255 tokens and
  * more or 2^30 sequences and more. */
 typedef struct {

@@ -6,12 +6,15 @@
 // the loss) is summed in three steps, in an order that depends on the sizes alone:
 //   parts    a wave takes a chunk of tokens, whatever sequences they are of, and leaves the sums of each of them: chunk c and
 //            sequence s share the place c + s, and no other pair does, since one of the two grows from pair to pair.  Long and short
-//            sequences are the same work, and nothing has to be cleared.
-//   join     every sequence's parts are added up, the loss formed, and what a token's gradient needs of its sequence
+//            sequences are the same work here and in the gradient, and nothing has to be cleared.
+//   join     every sequence's parts are added up by as many lanes as a sequence has parts on average, the loss formed, and what a
+//            token's gradient needs of its sequence.  One long sequence among short ones waits for its few lanes: 1024 sequences of
+//            4.2 million tokens take 38 us forward when they are equal and 289 when one of them holds nine tenths; 16 of 147 456
+//            16.1 and 17.6.
 //   gradient tokens as they lie (backward)
-// Some tens of megabytes at most are read.  Up to 100 000 tokens bound by the latency of two launches forward (10 to 16 us) and one
-// backward (3), so that a wave has a single row of 64 tokens until there are enough for every CU; 4.2 million tokens (89 MB) take 38 and 24
-// us, a sixth of it exponentials.  Terms are formed in float64: a ratio's side of a clipping border decides about its whole
+// Up to 100 000 tokens bound by the latency of two launches forward (7 to 17 us in a graph) and one backward (2 to 4), so that a wave
+// has a single row of 64 tokens until there are enough for every CU; 4.2 million tokens with everything that there is (89 MB) take 35 and
+// 21 us, a sixth of it exponentials.  Terms are formed in float64: a ratio's side of a clipping border decides about its whole
 // gradient, and the KL estimators are differences of nearly equal numbers.
 #include "mx_rows.h"
 
@@ -21,9 +24,11 @@ constexpr int kSeqGrad = 256;          // lanes of a workgroup of the gradient
 constexpr int kSeqFew = 1024;          // lanes of the workgroup that joins alone
 constexpr int kSeqMany = 256;          // lanes of a workgroup where several join
 constexpr int kSeqManyGroups = 1024;   // of which there are at most
-// Tokens from which on a wave takes 4 rows of 64 (us forward, 1 / 4 rows: 64 sequences of 600 13.6 / 12.7, one of 147 456 20.7 / 13.9,
-// 1024 of 4099 46.9 / 37.7; 8 rows 43.0 there, 16 63.6), and in the gradient (us, 1 / 4 rows, packed: 128 sequences of 4099 6.0 / 7.4, 1024 of
-// 4099 30.8 / 24.5).
+// Tokens from which on a wave takes 4 rows of 64 (us forward in a graph, 1 / 4 rows.  Below: 16 sequences of 61 10.0 / 15.9, 16 of 1024 9.7 /
+// 11.3, 64 of 400 11.6 / 12.4, 64 of 511 11.9 / 12.5, one of 30 000 12.0 / 11.8.  From there on: one of 34 000 11.6 / 12.1, 64 of 600 13.6 /
+// 12.5, 16 of 4096 14.0 / 11.8, one of 147 456 20.7 / 13.9, 1024 of 4099 46.9 / 37.7, 8 rows 43.0 there, 16 63.6.  Short sequences
+// would want single rows for longer: 512 of 70 11.4 / 16.6), and in the gradient (us, 1 / 4 rows, packed: 128 sequences of 4099 6.0 /
+// 7.4, 1024 of 4099 30.8 / 24.5).
 constexpr int64_t kSeqLong = 32768, kSeqGradLong = 1 << 20;
 __host__ __device__ __forceinline__ int seq_rows(int64_t tokens) { return tokens < kSeqLong ? 1 : 4; }
 __host__ __device__ __forceinline__ int64_t seq_chunks(int64_t tokens) {
@@ -359,7 +364,8 @@ __device__ __forceinline__ void seq_finish(const Policy& f, const Sequences& q, 
   if (each) each[2 * q.count] = tokens, each[2 * q.count + 1] = filled;
 }
 
-// Of the pair: for the gradient, each[s] that of a token of either sequence (but for the mean over the pairs).
+// Of the pair: for the gradient, each[s] that of a token of either sequence (but for the mean over the pairs).  A sequence without
+// tokens beside one that has some has h = 0.
 __device__ __forceinline__ void seq_take(const Preference& f, const Sequences& q, const double* parts, int64_t p, int lane,
                                          int lanes, double* __restrict__ each, float* __restrict__ rewards,
                                          double (&total)[kPreferenceTotals]) {

@@ -146,8 +146,11 @@ class AdamW(torch.optim.Optimizer):
     ``step(total_norm=..., max_norm=...)`` scales the gradients by min(1, max_norm / (total_norm + 1e-6)) as they are read:
     ``clip_grads_with_norm_`` without its pass over memory (the gradients stay as they are, and of bf16 ones no scaled rounding).
 
+    Gradients are read in float32 (float32 ones of bf16 parameters as they are).
+
     With `capturable` the step counters are on the device and `lr` may be a float32 tensor there: a step can be captured into a
-    graph once a step has run outside of one."""
+    graph once a step has run outside of one.  A graph goes on with the tensors that it was captured with: a state that is loaded
+    afterwards wants a new one."""
 
     def __init__(self, params, lr: float | torch.Tensor = 1e-3, betas: tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
                  weight_decay: float = 1e-2, *, state_bits: int = 32, master_weights: bool = False, maximize: bool = False,

@@ -308,11 +308,12 @@ def policy_loss(log_probs: torch.Tensor, advantages: torch.Tensor, old_log_probs
     the tokens from offsets[s] to offsets[s + 1]; rising, not behind the last token).  `mask` (bool) says which of them count.  What a token
     that does not count holds has no influence, and its gradient is 0; sequences without a token that counts are left out of
     every mean.  advantages: [sequences], or of every token (ratio="token"); their shape says which, but for packed tokens as many as
-    there are sequences, where `advantage`, "sequence" or "token", must (on the GPU they are read in float32, whatever their type).  Without `old_log_probs` the policy has not moved: r is
-    1, with its gradient.  kl, at x = log_probs - ref_log_probs: "k1" x, "k2" x^2 / 2, "k3" exp(-x) - 1 + x, "k3_swapped" exp(x) - 1 - x.
+    there are sequences, where `advantage`, "sequence" or "token", must (on the GPU they are read in float32, whatever their type).
+    Without `old_log_probs` the policy has not moved: r is 1, with its gradient.  kl, at x = log_probs - ref_log_probs: "k1" x, "k2"
+    x^2 / 2, "k3" exp(-x) - 1 + x, "k3_swapped" exp(x) - 1 - x.
     The entropy is minus the mean of log_probs.  average: means of pg and KL over all tokens, or over sequences of the means
-    over their tokens.  A coefficient of 0 leaves its term out of the loss, whatever it is.  Only log_probs gets a gradient, which on the GPU cannot be differentiated again; terms and sums
-    are in float64."""
+    over their tokens.  A coefficient of 0 leaves its term out of the loss, whatever it is.  Only log_probs gets a gradient, which on the GPU
+    cannot be differentiated again; terms and sums are in float64."""
     if ratio not in ("token", "sequence") or average not in ("token", "sequence"):
         raise ValueError(f"ratio and average must be 'token' or 'sequence', got {ratio!r} and {average!r}")
     if kl not in _KL:
@@ -380,7 +381,8 @@ def preference_loss(log_probs: torch.Tensor, ref_log_probs: torch.Tensor | None 
         "hinge":   max(0, 1 - beta z)              "ipo": (z - 1 / (2 beta))^2
 
     averaged over the pairs.  The first half of the sequences are the preferred ones, the second half the others, in the same
-    order.  Tokens, `offsets` and `mask` as for ``policy_loss``; a pair without a token that counts is left out.  Without
+    order.  Tokens, `offsets` and `mask` as for ``policy_loss``; a pair without a token that counts is left out, and a sequence without
+    one beside an answer that has some has h = 0.  Without
     `ref_log_probs` h is of log_probs alone.  Only log_probs gets a gradient, which on the GPU cannot be differentiated
     again; terms and sums are in float64."""
     if kind not in _PREFERENCES:
