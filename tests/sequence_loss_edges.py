@@ -1,6 +1,7 @@
 """Infinite values, equal shapes and wide operands in the policy and preference losses, on any device."""
 import math
 
+import pytest
 import torch
 
 from torchtitan_amd.rl import policy_loss, preference_loss
@@ -38,8 +39,6 @@ def a_token_that_the_reference_rules_out(device):
 
 def as_many_tokens_as_sequences(device):
     """Packed, the shape of the advantages does not say what they belong to."""
-    import pytest
-
     lp = torch.zeros(4, device=device, requires_grad=True)
     A = torch.tensor([1.0, 2.0, 3.0, 4.0], device=device)
     for bounds, by_token, by_sequence in (([0, 3, 3, 3, 4], [1.0, 2.0, 3.0, 4.0], [1.0, 1.0, 1.0, 4.0]),

@@ -141,7 +141,7 @@ class AdamW(torch.optim.Optimizer):
     up or down by chance so that their mean is the exact one; `seed` decides about that chance, the same seed gives the same
     bits.  A block whose gradients hold an infinity or a NaN becomes NaN.  Such parameters must be contiguous.  (On the GPU, with
     eps of 1e-9 or more, the root of such an update is within an ulp and the quotient within two, else rounded right as all others;
-    a value's bits do not depend on the parameters beside it.)
+    whatever else is in the list, a value has the same bits, but for its parameter's number there, by which the chance goes too.)
 
     ``step(total_norm=..., max_norm=...)`` scales the gradients by min(1, max_norm / (total_norm + 1e-6)) as they are read:
     ``clip_grads_with_norm_`` without its pass over memory (the gradients stay as they are, and of bf16 ones no scaled rounding).
